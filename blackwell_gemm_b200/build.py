@@ -31,6 +31,10 @@ LIB = PKG / "libb200gemm.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
+# The shared C++ runtime by name: a toolchain whose libstdc++.so link is
+# missing would take the static archive instead, and the process would hold
+# two copies of it -- formatting a number into an error message then crashes.
+STDCXX = "-l:libstdc++.so.6"
 
 
 def _nvcc() -> str:
@@ -67,7 +71,7 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
     tmp = LIB.with_suffix(".so.tmp")
     log = _run([_nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, "-Xptxas", "-v",
                 "-I", INCLUDE, "-I", CSRC, "-shared", "-Xcompiler", "-fPIC",
-                "-o", tmp, CSRC / "gemm_capi.cu"], verbose)
+                "-o", tmp, CSRC / "gemm_capi.cu", "-Xlinker", STDCXX], verbose)
     os.replace(tmp, LIB)
     (PKG / "_build_ptxas.txt").write_text(log)
     return LIB
@@ -91,7 +95,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
            "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{i}" for i in incs],
            CSRC / "matmul.cpp", "-o", tmp,
            f"-L{PKG}", "-lb200gemm", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch",
-           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python",
+           "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", STDCXX,
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
     _run(cmd, verbose)
     os.replace(tmp, EXT)

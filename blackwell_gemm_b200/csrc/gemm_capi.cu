@@ -402,6 +402,12 @@ int device_state(DeviceState** out) {
     return B200_ERR_UNSUPPORTED_DEVICE;
   }
   if (dev < 0 || dev >= kMaxDevices) return B200_ERR_UNSUPPORTED_DEVICE;
+  // A thread that has not used this runtime yet (an autograd thread) has no
+  // current context, and the tensor-map encoder refuses to work without one.
+  if (cudaSetDevice(dev) != cudaSuccess) {
+    cudaGetLastError();
+    return B200_ERR_UNSUPPORTED_DEVICE;
+  }
   std::lock_guard<std::mutex> lock(g_mu);
   DeviceState& d = g_dev[dev];
   if (!d.ready) {
