@@ -21,9 +21,10 @@ import importlib
 import types
 
 from . import capi  # noqa: F401
+from .moe import matmul_b200_grouped
 
 __all__ = ["module", "matmul_b200", "profile_matmul_b200", "matmul_b200_epilogue",
-           "matmul_b200_host", "profile_rows", "capi", "load"]
+           "matmul_b200_host", "matmul_b200_grouped", "profile_rows", "capi", "load"]
 
 _ext = None
 

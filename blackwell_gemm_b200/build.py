@@ -4,7 +4,7 @@ Two artefacts, both written next to this file so they travel with the source
 tree and are found without installation:
 
 * ``libb200gemm.so`` -- the sm_100a kernels and the C ABI of
-  ``include/b200_gemm.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
+  ``include/b200_gemm.h`` and ``include/b200_moe.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
   static CUDA runtime, the driver's tensor-map encoder looked up at run time so
   no ``-lcuda`` is needed);
 * ``_C<ext-suffix>`` -- the torch extension with the reference-compatible
@@ -21,12 +21,14 @@ import shutil
 import subprocess
 import sys
 import sysconfig
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 INCLUDE = ROOT / "include"
+OBJ = PKG / "_build"   # object files, one per source
 LIB = PKG / "libb200gemm.so"
 EXT = PKG / ("_C" + sysconfig.get_config_var("EXT_SUFFIX"))
 
@@ -63,22 +65,41 @@ def _run(cmd, verbose: bool) -> str:
 
 
 def build_lib(force: bool = False, verbose: bool = False) -> Path:
-    srcs = [CSRC / "gemm_capi.cu", CSRC / "gemm_kernel.cuh", CSRC / "gemm_layout.h",
-            CSRC / "gemm_skinny.cuh", CSRC / "ksplit_fused.cuh", CSRC / "sm100_ptx.cuh",
-            INCLUDE / "b200_gemm.h"]
-    if not force and not _stale(LIB, srcs):
+    common = [CSRC / "device_state.h", CSRC / "gemm_kernel.cuh", CSRC / "gemm_layout.h",
+              CSRC / "ksplit_fused.cuh", CSRC / "sm100_ptx.cuh", INCLUDE / "b200_gemm.h"]
+    units = {  # source -> what else it includes
+        "gemm_capi.cu": [CSRC / "gemm_skinny.cuh"],
+        "moe_capi.cu": [*sorted(CSRC.glob("grouped_*.cuh")), *sorted(CSRC.glob("moe_*.cuh")),
+                        INCLUDE / "b200_moe.h"],
+    }
+    OBJ.mkdir(exist_ok=True)
+    stale = [name for name, more in units.items()
+             if force or _stale(OBJ / f"{name}.o", [CSRC / name, *common, *more])]
+    if not stale and not _stale(LIB, [OBJ / f"{name}.o" for name in units]):
         return LIB
+
+    def compile_one(name: str) -> None:
+        tmp = OBJ / f"{name}.o.tmp"
+        log = _run([_nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, "-Xptxas", "-v",
+                    "-I", INCLUDE, "-I", CSRC, "-c", "-Xcompiler", "-fPIC", "-o", tmp,
+                    CSRC / name], verbose)
+        os.replace(tmp, OBJ / f"{name}.o")
+        (OBJ / f"{name}.ptxas.txt").write_text(log)
+
+    with ThreadPoolExecutor(max(1, len(stale))) as pool:
+        list(pool.map(compile_one, stale))
     tmp = LIB.with_suffix(".so.tmp")
-    log = _run([_nvcc(), "-std=c++17", "-O3", "-lineinfo", *ARCH_FLAGS, "-Xptxas", "-v",
-                "-I", INCLUDE, "-I", CSRC, "-shared", "-Xcompiler", "-fPIC",
-                "-o", tmp, CSRC / "gemm_capi.cu", "-Xlinker", STDCXX], verbose)
+    _run([_nvcc(), *ARCH_FLAGS, "-shared", "-Xcompiler", "-fPIC", "-o", tmp,
+          *[OBJ / f"{name}.o" for name in units], "-Xlinker", STDCXX], verbose)
     os.replace(tmp, LIB)
-    (PKG / "_build_ptxas.txt").write_text(log)
+    (PKG / "_build_ptxas.txt").write_text(
+        "".join((OBJ / f"{name}.ptxas.txt").read_text() for name in units))
     return LIB
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
-    srcs = [CSRC / "matmul.cpp", INCLUDE / "b200_gemm.h", LIB]
+    srcs = [CSRC / "matmul.cpp", CSRC / "moe_torch.cpp", CSRC / "moe_torch.h",
+            INCLUDE / "b200_gemm.h", INCLUDE / "b200_moe.h"]
     if not force and not _stale(EXT, srcs):
         return EXT
     import torch
@@ -93,7 +114,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
            "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{i}" for i in incs],
-           CSRC / "matmul.cpp", "-o", tmp,
+           CSRC / "matmul.cpp", CSRC / "moe_torch.cpp", "-o", tmp,
            f"-L{PKG}", "-lb200gemm", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", STDCXX,
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]

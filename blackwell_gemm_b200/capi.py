@@ -32,6 +32,7 @@ DEVICE_WAIT_CODES = {
     0x1007: "K-split: a peer's piece of an own tile never arrived",
     0x1008: "stream-K: an earlier CTA's partial tile never arrived",
     0x1009: "dynamic dealing: a slot of the pair's unit ring",
+    0x100A: "grouped rows: offsets that decrease or leave the rows (clamped)",
 }
 
 KSPLIT_HANDLE_BYTES = 128
@@ -39,6 +40,7 @@ KSPLIT_HANDLE_BYTES = 128
 # Every symbol the header declares, with (restype, argtypes).
 _vp, _i, _u32, _u64, _ull = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64, \
     ctypes.c_ulonglong
+_ll = ctypes.c_longlong
 _ip = ctypes.POINTER(ctypes.c_int)
 SIGNATURES = {
     "b200_gemm_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
@@ -79,6 +81,11 @@ SIGNATURES = {
     "b200_ksplit_gemm_bf16": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "b200_ksplit_epoch": (_i, [_vp, ctypes.POINTER(ctypes.c_uint)]),
     "b200_ksplit_destroy": (_i, [_vp]),
+    # include/b200_moe.h
+    "b200_grouped_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _i, _i, _vp]),
+    "b200_grouped_gemm_da": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _i, _i, _vp]),
+    "b200_grouped_gemm_db": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _vp]),
+    "b200_grouped_set_kernel": (_i, [_i]),
 }
 
 _lib = None
@@ -282,6 +289,15 @@ def launch_shape(M: int, N: int, K: int) -> dict:
     check(lib().b200_gemm_launch_shape(M, N, K, ctypes.byref(t), ctypes.byref(g), ctypes.byref(s),
                                        ctypes.byref(th)), "launch_shape")
     return {"tiles": t.value, "grid": g.value, "smem_bytes": s.value, "threads": th.value}
+
+
+# ---------------------------------------------------------- mixture of experts
+BF16, FP16 = 0, 1
+
+
+def grouped_set_kernel(kernel: int) -> None:
+    """0 chosen by rows per expert (default), 1 streaming kernel, 2 pair kernel."""
+    check(lib().b200_grouped_set_kernel(int(kernel)), "b200_grouped_set_kernel")
 
 
 # ------------------------------------------------- fused K-split over NVLink

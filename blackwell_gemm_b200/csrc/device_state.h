@@ -1,0 +1,26 @@
+// What the launchers of one library share about a device: set up once by
+// gemm_capi.cu, read by the mixture-of-experts launchers (moe_capi.cu).
+#pragma once
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+namespace b200 {
+
+struct DeviceView {
+  int device = -1;
+  int sms = 0;
+  int* status = nullptr;             // device error word
+  cudaMemPool_t pool = nullptr;      // stream-ordered workspaces
+  unsigned long long timeout_ns = 0; // bound on any single pipeline wait
+};
+
+// The current device, set up on its first call.  Returns a status code.
+int device_view(DeviceView* out);
+
+// A tiled tensor map of rank 2 or 3 over 1-, 2- or 4-byte elements, 128-byte
+// swizzle, zero fill out of bounds.  strides_bytes: rank - 1 strides of the
+// outer dimensions.  Returns a status code.
+int encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box);
+
+}  // namespace b200

@@ -21,6 +21,7 @@
 #include <mutex>
 
 #include "b200_gemm.h"
+#include "device_state.h"
 #include "gemm_kernel.cuh"
 #include "gemm_skinny.cuh"
 
@@ -2194,3 +2195,35 @@ extern "C" int b200_gemm_noalloc_wait_probe(unsigned long long timeout_ns, void*
   wait_probe_kernel<<<2, 32, 0, static_cast<cudaStream_t>(stream)>>>(nd->launch.status, timeout_ns);
   return cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_LAUNCH;
 }
+
+// ------------------------------------------- shared with the other launchers
+namespace b200 {
+
+int device_view(DeviceView* out) {
+  DeviceState* d = nullptr;
+  const int st = device_state(&d);
+  if (st != B200_OK) return st;
+  int dev = -1;
+  if (cudaGetDevice(&dev) != cudaSuccess) {
+    cudaGetLastError();
+    return B200_ERR_UNSUPPORTED_DEVICE;
+  }
+  out->device = dev;
+  out->sms = d->sms;
+  out->status = d->status;
+  out->pool = d->pool;
+  out->timeout_ns = g_timeout_ns.load();
+  return B200_OK;
+}
+
+int encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,
+                  const cuuint64_t* dims, const cuuint64_t* strides_bytes, const cuuint32_t* box) {
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      encode_tiled()(map, type, (cuuint32_t)rank, const_cast<void*>(base), dims, strides_bytes, box,
+                     estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     l2_promotion(), CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? B200_OK : B200_ERR_TENSOR_MAP;
+}
+
+}  // namespace b200

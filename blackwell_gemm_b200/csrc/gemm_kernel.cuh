@@ -1036,7 +1036,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
 // Self-test of the bounded wait: one CTA pair waits on a barrier that nothing
 // ever arrives on.  The wait must give up after timeout_ns, record
 // kErrWaitProbe in *status and return; nothing faults or hangs.
-__global__ void __cluster_dims__(2, 1, 1) wait_probe_kernel(int* status,
+static __global__ void __cluster_dims__(2, 1, 1) wait_probe_kernel(int* status,
                                                             unsigned long long timeout_ns) {
   __shared__ alignas(8) uint64_t bar;
   __shared__ uint32_t abort_word;
@@ -1060,7 +1060,7 @@ __global__ void __cluster_dims__(2, 1, 1) wait_probe_kernel(int* status,
 // fp32 workspace (row stride ldw) -> bf16 C (row stride ldc), round to
 // nearest even.  Eight columns per thread; vector loads and stores when the
 // row has eight columns left and both rows are 16-byte aligned there.
-__global__ void __launch_bounds__(256) cast_f32_to_bf16_kernel(const float* __restrict__ W,
+static __global__ void __launch_bounds__(256) cast_f32_to_bf16_kernel(const float* __restrict__ W,
                                                                int ldw, __nv_bfloat16* C,
                                                                int ldc, int M, int N,
                                                                EpiArgs epi, bool fused) {

@@ -96,6 +96,15 @@ B200_HD uint32_t make_idesc_bf16_f32(int mma_m, int mma_n) {
          ((uint32_t)(mma_n >> 3) << 17) | ((uint32_t)(mma_m >> 4) << 24);
 }
 
+// The same descriptor for either 16-bit format (0 = f16, 1 = bf16; A and B
+// alike) and for operands whose M or N index runs along the 128-byte rows
+// (bits 15 and 16: A, B are MN-major).
+B200_HD uint32_t make_idesc_16bit(int mma_m, int mma_n, int format, bool a_mn, bool b_mn) {
+  return (1u << 4) | ((uint32_t)format << 7) | ((uint32_t)format << 10) |
+         ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(mma_n >> 3) << 17) |
+         ((uint32_t)(mma_m >> 4) << 24);
+}
+
 // Shared-memory matrix descriptor for a K-major operand tile written by TMA
 // with 128 B swizzling: rows of 128 B, 8-row swizzle atoms of 1024 B.
 //   bits  0-13 start address >> 4
@@ -107,6 +116,19 @@ B200_HD uint32_t make_idesc_bf16_f32(int mma_m, int mma_n) {
 // Same encoding as the reference's make_smem_desc (kernel_v1.cu:159-164).
 B200_HD uint64_t make_sdesc_k128(uint32_t smem_addr) {
   return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) |
+         ((uint64_t)(1024u >> 4) << 32) |
+         (1ull << 46) |
+         (2ull << 61);
+}
+
+// Descriptor for an MN-major operand tile written by TMA with 128 B
+// swizzling: slabs of 64 M (or N) elements, each K index one 128 B row, 8 K
+// rows to a swizzle atom of 1024 B.  Leading byte offset: from one 64-wide
+// slab to the next; stride byte offset: from one 8-row K group to the next.
+// A K16 step is two groups: start address + 2048 B.
+B200_HD uint64_t make_sdesc_mn128(uint32_t smem_addr, uint32_t slab_bytes) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) |
+         ((uint64_t)(slab_bytes >> 4) << 16) |
          ((uint64_t)(1024u >> 4) << 32) |
          (1ull << 46) |
          (2ull << 61);

@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include "b200_gemm.h"
+#include "moe_torch.h"
 
 namespace {
 
@@ -129,4 +130,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("profile_matmul_b200", &profile_matmul_b200,
         "matmul_b200 with the intra-kernel profiler writing into `profiler`");
   m.def("profile_rows", &profile_rows, "profiler rows needed for an M x N x K call on this device");
+  register_moe(m);
 }

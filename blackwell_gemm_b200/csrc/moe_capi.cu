@@ -1,0 +1,371 @@
+// C-ABI launchers of the mixture-of-experts operators (include/b200_moe.h).
+//
+// Per call: check the arguments, encode the tensor maps, choose a kernel and
+// launch it on the caller's stream.  Per device, once: shared-memory limits
+// and the number of 2-CTA clusters that can be resident.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <atomic>
+#include <mutex>
+
+#include "b200_moe.h"
+#include "device_state.h"
+#include "grouped_gemm.cuh"
+#include "moe_stream.cuh"
+
+using namespace b200;
+
+namespace {
+
+constexpr int kMaxDevices = 64;
+
+struct MoeDevice {
+  bool ready = false;
+  int init_status = B200_OK;
+  int pairs[3] = {};  // resident clusters per GroupedMode
+};
+
+std::mutex g_mu;
+MoeDevice g_moe[kMaxDevices];
+std::atomic<int> g_kernel{0};
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+template <class F>
+bool set_smem(F* fn, int bytes) {
+  return cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) ==
+         cudaSuccess;
+}
+
+template <int kMode, class T>
+bool init_pair(int sms, int* pairs) {
+  using C = GroupedCfg<kMode>;
+  auto* fn = grouped_pair_kernel<kMode, T>;
+  if (!set_smem(fn, C::smem_bytes(kMaxExperts))) return false;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sms);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::smem_bytes(kMaxExperts);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n < 1) return false;
+  if (*pairs == 0 || n < *pairs) *pairs = n;
+  return true;
+}
+
+template <bool kDA, class T>
+bool init_stream() {
+  return set_smem(grouped_stream_kernel<kDA, 16, T>, StreamCfg<16>::smem_bytes(kMaxExperts)) &&
+         set_smem(grouped_stream_kernel<kDA, 64, T>, StreamCfg<64>::smem_bytes(kMaxExperts));
+}
+
+template <class T>
+bool init_type(MoeDevice& m, int sms) {
+  return init_pair<kGroupedFwd, T>(sms, &m.pairs[0]) && init_pair<kGroupedDA, T>(sms, &m.pairs[1]) &&
+         init_pair<kGroupedDB, T>(sms, &m.pairs[2]) && init_stream<false, T>() &&
+         init_stream<true, T>();
+}
+
+int moe_device(DeviceView* v, MoeDevice** out) {
+  const int st = device_view(v);
+  if (st != B200_OK) return st;
+  std::lock_guard<std::mutex> lock(g_mu);
+  MoeDevice& m = g_moe[v->device];
+  if (!m.ready) {
+    m.ready = true;
+    m.init_status = init_type<__nv_bfloat16>(m, v->sms) && init_type<__half>(m, v->sms)
+                        ? B200_OK
+                        : B200_ERR_LAUNCH;
+    if (m.init_status != B200_OK) cudaGetLastError();
+  }
+  if (m.init_status != B200_OK) return m.init_status;
+  *out = &m;
+  return B200_OK;
+}
+
+// Arrival counts of the streaming kernels: one array per (device, stream),
+// made on the stream's first call; every launch leaves it at zero.  Null when
+// none can be made (the caller then clears counts of its own).
+constexpr size_t kCountBytes = 4096 * sizeof(unsigned int);
+struct StreamCounts {
+  int device;
+  cudaStream_t stream;
+  unsigned int* counts;
+};
+constexpr int kMaxStreamCounts = 256;
+StreamCounts g_counts[kMaxStreamCounts];
+int g_num_counts = 0;
+
+unsigned int* stream_counts(int device, cudaStream_t stream) {
+  std::lock_guard<std::mutex> lock(g_mu);
+  for (int i = 0; i < g_num_counts; ++i)
+    if (g_counts[i].device == device && g_counts[i].stream == stream) return g_counts[i].counts;
+  if (g_num_counts == kMaxStreamCounts) return nullptr;
+  unsigned int* p = nullptr;
+  if (cudaMalloc(&p, kCountBytes) != cudaSuccess ||
+      cudaMemsetAsync(p, 0, kCountBytes, stream) != cudaSuccess) {
+    cudaGetLastError();
+    if (p) cudaFree(p);
+    return nullptr;
+  }
+  g_counts[g_num_counts++] = {device, stream, p};
+  return p;
+}
+
+// Slots and counts of one streaming launch.  Counts are the stream's own
+// array, except under capture (a graph may be replayed on another stream),
+// where they come with the slots and are cleared in the graph.
+struct Workspace {
+  char* base = nullptr;
+  cudaStream_t stream = nullptr;
+  int take(const DeviceView& v, size_t slot_bytes, cudaStream_t s, StreamArgs* args) {
+    stream = s;
+    cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(s, &cap) != cudaSuccess) {
+      cudaGetLastError();
+      cap = cudaStreamCaptureStatusActive;
+    }
+    args->counts = cap == cudaStreamCaptureStatusNone ? stream_counts(v.device, s) : nullptr;
+    if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&base), kCountBytes + slot_bytes, v.pool,
+                                s) != cudaSuccess) {
+      cudaGetLastError();
+      base = nullptr;
+      return B200_ERR_LAUNCH;
+    }
+    args->slots = reinterpret_cast<float*>(base + kCountBytes);
+    if (args->counts == nullptr) {
+      args->counts = reinterpret_cast<unsigned int*>(base);
+      if (cudaMemsetAsync(base, 0, kCountBytes, s) != cudaSuccess) {
+        cudaGetLastError();
+        return B200_ERR_LAUNCH;
+      }
+    }
+    return B200_OK;
+  }
+  ~Workspace() {
+    if (base) cudaFreeAsync(base, stream);
+  }
+};
+
+CUtensorMapDataType map_type(int dtype) {
+  return dtype == B200_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+}
+
+int map_rows(CUtensorMap* m, int dtype, const void* p, int cols, int rows, int ld, int box_rows) {
+  const cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
+  const cuuint32_t box[2] = {kSlabK, (cuuint32_t)box_rows};
+  return encode_tensor(m, map_type(dtype), 2, p, dims, strides, box);
+}
+
+int map_bank(CUtensorMap* m, int dtype, const void* p, int K, int N, int experts, int ld,
+             long long expert_stride, int box_rows) {
+  const cuuint64_t dims[3] = {(cuuint64_t)K, (cuuint64_t)N, (cuuint64_t)experts};
+  // (the stride of a bank of one is never used; any valid one will do)
+  const cuuint64_t far = experts > 1 ? (cuuint64_t)expert_stride * 2 : (cuuint64_t)N * ld * 2;
+  const cuuint64_t strides[2] = {(cuuint64_t)ld * 2, far};
+  const cuuint32_t box[3] = {kSlabK, (cuuint32_t)box_rows, 1};
+  return encode_tensor(m, map_type(dtype), 3, p, dims, strides, box);
+}
+
+// One call's operands: t the token operand read (A or dC), u the token
+// operand written (C or dA) or, for dB, the other one read (A).
+struct Call {
+  const void* t;
+  void* u;
+  void* bank;
+  const int* offsets;
+  int rows, experts, N, K;
+  int ldt, ldu, ldb;
+  long long expert_stride;
+  int dtype;
+};
+
+int check_call(const Call& c, int mode) {
+  if (c.rows < 0 || c.experts < 0 || c.N < 0 || c.K < 0) return B200_ERR_INVALID_ARGUMENT;
+  if (c.dtype != B200_BF16 && c.dtype != B200_FP16) return B200_ERR_INVALID_ARGUMENT;
+  if (c.experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  const int wt = mode == kGroupedFwd ? c.K : c.N;  // width of t
+  const int wu = mode == kGroupedFwd ? c.N : c.K;  // width of u
+  const bool has_t = c.rows > 0 && wt > 0, has_u = c.rows > 0 && wu > 0;
+  const bool has_bank = c.experts > 0 && c.N > 0 && c.K > 0;
+  if ((has_t && !c.t) || (has_u && !c.u) || (has_bank && !c.bank) || (c.experts > 0 && !c.offsets))
+    return B200_ERR_INVALID_ARGUMENT;
+  if ((has_t && c.ldt < wt) || (has_u && c.ldu < wu) || (has_bank && c.ldb < c.K) ||
+      (has_bank && c.experts > 1 && c.expert_stride < (long long)c.N * c.ldb))
+    return B200_ERR_INVALID_ARGUMENT;
+  if ((has_t && (!aligned16(c.t) || (c.ldt & 7))) || (has_u && (!aligned16(c.u) || (c.ldu & 7))) ||
+      (has_bank && (!aligned16(c.bank) || (c.ldb & 7) ||
+                    (c.experts > 1 && (c.expert_stride & 7)))) ||
+      (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
+    return B200_ERR_ALIGNMENT;
+  // unit numbers are 32-bit
+  const int feat = mode == kGroupedDA ? c.K : c.N;
+  const long long units = mode == kGroupedDB
+                              ? ceil_div(c.N, 256) * ceil_div(c.K, 256) * c.experts
+                              : (ceil_div(c.rows, 16) + c.experts) * ceil_div(feat, 128);
+  return units < (1ll << 30) ? B200_OK : B200_ERR_TOO_LARGE;
+}
+
+int zero_rows(void* p, int ld, int width, int rows, cudaStream_t stream) {
+  if (rows == 0 || width == 0) return B200_OK;
+  return cudaMemset2DAsync(p, (size_t)ld * 2, 0, (size_t)width * 2, rows, stream) == cudaSuccess
+             ? B200_OK
+             : B200_ERR_LAUNCH;
+}
+
+int launched() {
+  if (cudaGetLastError() == cudaSuccess) return B200_OK;
+  return B200_ERR_LAUNCH;
+}
+
+template <int kMode, class T>
+int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStream_t stream) {
+  using C = GroupedCfg<kMode>;
+  CUtensorMap tw, tt, ts;
+  int st;
+  if (kMode == kGroupedDB) {
+    st = map_rows(&tw, c.dtype, c.t, c.N, c.rows, c.ldt, 64);
+    if (st == B200_OK) st = map_rows(&tt, c.dtype, c.u, c.K, c.rows, c.ldu, 64);
+    if (st == B200_OK)
+      st = map_bank(&ts, c.dtype, c.bank, c.K, c.N, c.experts, c.ldb, c.expert_stride, 32);
+  } else {
+    const int red = kMode == kGroupedFwd ? c.K : c.N;
+    st = map_bank(&tw, c.dtype, c.bank, c.K, c.N, c.experts, c.ldb, c.expert_stride,
+                  kMode == kGroupedFwd ? 128 : 64);
+    if (st == B200_OK) st = map_rows(&tt, c.dtype, c.t, red, c.rows, c.ldt, 128);
+    if (st == B200_OK) st = map_rows(&ts, c.dtype, c.t, red, c.rows, c.ldt, 16);
+  }
+  if (st != B200_OK) return st;
+  GroupedArgs a = {};
+  a.offsets = c.offsets;
+  a.experts = c.experts;
+  a.rows = c.rows;
+  a.feat = kMode == kGroupedDA ? c.K : c.N;
+  a.red = kMode == kGroupedFwd ? c.K : c.N;
+  a.cols = c.K;
+  a.out = kMode == kGroupedDB ? nullptr : c.u;
+  a.ldo = c.ldu;
+  a.group = 8;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  const long long tf = ceil_div(a.feat, 256);
+  const long long most = kMode == kGroupedDB
+                             ? tf * ceil_div(c.K, 256) * c.experts
+                             : tf * (ceil_div(c.rows, 256) + (c.experts < c.rows ? c.experts : c.rows));
+  const int pairs = (int)(most < m.pairs[kMode] ? most : m.pairs[kMode]);
+  grouped_pair_kernel<kMode, T>
+      <<<2 * pairs, C::kThreads, C::smem_bytes(c.experts), stream>>>(tw, tt, ts, a);
+  return launched();
+}
+
+template <bool kDA, int kTok, class T>
+int launch_stream(const Call& c, const DeviceView& v, cudaStream_t stream) {
+  using C = StreamCfg<kTok>;
+  CUtensorMap tw, tt;
+  int st = map_bank(&tw, c.dtype, c.bank, c.K, c.N, c.experts, c.ldb, c.expert_stride,
+                    kDA ? 64 : 128);
+  const int red = kDA ? c.N : c.K;
+  if (st == B200_OK) st = map_rows(&tt, c.dtype, c.t, red, c.rows, c.ldt, 16);
+  if (st != B200_OK) return st;
+  StreamArgs a = {};
+  a.offsets = c.offsets;
+  a.experts = c.experts;
+  a.rows = c.rows;
+  a.feat = kDA ? c.K : c.N;
+  a.feat_blocks = (int)ceil_div(a.feat, 128);
+  a.red = red;
+  a.red_blocks = (int)ceil_div(red, kSlabK);
+  a.min_items = 4;
+  a.out = c.u;
+  a.ldo = c.ldu;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  Workspace ws;
+  st = ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a);
+  if (st != B200_OK) return st;
+  grouped_stream_kernel<kDA, kTok, T>
+      <<<v.sms, C::kThreads, C::smem_bytes(c.experts), stream>>>(tw, tt, a);
+  return launched();
+}
+
+template <int kMode, class T>
+int run_typed(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStream_t stream) {
+  if constexpr (kMode != kGroupedDB) {
+    constexpr bool kDA = kMode == kGroupedDA;
+    const int k = g_kernel.load();
+    const bool few = k == 1 || (k == 0 && (long long)c.rows <= 64ll * c.experts);
+    if (few)
+      return c.rows <= 16 ? launch_stream<kDA, 16, T>(c, v, stream)
+                          : launch_stream<kDA, 64, T>(c, v, stream);
+  }
+  return launch_pair<kMode, T>(c, v, m, stream);
+}
+
+template <int kMode>
+int run_grouped(const Call& c, cudaStream_t stream) {
+  int st = check_call(c, kMode);
+  if (st != B200_OK) return st;
+  const bool no_bank = c.experts == 0 || c.N == 0 || c.K == 0;
+  if (kMode == kGroupedDB ? no_bank : c.rows == 0 || (kMode == kGroupedDA ? c.K : c.N) == 0)
+    return B200_OK;  // nothing to write
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  if (kMode != kGroupedDB && no_bank)  // an empty contraction, or no expert at all
+    return zero_rows(c.u, c.ldu, kMode == kGroupedDA ? c.K : c.N, c.rows, stream);
+  if (kMode == kGroupedDB && c.rows == 0) {
+    for (int e = 0; e < c.experts; ++e) {
+      st = zero_rows(static_cast<char*>(c.bank) + 2 * e * c.expert_stride, c.ldb, c.K, c.N, stream);
+      if (st != B200_OK) return st;
+    }
+    return B200_OK;
+  }
+  return c.dtype == B200_FP16 ? run_typed<kMode, __half>(c, v, *m, stream)
+                              : run_typed<kMode, __nv_bfloat16>(c, v, *m, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_grouped_gemm(const void* A, const void* B, void* C, const int* offsets, int rows,
+                      int experts, int N, int K, int lda, int ldb, long long expert_stride,
+                      int ldc, int dtype, void* stream) {
+  const Call c = {A, C, const_cast<void*>(B), offsets, rows, experts, N, K,
+                  lda, ldc, ldb, expert_stride, dtype};
+  return run_grouped<kGroupedFwd>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_grouped_gemm_da(const void* dC, const void* B, void* dA, const int* offsets, int rows,
+                         int experts, int N, int K, int ldc, int ldb, long long expert_stride,
+                         int lda, int dtype, void* stream) {
+  const Call c = {dC, dA, const_cast<void*>(B), offsets, rows, experts, N, K,
+                  ldc, lda, ldb, expert_stride, dtype};
+  return run_grouped<kGroupedDA>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* offsets, int rows,
+                         int experts, int N, int K, int ldc, int lda, int ldb,
+                         long long expert_stride, int dtype, void* stream) {
+  const Call c = {dC, const_cast<void*>(A), dB, offsets, rows, experts, N, K,
+                  ldc, lda, ldb, expert_stride, dtype};
+  return run_grouped<kGroupedDB>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_grouped_set_kernel(int kernel) {
+  if (kernel < 0 || kernel > 2) return B200_ERR_INVALID_ARGUMENT;
+  g_kernel.store(kernel);
+  return B200_OK;
+}
+
+}  // extern "C"

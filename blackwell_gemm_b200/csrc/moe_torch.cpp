@@ -1,0 +1,204 @@
+// Torch bindings of the mixture-of-experts operators (include/b200_moe.h).
+//
+// As for matmul_b200: dtype, device, rank and shape are checked and raise
+// RuntimeError; an operand whose rows are not 16-byte aligned is first copied
+// into a layout the kernels read; launches go on the current torch stream.
+// Operators with gradients are autograd functions here in C++, so a training
+// step pays no Python call per node.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "b200_moe.h"
+#include "moe_torch.h"
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void check_status(int st, const char* what) {
+  TORCH_CHECK(st == B200_OK, what, " failed: ", b200_gemm_status_string(st), " (status ", st, ")");
+}
+
+int64_t round_up8(int64_t x) { return (x + 7) / 8 * 8; }
+
+bool aligned16(const at::Tensor& t) {
+  return (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0;
+}
+
+void* current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+int dtype_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kHalf ? B200_FP16 : B200_BF16;
+}
+
+void check_16bit(const at::Tensor& t, const char* who, const char* name) {
+  TORCH_CHECK(t.is_cuda(), who, ": ", name, " must be a CUDA tensor");
+  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, who, ": ", name,
+              " must be bfloat16 or float16");
+}
+
+void check_same(const at::Tensor& t, const at::Tensor& like, const char* who, const char* name) {
+  TORCH_CHECK(t.device() == like.device(), who, ": ", name, " is on another device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), who, ": ", name, " has another dtype");
+}
+
+// A rows x cols operand as the kernels read it (unit column stride, rows and
+// base on 16 bytes): `t` itself where it is one, else a copy.
+struct Rows {
+  at::Tensor t;
+  int ld;
+};
+
+Rows as_rows(const at::Tensor& t) {
+  const int64_t rows = t.size(0), cols = t.size(1), pad = std::max<int64_t>(round_up8(cols), 8);
+  if (rows == 0 || cols == 0) return {t, (int)pad};
+  const int64_t ld = rows > 1 ? t.stride(0) : pad;
+  if ((cols == 1 || t.stride(1) == 1) && ld >= cols && ld % 8 == 0 && ld < (1ll << 31) &&
+      aligned16(t))
+    return {t, (int)ld};
+  auto buf = at::empty({rows, pad}, t.options());
+  auto view = buf.narrow(1, 0, cols);
+  view.copy_(t);
+  return {view, (int)pad};
+}
+
+// The same for a bank of matrices, given as (experts, N, K).
+struct Bank {
+  at::Tensor t;
+  int ld;
+  int64_t stride;
+};
+
+Bank as_bank(const at::Tensor& t) {
+  const int64_t e = t.size(0), n = t.size(1), k = t.size(2);
+  const int64_t pad = std::max<int64_t>(round_up8(k), 8);
+  if (t.numel() == 0) return {t, (int)pad, n * pad};
+  const int64_t ld = n > 1 ? t.stride(1) : pad;
+  const int64_t stride = e > 1 ? t.stride(0) : n * ld;
+  if ((k == 1 || t.stride(2) == 1) && ld >= k && ld % 8 == 0 && ld < (1ll << 31) &&
+      stride % 8 == 0 && stride >= n * ld && aligned16(t))
+    return {t, (int)ld, stride};
+  auto buf = at::empty({e, n, pad}, t.options());
+  auto view = buf.narrow(2, 0, k);
+  view.copy_(t);
+  return {view, (int)pad, n * pad};
+}
+
+// A new rows x cols result whose rows are on 16 bytes; `done` gives the
+// caller a contiguous tensor.
+struct Result {
+  at::Tensor buf;
+  int64_t cols;
+  int ld;
+  at::Tensor done() const {
+    return buf.size(1) == cols ? buf : buf.narrow(1, 0, cols).contiguous();
+  }
+};
+
+Result new_rows(int64_t rows, int64_t cols, const at::Tensor& like) {
+  const int64_t pad = round_up8(cols);
+  return {at::empty({rows, pad}, like.options()), cols, (int)std::max<int64_t>(pad, 8)};
+}
+
+at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::Tensor& like,
+                         const char* who) {
+  TORCH_CHECK(offsets.dim() == 1 && offsets.size(0) == experts + 1, who, ": offsets must have ",
+              experts + 1, " entries (one more than there are experts)");
+  TORCH_CHECK(offsets.device() == like.device(), who, ": offsets must be on the operands' device");
+  TORCH_CHECK(offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong, who,
+              ": offsets must be int32 or int64");
+  return offsets.to(at::kInt).contiguous();
+}
+
+void check_sizes(std::initializer_list<int64_t> sizes, const char* who) {
+  for (int64_t s : sizes)
+    TORCH_CHECK(s < (1ll << 31) - 8, who, ": dimension exceeds 2^31-1");
+}
+
+// ------------------------------------------------------------ grouped product
+constexpr const char* kGrouped = "matmul_b200_grouped";
+
+at::Tensor grouped_forward(const at::Tensor& a, const at::Tensor& bank, const at::Tensor& offsets) {
+  const c10::cuda::CUDAGuard guard(a.device());
+  const Rows ra = as_rows(a);
+  const Bank rb = as_bank(bank);
+  const Result c = new_rows(a.size(0), bank.size(1), a);
+  check_status(b200_grouped_gemm(ra.t.data_ptr(), rb.t.data_ptr(), c.buf.data_ptr(),
+                                 offsets.data_ptr<int>(), (int)a.size(0), (int)bank.size(0),
+                                 (int)bank.size(1), (int)bank.size(2), ra.ld, rb.ld, rb.stride,
+                                 c.ld, dtype_code(a), current_stream()),
+               kGrouped);
+  return c.done();
+}
+
+at::Tensor grouped_da(const at::Tensor& dc, const at::Tensor& bank, const at::Tensor& offsets) {
+  const Rows rc = as_rows(dc);
+  const Bank rb = as_bank(bank);
+  const Result da = new_rows(dc.size(0), bank.size(2), dc);
+  check_status(b200_grouped_gemm_da(rc.t.data_ptr(), rb.t.data_ptr(), da.buf.data_ptr(),
+                                    offsets.data_ptr<int>(), (int)dc.size(0), (int)bank.size(0),
+                                    (int)bank.size(1), (int)bank.size(2), rc.ld, rb.ld, rb.stride,
+                                    da.ld, dtype_code(dc), current_stream()),
+               "matmul_b200_grouped backward (A)");
+  return da.done();
+}
+
+at::Tensor grouped_db(const at::Tensor& dc, const at::Tensor& a, const at::Tensor& offsets) {
+  const int64_t experts = offsets.size(0) - 1, n = dc.size(1), k = a.size(1), pad = round_up8(k);
+  const Rows rc = as_rows(dc);
+  const Rows ra = as_rows(a);
+  auto db = at::empty({experts, n, pad}, dc.options());
+  check_status(b200_grouped_gemm_db(rc.t.data_ptr(), ra.t.data_ptr(), db.data_ptr(),
+                                    offsets.data_ptr<int>(), (int)dc.size(0), (int)experts, (int)n,
+                                    (int)k, rc.ld, ra.ld, (int)std::max<int64_t>(pad, 8), n * pad,
+                                    dtype_code(dc), current_stream()),
+               "matmul_b200_grouped backward (B)");
+  return pad == k ? db : db.narrow(2, 0, k).contiguous();
+}
+
+struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& a, const at::Tensor& b,
+                            const at::Tensor& offsets) {
+    ctx->save_for_backward({a, b, offsets});
+    return grouped_forward(a, b.transpose(1, 2), offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &a = saved[0], &b = saved[1], &offsets = saved[2];
+    at::Tensor da, db;
+    if (grads[0].defined()) {
+      const c10::cuda::CUDAGuard guard(a.device());
+      const at::Tensor dc = grads[0].to(a.scalar_type());
+      if (ctx->needs_input_grad(0)) da = grouped_da(dc, b.transpose(1, 2), offsets);
+      if (ctx->needs_input_grad(1)) db = grouped_db(dc, a, offsets).transpose(1, 2);
+    }
+    return {da, db, at::Tensor()};
+  }
+};
+
+at::Tensor matmul_b200_grouped(const at::Tensor& A, const at::Tensor& B,
+                               const at::Tensor& offsets) {
+  TORCH_CHECK(A.dim() == 2 && B.dim() == 3, kGrouped,
+              ": A must be (rows, K) and B (experts, K, N)");
+  check_16bit(A, kGrouped, "A");
+  check_16bit(B, kGrouped, "B");
+  check_same(B, A, kGrouped, "B");
+  TORCH_CHECK(B.size(1) == A.size(1), kGrouped, ": inner dimensions differ (A has K = ", A.size(1),
+              ", B has K = ", B.size(1), ")");
+  TORCH_CHECK(B.size(0) <= B200_MAX_EXPERTS, kGrouped, ": more than ", B200_MAX_EXPERTS,
+              " experts");
+  check_sizes({A.size(0), A.size(1), B.size(2)}, kGrouped);
+  const at::Tensor off = check_offsets(offsets, B.size(0), A, kGrouped);
+  if (at::GradMode::is_enabled() && (A.requires_grad() || B.requires_grad()))
+    return GroupedMatmul::apply(A, B, off);
+  return grouped_forward(A, B.transpose(1, 2), off);
+}
+
+}  // namespace
+
+void register_moe(pybind11::module_& m) {
+  m.def("matmul_b200_grouped", &matmul_b200_grouped,
+        "C[r] = A[r] @ B[e] for rows r of expert e (offsets on the device)");
+}

@@ -1,0 +1,83 @@
+"""What the mixture-of-experts operators refuse, checked before any device is
+touched (so this runs without a GPU)."""
+import pytest
+import torch
+
+import blackwell_gemm_b200 as bg
+from blackwell_gemm_b200 import capi
+
+FAKE = 0x7F0000000000  # never dereferenced: validation fails or returns first
+INT_MAX = 2 ** 31 - 1
+
+
+def grouped(a=FAKE, b=FAKE, c=FAKE, off=FAKE, rows=8, experts=2, n=8, k=8, lda=8, ldb=8,
+            stride=64, ldc=8, dtype=capi.BF16):
+    return capi.lib().b200_grouped_gemm(a, b, c, off, rows, experts, n, k, lda, ldb, stride, ldc,
+                                        dtype, None)
+
+
+@pytest.mark.parametrize("change,expect", [
+    (dict(rows=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(experts=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(n=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(k=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(dtype=2), capi.ERR_INVALID_ARGUMENT),
+    (dict(a=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(b=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(c=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(off=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(k=16, ldb=16, stride=128), capi.ERR_INVALID_ARGUMENT),    # lda < K
+    (dict(k=16, lda=16, stride=128), capi.ERR_INVALID_ARGUMENT),    # ldb < K
+    (dict(n=16, stride=128), capi.ERR_INVALID_ARGUMENT),            # ldc < N
+    (dict(stride=56), capi.ERR_INVALID_ARGUMENT),                   # matrices overlap
+    (dict(a=FAKE + 2), capi.ERR_ALIGNMENT),
+    (dict(b=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(c=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(off=FAKE + 2), capi.ERR_ALIGNMENT),
+    (dict(lda=12), capi.ERR_ALIGNMENT),
+    (dict(ldb=12, stride=96), capi.ERR_ALIGNMENT),
+    (dict(ldc=12), capi.ERR_ALIGNMENT),
+    (dict(stride=68), capi.ERR_ALIGNMENT),
+    (dict(experts=1025), capi.ERR_TOO_LARGE),
+    (dict(rows=INT_MAX, n=INT_MAX, ldc=INT_MAX - 7, stride=2 ** 40), capi.ERR_INVALID_ARGUMENT),
+    (dict(rows=2 ** 30, n=2 ** 30, ldc=2 ** 30, stride=2 ** 33), capi.ERR_TOO_LARGE),
+    (dict(rows=0, a=0, c=0), capi.OK),
+    (dict(n=0, b=0, c=0), capi.OK),
+])
+def test_grouped_c_abi(change, expect):
+    assert grouped(**change) == expect
+
+
+def test_grouped_gradients_c_abi():
+    lib = capi.lib()
+    da = lambda **k: lib.b200_grouped_gemm_da(*_args(k, ldc=8, ldb=8, stride=64, last=8))  # noqa: E731
+    assert da(rows=-1) == capi.ERR_INVALID_ARGUMENT
+    assert da(p0=FAKE + 2) == capi.ERR_ALIGNMENT
+    assert da(rows=0) == capi.OK
+    args = [FAKE, FAKE, FAKE, FAKE, 8, 2, 8, 8, 8, 8, 8, 64, capi.BF16, None]
+    for at, value, expect in [(0, 0, capi.ERR_INVALID_ARGUMENT), (2, FAKE + 4, capi.ERR_ALIGNMENT),
+                              (8, 4, capi.ERR_INVALID_ARGUMENT), (11, 8, capi.ERR_INVALID_ARGUMENT),
+                              (5, 0, capi.OK), (6, 0, capi.OK), (12, 7, capi.ERR_INVALID_ARGUMENT)]:
+        changed = list(args)
+        changed[at] = value
+        assert lib.b200_grouped_gemm_db(*changed) == expect, (at, value)
+    for bad in (-1, 3):
+        with pytest.raises(capi.GemmError):
+            capi.grouped_set_kernel(bad)
+
+
+def _args(k, ldc, ldb, stride, last):
+    return [k.get("p0", FAKE), FAKE, FAKE, FAKE, k.get("rows", 8), 2, 8, 8, ldc, ldb, stride, last,
+            capi.BF16, None]
+
+
+def test_grouped_torch_checks():
+    x = torch.zeros(4, 8, dtype=torch.bfloat16)
+    w = torch.zeros(2, 8, 8, dtype=torch.bfloat16)
+    off = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        bg.matmul_b200_grouped(x, w, off)
+    with pytest.raises(RuntimeError, match="experts, K, N"):
+        bg.matmul_b200_grouped(x, w[0], off)
+    with pytest.raises(RuntimeError, match="rows, K"):
+        bg.matmul_b200_grouped(x[0], w, off)
