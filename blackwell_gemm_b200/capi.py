@@ -86,6 +86,9 @@ SIGNATURES = {
     "b200_grouped_gemm_da": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _i, _i, _vp]),
     "b200_grouped_gemm_db": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _vp]),
     "b200_grouped_set_kernel": (_i, [_i]),
+    "b200_w4_packed_bytes": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
+    "b200_w4_pack": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
+    "b200_w4_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
 }
 
 _lib = None

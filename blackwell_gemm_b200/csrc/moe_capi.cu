@@ -13,6 +13,7 @@
 #include "device_state.h"
 #include "grouped_gemm.cuh"
 #include "moe_stream.cuh"
+#include "moe_w4.cuh"
 
 using namespace b200;
 
@@ -67,11 +68,23 @@ bool init_stream() {
          set_smem(grouped_stream_kernel<kDA, 64, T>, StreamCfg<64>::smem_bytes(kMaxExperts));
 }
 
+// Token tile of the 4-bit kernel: all rows of a small call in one tile of 16;
+// else the widest whose products (one set of columns per group of a record)
+// fit the kernel's TMEM.
+constexpr int w4_tokens(int group) { return group == 32 ? 32 : 64; }
+
+template <int kGroup, class T>
+bool init_w4() {
+  constexpr int wide = w4_tokens(kGroup);
+  return set_smem(w4_stream_kernel<16, kGroup, T>, W4Cfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
+         set_smem(w4_stream_kernel<wide, kGroup, T>, W4Cfg<wide, kGroup>::smem_bytes(kMaxExperts));
+}
+
 template <class T>
 bool init_type(MoeDevice& m, int sms) {
   return init_pair<kGroupedFwd, T>(sms, &m.pairs[0]) && init_pair<kGroupedDA, T>(sms, &m.pairs[1]) &&
          init_pair<kGroupedDB, T>(sms, &m.pairs[2]) && init_stream<false, T>() &&
-         init_stream<true, T>();
+         init_stream<true, T>() && init_w4<32, T>() && init_w4<64, T>() && init_w4<128, T>();
 }
 
 int moe_device(DeviceView* v, MoeDevice** out) {
@@ -334,6 +347,114 @@ int run_grouped(const Call& c, cudaStream_t stream) {
                               : run_typed<kMode, __nv_bfloat16>(c, v, *m, stream);
 }
 
+// ------------------------------------------------------------- 4-bit weights
+struct W4Call {
+  const void* a;
+  const void* packed;
+  void* c;
+  const int* offsets;
+  int rows, experts, N, K, group, zeros, lda, ldc, dtype;
+};
+
+int check_w4_shape(int experts, int N, int K, int group) {
+  if (experts < 0 || N < 0 || K < 0) return B200_ERR_INVALID_ARGUMENT;
+  if ((group != 32 && group != 64 && group != 128) || K % group != 0)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  // record numbers are launch indexes
+  return (long long)experts * ceil_div(N, kW4Rows) * ceil_div(K, kW4K) < (1ll << 31)
+             ? B200_OK
+             : B200_ERR_TOO_LARGE;
+}
+
+template <int kTok, int kGroup, class T>
+int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
+  using C = W4Cfg<kTok, kGroup>;
+  CUtensorMap tt;
+  int st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, 16);
+  if (st != B200_OK) return st;
+  StreamArgs a = {};
+  a.offsets = c.offsets;
+  a.experts = c.experts;
+  a.rows = c.rows;
+  a.feat = c.N;
+  a.feat_blocks = (int)ceil_div(c.N, kW4Rows);
+  a.red = c.K;
+  a.red_blocks = (int)ceil_div(c.K, kW4K);
+  a.min_items = 4;
+  a.out = c.c;
+  a.ldo = c.ldc;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  a.packed = static_cast<const uint8_t*>(c.packed);
+  a.record_bytes = w4_record_bytes(kGroup, c.zeros != 0);
+  a.expert_bytes = (long long)a.feat_blocks * a.red_blocks * a.record_bytes;
+  Workspace ws;
+  st = ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a);
+  if (st != B200_OK) return st;
+  w4_stream_kernel<kTok, kGroup, T>
+      <<<v.sms, C::kThreads, C::smem_bytes(c.experts), stream>>>(tt, a, c.zeros != 0);
+  return launched();
+}
+
+template <int kGroup, class T>
+int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
+  return c.rows <= 16 ? launch_w4<16, kGroup, T>(c, v, stream)
+                      : launch_w4<w4_tokens(kGroup), kGroup, T>(c, v, stream);
+}
+
+template <class T>
+int run_w4_typed(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
+  return c.group == 32   ? run_w4_group<32, T>(c, v, stream)
+         : c.group == 64 ? run_w4_group<64, T>(c, v, stream)
+                         : run_w4_group<128, T>(c, v, stream);
+}
+
+int run_w4(const W4Call& c, cudaStream_t stream) {
+  int st = check_w4_shape(c.experts, c.N, c.K, c.group);
+  if (st != B200_OK) return st;
+  if (c.rows < 0 || (c.dtype != B200_BF16 && c.dtype != B200_FP16) ||
+      (c.offsets == nullptr && c.experts > 1))
+    return B200_ERR_INVALID_ARGUMENT;
+  if (c.rows == 0 || c.N == 0) return B200_OK;
+  const bool empty = c.K == 0 || c.experts == 0;
+  if (!c.c || c.ldc < c.N || (!empty && (!c.a || !c.packed || c.lda < c.K)))
+    return B200_ERR_INVALID_ARGUMENT;
+  if (!aligned16(c.c) || (c.ldc & 7) ||
+      (!empty && (!aligned16(c.a) || (c.lda & 7) || !aligned16(c.packed))) ||
+      (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
+    return B200_ERR_ALIGNMENT;
+  if ((ceil_div(c.rows, 16) + c.experts) * ceil_div(c.N, kW4Rows) >= (1ll << 30))
+    return B200_ERR_TOO_LARGE;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  if (empty) return zero_rows(c.c, c.ldc, c.N, c.rows, stream);
+  return c.dtype == B200_FP16 ? run_w4_typed<__half>(c, v, stream)
+                              : run_w4_typed<__nv_bfloat16>(c, v, stream);
+}
+
+int run_w4_pack(const void* q, const void* scales, const void* zeros, void* packed, int experts,
+                int N, int K, int group, cudaStream_t stream) {
+  int st = check_w4_shape(experts, N, K, group);
+  if (st != B200_OK) return st;
+  const int blocks = (int)ceil_div(N, kW4Rows), red = (int)ceil_div(K, kW4K);
+  const long long records = (long long)experts * blocks * red;
+  if (records == 0) return B200_OK;
+  if (!q || !scales || !packed) return B200_ERR_INVALID_ARGUMENT;
+  if (!aligned16(packed) || (reinterpret_cast<uintptr_t>(scales) & 1u)) return B200_ERR_ALIGNMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  w4_pack_kernel<<<(unsigned)records, 256, 0, stream>>>(
+      static_cast<const uint8_t*>(q), static_cast<const uint16_t*>(scales),
+      static_cast<const uint8_t*>(zeros), static_cast<uint8_t*>(packed), N, K, group, blocks, red,
+      w4_record_bytes(group, zeros != nullptr));
+  return launched();
+}
+
 }  // namespace
 
 extern "C" {
@@ -366,6 +487,28 @@ int b200_grouped_set_kernel(int kernel) {
   if (kernel < 0 || kernel > 2) return B200_ERR_INVALID_ARGUMENT;
   g_kernel.store(kernel);
   return B200_OK;
+}
+
+int b200_w4_packed_bytes(int experts, int N, int K, int group, int zeros, size_t* bytes) {
+  if (!bytes) return B200_ERR_INVALID_ARGUMENT;
+  const int st = check_w4_shape(experts, N, K, group);
+  if (st != B200_OK) return st;
+  *bytes = (size_t)experts * ceil_div(N, kW4Rows) * ceil_div(K, kW4K) *
+           w4_record_bytes(group, zeros != 0);
+  return B200_OK;
+}
+
+int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* packed, int experts,
+                 int N, int K, int group, void* stream) {
+  return run_w4_pack(q, scales, zeros, packed, experts, N, K, group,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets, int rows,
+                 int experts, int N, int K, int group, int zeros, int lda, int ldc, int dtype,
+                 void* stream) {
+  const W4Call c = {A, packed, C, offsets, rows, experts, N, K, group, zeros, lda, ldc, dtype};
+  return run_w4(c, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

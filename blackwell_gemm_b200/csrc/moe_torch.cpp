@@ -196,9 +196,84 @@ at::Tensor matmul_b200_grouped(const at::Tensor& A, const at::Tensor& B,
   return grouped_forward(A, B.transpose(1, 2), off);
 }
 
+// -------------------------------------------------------------- 4-bit weights
+constexpr const char* kPack = "pack_w4";
+constexpr const char* kW4 = "matmul_b200_w4";
+
+// q (experts, N, K / 2), scales and zeros (experts, N, K / group): the packed bytes.
+at::Tensor w4_pack(const at::Tensor& q, const at::Tensor& scales,
+                   const std::optional<at::Tensor>& zeros) {
+  TORCH_CHECK(q.dim() == 3 && scales.dim() == 3, kPack,
+              ": q must be (N, K/2) or (experts, N, K/2) and scales (.., N, K/group)");
+  TORCH_CHECK(q.is_cuda() && q.scalar_type() == at::kByte, kPack,
+              ": q must be a uint8 CUDA tensor");
+  check_16bit(scales, kPack, "scales");
+  TORCH_CHECK(scales.device() == q.device(), kPack, ": scales is on another device");
+  const int64_t e = q.size(0), n = q.size(1), k = 2 * q.size(2), groups = scales.size(2);
+  TORCH_CHECK(scales.size(0) == e && scales.size(1) == n, kPack,
+              ": scales must have q's experts and rows");
+  check_sizes({n, k}, kPack);
+  TORCH_CHECK(groups > 0 ? k % groups == 0 : k == 0, kPack, ": K = ", k,
+              " is not a whole number of groups (", groups, " scales to a row)");
+  const int64_t group = groups > 0 ? k / groups : 128;
+  TORCH_CHECK(group == 32 || group == 64 || group == 128, kPack,
+              ": groups must hold 32, 64 or 128 weights, not ", group);
+  TORCH_CHECK(e <= B200_MAX_EXPERTS, kPack, ": more than ", B200_MAX_EXPERTS, " experts");
+  at::Tensor z;
+  if (zeros.has_value()) {
+    TORCH_CHECK(zeros->sizes() == scales.sizes() && zeros->scalar_type() == at::kByte &&
+                    zeros->device() == q.device(),
+                kPack, ": zeros must be uint8, of scales' shape, on q's device");
+    z = zeros->contiguous();
+  }
+  const c10::cuda::CUDAGuard guard(q.device());
+  size_t bytes = 0;
+  check_status(b200_w4_packed_bytes((int)e, (int)n, (int)k, (int)group, z.defined(), &bytes),
+               kPack);
+  auto packed = at::empty({(int64_t)bytes}, q.options());
+  const at::Tensor qc = q.contiguous(), sc = scales.contiguous();
+  check_status(b200_w4_pack(qc.data_ptr(), sc.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
+                            packed.data_ptr(), (int)e, (int)n, (int)k, (int)group,
+                            current_stream()),
+               kPack);
+  return packed;
+}
+
+at::Tensor w4_matmul(const at::Tensor& A, const at::Tensor& packed, int64_t experts, int64_t N,
+                     int64_t K, int64_t group, bool zeros, bool half,
+                     const std::optional<at::Tensor>& offsets) {
+  TORCH_CHECK(A.dim() == 2, kW4, ": A must be (rows, K)");
+  check_16bit(A, kW4, "A");
+  TORCH_CHECK(A.scalar_type() == (half ? at::kHalf : at::kBFloat16), kW4,
+              ": A and the scales must have the same dtype");
+  TORCH_CHECK(A.device() == packed.device(), kW4, ": A and the weight are on different devices");
+  TORCH_CHECK(A.size(1) == K, kW4, ": inner dimensions differ (A has K = ", A.size(1),
+              ", the weight has K = ", K, ")");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && A.requires_grad()), kW4,
+              ": no gradient is defined (4-bit weights serve); use torch.no_grad()");
+  check_sizes({A.size(0)}, kW4);
+  at::Tensor off;
+  if (offsets.has_value())
+    off = check_offsets(*offsets, experts, A, kW4);
+  else
+    TORCH_CHECK(experts == 1, kW4, ": a bank of experts needs offsets");
+  const c10::cuda::CUDAGuard guard(A.device());
+  const Rows ra = as_rows(A);
+  const Result c = new_rows(A.size(0), N, A);
+  check_status(b200_w4_gemm(ra.t.data_ptr(), packed.data_ptr(), c.buf.data_ptr(),
+                            off.defined() ? off.data_ptr<int>() : nullptr, (int)A.size(0),
+                            (int)experts, (int)N, (int)K, (int)group, zeros, ra.ld, c.ld,
+                            dtype_code(A), current_stream()),
+               kW4);
+  return c.done();
+}
+
 }  // namespace
 
 void register_moe(pybind11::module_& m) {
   m.def("matmul_b200_grouped", &matmul_b200_grouped,
         "C[r] = A[r] @ B[e] for rows r of expert e (offsets on the device)");
+  m.def("w4_pack", &w4_pack, "4-bit weights in the order the kernel reads them",
+        pybind11::arg("q"), pybind11::arg("scales"), pybind11::arg("zeros") = std::nullopt);
+  m.def("w4_matmul", &w4_matmul, "C = A @ W^T with packed 4-bit weights");
 }

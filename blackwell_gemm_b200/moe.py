@@ -7,7 +7,9 @@ runs on the current stream and is computed by libb200gemm.so
 """
 from __future__ import annotations
 
-__all__ = ["matmul_b200_grouped"]
+from typing import NamedTuple
+
+__all__ = ["matmul_b200_grouped", "W4Weight", "pack_w4", "quantize_w4", "matmul_b200_w4"]
 
 
 def _ext():
@@ -30,3 +32,74 @@ def matmul_b200_grouped(A, B, offsets):
     rows) costs a copy of that operand per call.  Offsets that decrease or
     leave [0, rows] are clamped and reported by ``capi.device_status``."""
     return _ext().matmul_b200_grouped(A, B, offsets)
+
+
+class W4Weight(NamedTuple):
+    """4-bit weights laid out for matmul_b200_w4 (see pack_w4)."""
+    data: "torch.Tensor"    # noqa: F821  packed bytes, on the device
+    experts: int            # matrices; 1 and bank = False for a single one
+    N: int
+    K: int
+    group: int
+    zeros: bool
+    half: bool              # fp16 scales and rows (else bf16)
+    bank: bool
+
+
+def pack_w4(q, scales, zeros=None) -> W4Weight:
+    """Lay 4-bit weights out, once, in the order matmul_b200_w4 reads them.
+
+    The weight of row n and column k is (q - zero) * scale, with one scale and
+    one zero point per group of 32, 64 or 128 consecutive k.  q: uint8
+    (N, K/2) or (experts, N, K/2), the low nibble the even k.  scales: bf16 or
+    fp16, (.., N, K/group); the rows multiplied later must have the same dtype.
+    zeros: uint8 0..15 of scales' shape, or None for 8 everywhere."""
+    bank = q.dim() == 3
+    if not bank:
+        if q.dim() != 2:
+            raise RuntimeError("pack_w4: q must be (N, K/2) or (experts, N, K/2)")
+        if scales.dim() != 2 or (zeros is not None and zeros.dim() != 2):
+            raise RuntimeError("pack_w4: scales and zeros must be (N, K/group), like q")
+        q, scales = q[None], scales[None]
+        zeros = None if zeros is None else zeros[None]
+    data = _ext().w4_pack(q, scales, zeros)
+    import torch
+    experts, N, K = q.shape[0], q.shape[1], 2 * q.shape[2]
+    group = K // scales.shape[2] if scales.shape[2] else 128
+    return W4Weight(data, experts, N, K, group, zeros is not None,
+                    scales.dtype == torch.float16, bank)
+
+
+def quantize_w4(w, group: int = 128):
+    """(q, scales) of a bf16 or fp16 weight (.., N, K), rounded to nearest with
+    symmetric scales: |w| / 7 of each group's largest.  A plain helper; any
+    quantiser that yields pack_w4's operands will do."""
+    *lead, n, k = w.shape
+    if k % group:
+        raise RuntimeError(f"quantize_w4: K = {k} is not a multiple of group = {group}")
+    parts = w.float().reshape(*lead, n, k // group, group)
+    scales = (parts.abs().amax(-1) / 7).to(w.dtype)
+    step = scales.float().clamp(min=1e-30)[..., None]
+    q = ((parts / step).round().clamp(-8, 7) + 8).to(dtype=_uint8()).reshape(*lead, n, k)
+    return q[..., 0::2] | (q[..., 1::2] << 4), scales
+
+
+def _uint8():
+    import torch
+    return torch.uint8
+
+
+def matmul_b200_w4(A, weight: W4Weight, offsets=None):
+    """C = A @ W.T for 4-bit weights; with a bank, by expert as
+    matmul_b200_grouped.
+
+    A: (rows, K) CUDA, bf16 or fp16 like the weight's scales.  offsets:
+    (experts + 1,) int32 or int64 on the device, for a bank.  Returns
+    (rows, N).  The 4-bit integers enter the product exactly, the scales
+    multiply fp32 sums, and the result is rounded once.  Made for few rows (the
+    weights are read once per 64 rows of an expert); correct for any number.
+    No gradient."""
+    if offsets is None and weight.bank and weight.experts != 1:
+        raise RuntimeError("matmul_b200_w4: a bank of experts needs offsets")
+    return _ext().w4_matmul(A, weight.data, weight.experts, weight.N, weight.K, weight.group,
+                            weight.zeros, weight.half, offsets)

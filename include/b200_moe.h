@@ -17,6 +17,7 @@
 #ifndef B200_MOE_H_
 #define B200_MOE_H_
 
+#include <stddef.h>
 #include <stdint.h>
 
 #include "b200_gemm.h"
@@ -55,6 +56,30 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
 /* Kernel for b200_grouped_gemm and _da: 0 = chosen by rows per expert
  * (default), 1 = the streaming kernel (few rows), 2 = the pair kernel. */
 int b200_grouped_set_kernel(int kernel);
+
+/* ---- 4-bit weights with group scales ---------------------------------------
+ * A weight is (q - z) * s: q in 0..15, one scale s (16-bit, the type of A) and
+ * one zero point z in 0..15 (8 where none are given) per `group` consecutive
+ * k of a row; group = 32, 64 or 128 and K a multiple of it.
+ *
+ * b200_w4_pack lays a matrix, or a bank of them, out once in the order the
+ * kernel reads it.  q: experts x N x K/2 bytes, the low nibble the even k;
+ * scales: experts x N x K/group; zeros: the same shape, one byte each, or
+ * NULL; all contiguous.  packed: b200_w4_packed_bytes bytes, 16-byte aligned
+ * (zeros != 0 when zero points are given). */
+int b200_w4_packed_bytes(int experts, int N, int K, int group, int zeros, size_t* bytes);
+int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* packed, int experts,
+                 int N, int K, int group, void* stream);
+
+/* C[r, :] = A[r, :] W[e]^T with packed weights.  offsets as for
+ * b200_grouped_gemm, or NULL for experts = 1: every row takes the one matrix.
+ * A: rows x K, stride lda; C: rows x N, stride ldc; alignment as above.  The
+ * weights enter as exact integers, the scales multiply fp32 sums.  Any number
+ * of rows; made for few (the weights are read once per 64 rows of an expert,
+ * 32 when group is 32). */
+int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets, int rows,
+                 int experts, int N, int K, int group, int zeros, int lda, int ldc, int dtype,
+                 void* stream);
 
 #ifdef __cplusplus
 }

@@ -81,3 +81,65 @@ def test_grouped_torch_checks():
         bg.matmul_b200_grouped(x, w[0], off)
     with pytest.raises(RuntimeError, match="rows, K"):
         bg.matmul_b200_grouped(x[0], w, off)
+
+
+def w4(a=FAKE, p=FAKE, c=FAKE, off=0, rows=8, experts=1, n=8, k=64, group=64, zeros=0, lda=64,
+       ldc=8, dtype=capi.BF16):
+    return capi.lib().b200_w4_gemm(a, p, c, off, rows, experts, n, k, group, zeros, lda, ldc,
+                                   dtype, None)
+
+
+@pytest.mark.parametrize("change,expect", [
+    (dict(rows=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(experts=-1), capi.ERR_INVALID_ARGUMENT),
+    (dict(experts=2), capi.ERR_INVALID_ARGUMENT),          # a bank without offsets
+    (dict(group=16), capi.ERR_INVALID_ARGUMENT),
+    (dict(k=96, lda=96), capi.ERR_INVALID_ARGUMENT),       # not whole groups
+    (dict(dtype=5), capi.ERR_INVALID_ARGUMENT),
+    (dict(a=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(p=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(c=0), capi.ERR_INVALID_ARGUMENT),
+    (dict(lda=56), capi.ERR_INVALID_ARGUMENT),
+    (dict(n=16), capi.ERR_INVALID_ARGUMENT),               # ldc < N
+    (dict(lda=68), capi.ERR_ALIGNMENT),
+    (dict(ldc=12), capi.ERR_ALIGNMENT),
+    (dict(a=FAKE + 2), capi.ERR_ALIGNMENT),
+    (dict(p=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(c=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(off=FAKE + 1, experts=2), capi.ERR_ALIGNMENT),
+    (dict(experts=1025, off=FAKE), capi.ERR_TOO_LARGE),
+    (dict(n=INT_MAX - 7, ldc=INT_MAX - 7, rows=INT_MAX), capi.ERR_TOO_LARGE),
+    (dict(rows=0, a=0, c=0), capi.OK),
+    (dict(n=0, c=0), capi.OK),
+])
+def test_w4_c_abi(change, expect):
+    assert w4(**change) == expect
+
+
+def test_w4_packed_bytes():
+    import ctypes
+    size = ctypes.c_size_t(0)
+    lib = capi.lib()
+    for args, want in [((1, 128, 128, 128, 0), 8192 + 256), ((1, 1, 32, 32, 1), 8192 + 1024 + 512),
+                       ((3, 129, 192, 64, 0), 3 * 2 * 2 * (8192 + 512)), ((0, 8, 64, 64, 0), 0),
+                       ((1, 0, 64, 64, 0), 0)]:
+        assert lib.b200_w4_packed_bytes(*args, ctypes.byref(size)) == capi.OK
+        assert size.value == want, args
+    assert lib.b200_w4_packed_bytes(1, 8, 64, 64, 0, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.b200_w4_packed_bytes(1, 8, 60, 64, 0, ctypes.byref(size)) == \
+        capi.ERR_INVALID_ARGUMENT
+    assert lib.b200_w4_pack(0, FAKE, 0, FAKE, 1, 8, 64, 64, None) == capi.ERR_INVALID_ARGUMENT
+    assert lib.b200_w4_pack(FAKE, FAKE, 0, FAKE + 4, 1, 8, 64, 64, None) == capi.ERR_ALIGNMENT
+
+
+def test_w4_torch_checks():
+    q = torch.zeros(8, 32, dtype=torch.uint8)
+    s = torch.zeros(8, 1, dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        bg.pack_w4(q, s)
+    with pytest.raises(RuntimeError, match="like q"):
+        bg.pack_w4(q, s[None])
+    with pytest.raises(RuntimeError, match="experts, N, K/2"):
+        bg.pack_w4(q[0], s)
+    with pytest.raises(RuntimeError, match="multiple of group"):
+        bg.quantize_w4(torch.zeros(4, 100, dtype=torch.bfloat16), 64)
