@@ -21,11 +21,13 @@ import importlib
 import types
 
 from . import capi  # noqa: F401
-from .moe import W4Weight, matmul_b200_grouped, matmul_b200_w4, pack_w4, quantize_w4
+from .moe import (Routing, W4Weight, combine_b200, dispatch_b200, matmul_b200_grouped,
+                  matmul_b200_w4, pack_w4, quantize_w4, route_b200)
 
 __all__ = ["module", "matmul_b200", "profile_matmul_b200", "matmul_b200_epilogue",
-           "matmul_b200_host", "matmul_b200_grouped", "matmul_b200_w4",
-           "pack_w4", "quantize_w4", "W4Weight", "profile_rows", "capi", "load"]
+           "matmul_b200_host", "route_b200", "dispatch_b200", "combine_b200", "Routing",
+           "matmul_b200_grouped", "matmul_b200_w4", "pack_w4", "quantize_w4", "W4Weight",
+           "profile_rows", "capi", "load"]
 
 _ext = None
 

@@ -86,6 +86,12 @@ SIGNATURES = {
     "b200_grouped_gemm_da": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _ll, _i, _i, _vp]),
     "b200_grouped_gemm_db": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _vp]),
     "b200_grouped_set_kernel": (_i, [_i]),
+    "b200_route": (_i, [_vp, _i, _i, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_route_grad": (_i, [_vp, _i, _i, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
+    "b200_dispatch": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _i, _vp]),
+    "b200_combine": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _i, _vp]),
+    "b200_combine_grad": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _ll, _i,
+                               _vp]),
     "b200_w4_packed_bytes": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "b200_w4_pack": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "b200_w4_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
@@ -295,7 +301,7 @@ def launch_shape(M: int, N: int, K: int) -> dict:
 
 
 # ---------------------------------------------------------- mixture of experts
-BF16, FP16 = 0, 1
+BF16, FP16, FP32 = 0, 1, 2
 
 
 def grouped_set_kernel(kernel: int) -> None:

@@ -12,6 +12,7 @@
 #include "b200_moe.h"
 #include "device_state.h"
 #include "grouped_gemm.cuh"
+#include "moe_route.cuh"
 #include "moe_stream.cuh"
 #include "moe_w4.cuh"
 
@@ -87,6 +88,17 @@ bool init_type(MoeDevice& m, int sms) {
          init_stream<true, T>() && init_w4<32, T>() && init_w4<64, T>() && init_w4<128, T>();
 }
 
+template <int kPer>
+bool init_choose() {
+  return set_smem(route_choose_kernel<kPer>, (1 + kRouteWarps) * kMaxExperts * (int)sizeof(int));
+}
+
+bool init_route() {
+  return init_choose<1>() && init_choose<2>() && init_choose<4>() && init_choose<8>() &&
+         init_choose<32>() &&
+         set_smem(route_rank_kernel, (1 + kRouteWarps) * kMaxExperts * (int)sizeof(int));
+}
+
 int moe_device(DeviceView* v, MoeDevice** out) {
   const int st = device_view(v);
   if (st != B200_OK) return st;
@@ -94,9 +106,10 @@ int moe_device(DeviceView* v, MoeDevice** out) {
   MoeDevice& m = g_moe[v->device];
   if (!m.ready) {
     m.ready = true;
-    m.init_status = init_type<__nv_bfloat16>(m, v->sms) && init_type<__half>(m, v->sms)
-                        ? B200_OK
-                        : B200_ERR_LAUNCH;
+    m.init_status =
+        init_type<__nv_bfloat16>(m, v->sms) && init_type<__half>(m, v->sms) && init_route()
+            ? B200_OK
+            : B200_ERR_LAUNCH;
     if (m.init_status != B200_OK) cudaGetLastError();
   }
   if (m.init_status != B200_OK) return m.init_status;
@@ -455,6 +468,89 @@ int run_w4_pack(const void* q, const void* scales, const void* zeros, void* pack
   return launched();
 }
 
+// -------------------------------------------------------------------- routing
+template <int kPer>
+int launch_choose(const RouteArgs& a, int blocks, size_t smem, cudaStream_t stream) {
+  route_choose_kernel<kPer><<<blocks, kRouteThreads, smem, stream>>>(a);
+  return launched();
+}
+
+int run_route(RouteArgs a, const DeviceView& v, cudaStream_t stream) {
+  // Up to 256 tokens one block does everything in one launch; beyond that
+  // one chunk per SM.
+  a.chunk = a.tokens <= 256 ? a.tokens : (int)ceil_div(a.tokens, v.sms);
+  const int blocks = (int)ceil_div(a.tokens, a.chunk);
+  const size_t smem = (size_t)(1 + kRouteWarps) * a.experts * sizeof(int);
+  int* counts = nullptr;
+  if (blocks > 1) {
+    if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&counts),
+                                (size_t)blocks * a.experts * sizeof(int), v.pool,
+                                stream) != cudaSuccess) {
+      cudaGetLastError();
+      return B200_ERR_LAUNCH;
+    }
+    a.counts = counts;
+  }
+  int st = a.experts <= 32    ? launch_choose<1>(a, blocks, smem, stream)
+           : a.experts <= 64  ? launch_choose<2>(a, blocks, smem, stream)
+           : a.experts <= 128 ? launch_choose<4>(a, blocks, smem, stream)
+           : a.experts <= 256 ? launch_choose<8>(a, blocks, smem, stream)
+                              : launch_choose<32>(a, blocks, smem, stream);
+  if (st == B200_OK && blocks > 1) {
+    route_rank_kernel<<<blocks, kRouteThreads, smem, stream>>>(a);
+    st = launched();
+  }
+  if (counts) cudaFreeAsync(counts, stream);
+  return st;
+}
+
+enum Move { kDispatch, kCombine, kCombineGrad };
+
+template <class T, int kVec>
+int launch_move(Move what, const MoveArgs& a, cudaStream_t stream) {
+  const long long lanes = ceil_div(a.width, kVec);
+  const int threads = lanes >= 256 ? 256 : (int)(lanes < 32 ? 32 : (lanes + 31) / 32 * 32);
+  switch (what) {
+    case kDispatch: dispatch_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
+    case kCombine: combine_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
+    default: combine_grad_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
+  }
+  return launched();
+}
+
+int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
+  if (a.tokens < 0 || a.top_k < 0 || a.width < 0 || a.top_k > kMaxTopK ||
+      (dtype != B200_BF16 && dtype != B200_FP16))
+    return B200_ERR_INVALID_ARGUMENT;
+  if ((long long)a.tokens * a.top_k >= (1ll << 31)) return B200_ERR_TOO_LARGE;
+  // no slots: dispatch and the gradient write nothing, combine writes zeros
+  if (a.tokens == 0 || (a.top_k == 0 && what != kCombine)) return B200_OK;
+  if (a.width == 0 && what != kCombineGrad) return B200_OK;
+  const bool any = a.top_k > 0, wide = a.width > 0;
+  if ((any && !a.rows) || (wide && (!a.out || (any && !a.in))) ||
+      (what != kCombine && !a.total) ||
+      (what == kCombineGrad && ((wide && !a.in2) || !a.weights)))
+    return B200_ERR_INVALID_ARGUMENT;
+  if (wide && (a.ld_in < a.width || a.ld_out < a.width ||
+               (what == kCombineGrad && a.ld_in2 < a.width)))
+    return B200_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(a.in) | reinterpret_cast<uintptr_t>(a.in2) |
+        reinterpret_cast<uintptr_t>(a.out)) & 1u) ||
+      ((reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.total) |
+        reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.dweights)) & 3u))
+    return B200_ERR_ALIGNMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  const int st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  const bool vec = aligned16(a.in) && aligned16(a.out) && aligned16(a.in2) &&
+                   ((a.width | a.ld_in | a.ld_out | a.ld_in2) & 7) == 0;
+  if (dtype == B200_FP16)
+    return vec ? launch_move<__half, 8>(what, a, stream) : launch_move<__half, 1>(what, a, stream);
+  return vec ? launch_move<__nv_bfloat16, 8>(what, a, stream)
+             : launch_move<__nv_bfloat16, 1>(what, a, stream);
+}
+
 }  // namespace
 
 extern "C" {
@@ -509,6 +605,116 @@ int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets,
                  void* stream) {
   const W4Call c = {A, packed, C, offsets, rows, experts, N, K, group, zeros, lda, ldc, dtype};
   return run_w4(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_route(const void* logits, int tokens, int experts, long long ld, int type, int top_k,
+               int normalize, float* weights, int* chosen, int* rows, int* sources, int* offsets,
+               void* stream) {
+  if (tokens < 0 || experts < 0 || top_k < 0 || top_k > experts || top_k > kMaxTopK ||
+      type < B200_BF16 || type > B200_FP32)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (experts > kMaxExperts || (long long)tokens * top_k >= (1ll << 31)) return B200_ERR_TOO_LARGE;
+  if (!offsets) return B200_ERR_INVALID_ARGUMENT;
+  const bool any = tokens > 0 && top_k > 0;
+  if (any && (!logits || ld < experts || !weights || !chosen || !rows || !sources))
+    return B200_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(logits) & (type == B200_FP32 ? 3u : 1u)) ||
+      ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(chosen) |
+        reinterpret_cast<uintptr_t>(rows) | reinterpret_cast<uintptr_t>(sources) |
+        reinterpret_cast<uintptr_t>(offsets)) & 3u))
+    return B200_ERR_ALIGNMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  const int st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (!any)
+    return cudaMemsetAsync(offsets, 0, (size_t)(experts + 1) * sizeof(int), s) == cudaSuccess
+               ? B200_OK
+               : B200_ERR_LAUNCH;
+  RouteArgs a = {};
+  a.logits = logits;
+  a.ld = ld;
+  a.type = type;
+  a.tokens = tokens;
+  a.experts = experts;
+  a.top_k = top_k;
+  a.normalize = normalize != 0;
+  a.weights = weights;
+  a.chosen = chosen;
+  a.rows = rows;
+  a.sources = sources;
+  a.offsets = offsets;
+  return run_route(a, v, s);
+}
+
+int b200_route_grad(const void* logits, int tokens, int experts, long long ld, int type, int top_k,
+                    int normalize, const int* chosen, const float* weights, const float* dweights,
+                    void* dlogits, void* stream) {
+  if (tokens < 0 || experts < 0 || top_k < 0 || top_k > experts || top_k > kMaxTopK ||
+      type < B200_BF16 || type > B200_FP32)
+    return B200_ERR_INVALID_ARGUMENT;
+  if (experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  if (tokens == 0 || experts == 0) return B200_OK;
+  if (!logits || ld < experts || !dlogits || (top_k > 0 && (!chosen || !weights || !dweights)))
+    return B200_ERR_INVALID_ARGUMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  const int st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  route_grad_kernel<<<(unsigned)ceil_div(tokens, 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
+      logits, ld, type, chosen, weights, dweights, dlogits, tokens, experts, top_k, normalize != 0);
+  return launched();
+}
+
+int b200_dispatch(const void* x, const int* rows, const int* total, void* xs, int tokens, int top_k,
+                  int width, long long ldx, long long ldxs, int dtype, void* stream) {
+  MoveArgs a = {};
+  a.in = x;
+  a.ld_in = ldx;
+  a.out = xs;
+  a.ld_out = ldxs;
+  a.rows = rows;
+  a.total = total;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.width = width;
+  return run_move(kDispatch, a, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200_combine(const void* y, const float* weights, const int* rows, void* out, int tokens,
+                 int top_k, int width, long long ldy, long long ldo, int dtype, void* stream) {
+  MoveArgs a = {};
+  a.in = y;
+  a.ld_in = ldy;
+  a.out = out;
+  a.ld_out = ldo;
+  a.weights = weights;
+  a.rows = rows;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.width = width;
+  return run_move(kCombine, a, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200_combine_grad(const void* dout, const void* y, const float* weights, const int* rows,
+                      const int* total, void* dy, float* dweights, int tokens, int top_k, int width,
+                      long long ldo, long long ldy, long long lddy, int dtype, void* stream) {
+  MoveArgs a = {};
+  a.in = dout;
+  a.ld_in = ldo;
+  a.in2 = y;
+  a.ld_in2 = ldy;
+  a.out = dy;
+  a.ld_out = lddy;
+  a.weights = weights;
+  a.dweights = dweights;
+  a.rows = rows;
+  a.total = total;
+  a.tokens = tokens;
+  a.top_k = top_k;
+  a.width = width;
+  return run_move(kCombineGrad, a, dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

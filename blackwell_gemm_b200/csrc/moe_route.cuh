@@ -1,0 +1,453 @@
+// Routing: each token's top-k experts, their softmax weights, and the order
+// that sorts (token, slot) pairs by expert; rows moved there and back.
+//
+//   chosen     the k largest logits of a token, the lower index first on a
+//              tie; NaN counts as largest, -inf is a closed expert: never
+//              chosen, its slot stays empty (expert, row -1, weight 0)
+//   weights    softmax over the chosen, or over all, experts; fp32
+//   row        offsets[e] + the number of earlier pairs, by token then slot,
+//              that chose e too: the order does not depend on timing
+//   dispatch   xs[row(t, j)] = x[t]          combine  out[t] = sum_j w y[row]
+//
+// A warp holds a token's logits in registers.  The tokens are cut into one
+// chunk per block: counts per (chunk, expert) first, then every block adds
+// up the chunks before its own and ranks its pairs (two launches; one when a
+// single block does it all).  Moving rows is bound by memory: one block per
+// token, every row read once and written once, sums in fp32.
+#pragma once
+#include "moe_groups.cuh"
+
+namespace b200 {
+
+constexpr int kRouteThreads = 512;
+constexpr int kRouteWarps = kRouteThreads / 32;
+constexpr int kMaxTopK = 32;
+
+// Logit types: 0 bf16, 1 f16, 2 f32.
+struct RouteArgs {
+  const void* logits;
+  long long ld;
+  int type;
+  int tokens, experts, top_k;
+  int chunk;        // tokens per block
+  bool normalize;
+  float* weights;   // tokens x top_k
+  int* chosen;      // tokens x top_k
+  int* rows;        // tokens x top_k
+  int* sources;     // tokens * top_k
+  int* offsets;     // experts + 1
+  int* counts;      // blocks x experts (several blocks)
+};
+
+__device__ __forceinline__ float load_logit(const void* p, int type, long long i) {
+  if (type == 2) return static_cast<const float*>(p)[i];
+  if (type == 1) return __half2float(static_cast<const __half*>(p)[i]);
+  return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// An unsigned key in the order of the values: NaN above all, -0 = +0.
+__device__ __forceinline__ uint32_t order_key(float v) {
+  if (v != v) return 0xFFFFFFFFu;
+  const uint32_t b = __float_as_uint(v + 0.0f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+constexpr uint32_t kClosedKey = 0x007FFFFFu;  // order_key(-inf)
+
+__device__ __forceinline__ float warp_sum(float v) {
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(0xffffffffu, v, d);
+  return v;
+}
+
+// One warp, one token: expert i of the row is value i / 32 of lane i % 32.
+template <int kPer>
+__device__ __forceinline__ void choose_token(const RouteArgs& a, int t, int* hist) {
+  const int lane = threadIdx.x & 31;
+  float v[kPer];
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int e = i * 32 + lane;
+    v[i] = e < a.experts ? load_logit(a.logits, a.type, t * a.ld + e) : -INFINITY;
+    key[i] = order_key(v[i]);
+  }
+  float base = 0.0f, mine = 0.0f, sum = 0.0f;
+  int slot_expert = -1;  // lane j keeps slot j
+  for (int j = 0; j < a.top_k; ++j) {
+    uint32_t best = 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) best = max(best, key[i]);
+    best = __reduce_max_sync(0xffffffffu, best);
+    if (best <= kClosedKey) break;
+    int at = 0x7FFFFFFF;
+#pragma unroll
+    for (int i = kPer - 1; i >= 0; --i)
+      if (key[i] == best) at = i * 32 + lane;
+    at = __reduce_min_sync(0xffffffffu, at);
+    float val = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (at == i * 32 + lane) {
+        val = v[i];
+        key[i] = 0;
+      }
+    val = __shfl_sync(0xffffffffu, val, at & 31);
+    if (j == 0) base = val;
+    const float p = expf(val - base);
+    if (a.normalize) sum += p;
+    if (lane == j) {
+      slot_expert = at;
+      mine = p;
+    }
+  }
+  if (!a.normalize) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 32 + lane < a.experts) sum += expf(v[i] - base);
+    sum = warp_sum(sum);
+  }
+  if (lane < a.top_k) {
+    const long long at = (long long)t * a.top_k + lane;
+    a.weights[at] = slot_expert >= 0 ? mine / sum : 0.0f;
+    a.chosen[at] = slot_expert;
+    if (slot_expert >= 0) atomicAdd(hist + slot_expert, 1);
+  }
+}
+
+template <int kPer>
+__device__ __forceinline__ void choose_chunk(const RouteArgs& a, int first, int last, int* hist) {
+  for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) hist[i] = 0;
+  __syncthreads();
+  for (int t = first + (threadIdx.x >> 5); t < last; t += kRouteWarps)
+    choose_token<kPer>(a, t, hist);
+  __syncthreads();
+}
+
+// Exclusive prefix sum of totals[0 .. n) by one warp; returns the sum.
+__device__ __forceinline__ int scan_experts(int* totals, int n) {
+  const int lane = threadIdx.x & 31;
+  int run = 0;
+  for (int base = 0; base < n; base += 32) {
+    const int i = base + lane;
+    const int own = i < n ? totals[i] : 0;
+    int v = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, v, d);
+      if (lane >= d) v += o;
+    }
+    if (i < n) totals[i] = run + v - own;
+    run += __shfl_sync(0xffffffffu, v, 31);
+  }
+  return run;
+}
+
+// Rows of the chunk's pairs.  start[e]: offsets[e] + pairs of earlier chunks;
+// cursor[warp][e]: next row of this warp's part of the chunk.
+__device__ __forceinline__ void rank_chunk(const RouteArgs& a, int first, int last,
+                                           const int* start, int* cursor) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int pairs = (last - first) * a.top_k;
+  const int part = ((pairs + kRouteWarps - 1) / kRouteWarps + 31) & ~31;
+  const long long base = (long long)first * a.top_k;
+  const int lo = min(warp * part, pairs), hi = min(lo + part, pairs);
+  for (int i = threadIdx.x; i < kRouteWarps * a.experts; i += kRouteThreads) cursor[i] = 0;
+  __syncthreads();
+  int* mine = cursor + warp * a.experts;
+  for (int i = lo + lane; i < hi; i += 32) {
+    const int e = a.chosen[base + i];
+    if (e >= 0) atomicAdd(mine + e, 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+    int at = start[e];
+    for (int w = 0; w < kRouteWarps; ++w) {
+      const int n = cursor[w * a.experts + e];
+      cursor[w * a.experts + e] = at;
+      at += n;
+    }
+  }
+  __syncthreads();
+  for (int i = lo; i < hi; i += 32) {
+    const bool in = i + lane < hi;
+    const int e = in ? a.chosen[base + i + lane] : -1;
+    const unsigned int same = __match_any_sync(0xffffffffu, e);
+    const int before = __popc(same & ((1u << lane) - 1u));
+    int row = -1;
+    if (e >= 0) {
+      row = mine[e] + before;
+      a.sources[row] = (int)((base + i + lane) / a.top_k);
+    }
+    __syncwarp();
+    if (e >= 0 && before == 0) mine[e] += __popc(same);
+    __syncwarp();
+    if (in) a.rows[base + i + lane] = row;
+  }
+}
+
+// Pairs that went nowhere leave rows without an expert at the end.
+__device__ __forceinline__ void mark_unowned(const RouteArgs& a, int total) {
+  const long long pairs = (long long)a.tokens * a.top_k;
+  for (long long r = total + (long long)blockIdx.x * kRouteThreads + threadIdx.x; r < pairs;
+       r += (long long)gridDim.x * kRouteThreads)
+    a.sources[r] = -1;
+}
+
+// Dynamic shared memory: hist/start [experts], cursor [warps][experts].
+template <int kPer>
+__global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs a) {
+  extern __shared__ int s_route[];
+  int* hist = s_route;
+  const int first = blockIdx.x * a.chunk;
+  const int last = min(a.tokens, first + a.chunk);
+  choose_chunk<kPer>(a, first, last, hist);
+  if (gridDim.x > 1) {
+    for (int e = threadIdx.x; e < a.experts; e += kRouteThreads)
+      a.counts[(long long)blockIdx.x * a.experts + e] = hist[e];
+    return;
+  }
+  __shared__ int total;
+  if (threadIdx.x < 32) {
+    const int n = scan_experts(hist, a.experts);
+    if (threadIdx.x == 0) total = n;
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads)
+    a.offsets[e] = e < a.experts ? hist[e] : total;
+  rank_chunk(a, first, last, hist, s_route + a.experts);
+  mark_unowned(a, total);
+}
+
+__global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteArgs a) {
+  extern __shared__ int s_route[];
+  int* start = s_route;                 // totals, then offsets, then + earlier chunks
+  int* earlier = s_route + a.experts;   // (the cursors take this over)
+  __shared__ int total;
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+    int all = 0, before = 0;
+    for (int b = 0; b < (int)gridDim.x; ++b) {
+      const int n = a.counts[(long long)b * a.experts + e];
+      all += n;
+      if (b < (int)blockIdx.x) before += n;
+    }
+    start[e] = all;
+    earlier[e] = before;
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    const int n = scan_experts(start, a.experts);
+    if (threadIdx.x == 0) total = n;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads)
+      a.offsets[e] = e < a.experts ? start[e] : total;
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] += earlier[e];
+  __syncthreads();
+  const int first = blockIdx.x * a.chunk;
+  rank_chunk(a, first, min(a.tokens, first + a.chunk), start, s_route + a.experts);
+  mark_unowned(a, total);
+}
+
+// Gradient in the logits, one warp per token:
+//   over the chosen:  w_j (dw_j - sum_i w_i dw_i) at chosen experts, else 0
+//   over all:         p_e ([e chosen] dw_e - sum_j w_j dw_j)
+__global__ void __launch_bounds__(256)
+route_grad_kernel(const void* logits, long long ld, int type, const int* __restrict__ chosen,
+                  const float* __restrict__ weights, const float* __restrict__ dweights,
+                  void* dlogits, int tokens, int experts, int top_k, bool normalize) {
+  const int lane = threadIdx.x & 31;
+  const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t >= tokens) return;
+  const long long at = t * top_k + lane;
+  const int e = lane < top_k ? chosen[at] : -1;
+  const float w = e >= 0 ? weights[at] : 0.0f;
+  const float dw = e >= 0 ? dweights[at] : 0.0f;
+  const float inner = warp_sum(e >= 0 ? w * dw : 0.0f);
+  const int top = __shfl_sync(0xffffffffu, e, 0);
+  float base = 0.0f, sum = 1.0f;
+  if (!normalize && top >= 0) {
+    base = load_logit(logits, type, t * ld + top);
+    float part = 0.0f;
+    for (int i = lane; i < experts; i += 32)
+      part += expf(load_logit(logits, type, t * ld + i) - base);
+    sum = warp_sum(part);
+  }
+  for (int i0 = 0; i0 < experts; i0 += 32) {
+    const int i = i0 + lane;
+    float hit = 0.0f, share = 0.0f;
+    bool took = false;
+    for (int j = 0; j < top_k; ++j) {
+      const int ej = __shfl_sync(0xffffffffu, e, j);
+      const float wj = __shfl_sync(0xffffffffu, w, j), dj = __shfl_sync(0xffffffffu, dw, j);
+      if (ej == i) {
+        took = true;
+        hit = dj;
+        share = wj;
+      }
+    }
+    if (i >= experts) continue;
+    float g = 0.0f;
+    if (normalize) {
+      if (took) g = share * (hit - inner);
+    } else if (top >= 0) {
+      const float l = load_logit(logits, type, t * ld + i);
+      // (a closed expert has no share; NaN and inf take part as they are)
+      if (l != -INFINITY) g = (took ? share : expf(l - base) / sum) * (hit - inner);
+    }
+    const long long o = t * experts + i;
+    if (type == 2) static_cast<float*>(dlogits)[o] = g;
+    else if (type == 1) static_cast<__half*>(dlogits)[o] = __float2half_rn(g);
+    else static_cast<__nv_bfloat16*>(dlogits)[o] = __float2bfloat16_rn(g);
+  }
+}
+
+// ------------------------------------------------------------------ moving rows
+struct MoveArgs {
+  const void* in;         // x, y or dout
+  long long ld_in;
+  const void* in2;        // combine's gradient: y
+  long long ld_in2;
+  void* out;              // xs, out or dy
+  long long ld_out;
+  const float* weights;   // tokens x top_k, or null: 1
+  float* dweights;        // combine's gradient
+  const int* rows;        // tokens x top_k
+  const int* total;       // rows that have an expert
+  int tokens, top_k, width;
+};
+
+// kVec elements of a row at once: 8 (16 bytes, aligned rows) or 1.
+template <class T, int kVec>
+struct Pack {
+  T v[kVec];
+};
+template <class T, int kVec>
+__device__ __forceinline__ Pack<T, kVec> load_pack(const void* base, long long i) {
+  Pack<T, kVec> p;
+  if constexpr (kVec == 8)
+    *reinterpret_cast<uint4*>(&p) =
+        __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + i));
+  else
+    p.v[0] = static_cast<const T*>(base)[i];
+  return p;
+}
+template <class T, int kVec>
+__device__ __forceinline__ void store_pack(void* base, long long i, const Pack<T, kVec>& p) {
+  if constexpr (kVec == 8)
+    *reinterpret_cast<uint4*>(static_cast<T*>(base) + i) = *reinterpret_cast<const uint4*>(&p);
+  else
+    static_cast<T*>(base)[i] = p.v[0];
+}
+__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+
+// A token's rows and weights into shared memory; a row that is no row of the
+// operand is treated as none.
+__device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* s_row, float* s_w) {
+  if ((int)threadIdx.x < a.top_k) {
+    const long long at = t * a.top_k + threadIdx.x;
+    const int r = a.rows[at];
+    s_row[threadIdx.x] = r >= 0 && r < (long long)a.tokens * a.top_k ? r : -1;
+    s_w[threadIdx.x] = a.weights != nullptr ? a.weights[at] : 1.0f;
+  }
+  __syncthreads();
+}
+
+// Rows t * top_k .. of the sorted operand that no expert owns are zeroed by
+// token t's block.
+template <class T, int kVec>
+__device__ __forceinline__ void zero_tail(const MoveArgs& a, long long t) {
+  const int total = *a.total;
+  for (int j = 0; j < a.top_k; ++j) {
+    const long long r = t * a.top_k + j;
+    if (r < total) continue;
+    Pack<T, kVec> z;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) z.v[i] = round_one<T>(0.0f);
+    for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec)
+      store_pack<T, kVec>(a.out, r * a.ld_out + c, z);
+  }
+}
+
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
+  __shared__ int s_row[kMaxTopK];
+  __shared__ float s_w[kMaxTopK];
+  const long long t = blockIdx.x;
+  load_slots(a, t, s_row, s_w);
+  for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec) {
+    const Pack<T, kVec> p = load_pack<T, kVec>(a.in, t * a.ld_in + c);
+    for (int j = 0; j < a.top_k; ++j)
+      if (s_row[j] >= 0) store_pack<T, kVec>(a.out, (long long)s_row[j] * a.ld_out + c, p);
+  }
+  zero_tail<T, kVec>(a, t);
+}
+
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
+  __shared__ int s_row[kMaxTopK];
+  __shared__ float s_w[kMaxTopK];
+  const long long t = blockIdx.x;
+  load_slots(a, t, s_row, s_w);
+  for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec) {
+    float sum[kVec];
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) sum[i] = 0.0f;
+#pragma unroll 4
+    for (int j = 0; j < a.top_k; ++j) {
+      if (s_row[j] < 0) continue;
+      const Pack<T, kVec> p = load_pack<T, kVec>(a.in, (long long)s_row[j] * a.ld_in + c);
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) sum[i] = fmaf(s_w[j], widen(p.v[i]), sum[i]);
+    }
+    Pack<T, kVec> o;
+#pragma unroll
+    for (int i = 0; i < kVec; ++i) o.v[i] = round_one<T>(sum[i]);
+    store_pack<T, kVec>(a.out, t * a.ld_out + c, o);
+  }
+}
+
+// dy[row] = w dout[t], dw[t, j] = <dout[t], y[row]>: dout is read once per
+// slot (from cache after the first), y once.
+template <class T, int kVec>
+__global__ void __launch_bounds__(256) combine_grad_kernel(const MoveArgs a) {
+  __shared__ int s_row[kMaxTopK];
+  __shared__ float s_w[kMaxTopK];
+  __shared__ float s_part[8];
+  const long long t = blockIdx.x;
+  load_slots(a, t, s_row, s_w);
+  for (int j = 0; j < a.top_k; ++j) {
+    const long long r = s_row[j];
+    float dot = 0.0f;
+    if (r >= 0) {
+      for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec) {
+        const Pack<T, kVec> d = load_pack<T, kVec>(a.in, t * a.ld_in + c);
+        const Pack<T, kVec> y = load_pack<T, kVec>(a.in2, r * a.ld_in2 + c);
+        Pack<T, kVec> o;
+#pragma unroll
+        for (int i = 0; i < kVec; ++i) {
+          const float v = widen(d.v[i]);
+          dot = fmaf(v, widen(y.v[i]), dot);
+          o.v[i] = round_one<T>(s_w[j] * v);
+        }
+        store_pack<T, kVec>(a.out, r * a.ld_out + c, o);
+      }
+    }
+    if (a.dweights != nullptr) {
+      dot = warp_sum(dot);
+      if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = dot;
+      __syncthreads();
+      if (threadIdx.x == 0) {
+        float all = 0.0f;
+        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all += s_part[w];
+        a.dweights[t * a.top_k + j] = all;
+      }
+      __syncthreads();
+    }
+  }
+  zero_tail<T, kVec>(a, t);
+}
+
+}  // namespace b200

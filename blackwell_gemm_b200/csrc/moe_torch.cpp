@@ -196,6 +196,191 @@ at::Tensor matmul_b200_grouped(const at::Tensor& A, const at::Tensor& B,
   return grouped_forward(A, B.transpose(1, 2), off);
 }
 
+// -------------------------------------------------------------------- routing
+constexpr const char* kRoute = "route_b200";
+constexpr const char* kDispatch = "dispatch_b200";
+constexpr const char* kCombine = "combine_b200";
+
+int logit_code(const at::Tensor& t) {
+  return t.scalar_type() == at::kFloat ? B200_FP32 : dtype_code(t);
+}
+
+// Rows with unit column stride; any row stride of at least the width.
+at::Tensor unit_rows(const at::Tensor& t) {
+  return (t.size(1) <= 1 || t.stride(1) == 1) && (t.size(0) <= 1 || t.stride(0) >= t.size(1))
+             ? t
+             : t.contiguous();
+}
+int64_t row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// weights, experts, rows, tokens, offsets
+std::vector<at::Tensor> route_forward(const at::Tensor& logits, int64_t top_k, bool normalize) {
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const int64_t t = logits.size(0), e = logits.size(1);
+  const at::Tensor l = unit_rows(logits);
+  const auto ints = logits.options().dtype(at::kInt);
+  auto weights = at::empty({t, top_k}, logits.options().dtype(at::kFloat));
+  auto chosen = at::empty({t, top_k}, ints), rows = at::empty({t, top_k}, ints);
+  auto sources = at::empty({t * top_k}, ints), offsets = at::empty({e + 1}, ints);
+  check_status(b200_route(l.data_ptr(), (int)t, (int)e, row_stride(l), logit_code(l), (int)top_k,
+                          normalize, weights.data_ptr<float>(), chosen.data_ptr<int>(),
+                          rows.data_ptr<int>(), sources.data_ptr<int>(), offsets.data_ptr<int>(),
+                          current_stream()),
+               kRoute);
+  return {weights, chosen, rows, sources, offsets};
+}
+
+struct Route : torch::autograd::Function<Route> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& logits, int64_t top_k,
+                               bool normalize) {
+    auto r = route_forward(logits, top_k, normalize);
+    ctx->save_for_backward({logits, r[1], r[0]});
+    ctx->saved_data["normalize"] = normalize;
+    ctx->mark_non_differentiable({r[1], r[2], r[3], r[4]});
+    return r;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &logits = saved[0], &chosen = saved[1], &weights = saved[2];
+    at::Tensor dlogits;
+    if (grads[0].defined()) {
+      const c10::cuda::CUDAGuard guard(logits.device());
+      const at::Tensor l = unit_rows(logits);
+      const at::Tensor dw = grads[0].to(at::kFloat).contiguous();
+      dlogits = at::empty({l.size(0), l.size(1)}, l.options());
+      check_status(b200_route_grad(l.data_ptr(), (int)l.size(0), (int)l.size(1), row_stride(l),
+                                   logit_code(l), (int)chosen.size(1),
+                                   ctx->saved_data["normalize"].toBool(), chosen.data_ptr<int>(),
+                                   weights.data_ptr<float>(), dw.data_ptr<float>(),
+                                   dlogits.data_ptr(), current_stream()),
+                   "route_b200 backward");
+    }
+    return {dlogits, at::Tensor(), at::Tensor()};
+  }
+};
+
+std::vector<at::Tensor> route_b200(const at::Tensor& logits, int64_t top_k, bool normalize) {
+  TORCH_CHECK(logits.dim() == 2, kRoute, ": logits must be (tokens, experts)");
+  TORCH_CHECK(logits.is_cuda(), kRoute, ": logits must be a CUDA tensor");
+  TORCH_CHECK(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 ||
+                  logits.scalar_type() == at::kHalf,
+              kRoute, ": logits must be float32, bfloat16 or float16");
+  const int64_t t = logits.size(0), e = logits.size(1);
+  TORCH_CHECK(e <= B200_MAX_EXPERTS, kRoute, ": more than ", B200_MAX_EXPERTS, " experts");
+  TORCH_CHECK(top_k >= 1 && top_k <= e && top_k <= B200_MAX_TOP_K, kRoute, ": top_k = ", top_k,
+              " must be 1 .. min(experts, ", B200_MAX_TOP_K, ")");
+  check_sizes({t * top_k}, kRoute);
+  if (at::GradMode::is_enabled() && logits.requires_grad())
+    return Route::apply(logits, top_k, normalize);
+  return route_forward(logits, top_k, normalize);
+}
+
+// A sorted operand's rows and a token operand's, checked against the routing.
+void check_routing(const at::Tensor& t, const at::Tensor& rows, const at::Tensor& offsets,
+                   bool sorted, const char* who, const char* name) {
+  TORCH_CHECK(t.dim() == 2, who, ": ", name, " must be 2-D");
+  check_16bit(t, who, name);
+  TORCH_CHECK(rows.dim() == 2 && rows.is_contiguous() && rows.scalar_type() == at::kInt &&
+                  offsets.dim() == 1 && offsets.size(0) >= 1 && offsets.is_contiguous() &&
+                  offsets.scalar_type() == at::kInt,
+              who, ": routing must come from route_b200");
+  TORCH_CHECK(rows.device() == t.device() && offsets.device() == t.device(), who, ": ", name,
+              " and the routing are on different devices");
+  TORCH_CHECK(rows.size(1) <= B200_MAX_TOP_K, who, ": more than ", B200_MAX_TOP_K, " slots");
+  const int64_t want = sorted ? rows.numel() : rows.size(0);
+  TORCH_CHECK(t.size(0) == want, who, ": ", name, " has ", t.size(0), " rows, the routing ", want);
+  check_sizes({rows.numel(), t.size(1)}, who);
+}
+
+const int* total_of(const at::Tensor& offsets) {
+  return offsets.data_ptr<int>() + (offsets.size(0) - 1);
+}
+
+at::Tensor dispatch_forward(const at::Tensor& x, const at::Tensor& rows,
+                            const at::Tensor& offsets) {
+  const c10::cuda::CUDAGuard guard(x.device());
+  const at::Tensor in = unit_rows(x);
+  auto xs = at::empty({rows.numel(), x.size(1)}, x.options());
+  check_status(b200_dispatch(in.data_ptr(), rows.data_ptr<int>(), total_of(offsets), xs.data_ptr(),
+                             (int)rows.size(0), (int)rows.size(1), (int)x.size(1), row_stride(in),
+                             x.size(1), dtype_code(x), current_stream()),
+               kDispatch);
+  return xs;
+}
+
+at::Tensor combine_forward(const at::Tensor& y, const float* weights, const at::Tensor& rows,
+                           const char* who) {
+  const c10::cuda::CUDAGuard guard(y.device());
+  const at::Tensor in = unit_rows(y);
+  auto out = at::empty({rows.size(0), y.size(1)}, y.options());
+  check_status(b200_combine(in.data_ptr(), weights, rows.data_ptr<int>(), out.data_ptr(),
+                            (int)rows.size(0), (int)rows.size(1), (int)y.size(1), row_stride(in),
+                            y.size(1), dtype_code(y), current_stream()),
+               who);
+  return out;
+}
+
+struct Dispatch : torch::autograd::Function<Dispatch> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& rows,
+                            const at::Tensor& offsets) {
+    ctx->save_for_backward({rows});
+    ctx->saved_data["dtype"] = x.scalar_type();
+    return dispatch_forward(x, rows, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    at::Tensor dx;
+    if (grads[0].defined())
+      dx = combine_forward(grads[0].to(ctx->saved_data["dtype"].toScalarType()), nullptr,
+                           ctx->get_saved_variables()[0], "dispatch_b200 backward");
+    return {dx, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor dispatch_b200(const at::Tensor& x, const at::Tensor& rows, const at::Tensor& offsets) {
+  check_routing(x, rows, offsets, false, kDispatch, "x");
+  if (at::GradMode::is_enabled() && x.requires_grad()) return Dispatch::apply(x, rows, offsets);
+  return dispatch_forward(x, rows, offsets);
+}
+
+struct Combine : torch::autograd::Function<Combine> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& weights,
+                            const at::Tensor& rows, const at::Tensor& offsets) {
+    ctx->save_for_backward({y, weights, rows, offsets});
+    return combine_forward(y, weights.data_ptr<float>(), rows, kCombine);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &y = saved[0], &weights = saved[1], &rows = saved[2], &offsets = saved[3];
+    at::Tensor dy, dweights;
+    if (grads[0].defined()) {
+      const c10::cuda::CUDAGuard guard(y.device());
+      const at::Tensor dout = unit_rows(grads[0].to(y.scalar_type())), in = unit_rows(y);
+      dy = at::empty({y.size(0), y.size(1)}, y.options());
+      if (ctx->needs_input_grad(1)) dweights = at::empty({rows.size(0), rows.size(1)}, weights.options());
+      check_status(
+          b200_combine_grad(dout.data_ptr(), in.data_ptr(), weights.data_ptr<float>(),
+                            rows.data_ptr<int>(), total_of(offsets), dy.data_ptr(),
+                            dweights.defined() ? dweights.data_ptr<float>() : nullptr,
+                            (int)rows.size(0), (int)rows.size(1), (int)y.size(1), row_stride(dout),
+                            row_stride(in), y.size(1), dtype_code(y), current_stream()),
+          "combine_b200 backward");
+    }
+    return {dy, dweights, at::Tensor(), at::Tensor()};
+  }
+};
+
+at::Tensor combine_b200(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& rows,
+                        const at::Tensor& offsets) {
+  check_routing(y, rows, offsets, true, kCombine, "y");
+  TORCH_CHECK(weights.sizes() == rows.sizes() && weights.scalar_type() == at::kFloat &&
+                  weights.device() == y.device(),
+              kCombine, ": weights must be float32 (tokens, top_k) on y's device");
+  const at::Tensor w = weights.contiguous();
+  if (at::GradMode::is_enabled() && (y.requires_grad() || w.requires_grad()))
+    return Combine::apply(y, w, rows, offsets);
+  return combine_forward(y, w.data_ptr<float>(), rows, kCombine);
+}
+
 // -------------------------------------------------------------- 4-bit weights
 constexpr const char* kPack = "pack_w4";
 constexpr const char* kW4 = "matmul_b200_w4";
@@ -273,6 +458,9 @@ at::Tensor w4_matmul(const at::Tensor& A, const at::Tensor& packed, int64_t expe
 void register_moe(pybind11::module_& m) {
   m.def("matmul_b200_grouped", &matmul_b200_grouped,
         "C[r] = A[r] @ B[e] for rows r of expert e (offsets on the device)");
+  m.def("route_b200", &route_b200, "top-k experts, weights and the order sorted by expert");
+  m.def("dispatch_b200", &dispatch_b200, "rows of x in the order sorted by expert");
+  m.def("combine_b200", &combine_b200, "weighted sum of each token's rows");
   m.def("w4_pack", &w4_pack, "4-bit weights in the order the kernel reads them",
         pybind11::arg("q"), pybind11::arg("scales"), pybind11::arg("zeros") = std::nullopt);
   m.def("w4_matmul", &w4_matmul, "C = A @ W^T with packed 4-bit weights");

@@ -9,12 +9,51 @@ from __future__ import annotations
 
 from typing import NamedTuple
 
-__all__ = ["matmul_b200_grouped", "W4Weight", "pack_w4", "quantize_w4", "matmul_b200_w4"]
+__all__ = ["Routing", "route_b200", "dispatch_b200", "combine_b200", "matmul_b200_grouped",
+           "W4Weight", "pack_w4", "quantize_w4", "matmul_b200_w4"]
 
 
 def _ext():
     from . import load
     return load()
+
+
+class Routing(NamedTuple):
+    """Where each token's top_k slots go (route_b200)."""
+    weights: "torch.Tensor"  # noqa: F821  (tokens, top_k) float32; differentiable
+    experts: "torch.Tensor"  # noqa: F821  (tokens, top_k) int32, -1 at an empty slot
+    rows: "torch.Tensor"     # noqa: F821  (tokens, top_k) int32, sorted row, -1 at an empty slot
+    tokens: "torch.Tensor"   # noqa: F821  (tokens * top_k,) int32, -1 past the last owned row
+    offsets: "torch.Tensor"  # noqa: F821  (experts + 1,) int32
+
+
+def route_b200(logits, top_k: int, *, normalize: bool = True) -> Routing:
+    """Each token's top_k experts, their weights, and the order by expert.
+
+    logits: (tokens, experts) float32, bf16 or fp16 CUDA; at most 1024
+    experts, top_k at most 32.  The largest logits are chosen, the lower index
+    first on a tie; NaN counts as largest; an expert at -inf is closed and
+    never chosen, and a token with fewer open experts than top_k has empty
+    slots (expert and row -1, weight 0).  weights: the softmax over the chosen
+    experts (normalize) or over all of them, in float32; differentiable in the
+    logits.  Rows are sorted by expert, then token, then slot."""
+    return Routing(*_ext().route_b200(logits, top_k, normalize))
+
+
+def dispatch_b200(x, routing: Routing):
+    """xs[row] = x[token of row]: (tokens, width) bf16 or fp16 to (tokens *
+    top_k, width), sorted by expert; rows of no expert are zero.
+    Differentiable: a token's gradient is its rows' sum, in fp32, rounded once."""
+    return _ext().dispatch_b200(x, routing.rows, routing.offsets)
+
+
+def combine_b200(y, routing: Routing, weights=None):
+    """out[t] = sum_j weights[t, j] * y[rows[t, j]] over t's non-empty slots:
+    (tokens * top_k, width) to (tokens, width), summed in fp32, rounded once.
+    weights: (tokens, top_k) float32, routing.weights by default.
+    Differentiable in y and the weights."""
+    w = routing.weights if weights is None else weights
+    return _ext().combine_b200(y, w, routing.rows, routing.offsets)
 
 
 def matmul_b200_grouped(A, B, offsets):

@@ -28,7 +28,9 @@ extern "C" {
 
 #define B200_BF16 0
 #define B200_FP16 1
+#define B200_FP32 2 /* logits only */
 #define B200_MAX_EXPERTS 1024
+#define B200_MAX_TOP_K 32
 
 /* C[r, :] = A[r, :] B[e]^T for the rows r of every expert e.
  * A: rows x K, stride lda.  B: experts x N x K, row stride ldb, matrix stride
@@ -56,6 +58,47 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
 /* Kernel for b200_grouped_gemm and _da: 0 = chosen by rows per expert
  * (default), 1 = the streaming kernel (few rows), 2 = the pair kernel. */
 int b200_grouped_set_kernel(int kernel);
+
+/* ---- Routing -----------------------------------------------------------------
+ * Each token's top_k experts (largest logits; the lower index first on a tie;
+ * NaN counts as largest), their softmax weights and the order that sorts the
+ * tokens * top_k (token, slot) pairs by expert, pairs of one expert by token
+ * and slot.  An expert whose logit is -inf is closed: never chosen.  A slot
+ * left empty for want of open experts has expert -1, row -1 and weight 0.
+ * logits: tokens x experts, stride ld, type B200_BF16, _FP16 or _FP32.
+ * normalize != 0: softmax over the chosen experts, else over all of them.
+ * weights, chosen, rows: tokens x top_k; sources: tokens * top_k, the token of
+ * each sorted row, -1 past the last owned row; offsets: experts + 1, what
+ * b200_grouped_gemm takes.  top_k <= experts, top_k <= 32. */
+int b200_route(const void* logits, int tokens, int experts, long long ld, int type, int top_k,
+               int normalize, float* weights, int* chosen, int* rows, int* sources, int* offsets,
+               void* stream);
+
+/* Gradient of the weights in the logits; dlogits: tokens x experts,
+ * contiguous, of the logits' type; zero at closed experts. */
+int b200_route_grad(const void* logits, int tokens, int experts, long long ld, int type, int top_k,
+                    int normalize, const int* chosen, const float* weights, const float* dweights,
+                    void* dlogits, void* stream);
+
+/* xs[rows[t][j], :] = x[t, :]; rows of xs from *total on (the last entry of
+ * offsets) are zero.  xs: tokens * top_k rows.  16-bit elements; strides in
+ * elements; 16-byte aligned rows of a multiple of 8 elements move fastest,
+ * any others work. */
+int b200_dispatch(const void* x, const int* rows, const int* total, void* xs, int tokens, int top_k,
+                  int width, long long ldx, long long ldxs, int dtype, void* stream);
+
+/* out[t, :] = sum over t's non-empty slots j of weights[t][j] y[rows[t][j], :],
+ * summed in fp32 in slot order, rounded once; weights NULL: all 1 (which is
+ * the gradient of b200_dispatch). */
+int b200_combine(const void* y, const float* weights, const int* rows, void* out, int tokens,
+                 int top_k, int width, long long ldy, long long ldo, int dtype, void* stream);
+
+/* Gradients of b200_combine: dy[rows[t][j], :] = weights[t][j] dout[t, :] (rows
+ * from *total on zero), dweights[t][j] = <dout[t, :], y[rows[t][j], :]> (0 at
+ * empty slots; dweights may be NULL). */
+int b200_combine_grad(const void* dout, const void* y, const float* weights, const int* rows,
+                      const int* total, void* dy, float* dweights, int tokens, int top_k, int width,
+                      long long ldo, long long ldy, long long lddy, int dtype, void* stream);
 
 /* ---- 4-bit weights with group scales ---------------------------------------
  * A weight is (q - z) * s: q in 0..15, one scale s (16-bit, the type of A) and

@@ -143,3 +143,68 @@ def test_w4_torch_checks():
         bg.pack_w4(q[0], s)
     with pytest.raises(RuntimeError, match="multiple of group"):
         bg.quantize_w4(torch.zeros(4, 100, dtype=torch.bfloat16), 64)
+
+
+def test_route_c_abi():
+    lib = capi.lib()
+
+    def route(logits=FAKE, tokens=4, experts=8, ld=8, type=capi.FP32, k=2, w=FAKE, ex=FAKE,
+              rows=FAKE, src=FAKE, off=FAKE):
+        return lib.b200_route(logits, tokens, experts, ld, type, k, 1, w, ex, rows, src, off, None)
+
+    for change, expect in [(dict(tokens=-1), capi.ERR_INVALID_ARGUMENT),
+                           (dict(k=9), capi.ERR_INVALID_ARGUMENT),
+                           (dict(k=-1), capi.ERR_INVALID_ARGUMENT),
+                           (dict(k=33, experts=64, ld=64), capi.ERR_INVALID_ARGUMENT),
+                           (dict(type=3), capi.ERR_INVALID_ARGUMENT),
+                           (dict(ld=7), capi.ERR_INVALID_ARGUMENT),
+                           (dict(logits=0), capi.ERR_INVALID_ARGUMENT),
+                           (dict(off=0), capi.ERR_INVALID_ARGUMENT),
+                           (dict(w=0), capi.ERR_INVALID_ARGUMENT),
+                           (dict(rows=FAKE + 2), capi.ERR_ALIGNMENT),
+                           (dict(logits=FAKE + 2), capi.ERR_ALIGNMENT),
+                           (dict(experts=1025, ld=1025), capi.ERR_TOO_LARGE),
+                           (dict(tokens=INT_MAX, k=2), capi.ERR_TOO_LARGE)]:
+        assert route(**change) == expect, change
+    assert lib.b200_route_grad(FAKE, 4, 8, 7, 2, 2, 1, FAKE, FAKE, FAKE, FAKE, None) == \
+        capi.ERR_INVALID_ARGUMENT
+    assert lib.b200_route_grad(FAKE, 0, 8, 8, 2, 2, 1, FAKE, FAKE, FAKE, FAKE, None) == capi.OK
+
+
+def test_moving_rows_c_abi():
+    lib = capi.lib()
+    dispatch = [FAKE, FAKE, FAKE, FAKE, 4, 2, 16, 16, 16, capi.BF16, None]
+    combine = [FAKE, FAKE, FAKE, FAKE, 4, 2, 16, 16, 16, capi.BF16, None]
+    grad = [FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, 4, 2, 16, 16, 16, 16, capi.BF16, None]
+    for fn, args, at, value, expect in [
+            (lib.b200_dispatch, dispatch, 4, -1, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_dispatch, dispatch, 5, 33, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_dispatch, dispatch, 7, 15, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_dispatch, dispatch, 2, 0, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_dispatch, dispatch, 9, 2, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_dispatch, dispatch, 0, FAKE + 1, capi.ERR_ALIGNMENT),
+            (lib.b200_dispatch, dispatch, 4, INT_MAX, capi.ERR_TOO_LARGE),
+            (lib.b200_dispatch, dispatch, 4, 0, capi.OK),
+            (lib.b200_combine, combine, 2, 0, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_combine, combine, 8, 8, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_combine, combine, 1, FAKE + 2, capi.ERR_ALIGNMENT),
+            (lib.b200_combine, combine, 6, 0, capi.OK),
+            (lib.b200_combine_grad, grad, 2, 0, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_combine_grad, grad, 4, 0, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_combine_grad, grad, 11, 8, capi.ERR_INVALID_ARGUMENT),
+            (lib.b200_combine_grad, grad, 7, 0, capi.OK)]:
+        changed = list(args)
+        changed[at] = value
+        assert fn(*changed) == expect, (fn, at, value)
+
+
+def test_route_torch_checks():
+    x = torch.zeros(4, 8)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        bg.route_b200(x, 2)
+    i = torch.zeros(4, 2, dtype=torch.int32)
+    r = bg.Routing(torch.zeros(4, 2), i, i, i.flatten(), torch.zeros(9, dtype=torch.int32))
+    with pytest.raises(RuntimeError, match="CUDA"):
+        bg.dispatch_b200(x.bfloat16(), r)
+    with pytest.raises(RuntimeError, match="2-D"):
+        bg.combine_b200(x[0].bfloat16(), r)
