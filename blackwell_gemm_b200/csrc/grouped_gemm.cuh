@@ -140,7 +140,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int pair = blockIdx.x >> 1;
@@ -194,7 +194,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
 
   if (warp == 0) {
     // ------------------------------------------------------------ producer
-    if (lane == 0) {
+    if (elect_one()) {
       const uint32_t full_leader = cluster_map(smem_u32(&bar_full[0]), 0);
       const uint32_t empty_peer = cluster_map(smem_u32(&bar_empty[0]), 1);
       const uint32_t edge_self = cluster_map(smem_u32(&bar_edge[0]), rank);
@@ -245,7 +245,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
-    if (rank == 0 && lane == 0) {
+    if (rank == 0 && elect_one()) {
       const uint32_t empty_self = cluster_map(smem_u32(&bar_empty[0]), 0);
       const uint32_t accf_self = cluster_map(smem_u32(&bar_acc_full[0]), 0);
       const uint32_t accf_peer = cluster_map(smem_u32(&bar_acc_full[0]), 1);

@@ -184,7 +184,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
   __shared__ uint32_t abort_word;
   constexpr uint32_t kCols = 2 * kTok < 32 ? 32 : 2 * kTok;  // two accumulators
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   int* s_off =
@@ -227,7 +227,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
   StreamSegment s;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
       uint32_t stage = 0, phase = 0;
       bool ok = true;
@@ -257,7 +257,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t stage = 0, phase = 0;
       int it = 0;
       bool ok = true;

@@ -104,7 +104,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
-  const int warp = threadIdx.x >> 5;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t exchange = smem_base + kStages * C::kStageBytes;
@@ -150,7 +150,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   StreamSegment s;
 
   if (warp == 0) {
-    if (lane == 0) {
+    if (elect_one()) {
       const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
       uint32_t stage = 0, phase = 0;
       bool ok = true;
@@ -179,7 +179,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
     }
     __syncwarp();
   } else if (warp == 1) {
-    if (lane == 0) {
+    if (elect_one()) {
       uint32_t stage = 0, phase = 0;
       uint32_t item = 0;
       bool ok = true;
