@@ -171,6 +171,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
     tmem_relinquish_pair();
   }
+  grid_wait();
   if (warp == 2) {
     const bool bad = build_groups(args.offsets, args.experts, args.rows, 256, s_off, s_tiles);
     if (bad && blockIdx.x == 0 && lane == 0) atomicCAS(args.status, 0, kErrOffsets);
@@ -178,6 +179,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();
+  grid_launch_next();
   const uint32_t tmem_base = tmem_slot;
 
   WaitCtx wctx;
@@ -208,7 +210,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         const int t0 = kMode == kGroupedDB ? w.col0 + (int)rank * 128 : w.row0 + (int)rank * half;
         const uint32_t bytes = C::kOperand + (half == 128 ? C::kOperand : half * 128);
         for (int kb = 0; kb < w.blocks; ++kb) {
-          if (!wait_bounded(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
+          if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
             ok = false;
             break;
           }
@@ -258,7 +260,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         const uint32_t idesc = make_idesc_16bit(kPairM, w.mma_n, kFormat<T>, kMnA, kMnB);
         const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
         ++it;
-        if (!wait_bounded(smem_u32(&bar_acc_empty[buf]), acc_phase ^ 1u, wctx, kErrWaitAccEmpty))
+        if (!wait_ready(smem_u32(&bar_acc_empty[buf]), acc_phase ^ 1u, wctx, kErrWaitAccEmpty))
           break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * 256;
@@ -269,7 +271,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
           const bool edge = kMode == kGroupedDB && left < kSlabK && (left & 15) != 0;
           const bool landed =
               edge ? wait_bounded_acq_cluster(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)
-                   : wait_bounded(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull);
+                   : wait_ready(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull);
           if (!landed) {
             ok = false;
             break;
@@ -318,7 +320,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         ++it;
         int ok = 0;
         if (lane == 0)
-          ok = wait_bounded(smem_u32(&bar_acc_full[buf]), acc_phase, wctx, kErrWaitAccFull);
+          ok = wait_ready(smem_u32(&bar_acc_full[buf]), acc_phase, wctx, kErrWaitAccFull);
         ok = __shfl_sync(0xffffffffu, ok, 0);
         if (!ok) break;
         tc_fence_after_sync();
@@ -403,7 +405,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
       if ((valid & 15) == 0) continue;
       int got = 0;
       if (lane == 0)
-        got = wait_bounded(smem_u32(&bar_edge[s]), (parity >> s) & 1u, wctx, kErrWaitFull);
+        got = wait_ready(smem_u32(&bar_edge[s]), (parity >> s) & 1u, wctx, kErrWaitFull);
       ok = __shfl_sync(0xffffffffu, got, 0) != 0;
       __syncwarp();
       if (!ok) break;

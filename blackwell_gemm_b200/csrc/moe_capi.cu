@@ -69,16 +69,24 @@ bool init_stream() {
          set_smem(grouped_stream_kernel<kDA, 64, T>, StreamCfg<64>::smem_bytes(kMaxExperts));
 }
 
-// Token tile of the 4-bit kernel: all rows of a small call in one tile of 16;
-// else the widest whose products (one set of columns per group of a record)
-// fit the kernel's TMEM.
+// Token tile of the 4-bit kernel that goes through TMEM: the widest whose
+// products (one set of columns per group of a record) fit there.
 constexpr int w4_tokens(int group) { return group == 32 ? 32 : 64; }
+
+template <int kGroup, bool kZeros, class T>
+bool init_w4_one() {
+  constexpr int wide = w4_tokens(kGroup);
+  return set_smem(w4_rows_kernel<8, kGroup, kZeros, T>,
+                  W4RowsCfg<8, kGroup>::smem_bytes(kMaxExperts)) &&
+         set_smem(w4_rows_kernel<16, kGroup, kZeros, T>,
+                  W4RowsCfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
+         set_smem(w4_stream_kernel<wide, kGroup, kZeros, T>,
+                  W4Cfg<wide, kGroup>::smem_bytes(kMaxExperts));
+}
 
 template <int kGroup, class T>
 bool init_w4() {
-  constexpr int wide = w4_tokens(kGroup);
-  return set_smem(w4_stream_kernel<16, kGroup, T>, W4Cfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
-         set_smem(w4_stream_kernel<wide, kGroup, T>, W4Cfg<wide, kGroup>::smem_bytes(kMaxExperts));
+  return init_w4_one<kGroup, false, T>() && init_w4_one<kGroup, true, T>();
 }
 
 template <class T>
@@ -248,8 +256,24 @@ int zero_rows(void* p, int ld, int width, int rows, cudaStream_t stream) {
              : B200_ERR_LAUNCH;
 }
 
-int launched() {
-  if (cudaGetLastError() == cudaSuccess) return B200_OK;
+// Launch with programmatic stream serialization: the kernel's set-up overlaps
+// the end of the one before it (every kernel of this file waits, grid_wait,
+// before it touches global memory).
+template <class... P, class... A>
+int launch(void (*fn)(P...), int blocks, int threads, size_t smem, cudaStream_t stream,
+           A&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...) == cudaSuccess) return B200_OK;
+  cudaGetLastError();
   return B200_ERR_LAUNCH;
 }
 
@@ -288,9 +312,8 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
                              ? tf * ceil_div(c.K, 256) * c.experts
                              : tf * (ceil_div(c.rows, 256) + (c.experts < c.rows ? c.experts : c.rows));
   const int pairs = (int)(most < m.pairs[kMode] ? most : m.pairs[kMode]);
-  grouped_pair_kernel<kMode, T>
-      <<<2 * pairs, C::kThreads, C::smem_bytes(c.experts), stream>>>(tw, tt, ts, a);
-  return launched();
+  return launch(grouped_pair_kernel<kMode, T>, 2 * pairs, C::kThreads, C::smem_bytes(c.experts),
+                stream, tw, tt, ts, a);
 }
 
 template <bool kDA, int kTok, class T>
@@ -318,9 +341,8 @@ int launch_stream(const Call& c, const DeviceView& v, cudaStream_t stream) {
   Workspace ws;
   st = ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a);
   if (st != B200_OK) return st;
-  grouped_stream_kernel<kDA, kTok, T>
-      <<<v.sms, C::kThreads, C::smem_bytes(c.experts), stream>>>(tw, tt, a);
-  return launched();
+  return launch(grouped_stream_kernel<kDA, kTok, T>, v.sms, C::kThreads,
+                C::smem_bytes(c.experts), stream, tw, tt, a);
 }
 
 template <int kMode, class T>
@@ -380,11 +402,19 @@ int check_w4_shape(int experts, int N, int K, int group) {
              : B200_ERR_TOO_LARGE;
 }
 
-template <int kTok, int kGroup, class T>
+template <bool kRows, int kTok, int kGroup, bool kZeros, class T>
 int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
-  using C = W4Cfg<kTok, kGroup>;
+  constexpr int box_rows = W4Ring<kTok, kGroup>::kSlabRows;
   CUtensorMap tt;
-  int st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, 16);
+  int st;
+  if (c.K % kSlabK == 0) {  // (k in a slab, row, slab)
+    const cuuint64_t dims[3] = {kSlabK, (cuuint64_t)c.rows, (cuuint64_t)(c.K / kSlabK)};
+    const cuuint64_t strides[2] = {(cuuint64_t)c.lda * 2, kSlabK * 2};
+    const cuuint32_t box[3] = {kSlabK, box_rows, 4};
+    st = encode_tensor(&tt, map_type(c.dtype), 3, c.a, dims, strides, box);
+  } else {
+    st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, box_rows);
+  }
   if (st != B200_OK) return st;
   StreamArgs a = {};
   a.offsets = c.offsets;
@@ -400,27 +430,38 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   a.status = v.status;
   a.timeout_ns = v.timeout_ns;
   a.packed = static_cast<const uint8_t*>(c.packed);
-  a.record_bytes = w4_record_bytes(kGroup, c.zeros != 0);
+  a.record_bytes = w4_record_bytes(kGroup, kZeros);
   a.expert_bytes = (long long)a.feat_blocks * a.red_blocks * a.record_bytes;
   Workspace ws;
   st = ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a);
   if (st != B200_OK) return st;
-  w4_stream_kernel<kTok, kGroup, T>
-      <<<v.sms, C::kThreads, C::smem_bytes(c.experts), stream>>>(tt, a, c.zeros != 0);
-  return launched();
+  if constexpr (kRows) {
+    using C = W4RowsCfg<kTok, kGroup>;
+    return launch(w4_rows_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
+                  C::smem_bytes(c.experts), stream, tt, a);
+  } else {
+    using C = W4Cfg<kTok, kGroup>;
+    return launch(w4_stream_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
+                  C::smem_bytes(c.experts), stream, tt, a);
+  }
 }
 
-template <int kGroup, class T>
+template <int kGroup, bool kZeros, class T>
 int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
-  return c.rows <= 16 ? launch_w4<16, kGroup, T>(c, v, stream)
-                      : launch_w4<w4_tokens(kGroup), kGroup, T>(c, v, stream);
+  if (c.rows <= 8) return launch_w4<true, 8, kGroup, kZeros, T>(c, v, stream);
+  if (c.rows <= 16) return launch_w4<true, 16, kGroup, kZeros, T>(c, v, stream);
+  return launch_w4<false, w4_tokens(kGroup), kGroup, kZeros, T>(c, v, stream);
 }
 
 template <class T>
 int run_w4_typed(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
-  return c.group == 32   ? run_w4_group<32, T>(c, v, stream)
-         : c.group == 64 ? run_w4_group<64, T>(c, v, stream)
-                         : run_w4_group<128, T>(c, v, stream);
+  if (c.zeros)
+    return c.group == 32   ? run_w4_group<32, true, T>(c, v, stream)
+           : c.group == 64 ? run_w4_group<64, true, T>(c, v, stream)
+                           : run_w4_group<128, true, T>(c, v, stream);
+  return c.group == 32   ? run_w4_group<32, false, T>(c, v, stream)
+         : c.group == 64 ? run_w4_group<64, false, T>(c, v, stream)
+                         : run_w4_group<128, false, T>(c, v, stream);
 }
 
 int run_w4(const W4Call& c, cudaStream_t stream) {
@@ -461,18 +502,16 @@ int run_w4_pack(const void* q, const void* scales, const void* zeros, void* pack
   MoeDevice* m = nullptr;
   st = moe_device(&v, &m);
   if (st != B200_OK) return st;
-  w4_pack_kernel<<<(unsigned)records, 256, 0, stream>>>(
-      static_cast<const uint8_t*>(q), static_cast<const uint16_t*>(scales),
-      static_cast<const uint8_t*>(zeros), static_cast<uint8_t*>(packed), N, K, group, blocks, red,
-      w4_record_bytes(group, zeros != nullptr));
-  return launched();
+  return launch(w4_pack_kernel, (int)records, 256, 0, stream, static_cast<const uint8_t*>(q),
+                static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros),
+                static_cast<uint8_t*>(packed), N, K, group, blocks, red,
+                w4_record_bytes(group, zeros != nullptr));
 }
 
 // -------------------------------------------------------------------- routing
 template <int kPer>
 int launch_choose(const RouteArgs& a, int blocks, size_t smem, cudaStream_t stream) {
-  route_choose_kernel<kPer><<<blocks, kRouteThreads, smem, stream>>>(a);
-  return launched();
+  return launch(route_choose_kernel<kPer>, blocks, kRouteThreads, smem, stream, a);
 }
 
 int run_route(RouteArgs a, const DeviceView& v, cudaStream_t stream) {
@@ -497,8 +536,7 @@ int run_route(RouteArgs a, const DeviceView& v, cudaStream_t stream) {
            : a.experts <= 256 ? launch_choose<8>(a, blocks, smem, stream)
                               : launch_choose<32>(a, blocks, smem, stream);
   if (st == B200_OK && blocks > 1) {
-    route_rank_kernel<<<blocks, kRouteThreads, smem, stream>>>(a);
-    st = launched();
+    st = launch(route_rank_kernel, blocks, kRouteThreads, smem, stream, a);
   }
   if (counts) cudaFreeAsync(counts, stream);
   return st;
@@ -511,11 +549,10 @@ int launch_move(Move what, const MoveArgs& a, cudaStream_t stream) {
   const long long lanes = ceil_div(a.width, kVec);
   const int threads = lanes >= 256 ? 256 : (int)(lanes < 32 ? 32 : (lanes + 31) / 32 * 32);
   switch (what) {
-    case kDispatch: dispatch_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
-    case kCombine: combine_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
-    default: combine_grad_kernel<T, kVec><<<a.tokens, threads, 0, stream>>>(a); break;
+    case kDispatch: return launch(dispatch_kernel<T, kVec>, a.tokens, threads, 0, stream, a);
+    case kCombine: return launch(combine_kernel<T, kVec>, a.tokens, threads, 0, stream, a);
+    default: return launch(combine_grad_kernel<T, kVec>, a.tokens, threads, 0, stream, a);
   }
-  return launched();
 }
 
 int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
@@ -662,9 +699,9 @@ int b200_route_grad(const void* logits, int tokens, int experts, long long ld, i
   MoeDevice* m = nullptr;
   const int st = moe_device(&v, &m);
   if (st != B200_OK) return st;
-  route_grad_kernel<<<(unsigned)ceil_div(tokens, 8), 256, 0, static_cast<cudaStream_t>(stream)>>>(
-      logits, ld, type, chosen, weights, dweights, dlogits, tokens, experts, top_k, normalize != 0);
-  return launched();
+  return launch(route_grad_kernel, (int)ceil_div(tokens, 8), 256, 0,
+                static_cast<cudaStream_t>(stream), logits, ld, type, chosen, weights, dweights,
+                dlogits, tokens, experts, top_k, normalize != 0);
 }
 
 int b200_dispatch(const void* x, const int* rows, const int* total, void* xs, int tokens, int top_k,

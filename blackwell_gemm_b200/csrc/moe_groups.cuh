@@ -9,6 +9,13 @@
 
 namespace b200 {
 
+// wait_bounded for a barrier that has usually completed already.
+__device__ __forceinline__ bool wait_ready(uint32_t bar, uint32_t parity, const WaitCtx& w,
+                                           int code) {
+  if (mbar_test_wait(bar, parity)) return true;
+  return wait_slow(bar, parity, w, code, true);
+}
+
 constexpr int kMaxExperts = 1024;
 // Device error word: offsets that fall or leave [0, rows] (they are clamped).
 constexpr int kErrOffsets = 0x100A;

@@ -196,6 +196,8 @@ __device__ __forceinline__ void mark_unowned(const RouteArgs& a, int total) {
 // Dynamic shared memory: hist/start [experts], cursor [warps][experts].
 template <int kPer>
 __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const RouteArgs a) {
+  grid_wait();
+  grid_launch_next();
   extern __shared__ int s_route[];
   int* hist = s_route;
   const int first = blockIdx.x * a.chunk;
@@ -219,6 +221,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
 }
 
 __global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteArgs a) {
+  grid_wait();
+  grid_launch_next();
   extern __shared__ int s_route[];
   int* start = s_route;                 // totals, then offsets, then + earlier chunks
   int* earlier = s_route + a.experts;   // (the cursors take this over)
@@ -257,6 +261,8 @@ __global__ void __launch_bounds__(256)
 route_grad_kernel(const void* logits, long long ld, int type, const int* __restrict__ chosen,
                   const float* __restrict__ weights, const float* __restrict__ dweights,
                   void* dlogits, int tokens, int experts, int top_k, bool normalize) {
+  grid_wait();
+  grid_launch_next();
   const int lane = threadIdx.x & 31;
   const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
   if (t >= tokens) return;
@@ -373,6 +379,8 @@ __device__ __forceinline__ void zero_tail(const MoveArgs& a, long long t) {
 
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
+  grid_wait();
+  grid_launch_next();
   __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
@@ -387,6 +395,8 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
 
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
+  grid_wait();
+  grid_launch_next();
   __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
@@ -413,6 +423,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
 // slot (from cache after the first), y once.
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const MoveArgs a) {
+  grid_wait();
+  grid_launch_next();
   __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   __shared__ float s_part[8];

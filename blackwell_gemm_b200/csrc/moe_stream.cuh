@@ -126,21 +126,32 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
       for (int c = 0; c < kTok; ++c)
         if (c < s.rows) __stcg(mine + c * 128, acc[c]);
     }
-    __threadfence();
     __syncwarp();
     unsigned int before = 0;
-    if (lane == 0) before = atomicAdd(a.counts + c0 * 4 + quarter, 1u);
+    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 4 + quarter, 1u);
     before = __shfl_sync(0xffffffffu, before, 0);
     if (before != (unsigned int)(c1 - c0)) return;
-    __threadfence();
+    __syncwarp();
     if (lane == 0) atomicExch(a.counts + c0 * 4 + quarter, 0u);
 #pragma unroll
     for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
-    for (int p = c0; p <= c1; ++p) {
+    // (two parts' loads in flight at a time; added in order)
+    constexpr int kBatch = kTok < 16 ? kTok : 16;
+    for (int p = c0; p <= c1; p += 2) {
       const float* from = slot(p);
+      const float* then = slot(p < c1 ? p + 1 : p);
 #pragma unroll
-      for (int c = 0; c < kTok; ++c)
-        if (c < s.rows) acc[c] += __ldcg(from + c * 128);
+      for (int b = 0; b < kTok; b += kBatch) {
+        float v[kBatch], u[kBatch];
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c) {
+          const bool in = b + c < s.rows;
+          v[c] = in ? __ldcg(from + (b + c) * 128) : 0.0f;
+          u[c] = in && p < c1 ? __ldcg(then + (b + c) * 128) : 0.0f;
+        }
+#pragma unroll
+        for (int c = 0; c < kBatch; ++c) acc[b + c] = (acc[b + c] + v[c]) + u[c];
+      }
     }
   }
   if (!valid || f >= a.feat) return;
@@ -210,10 +221,12 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
     tmem_alloc_1(smem_u32(&tmem_slot), kCols);
     tmem_relinquish_1();
   }
+  grid_wait();
   if (warp == 2) stream_groups(args, kTok, s_off, s_tiles);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  grid_launch_next();
   const uint32_t tmem_base = tmem_slot;
 
   WaitCtx wctx;
@@ -233,7 +246,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
       bool ok = true;
       while (ok && walk.next(&s)) {
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          if (!wait_bounded(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
+          if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
             ok = false;
             break;
           }
@@ -266,12 +279,12 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
             make_idesc_16bit(128, (s.rows + 15) & ~15, kFormat<T>, kDA, false);
         const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
         ++it;
-        if (!wait_bounded(smem_u32(&bar_acc_empty[buf]), acc_phase ^ 1u, wctx, kErrWaitAccEmpty))
+        if (!wait_ready(smem_u32(&bar_acc_empty[buf]), acc_phase ^ 1u, wctx, kErrWaitAccEmpty))
           break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * kTok;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          if (!wait_bounded(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)) {
+          if (!wait_ready(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)) {
             ok = false;
             break;
           }
@@ -306,7 +319,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
       ++it;
       if (ok) {
         if (lane == 0)
-          ok = wait_bounded(smem_u32(&bar_acc_full[buf]), acc_phase, wctx, kErrWaitAccFull);
+          ok = wait_ready(smem_u32(&bar_acc_full[buf]), acc_phase, wctx, kErrWaitAccFull);
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       tc_fence_after_sync();

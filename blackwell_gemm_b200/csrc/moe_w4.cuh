@@ -16,15 +16,17 @@
 // Weights are laid out once (w4_pack_kernel) in records of 128 rows x 128 k,
 // in the order a CTA walks them, so a record is one bulk copy and a CTA's
 // whole share one sequential read:
-//   8192 B  q: [4][128 rows][16 B], 32 k in 16 B; in a word the nibbles of
-//           k = 0, 2, 4, 6 fill the low half and 1, 3, 5, 7 the high half,
-//           so one shift and one mask give a pair in order
+//   8192 B  q: [4 t][128 rows][4 c] words, a word being k = 32 c + 8 t .. + 7:
+//           its nibbles k = 0, 2, 4, 6 fill the low half and 1, 3, 5, 7 the
+//           high half, so one mask gives a pair in order; row r of t stands
+//           at place r ^ 2 t (w4_q_offset)
 //   scales  [128 / G][128 rows], 16-bit
 //   zeros   [128 / G][128 rows], 8-bit, when there are any
 //
 // Work is divided as in moe_stream.cuh (items are records).  Warps: 0 bulk
-// and TMA copies, 1 MMA, 2-5 and 6-9 two sets of unpackers that take
-// records in turn; a set unpacks record j + 1 while the MMA works on j.
+// and TMA copies, 1 MMA, 2-9 two sets that take the products of every other
+// record (and finish tiles), 10-17 two sets that unpack every other one.  Several records' weights and
+// products are in TMEM at a time, so the three stages run beside one another.
 #pragma once
 #include "moe_stream.cuh"
 
@@ -36,70 +38,381 @@ __host__ __device__ constexpr int w4_record_bytes(int group, bool zeros) {
   return kW4Q + kW4K / group * kW4Rows * (zeros ? 3 : 2);
 }
 
-template <int kTok, int kGroup>
-struct W4Cfg {
-  static constexpr int kSub = kW4K / kGroup;       // groups per record
-  static_assert(kTok * kSub <= 128, "a set's products fill at most 128 TMEM columns");
-  static constexpr int kTokens = 2 * kTok * 128;   // two 64-k slabs of the token operand
-  static constexpr int kRecord = (w4_record_bytes(kGroup, true) + 1023) / 1024 * 1024;
-  static constexpr int kStageBytes = kTokens + kRecord;
-  static constexpr int kExchange = kTok * 128 * 4;
-  static constexpr int kStages = (214 * 1024 - kExchange) / kStageBytes < 16
-                                     ? (214 * 1024 - kExchange) / kStageBytes
-                                     : 16;
-  static constexpr int kThreads = 320;
-  static constexpr int smem_bytes(int experts) {
-    return kStages * kStageBytes + kExchange + group_table_bytes(experts) + 1024;
-  }
-};
+// Bytes from a record's start to row `row`'s 16 bytes of part t.  The order of
+// the rows lets both ways of reading use all banks: 32 rows of one t, or 8
+// rows of four.
+__host__ __device__ constexpr uint32_t w4_q_offset(int t, int row) {
+  return (uint32_t)(t * 2048 + ((row * 16) ^ (t * 32)));
+}
 
-// Pairs of 4-bit values (low and high half of `v`, already shifted) as 16-bit
-// floats: the nibble set into the mantissa of 2^7 (bf16) or 2^10 (f16) gives
-// that power plus q; both the sum and the difference taken from it are exact.
+// Unpacking.  The logic pipe takes a warp's instruction every other cycle and
+// limits this kernel, so a pair of 4-bit values costs one mask and half a
+// shift there; the rest is one fused multiply-add on the other pipe.  A
+// nibble at bits 0-3 or 4-7 of a 16-bit float is a subnormal (or, with bit 7
+// of a bf16, a number of the first binade, which has the same spacing): the
+// bits n stand for n 2^-133 (bf16) or n 2^-24 (f16).  Times a power of two
+// that is (q - z) kUnit, exactly; the sums are scaled back by 1 / kUnit.
 template <class T>
-struct W4Magic;
+struct W4Unpack;
 template <>
-struct W4Magic<__nv_bfloat16> {
-  static constexpr uint32_t kBits = 0x43004300u;
-  static __device__ __forceinline__ uint32_t bias(uint32_t z) { return (0x4300u + z) * 0x10001u; }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+struct W4Unpack<__nv_bfloat16> {
+  static constexpr float kUnit = 1.0f / 64;        // 2^-133 x 2^127
+  static constexpr uint32_t kLow = 0x7F007F00u;    // 2^127
+  static constexpr uint32_t kHigh = 0x7D007D00u;   // 2^123: bits 4-7 count 16
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t m, uint32_t b) {
+    const __nv_bfloat162 r = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&a),
+                                     *reinterpret_cast<const __nv_bfloat162*>(&m),
                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  static __device__ __forceinline__ uint32_t bias(uint32_t z) {
+    // -z / 64 in bf16: exact (z has four bits)
+    return pack_pair<__nv_bfloat16>(-kUnit * (float)z, -kUnit * (float)z);
+  }
   static __device__ __forceinline__ float wide(uint16_t s) {
-    return __uint_as_float((uint32_t)s << 16);
+    return __uint_as_float((uint32_t)s << 16) * (1.0f / kUnit);
   }
 };
 template <>
-struct W4Magic<__half> {
-  static constexpr uint32_t kBits = 0x64006400u;
-  static __device__ __forceinline__ uint32_t bias(uint32_t z) { return (0x6400u + z) * 0x10001u; }
-  static __device__ __forceinline__ uint32_t sub(uint32_t a, uint32_t b) {
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&a),
+struct W4Unpack<__half> {
+  static constexpr float kUnit = 1.0f / 512;       // 2^-24 x 2^15
+  static constexpr uint32_t kLow = 0x78007800u;    // 2^15
+  static constexpr uint32_t kHigh = 0x68006800u;   // 2^11
+  static __device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t m, uint32_t b) {
+    const __half2 r = __hfma2(*reinterpret_cast<const __half2*>(&a),
+                              *reinterpret_cast<const __half2*>(&m),
                               *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
+  static __device__ __forceinline__ uint32_t bias(uint32_t z) {
+    return pack_pair<__half>(-kUnit * (float)z, -kUnit * (float)z);
+  }
   static __device__ __forceinline__ float wide(uint16_t s) {
-    return __half2float(*reinterpret_cast<const __half*>(&s));
+    return __half2float(*reinterpret_cast<const __half*>(&s)) * (1.0f / kUnit);
   }
 };
 
-// tmap_t: the token operand (k, r), box 64 x 16.
-template <int kTok, int kGroup, class T>
-__global__ void __launch_bounds__(W4Cfg<kTok, kGroup>::kThreads, 1)
-w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args,
-                 const bool has_zeros) {
-  using C = W4Cfg<kTok, kGroup>;
-  using M = W4Magic<T>;
+// The eight weights of a word, k ascending, two to a register.
+template <class T>
+__device__ __forceinline__ void w4_pairs(uint32_t w, uint32_t bias, uint32_t* o) {
+  using U = W4Unpack<T>;
+  const uint32_t v = w >> 8;
+  o[0] = U::fma2(w & 0x000F000Fu, U::kLow, bias);
+  o[1] = U::fma2(w & 0x00F000F0u, U::kHigh, bias);
+  o[2] = U::fma2(v & 0x000F000Fu, U::kLow, bias);
+  o[3] = U::fma2(v & 0x00F000F0u, U::kHigh, bias);
+}
+
+// D += A B^T for 16 weight rows, 8 tokens, 16 k, in registers.
+template <class T>
+__device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                            uint32_t b1);
+template <>
+__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
+                                                           uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&a)[4],
+                                                    uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A ring stage holds up to two consecutive records of a segment (one bulk
+// copy) and the four 64-k slabs of the tile's tokens that go with them (one
+// TMA box): the producing thread shares its scheduler with busy warps, and
+// with a record and two boxes at a time it fell behind HBM (630 cycles a
+// record).
+template <int kTok, int kGroup>
+struct W4Ring {
+  static constexpr int kSub = kW4K / kGroup;               // groups per record
+  static constexpr int kSlabRows = kTok;                   // rows of a token box
+  static constexpr int kSlab = kSlabRows * 128;
+  static constexpr int kTokens = 4 * kSlab;
+  static constexpr int kStageBytes =
+      kTokens + (2 * w4_record_bytes(kGroup, true) + 1023) / 1024 * 1024;
+  static constexpr int stages(int other) {
+    return (214 * 1024 - other) / kStageBytes < 8 ? (214 * 1024 - other) / kStageBytes : 8;
+  }
+};
+
+// tmap_t: with K a multiple of 64, the token operand as (k in a slab, row,
+// slab), box 64 x kSlabRows x 4; else (k, row), box 64 x kSlabRows.
+template <int kTok, int kGroup, int kStages>
+__device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kTok> walk,
+                                           const CUtensorMap* tmap_t, uint32_t ring, uint32_t full,
+                                           uint32_t empty, const WaitCtx& wctx) {
+  using R = W4Ring<kTok, kGroup>;
+  const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
+  const bool slabs = args.red % kSlabK == 0;
+  uint32_t stage = 0, phase = 0;
+  StreamSegment s;
+  while (walk.next(&s)) {
+    const uint8_t* record = args.packed + (long long)s.e * args.expert_bytes +
+                            ((long long)s.block * args.red_blocks + s.kb0) * args.record_bytes;
+    for (int kb = s.kb0; kb < s.kb1; kb += 2) {
+      const uint32_t fb = full + stage * 8u;
+      const uint32_t sa = ring + stage * R::kStageBytes;
+      const uint32_t bytes = kb + 1 < s.kb1 ? 2 * args.record_bytes : args.record_bytes;
+      if (!wait_ready(empty + stage * 8u, phase ^ 1u, wctx, kErrWaitEmpty)) return;
+      mbar_arrive_expect_tx(fb, bytes + R::kTokens);
+      bulk_load_hint(sa + R::kTokens, record, bytes, fb, once);
+      if (slabs) {
+        tma_load_3d_hint(sa, tmap_t, 0, s.row0, 2 * kb, fb, keep);
+      } else {
+        for (int j = 0; j < 4; ++j)
+          tma_load_2d_hint(sa + j * R::kSlab, tmap_t, kb * kW4K + 64 * j, s.row0, fb, keep);
+      }
+      record += bytes;
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    }
+  }
+}
+
+// Few rows (at most 16 to a tile): unpacked weights go straight from
+// registers into warp-level MMAs.  A record then costs about 840 warp
+// instructions, where the way through TMEM takes 1780 (stores, loads and the
+// handshakes between its stages), and with so few tokens the tensor core's
+// rate does not matter.  Sixteen warps, four to a record: stage i's two records
+// go to groups 2 (i % 2) and 2 (i % 2) + 1, and of each a warp takes 32 rows.
+// Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
+// lets eight lanes read all banks of the swizzled token slab.
+template <int kTok, int kGroup>
+struct W4RowsCfg {
+  using Ring = W4Ring<kTok, kGroup>;
+  static constexpr int kPitch = 136;  // floats from token to token of the exchange
+  static constexpr int kExchange = 4 * kTok * kPitch * 4;
+  static constexpr int kStages = Ring::stages(kExchange) & ~1;  // a stage has its two groups
+  static constexpr int kThreads = 32 * 17;
+  static constexpr int smem_bytes(int experts) {
+    return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;
+  }
+};
+
+template <int kTok, int kGroup, bool kZeros, class T>
+__global__ void __launch_bounds__(W4RowsCfg<kTok, kGroup>::kThreads, 1)
+w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args) {
+  using C = W4RowsCfg<kTok, kGroup>;
+  using R = typename C::Ring;
+  using U = W4Unpack<T>;
   constexpr int kStages = C::kStages;
-  constexpr int kSub = C::kSub;
+  constexpr int kSub = R::kSub;
+  constexpr int kNt = kTok / 8;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t bar_full[kStages];
   __shared__ alignas(8) uint64_t bar_empty[kStages];
-  __shared__ alignas(8) uint64_t bar_a_full[2][2];  // [set][buffer]: unpacked weights in TMEM
-  __shared__ alignas(8) uint64_t bar_d_full[2];     // [set]: products in TMEM
-  __shared__ alignas(8) uint64_t bar_d_empty[2];
+  __shared__ uint32_t abort_word;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
+  const int lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t exchange = smem_base + kStages * R::kStageBytes;
+  int* s_off = reinterpret_cast<int*>(smem_raw + (exchange + C::kExchange - smem_u32(smem_raw)));
+  int* s_tiles = s_off + args.experts + 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 8);  // the two groups' warps
+    }
+    abort_word = 0;
+    fence_mbar_init_cluster();
+    prefetch_tmap(&tmap_t);
+  }
+  grid_wait();
+  if (warp == 1) stream_groups(args, kTok, s_off, s_tiles);
+  __syncthreads();
+  grid_launch_next();
+
+  WaitCtx wctx;
+  wctx.status = args.status;
+  wctx.timeout_ns = args.timeout_ns;
+  wctx.abort_local = smem_u32(&abort_word);
+  wctx.abort_peer = cluster_map(smem_u32(&abort_word), 0);
+
+  StreamWalk<kTok> walk;
+  walk.init(args, s_off, s_tiles);
+  StreamSegment s;
+
+  if (warp == 16) {
+    if (elect_one()) {
+      w4_produce<kTok, kGroup, kStages>(args, walk, &tmap_t, smem_base, smem_u32(&bar_full[0]),
+                                        smem_u32(&bar_empty[0]), wctx);
+    }
+    __syncwarp();
+    return;
+  }
+  const int g = lane >> 2, t = lane & 3;
+  const int row = (warp & 3) * 32 + g;  // + 0, 8 (first 16 rows), 16, 24 (second)
+  const uint32_t group = warp >> 2;
+  const int token = (g >> 1) + 4 * (g & 1);  // of column g of each eight
+  // bytes of this lane's token row in a slab; 16-byte chunk c at c ^ token
+  const uint32_t token_row = token * 128;
+  zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
+                    s_off[args.experts], args.rows,
+                    (long long)blockIdx.x * 512 + threadIdx.x, gridDim.x * 512ll);
+  // This group's stages: every other one, from group / 2.
+  uint32_t next = 0, stage = group >> 1, phase = 0;
+  const uint32_t second = group & 1;
+  bool ok = true;
+  while (walk.next(&s)) {
+    float acc[2][kNt][4];
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
+    for (int kb = s.kb0; ok && kb < s.kb1; kb += 2) {
+      const bool mine = next == group >> 1;
+      next ^= 1u;
+      if (!mine) continue;
+      const uint32_t bar = smem_u32(&bar_full[stage]), done = smem_u32(&bar_empty[stage]);
+      const uint32_t tokens = smem_base + stage * R::kStageBytes + second * 2 * R::kSlab;
+      const uint32_t record =
+          smem_base + stage * R::kStageBytes + R::kTokens + second * args.record_bytes;
+      const uint32_t parity = phase;
+      stage += 2;
+      if (stage >= kStages) { stage -= kStages; phase ^= 1u; }
+      if (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) {
+        int got = 0;
+        if (lane == 0) got = wait_ready(bar, parity, wctx, kErrWaitFull);
+        ok = __shfl_sync(0xffffffffu, got, 0) != 0;
+        __syncwarp();
+        if (!ok) break;
+      }
+      if (kb + (int)second >= s.kb1) {  // the segment's last stage holds one record
+        if (lane == 0) mbar_arrive_local(done);
+        continue;
+      }
+      uint32_t q[4][4];  // [row][c]
+#pragma unroll
+      for (int r = 0; r < 4; ++r) ld_shared_v4_u32(record + w4_q_offset(t, row + 8 * r), q[r]);
+      float part[2][kNt][4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        constexpr int kPer = kGroup / 32;  // words to a group
+        const int sub = c / kPer;
+        uint32_t x[kNt][4];
+#pragma unroll
+        for (int n = 0; n < kNt; ++n)
+          ld_shared_v4_u32(tokens + (c >> 1) * R::kSlab + n * 1024 + token_row +
+                               ((((c & 1) * 4 + t) ^ token) << 4),
+                           x[n]);
+        if (c % kPer == 0) {
+#pragma unroll
+          for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < kNt; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) part[m][n][i] = 0.0f;
+        }
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          uint32_t lo[4], hi[4];
+          uint32_t z0 = 8, z1 = 8;
+          if constexpr (kZeros) {
+            const uint32_t zeros = record + kW4Q + kSub * 256 + sub * 128 + row + 16 * m;
+            z0 = ld_shared_u8(zeros);
+            z1 = ld_shared_u8(zeros + 8);
+          }
+          w4_pairs<T>(q[2 * m][c], U::bias(z0), lo);
+          w4_pairs<T>(q[2 * m + 1][c], U::bias(z1), hi);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t a[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
+#pragma unroll
+            for (int n = 0; n < kNt; ++n)
+              mma_16x8x16<T>(part[m][n], a, x[n][2 * h], x[n][2 * h + 1]);
+          }
+        }
+        if (c % kPer == kPer - 1) {
+          const uint32_t scales = record + kW4Q + (sub * 128 + row) * 2;
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const float s0 = U::wide(ld_shared_u16(scales + 32 * m));
+            const float s1 = U::wide(ld_shared_u16(scales + 32 * m + 16));
+#pragma unroll
+            for (int n = 0; n < kNt; ++n)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                acc[m][n][i] = fmaf(i < 2 ? s0 : s1, part[m][n][i], acc[m][n][i]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive_local(done);
+    }
+    // The four groups' sums meet in shared memory; warps 0-3 finish the tile,
+    // lane = row.
+    float* sums = reinterpret_cast<float*>(smem_raw + (exchange - smem_u32(smem_raw)));
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int n = 0; n < kNt; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          sums[(group * kTok + n * 8 + t + 4 * (i & 1)) * C::kPitch + row + 16 * m + 8 * (i >> 1)] =
+              acc[m][n][i];
+    named_bar_sync(1, 512);
+    float total[kTok];
+    if (warp < 4) {
+#pragma unroll
+      for (int c = 0; c < kTok; ++c) {
+        const float* from = sums + c * C::kPitch + warp * 32 + lane;
+        total[c] = (from[0] + from[kTok * C::kPitch]) +
+                   (from[2 * kTok * C::kPitch] + from[3 * kTok * C::kPitch]);
+      }
+    }
+    named_bar_sync(1, 512);
+    if (warp < 4) {
+      const bool valid = __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
+      stream_finish<kTok, T>(args, walk, s, warp, total, valid);
+    }
+  }
+}
+
+// More rows: through TMEM, 64 tokens to a tile (32 where the groups are of 32).
+template <int kTok, int kGroup>
+struct W4Cfg {
+  using Ring = W4Ring<kTok, kGroup>;
+  // TMEM: kProducts records' products and kWeights records' unpacked weights.
+  static constexpr int kProductCols = kTok * Ring::kSub;
+  static constexpr int kProducts = kProductCols >= 128 ? 2 : kProductCols >= 64 ? 3 : 4;
+  static constexpr int kFree = (kTmemCols - kProducts * kProductCols) / 64;
+  static constexpr int kWeights = kFree < 6 ? kFree : 6;
+  static_assert(kWeights >= kProducts, "a product's barrier is its weights'");
+  static constexpr int kExchange = kTok * 128 * 4;
+  static constexpr int kStages = Ring::stages(kExchange + 8192);
+  static constexpr int kThreads = 32 * (2 + 8 + 8);
+  static constexpr int smem_bytes(int experts) {
+    return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;
+  }
+};
+
+// tmap_t: as w4_produce takes it.
+template <int kTok, int kGroup, bool kZeros, class T>
+__global__ void __launch_bounds__(W4Cfg<kTok, kGroup>::kThreads, 1)
+w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args) {
+  using C = W4Cfg<kTok, kGroup>;
+  using R = typename C::Ring;
+  using U = W4Unpack<T>;
+  constexpr int kStages = C::kStages;
+  constexpr int kSub = R::kSub;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ alignas(8) uint64_t bar_full[kStages];
+  __shared__ alignas(8) uint64_t bar_empty[kStages];
+  __shared__ alignas(8) uint64_t bar_a_full[C::kWeights];   // weights unpacked into TMEM
+  __shared__ alignas(8) uint64_t bar_done[C::kWeights];     // their MMAs are done
+  __shared__ alignas(8) uint64_t bar_taken[C::kProducts];   // products taken
   __shared__ alignas(8) uint64_t bar_drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
@@ -107,21 +420,20 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t exchange = smem_base + kStages * C::kStageBytes;
+  const uint32_t exchange = smem_base + kStages * R::kStageBytes;
   int* s_off = reinterpret_cast<int*>(smem_raw + (exchange + C::kExchange - smem_u32(smem_raw)));
   int* s_tiles = s_off + args.experts + 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 5);  // a set's four warps, and the MMA that read the tokens
+      mbar_init(smem_u32(&bar_empty[s]), 16);  // the unpackers, and those who take products
     }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(smem_u32(&bar_a_full[s][0]), 4);
-      mbar_init(smem_u32(&bar_a_full[s][1]), 4);
-      mbar_init(smem_u32(&bar_d_full[s]), 1);
-      mbar_init(smem_u32(&bar_d_empty[s]), 4);
+    for (int b = 0; b < C::kWeights; ++b) {
+      mbar_init(smem_u32(&bar_a_full[b]), 4);
+      mbar_init(smem_u32(&bar_done[b]), 1);
     }
+    for (int b = 0; b < C::kProducts; ++b) mbar_init(smem_u32(&bar_taken[b]), 4);
     mbar_init(smem_u32(&bar_drain), 1);
     abort_word = 0;
     fence_mbar_init_cluster();
@@ -131,13 +443,14 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
     tmem_alloc_1(smem_u32(&tmem_slot), kTmemCols);
     tmem_relinquish_1();
   }
+  grid_wait();
   if (warp == 2) stream_groups(args, kTok, s_off, s_tiles);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  grid_launch_next();
   const uint32_t tmem_base = tmem_slot;
-  // TMEM columns: weights [set][buffer] 64 each, then products [set] 128 each
-  const uint32_t tmem_d = tmem_base + 256;
+  const uint32_t tmem_d = tmem_base + C::kWeights * 64;
 
   WaitCtx wctx;
   wctx.status = args.status;
@@ -151,61 +464,44 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
 
   if (warp == 0) {
     if (elect_one()) {
-      const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
-      uint32_t stage = 0, phase = 0;
-      bool ok = true;
-      while (ok && walk.next(&s)) {
-        const uint8_t* records = args.packed + (long long)s.e * args.expert_bytes +
-                                 (long long)s.block * args.red_blocks * args.record_bytes;
-        const int boxes = (s.rows + 15) / 16;
-        for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          if (!wait_bounded(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
-            ok = false;
-            break;
-          }
-          const uint32_t fb = smem_u32(&bar_full[stage]);
-          const uint32_t sa = smem_base + stage * C::kStageBytes;
-          mbar_arrive_expect_tx(fb, args.record_bytes + boxes * 2 * 16 * 128);
-          bulk_load_hint(sa + C::kTokens, records + (long long)kb * args.record_bytes,
-                         args.record_bytes, fb, once);
-          for (int i = 0; i < boxes; ++i) {
-            tma_load_2d_hint(sa + i * 16 * 128, &tmap_t, kb * kW4K, s.row0 + i * 16, fb, keep);
-            tma_load_2d_hint(sa + (kTok + i * 16) * 128, &tmap_t, kb * kW4K + 64, s.row0 + i * 16,
-                             fb, keep);
-          }
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
-        }
-      }
+      w4_produce<kTok, kGroup, kStages>(args, walk, &tmap_t, smem_base, smem_u32(&bar_full[0]),
+                                        smem_u32(&bar_empty[0]), wctx);
     }
     __syncwarp();
   } else if (warp == 1) {
     if (elect_one()) {
       uint32_t stage = 0, phase = 0;
-      uint32_t item = 0;
+      uint32_t w = 0, wp = 0, p = 0, pp = 1;  // places in TMEM and their phases
       bool ok = true;
       while (ok && walk.next(&s)) {
         const uint32_t idesc = make_idesc_16bit(128, (s.rows + 15) & ~15, kFormat<T>, false, false);
-        for (int kb = s.kb0; kb < s.kb1; ++kb, ++item) {
-          const uint32_t set = item & 1, j = item >> 1, buf = j & 1;
-          if (!wait_bounded(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull) ||
-              !wait_bounded(smem_u32(&bar_a_full[set][buf]), (j >> 1) & 1, wctx, kErrWaitFull) ||
-              !wait_bounded(smem_u32(&bar_d_empty[set]), (j & 1) ^ 1, wctx, kErrWaitAccEmpty)) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          const uint32_t full = smem_u32(&bar_full[stage]), unpacked = smem_u32(&bar_a_full[w]),
+                         taken = smem_u32(&bar_taken[p]);
+          const bool r0 = mbar_test_wait(full, phase), r1 = mbar_test_wait(unpacked, wp),
+                     r2 = mbar_test_wait(taken, pp);
+          if (!(r0 && r1 && r2) && (!wait_ready(full, phase, wctx, kErrWaitFull) ||
+                                    !wait_ready(taken, pp, wctx, kErrWaitAccEmpty) ||
+                                    !wait_ready(unpacked, wp, wctx, kErrWaitFull))) {
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t sx = smem_base + stage * C::kStageBytes;
-          const uint32_t a = tmem_base + (set * 2 + buf) * 64;
-          const uint32_t d = tmem_d + set * 128;
+          const uint64_t bdesc =
+              make_sdesc_k128(smem_base + stage * R::kStageBytes + ((kb - s.kb0) & 1) * 2 * R::kSlab);
+          const uint32_t a = tmem_base + w * 64;
+          const uint32_t d = tmem_d + p * C::kProductCols;
 #pragma unroll
-          for (int k = 0; k < kW4K / kMmaK; ++k) {
-            const uint64_t bdesc = make_sdesc_k128(sx + (k >> 2) * kTok * 128) + 2ull * (k & 3);
-            umma_tmem_a_1(d + k * kMmaK / kGroup * kTok, a + k * 8, bdesc, idesc,
+          for (int k = 0; k < kW4K / kMmaK; ++k)
+            umma_tmem_a_1(d + k * kMmaK / kGroup * kTok, a + k * 8,
+                          bdesc + ((k >> 2) * R::kSlab + (k & 3) * 32) / 16, idesc,
                           k * kMmaK % kGroup != 0 ? 1u : 0u);
+          umma_commit_1(smem_u32(&bar_done[w]));
+          if (++w == C::kWeights) { w = 0; wp ^= 1u; }
+          if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+          if (((kb - s.kb0) & 1) != 0 || kb + 1 == s.kb1) {
+            if (++stage == kStages) { stage = 0; phase ^= 1u; }
           }
-          umma_commit_1(smem_u32(&bar_empty[stage]));
-          umma_commit_1(smem_u32(&bar_d_full[set]));
-          if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
       umma_commit_1(smem_u32(&bar_drain));
@@ -214,120 +510,141 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
     }
     __syncwarp();
   } else {
-    const int set = (warp - 2) >> 2;
     const int quarter = warp & 3;
     const int row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
-                      s_off[args.experts], args.rows,
-                      (long long)blockIdx.x * 256 + (threadIdx.x - 64), gridDim.x * 256ll);
-    uint32_t item = 0;  // records this CTA has passed; this set takes every other one
-    bool ok = true;
+    // All lanes look at once (one instruction, one answer); lane 0 waits.
     auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) {
+      if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
       int got = 0;
-      if (lane == 0) got = wait_bounded(bar, parity, wctx, code);
+      if (lane == 0) got = wait_ready(bar, parity, wctx, code);
       got = __shfl_sync(0xffffffffu, got, 0);
       __syncwarp();
       return got != 0;
     };
-    while (walk.next(&s)) {
-      float acc[kTok];
-#pragma unroll
-      for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
-      float scale[kSub];      // of the record whose products are still to be taken
-      bool pending = false;
-      uint32_t pending_j = 0;
-      // Products of record j times their scales into the running sums.
-      auto fold = [&]() {
-        if (!wait_warp(smem_u32(&bar_d_full[set]), pending_j & 1, kErrWaitAccFull)) {
-          ok = false;
-          return;
-        }
-        tc_fence_after_sync();
-#pragma unroll
-        for (int g = 0; g < kSub; ++g) {
-#pragma unroll
-          for (int c = 0; c < kTok; c += 16) {
-            if (c < s.rows) {
-              uint32_t v[16];
-              tmem_ld_32x32b_x16(tmem_d + set * 128 + g * kTok + c + lanes, v);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i)
-                acc[c + i] = fmaf(scale[g], __uint_as_float(v[i]), acc[c + i]);
+    // The stage and the places in TMEM of the next pair of records, and their
+    // phases.  Set 0 takes a pair's first record, set 1 its second.
+    uint32_t stage = 0, phase = 0, w = 0, wp = 0, p = 0;
+    auto next_place = [&]() {
+      if (++w == C::kWeights) { w = 0; wp ^= 1u; }
+      if (++p == C::kProducts) p = 0;
+    };
+    auto next_stage = [&]() {
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+    };
+    const uint32_t set = ((uint32_t)(warp - 2) >> 2) & 1u;
+    bool ok = true;
+    if (warp >= 10) {
+      // ----------------------------------------------------------- unpack
+      while (ok && walk.next(&s)) {
+        for (int kb = s.kb0; kb < s.kb1; kb += 2, next_stage()) {
+          const bool pair = kb + 1 < s.kb1;
+          if (set == 1) {
+            next_place();
+            if (!pair) {  // nothing to unpack; the stage still counts this warp
+              if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+              continue;
             }
           }
-        }
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_local(smem_u32(&bar_d_empty[set]));
-      };
-      for (int kb = s.kb0; kb < s.kb1; ++kb, ++item) {
-        if ((int)(item & 1) != set || !ok) continue;
-        const uint32_t stage = item % kStages, phase = (item / kStages) & 1;
-        const uint32_t j = item >> 1, buf = j & 1;
-        if (!wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull)) {
-          ok = false;
-          continue;
-        }
-        const uint32_t record = smem_base + stage * C::kStageBytes + C::kTokens;
-        float next_scale[kSub];
-        uint32_t bias[kSub];
+          ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull) &&
+               wait_warp(smem_u32(&bar_done[w]), wp ^ 1u, kErrWaitAccEmpty);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t record =
+              smem_base + stage * R::kStageBytes + R::kTokens + set * args.record_bytes;
+          uint32_t bias[kSub];
 #pragma unroll
-        for (int g = 0; g < kSub; ++g) {
-          next_scale[g] = M::wide(ld_shared_u16(record + kW4Q + (g * 128 + row) * 2));
-          bias[g] = M::bias(
-              has_zeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
-        }
-        // (this buffer's last MMA was record j - 2, whose products this warp
-        // has already taken)
+          for (int g = 0; g < kSub; ++g)
+            bias[g] = U::bias(
+                kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
+          uint32_t q[4][4];  // [t][c]
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          uint32_t r[32];
+          for (int t = 0; t < 4; ++t) ld_shared_v4_u32(record + w4_q_offset(t, row), q[t]);
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t w[4];
-            ld_shared_v4_u32(record + (2 * h + c) * 2048 + row * 16, w);
-            const uint32_t b = bias[(2 * h + c) * 32 / kGroup];
+          for (int h = 0; h < 2; ++h) {
+            uint32_t r[32];
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
+            for (int c = 0; c < 2; ++c)
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                r[c * 16 + q * 4 + i] =
-                    M::sub(((w[q] >> (4 * i)) & 0x000F000Fu) | M::kBits, b);
+              for (int t = 0; t < 4; ++t)
+                w4_pairs<T>(q[t][2 * h + c], bias[(2 * h + c) * 32 / kGroup], r + c * 16 + t * 4);
+            tmem_st_32x32b_x32(tmem_base + w * 64 + h * 32 + lanes, r);
           }
-          tmem_st_32x32b_x32(tmem_base + (set * 2 + buf) * 64 + h * 32 + lanes, r);
+          __syncwarp();
+          if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_local(smem_u32(&bar_a_full[w]));
+          next_place();
+          if (set == 0 && pair) next_place();
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
-        tmem_wait_st();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_local(smem_u32(&bar_a_full[set][buf]));
-        if (pending) fold();
-#pragma unroll
-        for (int g = 0; g < kSub; ++g) scale[g] = next_scale[g];
-        pending = true;
-        pending_j = j;
       }
-      if (pending && ok) fold();
-      // The second set hands its sums to the first, which finishes the tile.
+    } else {
+      // --------------------------------------------------- products, finish
+      zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
+                        s_off[args.experts], args.rows,
+                        (long long)blockIdx.x * 256 + (threadIdx.x - 64), gridDim.x * 256ll);
       float* sums = reinterpret_cast<float*>(smem_raw + (exchange - smem_u32(smem_raw))) + row;
-      if (set == 1) {
+      while (walk.next(&s)) {
+        float acc[kTok];
 #pragma unroll
-        for (int c = 0; c < kTok; ++c)
-          if (c < s.rows) sums[c * 128] = acc[c];
-        named_bar_sync(1 + quarter, 64);
-        named_bar_sync(1 + quarter, 64);
-      } else {
-        named_bar_sync(1 + quarter, 64);
+        for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
+        for (int kb = s.kb0; ok && kb < s.kb1; kb += 2, next_stage()) {
+          const bool pair = kb + 1 < s.kb1;
+          if (set == 1) {
+            next_place();
+            if (!pair) {
+              if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+              continue;
+            }
+          }
+          ok = wait_warp(smem_u32(&bar_done[w]), wp, kErrWaitAccFull);
+          if (!ok) break;
+          tc_fence_after_sync();
+          const uint32_t scales = smem_base + stage * R::kStageBytes + R::kTokens +
+                                  set * args.record_bytes + kW4Q + row * 2;
 #pragma unroll
-        for (int c = 0; c < kTok; ++c)
-          if (c < s.rows) acc[c] += sums[c * 128];
-        named_bar_sync(1 + quarter, 64);
-        const bool valid =
-            __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
-        stream_finish<kTok, T>(args, walk, s, quarter, acc, valid);
+          for (int g = 0; g < kSub; ++g) {
+            const float scale = U::wide(ld_shared_u16(scales + g * 256));
+#pragma unroll
+            for (int c = 0; c < kTok; c += 16) {
+              if (c < s.rows) {
+                uint32_t v[16];
+                tmem_ld_32x32b_x16(tmem_d + p * C::kProductCols + g * kTok + c + lanes, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                  acc[c + i] = fmaf(scale, __uint_as_float(v[i]), acc[c + i]);
+              }
+            }
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive_local(smem_u32(&bar_taken[p]));
+            mbar_arrive_local(smem_u32(&bar_empty[stage]));
+          }
+          next_place();
+          if (set == 0 && pair) next_place();
+        }
+        // The second set hands its sums to the first, which finishes the tile.
+        if (set == 1) {
+#pragma unroll
+          for (int c = 0; c < kTok; ++c)
+            if (c < s.rows) sums[c * 128] = acc[c];
+          named_bar_sync(1 + quarter, 64);
+          named_bar_sync(1 + quarter, 64);
+        } else {
+          named_bar_sync(1 + quarter, 64);
+#pragma unroll
+          for (int c = 0; c < kTok; ++c)
+            if (c < s.rows) acc[c] += sums[c * 128];
+          named_bar_sync(1 + quarter, 64);
+          const bool valid =
+              __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
+          stream_finish<kTok, T>(args, walk, s, quarter, acc, valid);
+        }
       }
     }
     __syncwarp();
@@ -347,6 +664,8 @@ __global__ void __launch_bounds__(256)
 w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scales,
                const uint8_t* __restrict__ zeros, uint8_t* __restrict__ out, int N, int K, int group,
                int blocks, int red_blocks, int record_bytes) {
+  grid_wait();
+  grid_launch_next();
   const long long rec = blockIdx.x;
   const int kb = (int)(rec % red_blocks);
   const long long eb = rec / red_blocks;
@@ -368,7 +687,7 @@ w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scale
       w |= (v >> (8 * j) & 15u) << (4 * j);
       w |= (v >> (8 * j + 4) & 15u) << (16 + 4 * j);
     }
-    *reinterpret_cast<uint32_t*>(dst + (word >> 2) * 2048 + row * 16 + (word & 3) * 4) = w;
+    *reinterpret_cast<uint32_t*>(dst + w4_q_offset(word & 3, row) + (word >> 2) * 4) = w;
   }
   const int sub = kW4K / group, groups = K / group;
   for (int i = threadIdx.x; i < kW4Rows * sub; i += blockDim.x) {

@@ -92,6 +92,19 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
   return done != 0;
 }
 
+// One look at a barrier, without a suspend time: 17 cycles when the phase is
+// complete, where the poll above takes 55.  For waits that are mostly over
+// before they begin.
+__device__ __forceinline__ bool mbar_test_wait(uint32_t bar, uint32_t parity) {
+  uint32_t done;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}\n"
+      : "=r"(done) : "r"(bar), "r"(parity) : "memory");
+  return done != 0;
+}
+
 // The same poll with acquire semantics at cluster scope: a thread of the
 // other CTA wrote shared memory of this CTA (st.shared::cluster) and then
 // arrived with mbar_arrive_release_cluster; after this wait succeeds those
@@ -412,6 +425,28 @@ __device__ __forceinline__ void st_shared_u16(uint32_t addr, uint16_t v) {
 
 __device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t b) {
   asm volatile("st.shared.v2.b32 [%0], {%1, %2};" :: "r"(addr), "r"(a), "r"(b) : "memory");
+}
+
+// --------------------------------------------------- programmatic launch order
+// A kernel launched with programmatic stream serialization may start while
+// the one before it is still running: grid_wait returns when that one has
+// finished and its writes are visible (nothing of its may be read before);
+// grid_launch_next lets the next such kernel start.  Without the launch
+// attribute both do nothing.
+__device__ __forceinline__ void grid_wait() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+__device__ __forceinline__ void grid_launch_next() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Count one in with release and acquire at GPU scope: what this thread's CTA
+// wrote and it has seen (a barrier away) is visible to whoever counts later.
+__device__ __forceinline__ unsigned int atomic_add_acq_rel(unsigned int* p, unsigned int v) {
+  unsigned int old;
+  asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], %2;"
+               : "=r"(old) : "l"(p), "r"(v) : "memory");
+  return old;
 }
 
 // ------------------------------------- three-dimensional tiles, bulk copies
