@@ -69,19 +69,13 @@ bool init_stream() {
          set_smem(grouped_stream_kernel<kDA, 64, T>, StreamCfg<64>::smem_bytes(kMaxExperts));
 }
 
-// Token tile of the 4-bit kernel that goes through TMEM: the widest whose
-// products (one set of columns per group of a record) fit there.
-constexpr int w4_tokens(int group) { return group == 32 ? 32 : 64; }
-
 template <int kGroup, bool kZeros, class T>
 bool init_w4_one() {
-  constexpr int wide = w4_tokens(kGroup);
   return set_smem(w4_rows_kernel<8, kGroup, kZeros, T>,
                   W4RowsCfg<8, kGroup>::smem_bytes(kMaxExperts)) &&
          set_smem(w4_rows_kernel<16, kGroup, kZeros, T>,
                   W4RowsCfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
-         set_smem(w4_stream_kernel<wide, kGroup, kZeros, T>,
-                  W4Cfg<wide, kGroup>::smem_bytes(kMaxExperts));
+         set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts));
 }
 
 template <int kGroup, class T>
@@ -440,17 +434,21 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
     return launch(w4_rows_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
                   C::smem_bytes(c.experts), stream, tt, a);
   } else {
-    using C = W4Cfg<kTok, kGroup>;
-    return launch(w4_stream_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
+    using C = W4Cfg<kGroup>;
+    return launch(w4_stream_kernel<kGroup, kZeros, T>, v.sms, C::kThreads,
                   C::smem_bytes(c.experts), stream, tt, a);
   }
 }
 
 template <int kGroup, bool kZeros, class T>
 int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
-  if (c.rows <= 8) return launch_w4<true, 8, kGroup, kZeros, T>(c, v, stream);
-  if (c.rows <= 16) return launch_w4<true, 16, kGroup, kZeros, T>(c, v, stream);
-  return launch_w4<false, w4_tokens(kGroup), kGroup, kZeros, T>(c, v, stream);
+  // A tile as wide as most experts' rows: an expert with more takes another
+  // tile, that is, reads its weights again.
+  if (c.rows <= 8 || c.rows <= 4ll * c.experts)
+    return launch_w4<true, 8, kGroup, kZeros, T>(c, v, stream);
+  if (c.rows <= 16 || c.rows <= 8ll * c.experts)
+    return launch_w4<true, 16, kGroup, kZeros, T>(c, v, stream);
+  return launch_w4<false, 64, kGroup, kZeros, T>(c, v, stream);
 }
 
 template <class T>

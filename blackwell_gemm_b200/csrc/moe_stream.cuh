@@ -30,7 +30,7 @@ struct StreamArgs {
   void* out;
   long long ldo;
   float* slots;           // [CTA][2][tok][128]
-  unsigned int* counts;   // [CTA][4], zero between launches
+  unsigned int* counts;   // [CTA][8], zero between launches
   int* status;
   unsigned long long timeout_ns;
   const uint8_t* packed;  // 4-bit weights (w4_stream.cuh)
@@ -100,16 +100,18 @@ __device__ __forceinline__ void stream_groups(const StreamArgs& a, int tile, int
 }
 
 // One warp's 32 weight rows of a finished segment: acc[c] is lane's row,
-// token c.  A whole contraction is rounded and stored; a part is left in
-// this CTA's slot, and the last contributor to arrive stores the sum.
+// token tok0 + c of the tile's kTile.  A whole contraction is rounded and
+// stored; a part is left in this CTA's slot, and the last contributor to
+// arrive stores the sum.  `piece` numbers the warps of a CTA that finish.
 // valid = false (a wait ran out): the part is only counted, so that the
 // counts are zero again when the launch ends.
-template <int kTok, class T>
-__device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamWalk<kTok>& walk,
-                                              const StreamSegment& s, int quarter,
-                                              float (&acc)[kTok], bool valid) {
+template <int kTok, class T, int kTile>
+__device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamWalk<kTile>& walk,
+                                              const StreamSegment& s, int quarter, int piece,
+                                              int tok0, float (&acc)[kTok], bool valid) {
   const int lane = threadIdx.x & 31;
   const int f = s.block * 128 + quarter * 32 + lane;
+  const int rows = s.rows - tok0;  // of this warp's tokens (may be none)
   if (s.kb0 != 0 || s.kb1 != walk.red_blocks) {
     const long long first = s.unit * walk.red_blocks;
     const int c0 = sk_owner(first, walk.items, walk.ranges);
@@ -118,21 +120,22 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
     auto slot = [&](int c) {
       // a CTA begins at most one divided tile (slot 1) and ends or crosses
       // at most one that an earlier CTA began (slot 0)
-      return a.slots + ((long long)c * 2 + (c == c0 ? 1 : 0)) * kTok * 128 + quarter * 32 + lane;
+      return a.slots + (((long long)c * 2 + (c == c0 ? 1 : 0)) * kTile + tok0) * 128 +
+             quarter * 32 + lane;
     };
     if (valid) {
       float* mine = slot(me);
 #pragma unroll
       for (int c = 0; c < kTok; ++c)
-        if (c < s.rows) __stcg(mine + c * 128, acc[c]);
+        if (c < rows) __stcg(mine + c * 128, acc[c]);
     }
     __syncwarp();
     unsigned int before = 0;
-    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 4 + quarter, 1u);
+    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 8 + piece, 1u);
     before = __shfl_sync(0xffffffffu, before, 0);
     if (before != (unsigned int)(c1 - c0)) return;
     __syncwarp();
-    if (lane == 0) atomicExch(a.counts + c0 * 4 + quarter, 0u);
+    if (lane == 0) atomicExch(a.counts + c0 * 8 + piece, 0u);
 #pragma unroll
     for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
     // (two parts' loads in flight at a time; added in order)
@@ -145,7 +148,7 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
         float v[kBatch], u[kBatch];
 #pragma unroll
         for (int c = 0; c < kBatch; ++c) {
-          const bool in = b + c < s.rows;
+          const bool in = b + c < rows;
           v[c] = in ? __ldcg(from + (b + c) * 128) : 0.0f;
           u[c] = in && p < c1 ? __ldcg(then + (b + c) * 128) : 0.0f;
         }
@@ -155,10 +158,10 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
     }
   }
   if (!valid || f >= a.feat) return;
-  T* col = static_cast<T*>(a.out) + (long long)s.row0 * a.ldo + f;
+  T* col = static_cast<T*>(a.out) + (long long)(s.row0 + tok0) * a.ldo + f;
 #pragma unroll
   for (int c = 0; c < kTok; ++c)
-    if (c < s.rows) col[c * a.ldo] = round_one<T>(acc[c]);
+    if (c < rows) col[c * a.ldo] = round_one<T>(acc[c]);
 }
 
 // ----------------------------------------------- 16-bit weights, few tokens
@@ -338,7 +341,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
         __syncwarp();
         if (lane == 0) mbar_arrive_local(smem_u32(&bar_acc_empty[buf]));
       }
-      stream_finish<kTok, T>(args, walk, s, quarter, acc, ok != 0);
+      stream_finish<kTok, T>(args, walk, s, quarter, quarter, 0, acc, ok != 0);
     }
     __syncwarp();
   }

@@ -51,7 +51,7 @@ __host__ __device__ constexpr uint32_t w4_q_offset(int t, int row) {
 // nibble at bits 0-3 or 4-7 of a 16-bit float is a subnormal (or, with bit 7
 // of a bf16, a number of the first binade, which has the same spacing): the
 // bits n stand for n 2^-133 (bf16) or n 2^-24 (f16).  Times a power of two
-// that is (q - z) kUnit, exactly; the sums are scaled back by 1 / kUnit.
+// that is (q - z) kUnit, exactly; finished sums are scaled back by 1 / kUnit.
 template <class T>
 struct W4Unpack;
 template <>
@@ -70,7 +70,7 @@ struct W4Unpack<__nv_bfloat16> {
     return pack_pair<__nv_bfloat16>(-kUnit * (float)z, -kUnit * (float)z);
   }
   static __device__ __forceinline__ float wide(uint16_t s) {
-    return __uint_as_float((uint32_t)s << 16) * (1.0f / kUnit);
+    return __uint_as_float((uint32_t)s << 16);
   }
 };
 template <>
@@ -88,7 +88,7 @@ struct W4Unpack<__half> {
     return pack_pair<__half>(-kUnit * (float)z, -kUnit * (float)z);
   }
   static __device__ __forceinline__ float wide(uint16_t s) {
-    return __half2float(*reinterpret_cast<const __half*>(&s)) * (1.0f / kUnit);
+    return __half2float(*reinterpret_cast<const __half*>(&s));
   }
 };
 
@@ -103,27 +103,37 @@ __device__ __forceinline__ void w4_pairs(uint32_t w, uint32_t bias, uint32_t* o)
   o[3] = U::fma2(v & 0x00F000F0u, U::kHigh, bias);
 }
 
-// D += A B^T for 16 weight rows, 8 tokens, 16 k, in registers.
+// D = A B^T (+ D unless `first`) for 16 weight rows, 8 tokens, 16 k, in registers.
 template <class T>
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
-                                            uint32_t b1);
-template <>
-__device__ __forceinline__ void mma_16x8x16<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4],
-                                                           uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma_16x8x16<__half>(float (&d)[4], const uint32_t (&a)[4],
-                                                    uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
-      "{%8, %9}, {%0, %1, %2, %3};"
-      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+                                            uint32_t b1, bool first) {
+  if constexpr (kFormat<T> == 1) {
+    if (first)
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    if (first)
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+          : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+      asm volatile(
+          "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, "
+          "{%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+          : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+          : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
 }
 
 // A ring stage holds up to two consecutive records of a segment (one bulk
@@ -137,42 +147,63 @@ struct W4Ring {
   static constexpr int kSlabRows = kTok;                   // rows of a token box
   static constexpr int kSlab = kSlabRows * 128;
   static constexpr int kTokens = 4 * kSlab;
-  static constexpr int kStageBytes =
-      kTokens + (2 * w4_record_bytes(kGroup, true) + 1023) / 1024 * 1024;
+  static constexpr int kRecords = (2 * w4_record_bytes(kGroup, true) + 1023) / 1024 * 1024;
+  static constexpr int kStageBytes = kTokens + kRecords;
   static constexpr int stages(int other) {
     return (214 * 1024 - other) / kStageBytes < 8 ? (214 * 1024 - other) / kStageBytes : 8;
   }
 };
 
-// tmap_t: with K a multiple of 64, the token operand as (k in a slab, row,
-// slab), box 64 x kSlabRows x 4; else (k, row), box 64 x kSlabRows.
-template <int kTok, int kGroup, int kStages>
+// The two copies of a stage.  tmap_t: with K a multiple of 64, the token
+// operand as (k in a slab, row, slab), box 64 x kSlabRows x 4; else (k, row),
+// box 64 x kSlabRows.
+template <class R>
+__device__ __forceinline__ void w4_load_tokens(const CUtensorMap* tmap_t, bool slabs, uint32_t dst,
+                                               int kb, int row0, uint32_t bar, uint64_t policy) {
+  if (slabs) {
+    tma_load_3d_hint(dst, tmap_t, 0, row0, 2 * kb, bar, policy);
+  } else {
+    for (int j = 0; j < 4; ++j)
+      tma_load_2d_hint(dst + j * R::kSlab, tmap_t, kb * kW4K + 64 * j, row0, bar, policy);
+  }
+}
+__device__ __forceinline__ const uint8_t* w4_record(const StreamArgs& a, const StreamSegment& s,
+                                                    int kb) {
+  return a.packed + (long long)s.e * a.expert_bytes +
+         ((long long)s.block * a.red_blocks + kb) * a.record_bytes;
+}
+
+// Producing thread, both copies into stages of kStageBytes (tokens first), or
+// one of them into a ring of its own.
+enum W4Part { kW4Both, kW4Weights, kW4Tokens };
+template <W4Part kPart, int kTok, int kGroup, int kStages>
 __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kTok> walk,
                                            const CUtensorMap* tmap_t, uint32_t ring, uint32_t full,
                                            uint32_t empty, const WaitCtx& wctx) {
   using R = W4Ring<kTok, kGroup>;
+  constexpr uint32_t kTokenBytes = kPart == kW4Weights ? 0 : R::kTokens;
+  constexpr uint32_t kBytes = kTokenBytes + (kPart == kW4Tokens ? 0 : R::kRecords);
   const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
   const bool slabs = args.red % kSlabK == 0;
   uint32_t stage = 0, phase = 0;
+  // Looking at a barrier takes 100 cycles and more on a busy SM, so the next
+  // stage's is looked at before this stage's copies go out.
+  bool ready = true;
   StreamSegment s;
   while (walk.next(&s)) {
-    const uint8_t* record = args.packed + (long long)s.e * args.expert_bytes +
-                            ((long long)s.block * args.red_blocks + s.kb0) * args.record_bytes;
     for (int kb = s.kb0; kb < s.kb1; kb += 2) {
       const uint32_t fb = full + stage * 8u;
-      const uint32_t sa = ring + stage * R::kStageBytes;
-      const uint32_t bytes = kb + 1 < s.kb1 ? 2 * args.record_bytes : args.record_bytes;
-      if (!wait_ready(empty + stage * 8u, phase ^ 1u, wctx, kErrWaitEmpty)) return;
-      mbar_arrive_expect_tx(fb, bytes + R::kTokens);
-      bulk_load_hint(sa + R::kTokens, record, bytes, fb, once);
-      if (slabs) {
-        tma_load_3d_hint(sa, tmap_t, 0, s.row0, 2 * kb, fb, keep);
-      } else {
-        for (int j = 0; j < 4; ++j)
-          tma_load_2d_hint(sa + j * R::kSlab, tmap_t, kb * kW4K + 64 * j, s.row0, fb, keep);
-      }
-      record += bytes;
+      const uint32_t sa = ring + stage * kBytes;
+      const uint32_t bytes = kPart == kW4Tokens ? 0
+                             : kb + 1 < s.kb1   ? 2 * args.record_bytes
+                                                : args.record_bytes;
+      if (!ready && !wait_ready(empty + stage * 8u, phase ^ 1u, wctx, kErrWaitEmpty)) return;
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      ready = mbar_test_wait(empty + stage * 8u, phase ^ 1u);
+      mbar_arrive_expect_tx(fb, bytes + kTokenBytes);
+      if (kPart != kW4Tokens)
+        bulk_load_hint(sa + kTokenBytes, w4_record(args, s, kb), bytes, fb, once);
+      if (kPart != kW4Weights) w4_load_tokens<R>(tmap_t, slabs, sa, kb, s.row0, fb, keep);
     }
   }
 }
@@ -181,17 +212,20 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
 // registers into warp-level MMAs.  A record then costs about 840 warp
 // instructions, where the way through TMEM takes 1780 (stores, loads and the
 // handshakes between its stages), and with so few tokens the tensor core's
-// rate does not matter.  Sixteen warps, four to a record: stage i's two records
-// go to groups 2 (i % 2) and 2 (i % 2) + 1, and of each a warp takes 32 rows.
+// rate does not matter.  Groups of four warps take records in turn, a warp 32
+// rows of each: four groups for up to 8 tokens, three for 16, where a fourth
+// would leave 96 registers to a warp, which then spills (57344 x 8192, us:
+// 8 tokens 52.8 with four groups, 55.8 with three; 16 tokens 72.8 and 66.9).
 // Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
 // lets eight lanes read all banks of the swizzled token slab.
 template <int kTok, int kGroup>
 struct W4RowsCfg {
   using Ring = W4Ring<kTok, kGroup>;
   static constexpr int kPitch = 136;  // floats from token to token of the exchange
-  static constexpr int kExchange = 4 * kTok * kPitch * 4;
-  static constexpr int kStages = Ring::stages(kExchange) & ~1;  // a stage has its two groups
-  static constexpr int kThreads = 32 * 17;
+  static constexpr int kGroups = kTok <= 8 ? 4 : 3;
+  static constexpr int kExchange = kGroups * kTok * kPitch * 4;
+  static constexpr int kStages = Ring::stages(kExchange);
+  static constexpr int kThreads = 32 * (4 * kGroups + 1);
   static constexpr int smem_bytes(int experts) {
     return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;
   }
@@ -242,10 +276,11 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
   walk.init(args, s_off, s_tiles);
   StreamSegment s;
 
-  if (warp == 16) {
+  if (warp == 4 * C::kGroups) {
     if (elect_one()) {
-      w4_produce<kTok, kGroup, kStages>(args, walk, &tmap_t, smem_base, smem_u32(&bar_full[0]),
-                                        smem_u32(&bar_empty[0]), wctx);
+      w4_produce<kW4Both, kTok, kGroup, kStages>(args, walk, &tmap_t, smem_base,
+                                                 smem_u32(&bar_full[0]), smem_u32(&bar_empty[0]),
+                                                 wctx);
     }
     __syncwarp();
     return;
@@ -258,10 +293,10 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
   const uint32_t token_row = token * 128;
   zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
                     s_off[args.experts], args.rows,
-                    (long long)blockIdx.x * 512 + threadIdx.x, gridDim.x * 512ll);
-  // This group's stages: every other one, from group / 2.
-  uint32_t next = 0, stage = group >> 1, phase = 0;
-  const uint32_t second = group & 1;
+                    (long long)blockIdx.x * (128 * C::kGroups) + threadIdx.x,
+                    gridDim.x * (128ll * C::kGroups));
+  uint32_t stage = 0, phase = 0;
+  uint32_t turn = 0;  // group that takes the next record
   bool ok = true;
   while (walk.next(&s)) {
     float acc[2][kNt][4];
@@ -272,26 +307,24 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
     for (int kb = s.kb0; ok && kb < s.kb1; kb += 2) {
-      const bool mine = next == group >> 1;
-      next ^= 1u;
-      if (!mine) continue;
-      const uint32_t bar = smem_u32(&bar_full[stage]), done = smem_u32(&bar_empty[stage]);
-      const uint32_t tokens = smem_base + stage * R::kStageBytes + second * 2 * R::kSlab;
+      // a stage's records go to groups turn and turn + 1
+      const uint32_t records = kb + 1 < s.kb1 ? 2 : 1;
+      const uint32_t which = group >= turn ? group - turn : group + C::kGroups - turn;
+      const uint32_t at = stage, parity = phase;
+      turn += records;
+      if (turn >= C::kGroups) turn -= C::kGroups;
+      if (++stage == kStages) { stage = 0; phase ^= 1u; }
+      if (which >= records) continue;
+      const uint32_t bar = smem_u32(&bar_full[at]), done = smem_u32(&bar_empty[at]);
+      const uint32_t tokens = smem_base + at * R::kStageBytes + which * 2 * R::kSlab;
       const uint32_t record =
-          smem_base + stage * R::kStageBytes + R::kTokens + second * args.record_bytes;
-      const uint32_t parity = phase;
-      stage += 2;
-      if (stage >= kStages) { stage -= kStages; phase ^= 1u; }
+          smem_base + at * R::kStageBytes + R::kTokens + which * args.record_bytes;
       if (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) {
         int got = 0;
         if (lane == 0) got = wait_ready(bar, parity, wctx, kErrWaitFull);
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
         __syncwarp();
         if (!ok) break;
-      }
-      if (kb + (int)second >= s.kb1) {  // the segment's last stage holds one record
-        if (lane == 0) mbar_arrive_local(done);
-        continue;
       }
       uint32_t q[4][4];  // [row][c]
 #pragma unroll
@@ -307,14 +340,6 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
           ld_shared_v4_u32(tokens + (c >> 1) * R::kSlab + n * 1024 + token_row +
                                ((((c & 1) * 4 + t) ^ token) << 4),
                            x[n]);
-        if (c % kPer == 0) {
-#pragma unroll
-          for (int m = 0; m < 2; ++m)
-#pragma unroll
-            for (int n = 0; n < kNt; ++n)
-#pragma unroll
-              for (int i = 0; i < 4; ++i) part[m][n][i] = 0.0f;
-        }
 #pragma unroll
         for (int m = 0; m < 2; ++m) {
           uint32_t lo[4], hi[4];
@@ -331,7 +356,7 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
             const uint32_t a[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
 #pragma unroll
             for (int n = 0; n < kNt; ++n)
-              mma_16x8x16<T>(part[m][n], a, x[n][2 * h], x[n][2 * h + 1]);
+              mma_16x8x16<T>(part[m][n], a, x[n][2 * h], x[n][2 * h + 1], c % kPer == 0 && h == 0);
           }
         }
         if (c % kPer == kPer - 1) {
@@ -349,9 +374,12 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
         }
       }
       __syncwarp();
-      if (lane == 0) mbar_arrive_local(done);
+      if (lane == 0) {
+        mbar_arrive_local(done);
+        if (records == 1) mbar_arrive_local(done);  // for the record that is not there
+      }
     }
-    // The four groups' sums meet in shared memory; warps 0-3 finish the tile,
+    // The groups' sums meet in shared memory; warps 0-3 finish the tile,
     // lane = row.
     float* sums = reinterpret_cast<float*>(smem_raw + (exchange - smem_u32(smem_raw)));
 #pragma unroll
@@ -362,57 +390,75 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
         for (int i = 0; i < 4; ++i)
           sums[(group * kTok + n * 8 + t + 4 * (i & 1)) * C::kPitch + row + 16 * m + 8 * (i >> 1)] =
               acc[m][n][i];
-    named_bar_sync(1, 512);
+    named_bar_sync(1, 128 * C::kGroups);
     float total[kTok];
     if (warp < 4) {
 #pragma unroll
       for (int c = 0; c < kTok; ++c) {
         const float* from = sums + c * C::kPitch + warp * 32 + lane;
-        total[c] = (from[0] + from[kTok * C::kPitch]) +
-                   (from[2 * kTok * C::kPitch] + from[3 * kTok * C::kPitch]);
+        float sum = from[0];
+#pragma unroll
+        for (int i = 1; i < C::kGroups; ++i) sum += from[i * kTok * C::kPitch];
+        total[c] = sum * (1.0f / U::kUnit);
       }
     }
-    named_bar_sync(1, 512);
+    named_bar_sync(1, 128 * C::kGroups);
     if (warp < 4) {
       const bool valid = __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
-      stream_finish<kTok, T>(args, walk, s, warp, total, valid);
+      stream_finish<kTok, T>(args, walk, s, warp, warp, 0, total, valid);
     }
   }
 }
 
-// More rows: through TMEM, 64 tokens to a tile (32 where the groups are of 32).
-template <int kTok, int kGroup>
+// More rows: through TMEM, 64 tokens to a tile.  Warps: 0 records, 18 tokens
+// (each into a ring of its own: a record is free once it is unpacked, its
+// tokens when they are multiplied), 1 MMA, 2-9 take the products, 10-17
+// unpack.  Two sets unpack the first and
+// the second record of a stage into four places of 64 columns.  Products, 64
+// columns a group and at most two groups at a time, go through the other 256
+// columns, so unpacking, MMAs and the scaled sums run beside one another.
+// Two sets of warps take half of the tokens each.
+template <int kGroup>
 struct W4Cfg {
+  static constexpr int kTok = 64;
   using Ring = W4Ring<kTok, kGroup>;
-  // TMEM: kProducts records' products and kWeights records' unpacked weights.
-  static constexpr int kProductCols = kTok * Ring::kSub;
-  static constexpr int kProducts = kProductCols >= 128 ? 2 : kProductCols >= 64 ? 3 : 4;
-  static constexpr int kFree = (kTmemCols - kProducts * kProductCols) / 64;
-  static constexpr int kWeights = kFree < 6 ? kFree : 6;
-  static_assert(kWeights >= kProducts, "a product's barrier is its weights'");
-  static constexpr int kExchange = kTok * 128 * 4;
-  static constexpr int kStages = Ring::stages(kExchange + 8192);
-  static constexpr int kThreads = 32 * (2 + 8 + 8);
+  static constexpr int kPlaces = 4;                            // records' weights
+  static constexpr int kBatch = Ring::kSub < 2 ? 1 : 2;        // groups to a product
+  static constexpr int kProducts = 4 / kBatch;
+  static constexpr int kTokenStages = 3;
+  // Scales wait for their products in a ring of twice as many places: when
+  // record j - kPlaces is multiplied, the products of j - 2 kPlaces have been
+  // taken (there are never more than kPlaces records between the two).
+  static constexpr int kScalePlaces = 2 * kPlaces;
+  static constexpr int kScales = kScalePlaces * Ring::kSub * 128 * 2;
+  static constexpr int kStages =
+      (214 * 1024 - kTokenStages * Ring::kTokens - kScales) / Ring::kRecords;
+  static constexpr int kThreads = 32 * (2 + 8 + 8 + 1);
   static constexpr int smem_bytes(int experts) {
-    return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;
+    return kTokenStages * Ring::kTokens + kStages * Ring::kRecords + kScales +
+           group_table_bytes(experts) + 1024;
   }
 };
 
 // tmap_t: as w4_produce takes it.
-template <int kTok, int kGroup, bool kZeros, class T>
-__global__ void __launch_bounds__(W4Cfg<kTok, kGroup>::kThreads, 1)
+template <int kGroup, bool kZeros, class T>
+__global__ void __launch_bounds__(W4Cfg<kGroup>::kThreads, 1)
 w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args) {
-  using C = W4Cfg<kTok, kGroup>;
+  using C = W4Cfg<kGroup>;
   using R = typename C::Ring;
   using U = W4Unpack<T>;
+  constexpr int kTok = C::kTok;
   constexpr int kStages = C::kStages;
   constexpr int kSub = R::kSub;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t bar_full[kStages];
   __shared__ alignas(8) uint64_t bar_empty[kStages];
-  __shared__ alignas(8) uint64_t bar_a_full[C::kWeights];   // weights unpacked into TMEM
-  __shared__ alignas(8) uint64_t bar_done[C::kWeights];     // their MMAs are done
-  __shared__ alignas(8) uint64_t bar_taken[C::kProducts];   // products taken
+  __shared__ alignas(8) uint64_t bar_tok_full[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_tok_empty[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_unpacked[C::kPlaces];  // weights are in TMEM
+  __shared__ alignas(8) uint64_t bar_used[C::kPlaces];      // their MMAs are done
+  __shared__ alignas(8) uint64_t bar_product[C::kProducts]; // a batch of groups is in TMEM
+  __shared__ alignas(8) uint64_t bar_taken[C::kProducts];   // it has been read
   __shared__ alignas(8) uint64_t bar_drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
@@ -420,20 +466,28 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t exchange = smem_base + kStages * R::kStageBytes;
-  int* s_off = reinterpret_cast<int*>(smem_raw + (exchange + C::kExchange - smem_u32(smem_raw)));
+  const uint32_t records = smem_base + C::kTokenStages * R::kTokens;
+  const uint32_t scales = records + kStages * R::kRecords;  // [place][group][row], 16-bit
+  int* s_off = reinterpret_cast<int*>(smem_raw + (scales + C::kScales - smem_u32(smem_raw)));
   int* s_tiles = s_off + args.experts + 1;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 16);  // the unpackers, and those who take products
+      mbar_init(smem_u32(&bar_empty[s]), 8);  // the unpackers
     }
-    for (int b = 0; b < C::kWeights; ++b) {
-      mbar_init(smem_u32(&bar_a_full[b]), 4);
-      mbar_init(smem_u32(&bar_done[b]), 1);
+    for (int s = 0; s < C::kTokenStages; ++s) {
+      mbar_init(smem_u32(&bar_tok_full[s]), 1);
+      mbar_init(smem_u32(&bar_tok_empty[s]), 1);
     }
-    for (int b = 0; b < C::kProducts; ++b) mbar_init(smem_u32(&bar_taken[b]), 4);
+    for (int b = 0; b < C::kPlaces; ++b) {
+      mbar_init(smem_u32(&bar_unpacked[b]), 4);
+      mbar_init(smem_u32(&bar_used[b]), 1);
+    }
+    for (int b = 0; b < C::kProducts; ++b) {
+      mbar_init(smem_u32(&bar_product[b]), 1);
+      mbar_init(smem_u32(&bar_taken[b]), 8);
+    }
     mbar_init(smem_u32(&bar_drain), 1);
     abort_word = 0;
     fence_mbar_init_cluster();
@@ -450,7 +504,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   tc_fence_after_sync();
   grid_launch_next();
   const uint32_t tmem_base = tmem_slot;
-  const uint32_t tmem_d = tmem_base + C::kWeights * 64;
+  const uint32_t tmem_d = tmem_base + C::kPlaces * 64;
 
   WaitCtx wctx;
   wctx.status = args.status;
@@ -464,8 +518,16 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
 
   if (warp == 0) {
     if (elect_one()) {
-      w4_produce<kTok, kGroup, kStages>(args, walk, &tmap_t, smem_base, smem_u32(&bar_full[0]),
-                                        smem_u32(&bar_empty[0]), wctx);
+      w4_produce<kW4Weights, kTok, kGroup, kStages>(args, walk, &tmap_t, records,
+                                                    smem_u32(&bar_full[0]),
+                                                    smem_u32(&bar_empty[0]), wctx);
+    }
+    __syncwarp();
+  } else if (warp == 18) {
+    if (elect_one()) {
+      w4_produce<kW4Tokens, kTok, kGroup, C::kTokenStages>(args, walk, &tmap_t, smem_base,
+                                                           smem_u32(&bar_tok_full[0]),
+                                                           smem_u32(&bar_tok_empty[0]), wctx);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -473,35 +535,47 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
       uint32_t stage = 0, phase = 0;
       uint32_t w = 0, wp = 0, p = 0, pp = 1;  // places in TMEM and their phases
       bool ok = true;
+      // (looked at ahead, as by the producer)
+      bool landed = false, unpacked = false, taken = true;
       while (ok && walk.next(&s)) {
         const uint32_t idesc = make_idesc_16bit(128, (s.rows + 15) & ~15, kFormat<T>, false, false);
-        for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          const uint32_t full = smem_u32(&bar_full[stage]), unpacked = smem_u32(&bar_a_full[w]),
-                         taken = smem_u32(&bar_taken[p]);
-          const bool r0 = mbar_test_wait(full, phase), r1 = mbar_test_wait(unpacked, wp),
-                     r2 = mbar_test_wait(taken, pp);
-          if (!(r0 && r1 && r2) && (!wait_ready(full, phase, wctx, kErrWaitFull) ||
-                                    !wait_ready(taken, pp, wctx, kErrWaitAccEmpty) ||
-                                    !wait_ready(unpacked, wp, wctx, kErrWaitFull))) {
+        for (int kb = s.kb0; ok && kb < s.kb1; ++kb) {
+          if (!(landed || wait_ready(smem_u32(&bar_tok_full[stage]), phase, wctx, kErrWaitFull)) ||
+              !(unpacked || wait_ready(smem_u32(&bar_unpacked[w]), wp, wctx, kErrWaitFull))) {
             ok = false;
             break;
           }
-          tc_fence_after_sync();
+          const uint32_t second = (kb - s.kb0) & 1;
           const uint64_t bdesc =
-              make_sdesc_k128(smem_base + stage * R::kStageBytes + ((kb - s.kb0) & 1) * 2 * R::kSlab);
+              make_sdesc_k128(smem_base + stage * R::kTokens + second * 2 * R::kSlab);
           const uint32_t a = tmem_base + w * 64;
-          const uint32_t d = tmem_d + p * C::kProductCols;
 #pragma unroll
-          for (int k = 0; k < kW4K / kMmaK; ++k)
-            umma_tmem_a_1(d + k * kMmaK / kGroup * kTok, a + k * 8,
-                          bdesc + ((k >> 2) * R::kSlab + (k & 3) * 32) / 16, idesc,
-                          k * kMmaK % kGroup != 0 ? 1u : 0u);
-          umma_commit_1(smem_u32(&bar_done[w]));
-          if (++w == C::kWeights) { w = 0; wp ^= 1u; }
-          if (++p == C::kProducts) { p = 0; pp ^= 1u; }
-          if (((kb - s.kb0) & 1) != 0 || kb + 1 == s.kb1) {
-            if (++stage == kStages) { stage = 0; phase ^= 1u; }
+          for (int g = 0; g < kSub / C::kBatch; ++g) {
+            if (!taken && !wait_ready(smem_u32(&bar_taken[p]), pp, wctx, kErrWaitAccEmpty)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after_sync();
+            const uint32_t d = tmem_d + p * C::kBatch * 64;
+#pragma unroll
+            for (int i = 0; i < C::kBatch * kGroup / kMmaK; ++i) {
+              const int k = g * (C::kBatch * kGroup / kMmaK) + i;
+              umma_tmem_a_1(d + i * kMmaK / kGroup * 64, a + k * 8,
+                            bdesc + ((k >> 2) * R::kSlab + (k & 3) * 32) / 16, idesc,
+                            i * kMmaK % kGroup != 0 ? 1u : 0u);
+            }
+            umma_commit_1(smem_u32(&bar_product[p]));
+            if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+            taken = mbar_test_wait(smem_u32(&bar_taken[p]), pp);
           }
+          umma_commit_1(smem_u32(&bar_used[w]));
+          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+          if (second != 0 || kb + 1 == s.kb1) {
+            umma_commit_1(smem_u32(&bar_tok_empty[stage]));
+            if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+          }
+          landed = mbar_test_wait(smem_u32(&bar_tok_full[stage]), phase);
+          unpacked = mbar_test_wait(smem_u32(&bar_unpacked[w]), wp);
         }
       }
       umma_commit_1(smem_u32(&bar_drain));
@@ -522,20 +596,19 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
       __syncwarp();
       return got != 0;
     };
-    // The stage and the places in TMEM of the next pair of records, and their
-    // phases.  Set 0 takes a pair's first record, set 1 its second.
-    uint32_t stage = 0, phase = 0, w = 0, wp = 0, p = 0;
-    auto next_place = [&]() {
-      if (++w == C::kWeights) { w = 0; wp ^= 1u; }
-      if (++p == C::kProducts) p = 0;
-    };
+    const uint32_t set = ((uint32_t)(warp - 2) >> 2) & 1u;
+    uint32_t stage = 0, phase = 0;
     auto next_stage = [&]() {
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
     };
-    const uint32_t set = ((uint32_t)(warp - 2) >> 2) & 1u;
     bool ok = true;
     if (warp >= 10) {
       // ----------------------------------------------------------- unpack
+      uint32_t w = 0, wp = 0, n = 0;
+      auto next_place = [&]() {
+        if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+        if (++n == C::kScalePlaces) n = 0;
+      };
       while (ok && walk.next(&s)) {
         for (int kb = s.kb0; kb < s.kb1; kb += 2, next_stage()) {
           const bool pair = kb + 1 < s.kb1;
@@ -547,16 +620,19 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
             }
           }
           ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull) &&
-               wait_warp(smem_u32(&bar_done[w]), wp ^ 1u, kErrWaitAccEmpty);
+               wait_warp(smem_u32(&bar_used[w]), wp ^ 1u, kErrWaitAccEmpty);
           if (!ok) break;
           tc_fence_after_sync();
-          const uint32_t record =
-              smem_base + stage * R::kStageBytes + R::kTokens + set * args.record_bytes;
+          const uint32_t record = records + stage * R::kRecords + set * args.record_bytes;
           uint32_t bias[kSub];
 #pragma unroll
           for (int g = 0; g < kSub; ++g)
             bias[g] = U::bias(
                 kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
+#pragma unroll
+          for (int g = 0; g < kSub; ++g)
+            st_shared_u16(scales + ((n * kSub + g) * 128 + row) * 2,
+                          ld_shared_u16(record + kW4Q + (g * 128 + row) * 2));
           uint32_t q[4][4];  // [t][c]
 #pragma unroll
           for (int t = 0; t < 4; ++t) ld_shared_v4_u32(record + w4_q_offset(t, row), q[t]);
@@ -575,7 +651,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
           tmem_wait_st();
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive_local(smem_u32(&bar_a_full[w]));
+          if (lane == 0) mbar_arrive_local(smem_u32(&bar_unpacked[w]));
           next_place();
           if (set == 0 && pair) next_place();
         }
@@ -585,66 +661,53 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
       zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
                         s_off[args.experts], args.rows,
                         (long long)blockIdx.x * 256 + (threadIdx.x - 64), gridDim.x * 256ll);
-      float* sums = reinterpret_cast<float*>(smem_raw + (exchange - smem_u32(smem_raw))) + row;
+      const int tok0 = (int)set * 32;  // of this warp's tokens
+      uint32_t p = 0, pp = 0, n = 0;
+      bool ready = false;
       while (walk.next(&s)) {
-        float acc[kTok];
+        float acc[32];
 #pragma unroll
-        for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
-        for (int kb = s.kb0; ok && kb < s.kb1; kb += 2, next_stage()) {
-          const bool pair = kb + 1 < s.kb1;
-          if (set == 1) {
-            next_place();
-            if (!pair) {
-              if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
-              continue;
-            }
-          }
-          ok = wait_warp(smem_u32(&bar_done[w]), wp, kErrWaitAccFull);
-          if (!ok) break;
-          tc_fence_after_sync();
-          const uint32_t scales = smem_base + stage * R::kStageBytes + R::kTokens +
-                                  set * args.record_bytes + kW4Q + row * 2;
+        for (int c = 0; c < 32; ++c) acc[c] = 0.0f;
+        for (int kb = s.kb0; ok && kb < s.kb1; ++kb) {
+          const uint32_t mine = scales + (n * kSub * 128 + row) * 2;
+          if (++n == C::kScalePlaces) n = 0;
+#pragma unroll 1
+          for (int g = 0; g < kSub; g += C::kBatch) {
+            ok = ready || wait_warp(smem_u32(&bar_product[p]), pp, kErrWaitAccFull);
+            if (!ok) break;
+            tc_fence_after_sync();
+            float scale[C::kBatch];
 #pragma unroll
-          for (int g = 0; g < kSub; ++g) {
-            const float scale = U::wide(ld_shared_u16(scales + g * 256));
+            for (int j = 0; j < C::kBatch; ++j)
+              scale[j] = U::wide(ld_shared_u16(mine + (g + j) * 256));
+            const uint32_t d = tmem_d + p * C::kBatch * 64 + tok0 + lanes;
+            const uint32_t here = smem_u32(&bar_taken[p]);
+            if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+            ready = __all_sync(0xffffffffu, mbar_test_wait(smem_u32(&bar_product[p]), pp));
 #pragma unroll
-            for (int c = 0; c < kTok; c += 16) {
-              if (c < s.rows) {
-                uint32_t v[16];
-                tmem_ld_32x32b_x16(tmem_d + p * C::kProductCols + g * kTok + c + lanes, v);
+            for (int c = 0; c < 32; c += 16) {
+              if (tok0 + c < s.rows) {
+                uint32_t v[C::kBatch][16];
+#pragma unroll
+                for (int j = 0; j < C::kBatch; ++j) tmem_ld_32x32b_x16(d + j * 64 + c, v[j]);
                 tmem_wait_ld();
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  acc[c + i] = fmaf(scale, __uint_as_float(v[i]), acc[c + i]);
+                for (int j = 0; j < C::kBatch; ++j)
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    acc[c + i] = fmaf(scale[j], __uint_as_float(v[j][i]), acc[c + i]);
               }
             }
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_local(here);
           }
-          tc_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive_local(smem_u32(&bar_taken[p]));
-            mbar_arrive_local(smem_u32(&bar_empty[stage]));
-          }
-          next_place();
-          if (set == 0 && pair) next_place();
         }
-        // The second set hands its sums to the first, which finishes the tile.
-        if (set == 1) {
 #pragma unroll
-          for (int c = 0; c < kTok; ++c)
-            if (c < s.rows) sums[c * 128] = acc[c];
-          named_bar_sync(1 + quarter, 64);
-          named_bar_sync(1 + quarter, 64);
-        } else {
-          named_bar_sync(1 + quarter, 64);
-#pragma unroll
-          for (int c = 0; c < kTok; ++c)
-            if (c < s.rows) acc[c] += sums[c * 128];
-          named_bar_sync(1 + quarter, 64);
-          const bool valid =
-              __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
-          stream_finish<kTok, T>(args, walk, s, quarter, acc, valid);
-        }
+        for (int c = 0; c < 32; ++c) acc[c] *= 1.0f / U::kUnit;
+        const bool valid =
+            __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
+        stream_finish<32, T>(args, walk, s, quarter, (int)set * 4 + quarter, tok0, acc, valid);
       }
     }
     __syncwarp();
