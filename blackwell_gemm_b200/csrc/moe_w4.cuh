@@ -535,28 +535,43 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
       uint32_t stage = 0, phase = 0;
       uint32_t w = 0, wp = 0, p = 0, pp = 1;  // places in TMEM and their phases
       bool ok = true;
-      // (looked at ahead, as by the producer)
+      // (looked at before the MMAs ahead of them go out, as by the producer)
       bool landed = false, unpacked = false, taken = true;
+      const uint32_t tok_full = smem_u32(&bar_tok_full[0]), tok_empty = smem_u32(&bar_tok_empty[0]),
+                     unpacked0 = smem_u32(&bar_unpacked[0]), used0 = smem_u32(&bar_used[0]),
+                     product0 = smem_u32(&bar_product[0]), taken0 = smem_u32(&bar_taken[0]);
       while (ok && walk.next(&s)) {
         const uint32_t idesc = make_idesc_16bit(128, (s.rows + 15) & ~15, kFormat<T>, false, false);
+        uint32_t second = 0;
         for (int kb = s.kb0; ok && kb < s.kb1; ++kb) {
-          if (!(landed || wait_ready(smem_u32(&bar_tok_full[stage]), phase, wctx, kErrWaitFull)) ||
-              !(unpacked || wait_ready(smem_u32(&bar_unpacked[w]), wp, wctx, kErrWaitFull))) {
+          if (!(landed || wait_ready(tok_full + stage * 8u, phase, wctx, kErrWaitFull)) ||
+              !(unpacked || wait_ready(unpacked0 + w * 8u, wp, wctx, kErrWaitFull))) {
             ok = false;
             break;
           }
-          const uint32_t second = (kb - s.kb0) & 1;
           const uint64_t bdesc =
               make_sdesc_k128(smem_base + stage * R::kTokens + second * 2 * R::kSlab);
           const uint32_t a = tmem_base + w * 64;
+          const uint32_t my_tokens = tok_empty + stage * 8u, my_used = used0 + w * 8u;
+          const bool last = second != 0 || kb + 1 == s.kb1;  // of its stage
+          second = last ? 0u : 1u;
+          if (last) {
+            if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+          }
+          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+          landed = mbar_test_wait(tok_full + stage * 8u, phase);
+          unpacked = mbar_test_wait(unpacked0 + w * 8u, wp);
 #pragma unroll
           for (int g = 0; g < kSub / C::kBatch; ++g) {
-            if (!taken && !wait_ready(smem_u32(&bar_taken[p]), pp, wctx, kErrWaitAccEmpty)) {
+            if (!taken && !wait_ready(taken0 + p * 8u, pp, wctx, kErrWaitAccEmpty)) {
               ok = false;
               break;
             }
             tc_fence_after_sync();
             const uint32_t d = tmem_d + p * C::kBatch * 64;
+            const uint32_t my_product = product0 + p * 8u;
+            if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+            taken = mbar_test_wait(taken0 + p * 8u, pp);
 #pragma unroll
             for (int i = 0; i < C::kBatch * kGroup / kMmaK; ++i) {
               const int k = g * (C::kBatch * kGroup / kMmaK) + i;
@@ -564,18 +579,11 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
                             bdesc + ((k >> 2) * R::kSlab + (k & 3) * 32) / 16, idesc,
                             i * kMmaK % kGroup != 0 ? 1u : 0u);
             }
-            umma_commit_1(smem_u32(&bar_product[p]));
-            if (++p == C::kProducts) { p = 0; pp ^= 1u; }
-            taken = mbar_test_wait(smem_u32(&bar_taken[p]), pp);
+            umma_commit_1(my_product);
           }
-          umma_commit_1(smem_u32(&bar_used[w]));
-          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
-          if (second != 0 || kb + 1 == s.kb1) {
-            umma_commit_1(smem_u32(&bar_tok_empty[stage]));
-            if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
-          }
-          landed = mbar_test_wait(smem_u32(&bar_tok_full[stage]), phase);
-          unpacked = mbar_test_wait(smem_u32(&bar_unpacked[w]), wp);
+          // (with one product to a record its barrier serves the weights too)
+          if (C::kProducts != C::kPlaces) umma_commit_1(my_used);
+          if (last) umma_commit_1(my_tokens);
         }
       }
       umma_commit_1(smem_u32(&bar_drain));
@@ -620,7 +628,9 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
             }
           }
           ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull) &&
-               wait_warp(smem_u32(&bar_used[w]), wp ^ 1u, kErrWaitAccEmpty);
+               wait_warp(C::kProducts == C::kPlaces ? smem_u32(&bar_product[w % C::kProducts])
+                                                    : smem_u32(&bar_used[w]),
+                         wp ^ 1u, kErrWaitAccEmpty);
           if (!ok) break;
           tc_fence_after_sync();
           const uint32_t record = records + stage * R::kRecords + set * args.record_bytes;
