@@ -367,8 +367,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
           }
         }
       } else {
-        const int f = f0 + lane;
-        T* col = out + (long long)w.row0 * args.ldo + f;
+        // Lane = feature, column = token.  Neighbouring lanes trade values so
+        // that each holds two features of one token (even lanes even tokens):
+        // a store instruction then writes 64 bytes of each of two rows.
+        const int odd = lane & 1;
+        const int f = f0 + (lane & ~1);
+        T* row = out + (long long)(w.row0 + odd) * args.ldo + f;
+        const bool in = f < args.feat, both = f + 1 < args.feat;
 #pragma unroll 1
         for (int c = 0; c < w.mma_n; c += 32) {
           uint32_t v[32];
@@ -379,10 +384,20 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
             __syncwarp();
             if (lane == 0) mbar_arrive_cluster(acc_empty_leader + buf * 8u);
           }
-          if (f < args.feat) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (c + j < w.rows) col[(c + j) * args.ldo] = round_one<T>(__uint_as_float(v[j]));
+          for (int j = 0; j < 32; j += 2) {
+            const float give = __uint_as_float(odd ? v[j] : v[j + 1]);
+            const float keep = __uint_as_float(odd ? v[j + 1] : v[j]);
+            const float got = __shfl_xor_sync(0xffffffffu, give, 1);
+            const uint32_t pair = odd ? pack_pair<T>(got, keep) : pack_pair<T>(keep, got);
+            if (in && c + j + odd < w.rows) {
+              if (both) {
+                *reinterpret_cast<uint32_t*>(row) = pair;
+              } else {
+                *reinterpret_cast<uint16_t*>(row) = (uint16_t)pair;
+              }
+            }
+            row += 2 * args.ldo;
           }
         }
       }

@@ -339,13 +339,27 @@ int launch_stream(const Call& c, const DeviceView& v, cudaStream_t stream) {
                 C::smem_bytes(c.experts), stream, tw, tt, a);
 }
 
+// The streaming kernel splits every contraction evenly over the SMs and takes
+// 64 rows of an expert at a time; the pair kernel 256, but deals whole tiles.
+// Streaming is faster while most experts fit one of its tiles (48 rows on
+// average) and either the contraction is long or there are too few tiles to
+// go round.  Measured, us, streaming / pair, for experts x N x K at rows per
+// expert: 8 x 14336 x 4096 at 2: 112 / 122, at 48: 153 / 172, at 64: 205 /
+// 175; 16 x 512 x 8192 at 16: 32 / 40; 32 x 2056 x 1032 at 16: 33 / 32, its
+// gradient in A 45 / 37; 64 x 1024 x 2048 at 16: 54 / 55, 54 / 51.
+bool use_stream(const Call& c, int feat, int red, int pairs) {
+  const int k = g_kernel.load();
+  if (k != 0) return k == 1;
+  const long long groups = c.experts < c.rows ? c.experts : c.rows;
+  return c.rows <= 48ll * c.experts &&
+         (red >= 4096 || groups * ceil_div(feat, 256) < 2ll * pairs);
+}
+
 template <int kMode, class T>
 int run_typed(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStream_t stream) {
   if constexpr (kMode != kGroupedDB) {
     constexpr bool kDA = kMode == kGroupedDA;
-    const int k = g_kernel.load();
-    const bool few = k == 1 || (k == 0 && (long long)c.rows <= 64ll * c.experts);
-    if (few)
+    if (use_stream(c, kDA ? c.K : c.N, kDA ? c.N : c.K, m.pairs[kMode]))
       return c.rows <= 16 ? launch_stream<kDA, 16, T>(c, v, stream)
                           : launch_stream<kDA, 64, T>(c, v, stream);
   }
