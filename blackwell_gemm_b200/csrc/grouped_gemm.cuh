@@ -17,11 +17,13 @@
 // along rows (B in dA; both operands in dB) the tile is loaded as it lies
 // and the MMA reads it MN-major (make_sdesc_mn128).
 //
-// dB's contraction is ragged: the last 64-row block of an expert holds the
-// next expert's rows.  MMAs step 16 rows, so at most 15 rows of that block
-// must read as zero, in both operands (0 x inf is NaN): the block's loads
-// complete on a barrier of their own CTA, a warp set aside for it clears
-// those rows in shared memory and only then releases the block to the MMA.
+// dB's contraction is ragged: an expert's last 64-row block reaches into the
+// next expert's rows, which must read as zero in both operands (0 x inf is
+// NaN).  TMA fills what lies beyond a tensor's end with zeros, so a small
+// kernel first makes two tensor maps per expert that end at its last row
+// (grouped_maps_kernel).  (Clearing the rows in shared memory instead, by a
+// warp of its own between the load and the MMA, cost each tile 1.3 us: 8
+// experts x 1023 rows, 14336 x 4096, took 800 us where 1024 rows took 663.)
 // An expert without rows gets zeros.
 #pragma once
 #include <cuda_fp16.h>
@@ -41,22 +43,53 @@ struct GroupedArgs {
   void* out;     // forward, dA: rows x feat
   long long ldo;
   int group;     // raster band
+  const CUtensorMap* maps;  // dB: dC's and A's map of each expert, box 64 x 64
   int* status;
   unsigned long long timeout_ns;
 };
 
-template <int kMode>
+// dB stages its output in shared memory, two boxes to an epilogue warp; for
+// many experts (kMany) it gives up a stage for the table of their rows.
+template <int kMode, bool kMany = false>
 struct GroupedCfg {
-  static constexpr int kStages = 6;
+  static constexpr int kStages = kMany ? 5 : 6;
   static constexpr int kOperand = 128 * kSlabK * 2;  // 16 KiB: 128 x 64 of either operand
   static constexpr int kStageBytes = 2 * kOperand;
-  static constexpr int kWarps = kMode == kGroupedDB ? 7 : 6;  // + the edge warp
-  static constexpr int kThreads = 32 * kWarps;
-  static constexpr int kStaging = kMode == kGroupedDB ? 4 * kStoreBufBytes : 0;
+  static constexpr int kThreads = 32 * 6;
+  static constexpr int kStaging = kMode == kGroupedDB ? 4 * 2 * kStoreBufBytes : 0;
   static constexpr int smem_bytes(int experts) {
     return kStages * kStageBytes + kStaging + group_table_bytes(experts) + 1024;
   }
 };
+
+// dB: maps[2 e] and maps[2 e + 1] are dC's and A's tensor maps, ended at the
+// last row of expert e.  One warp per expert.
+__global__ void __launch_bounds__(32)
+grouped_maps_kernel(const __grid_constant__ CUtensorMap tmap_dc,
+                    const __grid_constant__ CUtensorMap tmap_a, const int* offsets, int rows,
+                    CUtensorMap* maps) {
+  __shared__ alignas(128) CUtensorMap map[2];
+  grid_wait();
+  grid_launch_next();
+  const int e = blockIdx.x, lane = threadIdx.x;
+  uint32_t* words = reinterpret_cast<uint32_t*>(map);
+  words[lane] = reinterpret_cast<const uint32_t*>(&tmap_dc)[lane];
+  words[32 + lane] = reinterpret_cast<const uint32_t*>(&tmap_a)[lane];
+  // The end of expert e as the other kernels read it (build_groups): the
+  // largest of the clamped offsets up to its own.
+  int end = 0;
+  for (int i = lane; i <= e + 1; i += 32) end = max(end, min(offsets[i], rows));
+  end = __reduce_max_sync(0xffffffffu, end);
+  __syncwarp();
+  if (lane == 0) {
+    // (an extent is at least 1; an expert that ends at row 0 has no rows)
+    tmap_set_rows(smem_u32(&map[0]), end > 0 ? (uint32_t)end : 1u);
+    tmap_set_rows(smem_u32(&map[1]), end > 0 ? (uint32_t)end : 1u);
+  }
+  __syncwarp();
+  tmap_publish(maps + 2 * e, smem_u32(&map[0]));
+  tmap_publish(maps + 2 * e + 1, smem_u32(&map[1]));
+}
 
 // One work unit: a tile of one expert's product.
 struct GroupedUnit {
@@ -116,24 +149,21 @@ struct GroupedWalk {
   }
 };
 
-// tmap_w: forward the bank (k, n, e), box 64 x 128; dA the bank, box 64 x 64;
-//         dB dC (n, r), box 64 x 64.
-// tmap_t: the token operand (forward A, dA dC), box 64 x 128; dB A (k, r),
-//         box 64 x 64.
+// tmap_w: forward the bank (k, n, e), box 64 x 128; dA the bank, box 64 x 64.
+// tmap_t: the token operand (forward A, dA dC), box 64 x 128.
 // tmap_s: forward, dA: the token operand, box 64 x 16; dB: dB (k, n, e), box 64 x 32.
-template <int kMode, class T>
+template <int kMode, bool kMany, class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(GroupedCfg<kMode>::kThreads, 1)
 grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
                     const __grid_constant__ CUtensorMap tmap_t,
                     const __grid_constant__ CUtensorMap tmap_s, const GroupedArgs args) {
-  using C = GroupedCfg<kMode>;
+  using C = GroupedCfg<kMode, kMany>;
   constexpr int kStages = C::kStages;
   constexpr bool kMnA = kMode != kGroupedFwd;  // the M operand lies along rows
   constexpr bool kMnB = kMode == kGroupedDB;
   extern __shared__ uint8_t smem_raw[];
   __shared__ alignas(8) uint64_t bar_full[kStages];
   __shared__ alignas(8) uint64_t bar_empty[kStages];
-  __shared__ alignas(8) uint64_t bar_edge[kStages];
   __shared__ alignas(8) uint64_t bar_acc_full[2];
   __shared__ alignas(8) uint64_t bar_acc_empty[2];
   __shared__ alignas(8) uint64_t bar_drain;
@@ -152,9 +182,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
-      mbar_init(smem_u32(&bar_full[s]), 2);  // one arrival per CTA: its producer or its edge warp
+      mbar_init(smem_u32(&bar_full[s]), 2);  // each CTA's producer
       mbar_init(smem_u32(&bar_empty[s]), 1);
-      mbar_init(smem_u32(&bar_edge[s]), 1);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bar_acc_full[b]), 1);
@@ -163,8 +192,10 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     mbar_init(smem_u32(&bar_drain), 1);
     abort_word = 0;
     fence_mbar_init_cluster();
-    prefetch_tmap(&tmap_w);
-    prefetch_tmap(&tmap_t);
+    if (kMode != kGroupedDB) {
+      prefetch_tmap(&tmap_w);
+      prefetch_tmap(&tmap_t);
+    }
     prefetch_tmap(&tmap_s);
   }
   if (warp == 1) {
@@ -191,17 +222,14 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
   GroupedWalk<kMode> walk;
   walk.init(args, s_off, s_tiles);
   const int total = walk.total(args);
-  // Rows of an expert's last block, and whether some must be cleared (dB).
-  auto last_rows = [](const GroupedUnit& w) { return w.rows - kSlabK * (w.blocks - 1); };
-
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
       const uint32_t full_leader = cluster_map(smem_u32(&bar_full[0]), 0);
       const uint32_t empty_peer = cluster_map(smem_u32(&bar_empty[0]), 1);
-      const uint32_t edge_self = cluster_map(smem_u32(&bar_edge[0]), rank);
       const uint64_t keep = l2_policy_evict_last();
       uint32_t stage = 0, phase = 0, filled = 0;
+      int last_e = -1;
       bool ok = true;
       for (int u = pair; ok && u < total; u += npairs) {
         const GroupedUnit w = walk.unit(args, u);
@@ -209,6 +237,19 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         const int half = w.mma_n / 2;
         const int t0 = kMode == kGroupedDB ? w.col0 + (int)rank * 128 : w.row0 + (int)rank * half;
         const uint32_t bytes = C::kOperand + (half == 128 ? C::kOperand : half * 128);
+        const CUtensorMap* maps = args.maps + 2 * w.e;
+        if constexpr (kMode == kGroupedDB) {
+          // A new expert's maps are fetched a unit ahead of their use.
+          for (int v = u; v < total && v <= u + npairs; v += npairs) {
+            const int e = v == u ? w.e : walk.unit(args, v).e;
+            if (e <= last_e) continue;
+            tmap_acquire(args.maps + 2 * e);
+            tmap_acquire(args.maps + 2 * e + 1);
+            prefetch_tmap(args.maps + 2 * e);
+            prefetch_tmap(args.maps + 2 * e + 1);
+            last_e = e;
+          }
+        }
         for (int kb = 0; kb < w.blocks; ++kb) {
           if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
             ok = false;
@@ -216,8 +257,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
           }
           if (rank == 0 && filled >= (uint32_t)kStages) mbar_arrive_cluster(empty_peer + stage * 8u);
           ++filled;
-          const bool edge = kMode == kGroupedDB && kb == w.blocks - 1 && (last_rows(w) & 15) != 0;
-          const uint32_t fb = (edge ? edge_self : full_leader) + stage * 8u;
+          const uint32_t fb = full_leader + stage * 8u;
           const uint32_t sa = smem_base + stage * C::kStageBytes;
           const uint32_t sb = sa + C::kOperand;
           mbar_arrive_expect_tx_cluster(fb, bytes);
@@ -228,12 +268,12 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
             tma_load_3d_pair_hint(sa, &tmap_w, f0, k0, w.e, fb, keep);
             tma_load_3d_pair_hint(sa + C::kOperand / 2, &tmap_w, f0 + 64, k0, w.e, fb, keep);
           } else {
-            tma_load_2d_pair_hint(sa, &tmap_w, f0, w.row0 + k0, fb, keep);
-            tma_load_2d_pair_hint(sa + C::kOperand / 2, &tmap_w, f0 + 64, w.row0 + k0, fb, keep);
+            tma_load_2d_pair_hint(sa, maps, f0, w.row0 + k0, fb, keep);
+            tma_load_2d_pair_hint(sa + C::kOperand / 2, maps, f0 + 64, w.row0 + k0, fb, keep);
           }
           if constexpr (kMode == kGroupedDB) {
-            tma_load_2d_pair_hint(sb, &tmap_t, t0, w.row0 + k0, fb, keep);
-            tma_load_2d_pair_hint(sb + C::kOperand / 2, &tmap_t, t0 + 64, w.row0 + k0, fb, keep);
+            tma_load_2d_pair_hint(sb, maps + 1, t0, w.row0 + k0, fb, keep);
+            tma_load_2d_pair_hint(sb + C::kOperand / 2, maps + 1, t0 + 64, w.row0 + k0, fb, keep);
           } else if (half == 128) {
             tma_load_2d_pair_hint(sb, &tmap_t, k0, t0, fb, keep);
           } else {
@@ -257,6 +297,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
       for (int u = pair; ok && u < total; u += npairs) {
         const GroupedUnit w = walk.unit(args, u);
         if (w.blocks == 0) continue;
+        const int red = kMode == kGroupedDB ? w.rows : args.red;
         const uint32_t idesc = make_idesc_16bit(kPairM, w.mma_n, kFormat<T>, kMnA, kMnB);
         const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
         ++it;
@@ -265,14 +306,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * 256;
         for (int kb = 0; kb < w.blocks; ++kb) {
-          // Blocks cleared by the edge warps were written by threads of both
-          // CTAs: those need the wait at cluster scope.
-          const int left = kMode == kGroupedDB ? w.rows - kb * kSlabK : args.red - kb * kSlabK;
-          const bool edge = kMode == kGroupedDB && left < kSlabK && (left & 15) != 0;
-          const bool landed =
-              edge ? wait_bounded_acq_cluster(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)
-                   : wait_ready(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull);
-          if (!landed) {
+          if (!wait_ready(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)) {
             ok = false;
             break;
           }
@@ -283,6 +317,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
               kMnA ? make_sdesc_mn128(sa, C::kOperand / 2) : make_sdesc_k128(sa);
           const uint64_t bdesc =
               kMnB ? make_sdesc_mn128(sb, C::kOperand / 2) : make_sdesc_k128(sb);
+          const int left = red - kb * kSlabK;
           const int steps = left >= kSlabK ? kSlabK / kMmaK : (left + kMmaK - 1) / kMmaK;
 #pragma unroll
           for (int k = 0; k < kSlabK / kMmaK; ++k) {
@@ -303,7 +338,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         wait_slow(smem_u32(&bar_drain), 0, wctx, kErrWaitDrain, false);
     }
     __syncwarp();
-  } else if (warp < 6) {
+  } else {
     // ----------------------------------------------------------- epilogue
     const int quarter = warp & 3;
     const uint32_t acc_empty_leader = cluster_map(smem_u32(&bar_acc_empty[0]), 0);
@@ -311,12 +346,13 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     if constexpr (kMode != kGroupedDB)
       zero_unowned_rows(out, args.ldo, args.feat, s_off[0], s_off[args.experts], args.rows,
                         (long long)blockIdx.x * 128 + (threadIdx.x - 64), gridDim.x * 128ll);
-    const uint32_t my_store = store_base + (uint32_t)(warp - 2) * kStoreBufBytes;
+    const uint32_t my_store = store_base + (uint32_t)(warp - 2) * 2 * kStoreBufBytes;
     int it = 0;
     for (int u = pair; u < total; u += npairs) {
       const GroupedUnit w = walk.unit(args, u);
       const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
-      if (w.blocks != 0) {
+      const bool any = w.blocks != 0;
+      if (any) {
         ++it;
         int ok = 0;
         if (lane == 0)
@@ -332,7 +368,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
 #pragma unroll 1
         for (int c = 0; c < 256 / kStoreCols; ++c) {
           uint32_t v0[32], v1[32];
-          if (w.blocks != 0) {
+          if (any) {
             tmem_ld_32x32b_x32(tbase + c * kStoreCols, v0);
             tmem_ld_32x32b_x32(tbase + c * kStoreCols + 32, v1);
             tmem_wait_ld();
@@ -345,7 +381,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
 #pragma unroll
             for (int j = 0; j < 32; ++j) v0[j] = v1[j] = 0;
           }
-          if (lane == 0) bulk_wait_group_read<0>();
+          const uint32_t box = my_store + (c & 1) * kStoreBufBytes;
+          if (lane == 0) bulk_wait_group_read<1>();  // the store before last has read it
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
@@ -354,15 +391,15 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
 #pragma unroll
             for (int q = 0; q < 4; ++q)
               p[q] = pack_pair<T>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
-            st_shared_v4(my_store + lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), p[0], p[1],
-                         p[2], p[3]);
+            st_shared_v4(box + lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), p[0], p[1], p[2],
+                         p[3]);
           }
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
             // (a box that starts past the matrix has nothing to write)
             if (f0 < args.feat && w.col0 + c * kStoreCols < args.cols)
-              tma_store_3d(&tmap_s, my_store, w.col0 + c * kStoreCols, f0, w.e);
+              tma_store_3d(&tmap_s, box, w.col0 + c * kStoreCols, f0, w.e);
             bulk_commit_group();
           }
         }
@@ -403,37 +440,6 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
       }
     }
     if (kMode == kGroupedDB && lane == 0) bulk_wait_group_read<0>();
-    __syncwarp();
-  } else {
-    // --------------------------------------------------------------- edge
-    // (dB) clear the rows of an expert's last block that its last K16 step
-    // would read beyond the group, in both operands of this CTA.
-    const uint32_t full_leader = cluster_map(smem_u32(&bar_full[0]), 0);
-    uint32_t stage = 0, parity = 0;  // parity: one bit per stage's edge barrier
-    bool ok = true;
-    for (int u = pair; ok && u < total; u += npairs) {
-      const GroupedUnit w = walk.unit(args, u);
-      if (w.blocks == 0) continue;
-      const int valid = last_rows(w);
-      const uint32_t s = (stage + w.blocks - 1) % kStages;
-      stage = (stage + w.blocks) % kStages;
-      if ((valid & 15) == 0) continue;
-      int got = 0;
-      if (lane == 0)
-        got = wait_ready(smem_u32(&bar_edge[s]), (parity >> s) & 1u, wctx, kErrWaitFull);
-      ok = __shfl_sync(0xffffffffu, got, 0) != 0;
-      __syncwarp();
-      if (!ok) break;
-      parity ^= 1u << s;
-      const int clear = 16 - (valid & 15);  // rows, 8 chunks of 16 B each, in 4 slabs of 64 rows
-      const uint32_t base = smem_base + s * C::kStageBytes + valid * 128u;
-      for (int i = lane; i < clear * 32; i += 32)
-        st_shared_v4(base + (uint32_t)(i & 3) * (C::kOperand / 2) + (uint32_t)(i >> 2) * 16u, 0, 0,
-                     0, 0);
-      fence_proxy_async_all();
-      __syncwarp();
-      if (lane == 0) mbar_arrive_release_cluster(full_leader + s * 8u);
-    }
     __syncwarp();
   }
 

@@ -41,15 +41,21 @@ bool set_smem(F* fn, int bytes) {
          cudaSuccess;
 }
 
-template <int kMode, class T>
+// dB: experts whose table fits beside six stages.
+constexpr int kFewExperts = 128;
+
+template <int kMode, bool kMany, class T>
 bool init_pair(int sms, int* pairs) {
-  using C = GroupedCfg<kMode>;
-  auto* fn = grouped_pair_kernel<kMode, T>;
-  if (!set_smem(fn, C::smem_bytes(kMaxExperts))) return false;
+  using C = GroupedCfg<kMode, kMany>;
+  constexpr int experts = kMode == kGroupedDB && !kMany ? kFewExperts : kMaxExperts;
+  // (512 B: more than the kernel's static shared memory)
+  static_assert(C::smem_bytes(experts) <= 227 * 1024 - 512, "shared memory of one CTA");
+  auto* fn = grouped_pair_kernel<kMode, kMany, T>;
+  if (!set_smem(fn, C::smem_bytes(experts))) return false;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * sms);
   cfg.blockDim = dim3(C::kThreads);
-  cfg.dynamicSmemBytes = C::smem_bytes(kMaxExperts);
+  cfg.dynamicSmemBytes = C::smem_bytes(experts);
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -85,8 +91,10 @@ bool init_w4() {
 
 template <class T>
 bool init_type(MoeDevice& m, int sms) {
-  return init_pair<kGroupedFwd, T>(sms, &m.pairs[0]) && init_pair<kGroupedDA, T>(sms, &m.pairs[1]) &&
-         init_pair<kGroupedDB, T>(sms, &m.pairs[2]) && init_stream<false, T>() &&
+  return init_pair<kGroupedFwd, false, T>(sms, &m.pairs[0]) &&
+         init_pair<kGroupedDA, false, T>(sms, &m.pairs[1]) &&
+         init_pair<kGroupedDB, false, T>(sms, &m.pairs[2]) &&
+         init_pair<kGroupedDB, true, T>(sms, &m.pairs[2]) && init_stream<false, T>() &&
          init_stream<true, T>() && init_w4<32, T>() && init_w4<64, T>() && init_w4<128, T>();
 }
 
@@ -183,6 +191,22 @@ struct Workspace {
   }
 };
 
+// A buffer of the device's pool for one call, freed in stream order.
+struct PoolBuffer {
+  void* p = nullptr;
+  cudaStream_t stream = nullptr;
+  int take(const DeviceView& v, size_t bytes, cudaStream_t s) {
+    stream = s;
+    if (cudaMallocFromPoolAsync(&p, bytes, v.pool, s) == cudaSuccess) return B200_OK;
+    cudaGetLastError();
+    p = nullptr;
+    return B200_ERR_LAUNCH;
+  }
+  ~PoolBuffer() {
+    if (p) cudaFreeAsync(p, stream);
+  }
+};
+
 CUtensorMapDataType map_type(int dtype) {
   return dtype == B200_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
 }
@@ -271,9 +295,9 @@ int launch(void (*fn)(P...), int blocks, int threads, size_t smem, cudaStream_t 
   return B200_ERR_LAUNCH;
 }
 
-template <int kMode, class T>
+template <int kMode, bool kMany, class T>
 int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStream_t stream) {
-  using C = GroupedCfg<kMode>;
+  using C = GroupedCfg<kMode, kMany>;
   CUtensorMap tw, tt, ts;
   int st;
   if (kMode == kGroupedDB) {
@@ -289,6 +313,14 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
     if (st == B200_OK) st = map_rows(&ts, c.dtype, c.t, red, c.rows, c.ldt, 16);
   }
   if (st != B200_OK) return st;
+  PoolBuffer maps;
+  if (kMode == kGroupedDB) {
+    st = maps.take(v, (size_t)c.experts * 2 * sizeof(CUtensorMap), stream);
+    if (st == B200_OK)
+      st = launch(grouped_maps_kernel, c.experts, 32, 0, stream, tw, tt, c.offsets, c.rows,
+                  static_cast<CUtensorMap*>(maps.p));
+    if (st != B200_OK) return st;
+  }
   GroupedArgs a = {};
   a.offsets = c.offsets;
   a.experts = c.experts;
@@ -299,6 +331,7 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
   a.out = kMode == kGroupedDB ? nullptr : c.u;
   a.ldo = c.ldu;
   a.group = 8;
+  a.maps = static_cast<const CUtensorMap*>(maps.p);
   a.status = v.status;
   a.timeout_ns = v.timeout_ns;
   const long long tf = ceil_div(a.feat, 256);
@@ -306,8 +339,8 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
                              ? tf * ceil_div(c.K, 256) * c.experts
                              : tf * (ceil_div(c.rows, 256) + (c.experts < c.rows ? c.experts : c.rows));
   const int pairs = (int)(most < m.pairs[kMode] ? most : m.pairs[kMode]);
-  return launch(grouped_pair_kernel<kMode, T>, 2 * pairs, C::kThreads, C::smem_bytes(c.experts),
-                stream, tw, tt, ts, a);
+  return launch(grouped_pair_kernel<kMode, kMany, T>, 2 * pairs, C::kThreads,
+                C::smem_bytes(c.experts), stream, tw, tt, ts, a);
 }
 
 template <bool kDA, int kTok, class T>
@@ -363,7 +396,10 @@ int run_typed(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStream
       return c.rows <= 16 ? launch_stream<kDA, 16, T>(c, v, stream)
                           : launch_stream<kDA, 64, T>(c, v, stream);
   }
-  return launch_pair<kMode, T>(c, v, m, stream);
+  if constexpr (kMode == kGroupedDB) {
+    if (c.experts > kFewExperts) return launch_pair<kMode, true, T>(c, v, m, stream);
+  }
+  return launch_pair<kMode, false, T>(c, v, m, stream);
 }
 
 template <int kMode>

@@ -449,6 +449,26 @@ __device__ __forceinline__ unsigned int atomic_add_acq_rel(unsigned int* p, unsi
   return old;
 }
 
+// ------------------------------------------------------ tensor maps made here
+// A tensor map (128 bytes, 128-byte aligned) in shared memory: the extent of
+// its dimension 1.
+__device__ __forceinline__ void tmap_set_rows(uint32_t smem_map, uint32_t rows) {
+  asm volatile("tensormap.replace.tile.global_dim.shared::cta.b1024.b32 [%0], 1, %1;"
+               :: "r"(smem_map), "r"(rows) : "memory");
+}
+// A whole warp copies it to global memory, to be used by TMA there after a
+// tmap_acquire.
+__device__ __forceinline__ void tmap_publish(CUtensorMap* global_map, uint32_t smem_map) {
+  asm volatile(
+      "tensormap.cp_fenceproxy.global.shared::cta.tensormap::generic.release.gpu.sync.aligned "
+      "[%0], [%1], 128;"
+      :: "l"(reinterpret_cast<uint64_t>(global_map)), "r"(smem_map) : "memory");
+}
+__device__ __forceinline__ void tmap_acquire(const CUtensorMap* m) {
+  asm volatile("fence.proxy.tensormap::generic.acquire.gpu [%0], 128;"
+               :: "l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
 // ------------------------------------- three-dimensional tiles, bulk copies
 // Three-dimensional forms of the pair load, the single-CTA load and the
 // store: the third coordinate selects a matrix of a bank.
