@@ -6,6 +6,7 @@
 // Operators with gradients are autograd functions here in C++, so a training
 // step pays no Python call per node.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -28,6 +29,12 @@ bool aligned16(const at::Tensor& t) {
 }
 
 void* current_stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+// A new contiguous tensor on `like`'s device, past the dispatcher (0.9 us a
+// tensor against 1.8: a decode step makes a dozen of them).
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor& like) {
+  return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
 
 int dtype_code(const at::Tensor& t) {
   return t.scalar_type() == at::kHalf ? B200_FP16 : B200_BF16;
@@ -58,7 +65,7 @@ Rows as_rows(const at::Tensor& t) {
   if ((cols == 1 || t.stride(1) == 1) && ld >= cols && ld % 8 == 0 && ld < (1ll << 31) &&
       aligned16(t))
     return {t, (int)ld};
-  auto buf = at::empty({rows, pad}, t.options());
+  auto buf = fresh({rows, pad}, t.scalar_type(), t);
   auto view = buf.narrow(1, 0, cols);
   view.copy_(t);
   return {view, (int)pad};
@@ -80,7 +87,7 @@ Bank as_bank(const at::Tensor& t) {
   if ((k == 1 || t.stride(2) == 1) && ld >= k && ld % 8 == 0 && ld < (1ll << 31) &&
       stride % 8 == 0 && stride >= n * ld && aligned16(t))
     return {t, (int)ld, stride};
-  auto buf = at::empty({e, n, pad}, t.options());
+  auto buf = fresh({e, n, pad}, t.scalar_type(), t);
   auto view = buf.narrow(2, 0, k);
   view.copy_(t);
   return {view, (int)pad, n * pad};
@@ -99,7 +106,7 @@ struct Result {
 
 Result new_rows(int64_t rows, int64_t cols, const at::Tensor& like) {
   const int64_t pad = round_up8(cols);
-  return {at::empty({rows, pad}, like.options()), cols, (int)std::max<int64_t>(pad, 8)};
+  return {fresh({rows, pad}, like.scalar_type(), like), cols, (int)std::max<int64_t>(pad, 8)};
 }
 
 at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::Tensor& like,
@@ -109,6 +116,7 @@ at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::T
   TORCH_CHECK(offsets.device() == like.device(), who, ": offsets must be on the operands' device");
   TORCH_CHECK(offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong, who,
               ": offsets must be int32 or int64");
+  if (offsets.scalar_type() == at::kInt && offsets.is_contiguous()) return offsets;
   return offsets.to(at::kInt).contiguous();
 }
 
@@ -149,7 +157,7 @@ at::Tensor grouped_db(const at::Tensor& dc, const at::Tensor& a, const at::Tenso
   const int64_t experts = offsets.size(0) - 1, n = dc.size(1), k = a.size(1), pad = round_up8(k);
   const Rows rc = as_rows(dc);
   const Rows ra = as_rows(a);
-  auto db = at::empty({experts, n, pad}, dc.options());
+  auto db = fresh({experts, n, pad}, dc.scalar_type(), dc);
   check_status(b200_grouped_gemm_db(rc.t.data_ptr(), ra.t.data_ptr(), db.data_ptr(),
                                     offsets.data_ptr<int>(), (int)dc.size(0), (int)experts, (int)n,
                                     (int)k, rc.ld, ra.ld, (int)std::max<int64_t>(pad, 8), n * pad,
@@ -218,10 +226,9 @@ std::vector<at::Tensor> route_forward(const at::Tensor& logits, int64_t top_k, b
   const c10::cuda::CUDAGuard guard(logits.device());
   const int64_t t = logits.size(0), e = logits.size(1);
   const at::Tensor l = unit_rows(logits);
-  const auto ints = logits.options().dtype(at::kInt);
-  auto weights = at::empty({t, top_k}, logits.options().dtype(at::kFloat));
-  auto chosen = at::empty({t, top_k}, ints), rows = at::empty({t, top_k}, ints);
-  auto sources = at::empty({t * top_k}, ints), offsets = at::empty({e + 1}, ints);
+  auto weights = fresh({t, top_k}, at::kFloat, logits);
+  auto chosen = fresh({t, top_k}, at::kInt, logits), rows = fresh({t, top_k}, at::kInt, logits);
+  auto sources = fresh({t * top_k}, at::kInt, logits), offsets = fresh({e + 1}, at::kInt, logits);
   check_status(b200_route(l.data_ptr(), (int)t, (int)e, row_stride(l), logit_code(l), (int)top_k,
                           normalize, weights.data_ptr<float>(), chosen.data_ptr<int>(),
                           rows.data_ptr<int>(), sources.data_ptr<int>(), offsets.data_ptr<int>(),
@@ -247,7 +254,7 @@ struct Route : torch::autograd::Function<Route> {
       const c10::cuda::CUDAGuard guard(logits.device());
       const at::Tensor l = unit_rows(logits);
       const at::Tensor dw = grads[0].to(at::kFloat).contiguous();
-      dlogits = at::empty({l.size(0), l.size(1)}, l.options());
+      dlogits = fresh({l.size(0), l.size(1)}, l.scalar_type(), l);
       check_status(b200_route_grad(l.data_ptr(), (int)l.size(0), (int)l.size(1), row_stride(l),
                                    logit_code(l), (int)chosen.size(1),
                                    ctx->saved_data["normalize"].toBool(), chosen.data_ptr<int>(),
@@ -300,7 +307,7 @@ at::Tensor dispatch_forward(const at::Tensor& x, const at::Tensor& rows,
                             const at::Tensor& offsets) {
   const c10::cuda::CUDAGuard guard(x.device());
   const at::Tensor in = unit_rows(x);
-  auto xs = at::empty({rows.numel(), x.size(1)}, x.options());
+  auto xs = fresh({rows.numel(), x.size(1)}, x.scalar_type(), x);
   check_status(b200_dispatch(in.data_ptr(), rows.data_ptr<int>(), total_of(offsets), xs.data_ptr(),
                              (int)rows.size(0), (int)rows.size(1), (int)x.size(1), row_stride(in),
                              x.size(1), dtype_code(x), current_stream()),
@@ -312,7 +319,7 @@ at::Tensor combine_forward(const at::Tensor& y, const float* weights, const at::
                            const char* who) {
   const c10::cuda::CUDAGuard guard(y.device());
   const at::Tensor in = unit_rows(y);
-  auto out = at::empty({rows.size(0), y.size(1)}, y.options());
+  auto out = fresh({rows.size(0), y.size(1)}, y.scalar_type(), y);
   check_status(b200_combine(in.data_ptr(), weights, rows.data_ptr<int>(), out.data_ptr(),
                             (int)rows.size(0), (int)rows.size(1), (int)y.size(1), row_stride(in),
                             y.size(1), dtype_code(y), current_stream()),
@@ -355,8 +362,9 @@ struct Combine : torch::autograd::Function<Combine> {
     if (grads[0].defined()) {
       const c10::cuda::CUDAGuard guard(y.device());
       const at::Tensor dout = unit_rows(grads[0].to(y.scalar_type())), in = unit_rows(y);
-      dy = at::empty({y.size(0), y.size(1)}, y.options());
-      if (ctx->needs_input_grad(1)) dweights = at::empty({rows.size(0), rows.size(1)}, weights.options());
+      dy = fresh({y.size(0), y.size(1)}, y.scalar_type(), y);
+      if (ctx->needs_input_grad(1))
+        dweights = fresh({rows.size(0), rows.size(1)}, at::kFloat, weights);
       check_status(
           b200_combine_grad(dout.data_ptr(), in.data_ptr(), weights.data_ptr<float>(),
                             rows.data_ptr<int>(), total_of(offsets), dy.data_ptr(),
@@ -375,7 +383,7 @@ at::Tensor combine_b200(const at::Tensor& y, const at::Tensor& weights, const at
   TORCH_CHECK(weights.sizes() == rows.sizes() && weights.scalar_type() == at::kFloat &&
                   weights.device() == y.device(),
               kCombine, ": weights must be float32 (tokens, top_k) on y's device");
-  const at::Tensor w = weights.contiguous();
+  const at::Tensor w = weights.is_contiguous() ? weights : weights.contiguous();
   if (at::GradMode::is_enabled() && (y.requires_grad() || w.requires_grad()))
     return Combine::apply(y, w, rows, offsets);
   return combine_forward(y, w.data_ptr<float>(), rows, kCombine);
@@ -415,7 +423,7 @@ at::Tensor w4_pack(const at::Tensor& q, const at::Tensor& scales,
   size_t bytes = 0;
   check_status(b200_w4_packed_bytes((int)e, (int)n, (int)k, (int)group, z.defined(), &bytes),
                kPack);
-  auto packed = at::empty({(int64_t)bytes}, q.options());
+  auto packed = fresh({(int64_t)bytes}, at::kByte, q);
   const at::Tensor qc = q.contiguous(), sc = scales.contiguous();
   check_status(b200_w4_pack(qc.data_ptr(), sc.data_ptr(), z.defined() ? z.data_ptr() : nullptr,
                             packed.data_ptr(), (int)e, (int)n, (int)k, (int)group,

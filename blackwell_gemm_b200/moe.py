@@ -13,9 +13,15 @@ __all__ = ["Routing", "route_b200", "dispatch_b200", "combine_b200", "matmul_b20
            "W4Weight", "pack_w4", "quantize_w4", "matmul_b200_w4"]
 
 
+_loaded = None
+
+
 def _ext():
-    from . import load
-    return load()
+    global _loaded
+    if _loaded is None:
+        from . import load
+        _loaded = load()
+    return _loaded
 
 
 class Routing(NamedTuple):
