@@ -19,7 +19,7 @@
 
 namespace b200 {
 
-constexpr int kRouteThreads = 512;
+constexpr int kRouteThreads = 1024;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kMaxTopK = 32;
 
@@ -59,18 +59,24 @@ __device__ __forceinline__ float warp_sum(float v) {
   return v;
 }
 
-// One warp, one token: expert i of the row is value i / 32 of lane i % 32.
+// A token's logits in a warp: expert i of the row is value i / 32 of lane i % 32.
 template <int kPer>
-__device__ __forceinline__ void choose_token(const RouteArgs& a, int t, int* hist) {
+__device__ __forceinline__ void load_token(const RouteArgs& a, int t, float (&v)[kPer]) {
   const int lane = threadIdx.x & 31;
-  float v[kPer];
-  uint32_t key[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int e = i * 32 + lane;
     v[i] = e < a.experts ? load_logit(a.logits, a.type, t * a.ld + e) : -INFINITY;
-    key[i] = order_key(v[i]);
   }
+}
+
+template <int kPer>
+__device__ __forceinline__ void choose_token(const RouteArgs& a, int t, const float (&v)[kPer],
+                                             int* hist) {
+  const int lane = threadIdx.x & 31;
+  uint32_t key[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) key[i] = order_key(v[i]);
   float base = 0.0f, mine = 0.0f, sum = 0.0f;
   int slot_expert = -1;  // lane j keeps slot j
   for (int j = 0; j < a.top_k; ++j) {
@@ -118,8 +124,16 @@ template <int kPer>
 __device__ __forceinline__ void choose_chunk(const RouteArgs& a, int first, int last, int* hist) {
   for (int i = threadIdx.x; i < a.experts; i += kRouteThreads) hist[i] = 0;
   __syncthreads();
-  for (int t = first + (threadIdx.x >> 5); t < last; t += kRouteWarps)
-    choose_token<kPer>(a, t, hist);
+  // (a warp's next token is on its way while it chooses for this one)
+  int t = first + (threadIdx.x >> 5);
+  float v[kPer], next[kPer];
+  if (t < last) load_token<kPer>(a, t, v);
+  for (; t < last; t += kRouteWarps) {
+    if (t + kRouteWarps < last) load_token<kPer>(a, t + kRouteWarps, next);
+    choose_token<kPer>(a, t, v, hist);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = next[i];
+  }
   __syncthreads();
 }
 
@@ -142,25 +156,40 @@ __device__ __forceinline__ int scan_experts(int* totals, int n) {
   return run;
 }
 
-// Rows of the chunk's pairs.  start[e]: offsets[e] + pairs of earlier chunks;
-// cursor[warp][e]: next row of this warp's part of the chunk.
-__device__ __forceinline__ void rank_chunk(const RouteArgs& a, int first, int last,
-                                           const int* start, int* cursor) {
+// A warp's part of a chunk's pairs, [lo, hi) from `base`, in steps of 32.
+struct RoutePart {
+  long long base;
+  int lo, hi;
+  int first;  // the expert of pair lo + lane, -1 past the end
+};
+__device__ __forceinline__ RoutePart route_part(const RouteArgs& a, int first, int last) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int pairs = (last - first) * a.top_k;
   const int part = ((pairs + kRouteWarps - 1) / kRouteWarps + 31) & ~31;
-  const long long base = (long long)first * a.top_k;
-  const int lo = min(warp * part, pairs), hi = min(lo + part, pairs);
+  RoutePart p;
+  p.base = (long long)first * a.top_k;
+  p.lo = min(warp * part, pairs);
+  p.hi = min(p.lo + part, pairs);
+  p.first = p.lo + lane < p.hi ? a.chosen[p.base + p.lo + lane] : -1;
+  return p;
+}
+
+// Rows of the chunk's pairs.  start[e]: offsets[e] + pairs of earlier chunks;
+// cursor[warp][e]: next row of this warp's part of the chunk.
+__device__ __forceinline__ void rank_chunk(const RouteArgs& a, const RoutePart& p,
+                                           const int* start, int* cursor) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int i = threadIdx.x; i < kRouteWarps * a.experts; i += kRouteThreads) cursor[i] = 0;
   __syncthreads();
   int* mine = cursor + warp * a.experts;
-  for (int i = lo + lane; i < hi; i += 32) {
-    const int e = a.chosen[base + i];
+  for (int i = p.lo + lane; i < p.hi; i += 32) {
+    const int e = i == p.lo + lane ? p.first : a.chosen[p.base + i];
     if (e >= 0) atomicAdd(mine + e, 1);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
     int at = start[e];
+#pragma unroll 8
     for (int w = 0; w < kRouteWarps; ++w) {
       const int n = cursor[w * a.experts + e];
       cursor[w * a.experts + e] = at;
@@ -168,20 +197,20 @@ __device__ __forceinline__ void rank_chunk(const RouteArgs& a, int first, int la
     }
   }
   __syncthreads();
-  for (int i = lo; i < hi; i += 32) {
-    const bool in = i + lane < hi;
-    const int e = in ? a.chosen[base + i + lane] : -1;
+  for (int i = p.lo; i < p.hi; i += 32) {
+    const bool in = i + lane < p.hi;
+    const int e = i == p.lo ? p.first : in ? a.chosen[p.base + i + lane] : -1;
     const unsigned int same = __match_any_sync(0xffffffffu, e);
     const int before = __popc(same & ((1u << lane) - 1u));
     int row = -1;
     if (e >= 0) {
       row = mine[e] + before;
-      a.sources[row] = (int)((base + i + lane) / a.top_k);
+      a.sources[row] = (int)((p.base + i + lane) / a.top_k);
     }
     __syncwarp();
     if (e >= 0 && before == 0) mine[e] += __popc(same);
     __syncwarp();
-    if (in) a.rows[base + i + lane] = row;
+    if (in) a.rows[p.base + i + lane] = row;
   }
 }
 
@@ -216,7 +245,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_choose_kernel(const Route
   __syncthreads();
   for (int e = threadIdx.x; e <= a.experts; e += kRouteThreads)
     a.offsets[e] = e < a.experts ? hist[e] : total;
-  rank_chunk(a, first, last, hist, s_route + a.experts);
+  rank_chunk(a, route_part(a, first, last), hist, s_route + a.experts);
   mark_unowned(a, total);
 }
 
@@ -227,15 +256,24 @@ __global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteAr
   int* start = s_route;                 // totals, then offsets, then + earlier chunks
   int* earlier = s_route + a.experts;   // (the cursors take this over)
   __shared__ int total;
-  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) {
+  const int first = blockIdx.x * a.chunk;
+  const RoutePart part = route_part(a, first, min(a.tokens, first + a.chunk));
+  // Counts of all chunks and of the earlier ones: a thread adds up a share of
+  // the chunks for one expert (16 loads in flight), shared memory the shares.
+  for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] = earlier[e] = 0;
+  __syncthreads();
+  const int shares = a.experts < kRouteThreads ? kRouteThreads / a.experts : 1;
+  for (int i = threadIdx.x; i < shares * a.experts; i += kRouteThreads) {
+    const int e = i % a.experts;
     int all = 0, before = 0;
-    for (int b = 0; b < (int)gridDim.x; ++b) {
-      const int n = a.counts[(long long)b * a.experts + e];
+#pragma unroll 16
+    for (int b = i / a.experts; b < (int)gridDim.x; b += shares) {
+      const int n = __ldg(a.counts + (long long)b * a.experts + e);
       all += n;
-      if (b < (int)blockIdx.x) before += n;
+      before += b < (int)blockIdx.x ? n : 0;
     }
-    start[e] = all;
-    earlier[e] = before;
+    atomicAdd(start + e, all);
+    atomicAdd(earlier + e, before);
   }
   __syncthreads();
   if (threadIdx.x < 32) {
@@ -249,62 +287,72 @@ __global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteAr
   __syncthreads();
   for (int e = threadIdx.x; e < a.experts; e += kRouteThreads) start[e] += earlier[e];
   __syncthreads();
-  const int first = blockIdx.x * a.chunk;
-  rank_chunk(a, first, min(a.tokens, first + a.chunk), start, s_route + a.experts);
+  rank_chunk(a, part, start, s_route + a.experts);
   mark_unowned(a, total);
 }
 
 // Gradient in the logits, one warp per token:
 //   over the chosen:  w_j (dw_j - sum_i w_i dw_i) at chosen experts, else 0
 //   over all:         p_e ([e chosen] dw_e - sum_j w_j dw_j)
+template <int kPer>
 __global__ void __launch_bounds__(256)
-route_grad_kernel(const void* logits, long long ld, int type, const int* __restrict__ chosen,
-                  const float* __restrict__ weights, const float* __restrict__ dweights,
-                  void* dlogits, int tokens, int experts, int top_k, bool normalize) {
+route_grad_kernel(const RouteArgs a, const float* __restrict__ dweights, void* dlogits) {
   grid_wait();
   grid_launch_next();
   const int lane = threadIdx.x & 31;
-  const long long t = (long long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (t >= tokens) return;
-  const long long at = t * top_k + lane;
-  const int e = lane < top_k ? chosen[at] : -1;
-  const float w = e >= 0 ? weights[at] : 0.0f;
+  const int t = blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (t >= a.tokens) return;
+  float v[kPer];
+  if (!a.normalize) load_token<kPer>(a, t, v);
+  const long long at = (long long)t * a.top_k + lane;
+  const int e = lane < a.top_k ? a.chosen[at] : -1;
+  const float w = e >= 0 ? a.weights[at] : 0.0f;
   const float dw = e >= 0 ? dweights[at] : 0.0f;
   const float inner = warp_sum(e >= 0 ? w * dw : 0.0f);
-  const int top = __shfl_sync(0xffffffffu, e, 0);
+  // what the chosen experts get: their weights and the weights' gradients
+  float share[kPer], hit[kPer];
+  uint32_t took = 0;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) share[i] = hit[i] = 0.0f;
+  for (int j = 0; j < a.top_k; ++j) {
+    const int ej = __shfl_sync(0xffffffffu, e, j);
+    const float wj = __shfl_sync(0xffffffffu, w, j), dj = __shfl_sync(0xffffffffu, dw, j);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (ej == i * 32 + lane) {
+        share[i] = wj;
+        hit[i] = dj;
+        took |= 1u << i;
+      }
+  }
   float base = 0.0f, sum = 1.0f;
-  if (!normalize && top >= 0) {
-    base = load_logit(logits, type, t * ld + top);
+  const int top = __shfl_sync(0xffffffffu, e, 0);
+  if (!a.normalize && top >= 0) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i == top >> 5) base = v[i];
+    base = __shfl_sync(0xffffffffu, base, top & 31);
     float part = 0.0f;
-    for (int i = lane; i < experts; i += 32)
-      part += expf(load_logit(logits, type, t * ld + i) - base);
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      if (i * 32 + lane < a.experts) part += expf(v[i] - base);
     sum = warp_sum(part);
   }
-  for (int i0 = 0; i0 < experts; i0 += 32) {
-    const int i = i0 + lane;
-    float hit = 0.0f, share = 0.0f;
-    bool took = false;
-    for (int j = 0; j < top_k; ++j) {
-      const int ej = __shfl_sync(0xffffffffu, e, j);
-      const float wj = __shfl_sync(0xffffffffu, w, j), dj = __shfl_sync(0xffffffffu, dw, j);
-      if (ej == i) {
-        took = true;
-        hit = dj;
-        share = wj;
-      }
-    }
-    if (i >= experts) continue;
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) {
+    const int ei = i * 32 + lane;
+    if (ei >= a.experts) continue;
+    const bool mine = took >> i & 1u;
     float g = 0.0f;
-    if (normalize) {
-      if (took) g = share * (hit - inner);
-    } else if (top >= 0) {
-      const float l = load_logit(logits, type, t * ld + i);
+    if (a.normalize) {
+      if (mine) g = share[i] * (hit[i] - inner);
+    } else if (top >= 0 && v[i] != -INFINITY) {
       // (a closed expert has no share; NaN and inf take part as they are)
-      if (l != -INFINITY) g = (took ? share : expf(l - base) / sum) * (hit - inner);
+      g = (mine ? share[i] : expf(v[i] - base) / sum) * (hit[i] - inner);
     }
-    const long long o = t * experts + i;
-    if (type == 2) static_cast<float*>(dlogits)[o] = g;
-    else if (type == 1) static_cast<__half*>(dlogits)[o] = __float2half_rn(g);
+    const long long o = (long long)t * a.experts + ei;
+    if (a.type == 2) static_cast<float*>(dlogits)[o] = g;
+    else if (a.type == 1) static_cast<__half*>(dlogits)[o] = __float2half_rn(g);
     else static_cast<__nv_bfloat16*>(dlogits)[o] = __float2bfloat16_rn(g);
   }
 }
@@ -349,9 +397,10 @@ __device__ __forceinline__ void store_pack(void* base, long long i, const Pack<T
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 
-// A token's rows and weights into shared memory; a row that is no row of the
-// operand is treated as none.
+// A token's rows and weights into shared memory, and the number of owned rows
+// behind the rows; a row that is no row of the operand is treated as none.
 __device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* s_row, float* s_w) {
+  if (threadIdx.x == kMaxTopK - 1 && a.total != nullptr) s_row[kMaxTopK] = *a.total;
   if ((int)threadIdx.x < a.top_k) {
     const long long at = t * a.top_k + threadIdx.x;
     const int r = a.rows[at];
@@ -364,8 +413,7 @@ __device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* 
 // Rows t * top_k .. of the sorted operand that no expert owns are zeroed by
 // token t's block.
 template <class T, int kVec>
-__device__ __forceinline__ void zero_tail(const MoveArgs& a, long long t) {
-  const int total = *a.total;
+__device__ __forceinline__ void zero_tail(const MoveArgs& a, long long t, int total) {
   for (int j = 0; j < a.top_k; ++j) {
     const long long r = t * a.top_k + j;
     if (r < total) continue;
@@ -381,7 +429,7 @@ template <class T, int kVec>
 __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK];
+  __shared__ int s_row[kMaxTopK + 1];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
   load_slots(a, t, s_row, s_w);
@@ -390,14 +438,14 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
     for (int j = 0; j < a.top_k; ++j)
       if (s_row[j] >= 0) store_pack<T, kVec>(a.out, (long long)s_row[j] * a.ld_out + c, p);
   }
-  zero_tail<T, kVec>(a, t);
+  zero_tail<T, kVec>(a, t, s_row[kMaxTopK]);
 }
 
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK];
+  __shared__ int s_row[kMaxTopK + 1];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
   load_slots(a, t, s_row, s_w);
@@ -419,47 +467,50 @@ __global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
   }
 }
 
-// dy[row] = w dout[t], dw[t, j] = <dout[t], y[row]>: dout is read once per
-// slot (from cache after the first), y once.
+// dy[row] = w dout[t], dw[t, j] = <dout[t], y[row]>.  Slot by slot, without a
+// barrier between them, so warps spread over the slots; dout comes from cache
+// after the first.  (All of a token's loads ahead of its stores takes twice
+// the registers and half the occupancy: 131 us against 108 for 16383 x 4 rows
+// of 2048.)
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK];
+  __shared__ int s_row[kMaxTopK + 1];
   __shared__ float s_w[kMaxTopK];
-  __shared__ float s_part[8];
+  __shared__ float s_part[8][kMaxTopK];
   const long long t = blockIdx.x;
   load_slots(a, t, s_row, s_w);
+#pragma unroll 1
   for (int j = 0; j < a.top_k; ++j) {
     const long long r = s_row[j];
+    const float w = s_w[j];
     float dot = 0.0f;
     if (r >= 0) {
       for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec) {
-        const Pack<T, kVec> d = load_pack<T, kVec>(a.in, t * a.ld_in + c);
         const Pack<T, kVec> y = load_pack<T, kVec>(a.in2, r * a.ld_in2 + c);
+        const Pack<T, kVec> d = load_pack<T, kVec>(a.in, t * a.ld_in + c);
         Pack<T, kVec> o;
 #pragma unroll
         for (int i = 0; i < kVec; ++i) {
           const float v = widen(d.v[i]);
           dot = fmaf(v, widen(y.v[i]), dot);
-          o.v[i] = round_one<T>(s_w[j] * v);
+          o.v[i] = round_one<T>(w * v);
         }
         store_pack<T, kVec>(a.out, r * a.ld_out + c, o);
       }
     }
-    if (a.dweights != nullptr) {
-      dot = warp_sum(dot);
-      if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5] = dot;
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        float all = 0.0f;
-        for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all += s_part[w];
-        a.dweights[t * a.top_k + j] = all;
-      }
-      __syncthreads();
-    }
+    dot = warp_sum(dot);
+    if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5][j] = dot;
   }
-  zero_tail<T, kVec>(a, t);
+  zero_tail<T, kVec>(a, t, s_row[kMaxTopK]);
+  if (a.dweights == nullptr) return;
+  __syncthreads();
+  if ((int)threadIdx.x < a.top_k) {
+    float all = 0.0f;
+    for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all += s_part[w][threadIdx.x];
+    a.dweights[t * a.top_k + threadIdx.x] = all;
+  }
 }
 
 }  // namespace b200
