@@ -40,8 +40,9 @@ struct GroupedArgs {
   int feat;      // extent of the MMA's M axis: N (forward, dB) or K (dA)
   int red;       // contraction extent: K (forward) or N (dA); unused in dB
   int cols;      // dB: extent of the MMA's N axis, K
-  void* out;     // forward, dA: rows x feat
+  void* out;     // forward, dA: rows x feat; dB: null, or dB where TMA cannot write it
   long long ldo;
+  long long expert_stride;  // of out, dB
   int group;     // raster band
   const CUtensorMap* maps;  // dB: dC's and A's map of each expert, box 64 x 64
   int* status;
@@ -346,6 +347,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     if constexpr (kMode != kGroupedDB)
       zero_unowned_rows(out, args.ldo, args.feat, s_off[0], s_off[args.experts], args.rows,
                         (long long)blockIdx.x * 128 + (threadIdx.x - 64), gridDim.x * 128ll);
+    // rows on 4 bytes take two elements at a time
+    const bool even_rows = (args.ldo & 1) == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
     const uint32_t my_store = store_base + (uint32_t)(warp - 2) * 2 * kStoreBufBytes;
     int it = 0;
     for (int u = pair; u < total; u += npairs) {
@@ -394,13 +397,30 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
             st_shared_v4(box + lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), p[0], p[1], p[2],
                          p[3]);
           }
-          fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            // (a box that starts past the matrix has nothing to write)
-            if (f0 < args.feat && w.col0 + c * kStoreCols < args.cols)
-              tma_store_3d(&tmap_s, box, w.col0 + c * kStoreCols, f0, w.e);
-            bulk_commit_group();
+          if (args.out == nullptr) {
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              // (a box that starts past the matrix has nothing to write)
+              if (f0 < args.feat && w.col0 + c * kStoreCols < args.cols)
+                tma_store_3d(&tmap_s, box, w.col0 + c * kStoreCols, f0, w.e);
+              bulk_commit_group();
+            }
+          } else {
+            // Rows that TMA cannot write: the box row by row, 64 bytes a store.
+            __syncwarp();
+            const int col = w.col0 + c * kStoreCols + lane;
+            T* to = out + w.e * args.expert_stride + (long long)f0 * args.ldo + col;
+            for (int r = 0; r < 32 && f0 + r < args.feat; ++r, to += args.ldo) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const int j = h * 32 + lane;  // element j of row r: 16-byte chunk j / 8
+                const uint16_t v = ld_shared_u16(box + r * 128 + (((j >> 3) ^ (r & 7)) << 4) +
+                                                 (j & 7) * 2);
+                if (col + h * 32 < args.cols) reinterpret_cast<uint16_t*>(to)[h * 32] = v;
+              }
+            }
+            __syncwarp();
           }
         }
       } else {
@@ -410,7 +430,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
         const int odd = lane & 1;
         const int f = f0 + (lane & ~1);
         T* row = out + (long long)(w.row0 + odd) * args.ldo + f;
-        const bool in = f < args.feat, both = f + 1 < args.feat;
+        const bool in = f < args.feat, second = f + 1 < args.feat;
+        const bool both = second && even_rows;
 #pragma unroll 1
         for (int c = 0; c < w.mma_n; c += 32) {
           uint32_t v[32];
@@ -431,7 +452,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
               if (both) {
                 *reinterpret_cast<uint32_t*>(row) = pair;
               } else {
-                *reinterpret_cast<uint16_t*>(row) = (uint16_t)pair;
+                uint16_t* half = reinterpret_cast<uint16_t*>(row);
+                half[0] = (uint16_t)pair;
+                if (second) half[1] = (uint16_t)(pair >> 16);
               }
             }
             row += 2 * args.ldo;

@@ -241,6 +241,11 @@ struct Call {
   int dtype;
 };
 
+bool tma_rows(const void* p, long long ld) { return aligned16(p) && (ld & 7) == 0; }
+bool tma_bank(const Call& c) {
+  return tma_rows(c.bank, c.ldb) && (c.experts <= 1 || (c.expert_stride & 7) == 0);
+}
+
 int check_call(const Call& c, int mode) {
   if (c.rows < 0 || c.experts < 0 || c.N < 0 || c.K < 0) return B200_ERR_INVALID_ARGUMENT;
   if (c.dtype != B200_BF16 && c.dtype != B200_FP16) return B200_ERR_INVALID_ARGUMENT;
@@ -254,9 +259,12 @@ int check_call(const Call& c, int mode) {
   if ((has_t && c.ldt < wt) || (has_u && c.ldu < wu) || (has_bank && c.ldb < c.K) ||
       (has_bank && c.experts > 1 && c.expert_stride < (long long)c.N * c.ldb))
     return B200_ERR_INVALID_ARGUMENT;
-  if ((has_t && (!aligned16(c.t) || (c.ldt & 7))) || (has_u && (!aligned16(c.u) || (c.ldu & 7))) ||
-      (has_bank && (!aligned16(c.bank) || (c.ldb & 7) ||
-                    (c.experts > 1 && (c.expert_stride & 7)))) ||
+  // What is read must suit TMA; what is written, its elements.
+  const bool bank_in = mode != kGroupedDB;
+  if ((has_t && !tma_rows(c.t, c.ldt)) ||
+      (has_u && (mode == kGroupedDB ? !tma_rows(c.u, c.ldu)
+                                    : (reinterpret_cast<uintptr_t>(c.u) & 1u) != 0)) ||
+      (has_bank && (bank_in ? !tma_bank(c) : (reinterpret_cast<uintptr_t>(c.bank) & 1u) != 0)) ||
       (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
     return B200_ERR_ALIGNMENT;
   // unit numbers are 32-bit
@@ -303,8 +311,10 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
   if (kMode == kGroupedDB) {
     st = map_rows(&tw, c.dtype, c.t, c.N, c.rows, c.ldt, 64);
     if (st == B200_OK) st = map_rows(&tt, c.dtype, c.u, c.K, c.rows, c.ldu, 64);
-    if (st == B200_OK)
+    if (st == B200_OK && tma_bank(c))
       st = map_bank(&ts, c.dtype, c.bank, c.K, c.N, c.experts, c.ldb, c.expert_stride, 32);
+    else
+      ts = tt;  // (not used: the kernel stores to `out`)
   } else {
     const int red = kMode == kGroupedFwd ? c.K : c.N;
     st = map_bank(&tw, c.dtype, c.bank, c.K, c.N, c.experts, c.ldb, c.expert_stride,
@@ -328,8 +338,9 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
   a.feat = kMode == kGroupedDA ? c.K : c.N;
   a.red = kMode == kGroupedFwd ? c.K : c.N;
   a.cols = c.K;
-  a.out = kMode == kGroupedDB ? nullptr : c.u;
-  a.ldo = c.ldu;
+  a.out = kMode != kGroupedDB ? c.u : tma_bank(c) ? nullptr : c.bank;
+  a.ldo = kMode == kGroupedDB ? c.ldb : c.ldu;
+  a.expert_stride = c.expert_stride;
   a.group = 8;
   a.maps = static_cast<const CUtensorMap*>(maps.p);
   a.status = v.status;
@@ -522,8 +533,8 @@ int run_w4(const W4Call& c, cudaStream_t stream) {
   const bool empty = c.K == 0 || c.experts == 0;
   if (!c.c || c.ldc < c.N || (!empty && (!c.a || !c.packed || c.lda < c.K)))
     return B200_ERR_INVALID_ARGUMENT;
-  if (!aligned16(c.c) || (c.ldc & 7) ||
-      (!empty && (!aligned16(c.a) || (c.lda & 7) || !aligned16(c.packed))) ||
+  if ((reinterpret_cast<uintptr_t>(c.c) & 1u) ||
+      (!empty && (!tma_rows(c.a, c.lda) || !aligned16(c.packed))) ||
       (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
     return B200_ERR_ALIGNMENT;
   if ((ceil_div(c.rows, 16) + c.experts) * ceil_div(c.N, kW4Rows) >= (1ll << 30))
@@ -663,6 +674,23 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
   const Call c = {dC, const_cast<void*>(A), dB, offsets, rows, experts, N, K,
                   ldc, lda, ldb, expert_stride, dtype};
   return run_grouped<kGroupedDB>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
+                    int matrices, int rows, int cols, int ld, void* stream) {
+  if (matrices < 0 || rows < 0 || cols < 0 || ld < cols) return B200_ERR_INVALID_ARGUMENT;
+  if (matrices == 0 || rows == 0 || cols == 0) return B200_OK;
+  if (!src || !dst || row_stride < 0 || matrix_stride < 0) return B200_ERR_INVALID_ARGUMENT;
+  if (!tma_rows(dst, ld) || (reinterpret_cast<uintptr_t>(src) & 1u)) return B200_ERR_ALIGNMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  const int st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  const long long blocks = ceil_div((long long)matrices * rows * (ld / 8), 256);
+  const long long most = 16ll * v.sms;
+  return launch(align_rows_kernel, (int)(blocks < most ? blocks : most), 256, 0,
+                static_cast<cudaStream_t>(stream), static_cast<const uint16_t*>(src),
+                matrix_stride, row_stride, static_cast<uint16_t*>(dst), matrices, rows, cols, ld);
 }
 
 int b200_grouped_set_kernel(int kernel) {

@@ -66,9 +66,14 @@ Rows as_rows(const at::Tensor& t) {
       aligned16(t))
     return {t, (int)ld};
   auto buf = fresh({rows, pad}, t.scalar_type(), t);
-  auto view = buf.narrow(1, 0, cols);
-  view.copy_(t);
-  return {view, (int)pad};
+  // (an expanded or transposed operand is made contiguous first)
+  const at::Tensor src = (cols == 1 || t.stride(1) == 1) && (rows == 1 || t.stride(0) >= 0)
+                             ? t
+                             : t.contiguous();
+  check_status(b200_align_rows(src.data_ptr(), 0, rows > 1 ? src.stride(0) : cols, buf.data_ptr(), 1,
+                               (int)rows, (int)cols, (int)pad, current_stream()),
+               "aligning rows");
+  return {buf.narrow(1, 0, cols), (int)pad};
 }
 
 // The same for a bank of matrices, given as (experts, N, K).
@@ -88,25 +93,12 @@ Bank as_bank(const at::Tensor& t) {
       stride % 8 == 0 && stride >= n * ld && aligned16(t))
     return {t, (int)ld, stride};
   auto buf = fresh({e, n, pad}, t.scalar_type(), t);
-  auto view = buf.narrow(2, 0, k);
-  view.copy_(t);
-  return {view, (int)pad, n * pad};
-}
-
-// A new rows x cols result whose rows are on 16 bytes; `done` gives the
-// caller a contiguous tensor.
-struct Result {
-  at::Tensor buf;
-  int64_t cols;
-  int ld;
-  at::Tensor done() const {
-    return buf.size(1) == cols ? buf : buf.narrow(1, 0, cols).contiguous();
-  }
-};
-
-Result new_rows(int64_t rows, int64_t cols, const at::Tensor& like) {
-  const int64_t pad = round_up8(cols);
-  return {fresh({rows, pad}, like.scalar_type(), like), cols, (int)std::max<int64_t>(pad, 8)};
+  const at::Tensor src =
+      (k == 1 || t.stride(2) == 1) && t.stride(1) >= 0 && t.stride(0) >= 0 ? t : t.contiguous();
+  check_status(b200_align_rows(src.data_ptr(), src.stride(0), src.stride(1), buf.data_ptr(), (int)e,
+                               (int)n, (int)k, (int)pad, current_stream()),
+               "aligning a bank");
+  return {buf.narrow(2, 0, k), (int)pad, n * pad};
 }
 
 at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::Tensor& like,
@@ -128,59 +120,60 @@ void check_sizes(std::initializer_list<int64_t> sizes, const char* who) {
 // ------------------------------------------------------------ grouped product
 constexpr const char* kGrouped = "matmul_b200_grouped";
 
-at::Tensor grouped_forward(const at::Tensor& a, const at::Tensor& bank, const at::Tensor& offsets) {
-  const c10::cuda::CUDAGuard guard(a.device());
-  const Rows ra = as_rows(a);
-  const Bank rb = as_bank(bank);
-  const Result c = new_rows(a.size(0), bank.size(1), a);
-  check_status(b200_grouped_gemm(ra.t.data_ptr(), rb.t.data_ptr(), c.buf.data_ptr(),
-                                 offsets.data_ptr<int>(), (int)a.size(0), (int)bank.size(0),
-                                 (int)bank.size(1), (int)bank.size(2), ra.ld, rb.ld, rb.stride,
-                                 c.ld, dtype_code(a), current_stream()),
+at::Tensor grouped_forward(const Rows& a, const Bank& bank, const at::Tensor& offsets) {
+  const int64_t rows = a.t.size(0), e = bank.t.size(0), n = bank.t.size(1), k = bank.t.size(2);
+  auto c = fresh({rows, n}, a.t.scalar_type(), a.t);
+  check_status(b200_grouped_gemm(a.t.data_ptr(), bank.t.data_ptr(), c.data_ptr(),
+                                 offsets.data_ptr<int>(), (int)rows, (int)e, (int)n, (int)k, a.ld,
+                                 bank.ld, bank.stride, (int)n, dtype_code(a.t), current_stream()),
                kGrouped);
-  return c.done();
+  return c;
 }
 
-at::Tensor grouped_da(const at::Tensor& dc, const at::Tensor& bank, const at::Tensor& offsets) {
-  const Rows rc = as_rows(dc);
-  const Bank rb = as_bank(bank);
-  const Result da = new_rows(dc.size(0), bank.size(2), dc);
-  check_status(b200_grouped_gemm_da(rc.t.data_ptr(), rb.t.data_ptr(), da.buf.data_ptr(),
-                                    offsets.data_ptr<int>(), (int)dc.size(0), (int)bank.size(0),
-                                    (int)bank.size(1), (int)bank.size(2), rc.ld, rb.ld, rb.stride,
-                                    da.ld, dtype_code(dc), current_stream()),
+at::Tensor grouped_da(const Rows& dc, const Bank& bank, const at::Tensor& offsets) {
+  const int64_t rows = dc.t.size(0), e = bank.t.size(0), n = bank.t.size(1), k = bank.t.size(2);
+  auto da = fresh({rows, k}, dc.t.scalar_type(), dc.t);
+  check_status(b200_grouped_gemm_da(dc.t.data_ptr(), bank.t.data_ptr(), da.data_ptr(),
+                                    offsets.data_ptr<int>(), (int)rows, (int)e, (int)n, (int)k,
+                                    dc.ld, bank.ld, bank.stride, (int)k, dtype_code(dc.t),
+                                    current_stream()),
                "matmul_b200_grouped backward (A)");
-  return da.done();
+  return da;
 }
 
-at::Tensor grouped_db(const at::Tensor& dc, const at::Tensor& a, const at::Tensor& offsets) {
-  const int64_t experts = offsets.size(0) - 1, n = dc.size(1), k = a.size(1), pad = round_up8(k);
-  const Rows rc = as_rows(dc);
-  const Rows ra = as_rows(a);
-  auto db = fresh({experts, n, pad}, dc.scalar_type(), dc);
-  check_status(b200_grouped_gemm_db(rc.t.data_ptr(), ra.t.data_ptr(), db.data_ptr(),
-                                    offsets.data_ptr<int>(), (int)dc.size(0), (int)experts, (int)n,
-                                    (int)k, rc.ld, ra.ld, (int)std::max<int64_t>(pad, 8), n * pad,
-                                    dtype_code(dc), current_stream()),
+at::Tensor grouped_db(const Rows& dc, const Rows& a, const at::Tensor& offsets) {
+  const int64_t e = offsets.size(0) - 1, rows = a.t.size(0), n = dc.t.size(1), k = a.t.size(1);
+  auto db = fresh({e, n, k}, dc.t.scalar_type(), dc.t);
+  check_status(b200_grouped_gemm_db(dc.t.data_ptr(), a.t.data_ptr(), db.data_ptr(),
+                                    offsets.data_ptr<int>(), (int)rows, (int)e, (int)n, (int)k,
+                                    dc.ld, a.ld, (int)k, n * k, dtype_code(dc.t),
+                                    current_stream()),
                "matmul_b200_grouped backward (B)");
-  return pad == k ? db : db.narrow(2, 0, k).contiguous();
+  return db;
 }
 
+// An operand that had to be copied into aligned rows is kept as that copy, so
+// that a training step copies it once.
 struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& a, const at::Tensor& b,
                             const at::Tensor& offsets) {
-    ctx->save_for_backward({a, b, offsets});
-    return grouped_forward(a, b.transpose(1, 2), offsets);
+    const c10::cuda::CUDAGuard guard(a.device());
+    const Rows ra = as_rows(a);
+    const Bank rb = as_bank(b.transpose(1, 2));
+    ctx->save_for_backward({ra.t, rb.t, offsets});
+    return grouped_forward(ra, rb, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const at::Tensor &a = saved[0], &b = saved[1], &offsets = saved[2];
+    const at::Tensor &a = saved[0], &bank = saved[1], &offsets = saved[2];
     at::Tensor da, db;
     if (grads[0].defined()) {
       const c10::cuda::CUDAGuard guard(a.device());
-      const at::Tensor dc = grads[0].to(a.scalar_type());
-      if (ctx->needs_input_grad(0)) da = grouped_da(dc, b.transpose(1, 2), offsets);
-      if (ctx->needs_input_grad(1)) db = grouped_db(dc, a, offsets).transpose(1, 2);
+      const Rows dc = as_rows(grads[0].scalar_type() == a.scalar_type()
+                                  ? grads[0]
+                                  : grads[0].to(a.scalar_type()));
+      if (ctx->needs_input_grad(0)) da = grouped_da(dc, as_bank(bank), offsets);
+      if (ctx->needs_input_grad(1)) db = grouped_db(dc, as_rows(a), offsets).transpose(1, 2);
     }
     return {da, db, at::Tensor()};
   }
@@ -201,7 +194,8 @@ at::Tensor matmul_b200_grouped(const at::Tensor& A, const at::Tensor& B,
   const at::Tensor off = check_offsets(offsets, B.size(0), A, kGrouped);
   if (at::GradMode::is_enabled() && (A.requires_grad() || B.requires_grad()))
     return GroupedMatmul::apply(A, B, off);
-  return grouped_forward(A, B.transpose(1, 2), off);
+  const c10::cuda::CUDAGuard guard(A.device());
+  return grouped_forward(as_rows(A), as_bank(B.transpose(1, 2)), off);
 }
 
 // -------------------------------------------------------------------- routing
@@ -452,13 +446,13 @@ at::Tensor w4_matmul(const at::Tensor& A, const at::Tensor& packed, int64_t expe
     TORCH_CHECK(experts == 1, kW4, ": a bank of experts needs offsets");
   const c10::cuda::CUDAGuard guard(A.device());
   const Rows ra = as_rows(A);
-  const Result c = new_rows(A.size(0), N, A);
-  check_status(b200_w4_gemm(ra.t.data_ptr(), packed.data_ptr(), c.buf.data_ptr(),
+  auto c = fresh({A.size(0), N}, A.scalar_type(), A);
+  check_status(b200_w4_gemm(ra.t.data_ptr(), packed.data_ptr(), c.data_ptr(),
                             off.defined() ? off.data_ptr<int>() : nullptr, (int)A.size(0),
-                            (int)experts, (int)N, (int)K, (int)group, zeros, ra.ld, c.ld,
+                            (int)experts, (int)N, (int)K, (int)group, zeros, ra.ld, (int)N,
                             dtype_code(A), current_stream()),
                kW4);
-  return c.done();
+  return c;
 }
 
 }  // namespace

@@ -35,9 +35,11 @@ extern "C" {
 /* C[r, :] = A[r, :] B[e]^T for the rows r of every expert e.
  * A: rows x K, stride lda.  B: experts x N x K, row stride ldb, matrix stride
  * expert_stride (elements).  C: rows x N, stride ldc; rows of no expert are
- * set to zero.  Pointers 16-byte aligned; lda, ldb, ldc and expert_stride
- * multiples of 8; lda, ldb >= K, ldc >= N, expert_stride >= N * ldb (or
- * experts <= 1); sizes >= 0.  K == 0 gives zeros. */
+ * set to zero.  What is read (here A and B) has 16-byte aligned pointers and
+ * strides that are multiples of 8 (b200_align_rows makes such rows); what is
+ * written (here C) may lie anywhere its elements can.  lda, ldb >= K, ldc >=
+ * N, expert_stride >= N * ldb (or experts <= 1); sizes >= 0.  K == 0 gives
+ * zeros. */
 int b200_grouped_gemm(const void* A, const void* B, void* C, const int* offsets, int rows,
                       int experts, int N, int K, int lda, int ldb, long long expert_stride,
                       int ldc, int dtype, void* stream);
@@ -54,6 +56,13 @@ int b200_grouped_gemm_da(const void* dC, const void* B, void* dA, const int* off
 int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* offsets, int rows,
                          int experts, int N, int K, int ldc, int lda, int ldb,
                          long long expert_stride, int dtype, void* stream);
+
+/* Copies `matrices` matrices of rows x cols 16-bit elements (strides in
+ * elements, unit column stride, any alignment) into rows of ld elements, ld a
+ * multiple of 8 and dst 16-byte aligned: what the products above can read.
+ * The columns past cols are zero. */
+int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
+                    int matrices, int rows, int cols, int ld, void* stream);
 
 /* Kernel for b200_grouped_gemm and _da: 0 = chosen by rows per expert
  * (default), 1 = the streaming kernel (few rows), 2 = the pair kernel. */
@@ -116,7 +125,7 @@ int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* pac
 
 /* C[r, :] = A[r, :] W[e]^T with packed weights.  offsets as for
  * b200_grouped_gemm, or NULL for experts = 1: every row takes the one matrix.
- * A: rows x K, stride lda; C: rows x N, stride ldc; alignment as above.  The
+ * A: rows x K, stride lda; C: rows x N, stride ldc; alignment as there.  The
  * weights enter as exact integers, the scales multiply fp32 sums.  Any number
  * of rows; made for few (the weights are read once per 64 rows of an expert). */
 int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets, int rows,

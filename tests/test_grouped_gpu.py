@@ -250,3 +250,31 @@ def test_other_stream_and_graph_capture():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, bg.matmul_b200_grouped(static, w.transpose(1, 2), off))
+
+
+def test_rows_anywhere():
+    # odd strides and starts in every operand that is read
+    def odd(t, pad):
+        wide = torch.full((*t.shape[:-1], t.shape[-1] + pad), float("nan"), dtype=t.dtype,
+                          device=t.device)
+        wide[..., pad // 2:pad // 2 + t.shape[-1]] = t
+        return wide[..., pad // 2:pad // 2 + t.shape[-1]].detach()
+
+    for n, k in ((33, 75), (64, 129), (131, 64), (9, 7)):
+        for pad in (1, 2, 5):
+            check_all([0, 30, 94, 101], 101, n, k, seed=pad, mangle=lambda t: odd(t, pad))
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 8), (17, 9), (64, 1033), (300, 250)])
+def test_align_rows(rows, cols):
+    from blackwell_gemm_b200 import capi as c
+    ld = (cols + 7) // 8 * 8
+    for stride in (cols, cols + 1, cols + 6):
+        for start in (0, 1, 2, 3, 7):
+            flat = torch.randn(2 * rows * stride + 8, device="cuda").bfloat16()
+            src = torch.as_strided(flat, (2, rows, cols), (rows * stride, stride, 1), start)
+            dst = torch.full((2, rows, ld), 9.0, device="cuda").bfloat16()
+            st = c.lib().b200_align_rows(src.data_ptr(), rows * stride, stride, dst.data_ptr(), 2,
+                                         rows, cols, ld, torch.cuda.current_stream().cuda_stream)
+            assert st == c.OK
+            assert torch.equal(dst[..., :cols], src) and not dst[..., cols:].any()

@@ -32,11 +32,10 @@ def grouped(a=FAKE, b=FAKE, c=FAKE, off=FAKE, rows=8, experts=2, n=8, k=8, lda=8
     (dict(stride=56), capi.ERR_INVALID_ARGUMENT),                   # matrices overlap
     (dict(a=FAKE + 2), capi.ERR_ALIGNMENT),
     (dict(b=FAKE + 8), capi.ERR_ALIGNMENT),
-    (dict(c=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(c=FAKE + 1), capi.ERR_ALIGNMENT),                         # (written: any 2 bytes)
     (dict(off=FAKE + 2), capi.ERR_ALIGNMENT),
     (dict(lda=12), capi.ERR_ALIGNMENT),
     (dict(ldb=12, stride=96), capi.ERR_ALIGNMENT),
-    (dict(ldc=12), capi.ERR_ALIGNMENT),
     (dict(stride=68), capi.ERR_ALIGNMENT),
     (dict(experts=1025), capi.ERR_TOO_LARGE),
     (dict(rows=INT_MAX, n=INT_MAX, ldc=INT_MAX - 7, stride=2 ** 40), capi.ERR_INVALID_ARGUMENT),
@@ -55,7 +54,8 @@ def test_grouped_gradients_c_abi():
     assert da(p0=FAKE + 2) == capi.ERR_ALIGNMENT
     assert da(rows=0) == capi.OK
     args = [FAKE, FAKE, FAKE, FAKE, 8, 2, 8, 8, 8, 8, 8, 64, capi.BF16, None]
-    for at, value, expect in [(0, 0, capi.ERR_INVALID_ARGUMENT), (2, FAKE + 4, capi.ERR_ALIGNMENT),
+    for at, value, expect in [(0, 0, capi.ERR_INVALID_ARGUMENT), (2, FAKE + 1, capi.ERR_ALIGNMENT),
+                              (1, FAKE + 4, capi.ERR_ALIGNMENT),
                               (8, 4, capi.ERR_INVALID_ARGUMENT), (11, 8, capi.ERR_INVALID_ARGUMENT),
                               (5, 0, capi.OK), (6, 0, capi.OK), (12, 7, capi.ERR_INVALID_ARGUMENT)]:
         changed = list(args)
@@ -102,10 +102,9 @@ def w4(a=FAKE, p=FAKE, c=FAKE, off=0, rows=8, experts=1, n=8, k=64, group=64, ze
     (dict(lda=56), capi.ERR_INVALID_ARGUMENT),
     (dict(n=16), capi.ERR_INVALID_ARGUMENT),               # ldc < N
     (dict(lda=68), capi.ERR_ALIGNMENT),
-    (dict(ldc=12), capi.ERR_ALIGNMENT),
     (dict(a=FAKE + 2), capi.ERR_ALIGNMENT),
     (dict(p=FAKE + 8), capi.ERR_ALIGNMENT),
-    (dict(c=FAKE + 8), capi.ERR_ALIGNMENT),
+    (dict(c=FAKE + 1), capi.ERR_ALIGNMENT),                # (written: any 2 bytes)
     (dict(off=FAKE + 1, experts=2), capi.ERR_ALIGNMENT),
     (dict(experts=1025, off=FAKE), capi.ERR_TOO_LARGE),
     (dict(n=INT_MAX - 7, ldc=INT_MAX - 7, rows=INT_MAX), capi.ERR_TOO_LARGE),
@@ -208,3 +207,16 @@ def test_route_torch_checks():
         bg.dispatch_b200(x.bfloat16(), r)
     with pytest.raises(RuntimeError, match="2-D"):
         bg.combine_b200(x[0].bfloat16(), r)
+
+
+def test_align_rows_c_abi():
+    lib = capi.lib()
+    args = [FAKE, 64, 8, FAKE, 2, 8, 7, 8, None]
+    for at, value, expect in [(4, -1, capi.ERR_INVALID_ARGUMENT), (5, -1, capi.ERR_INVALID_ARGUMENT),
+                              (7, 6, capi.ERR_INVALID_ARGUMENT), (0, 0, capi.ERR_INVALID_ARGUMENT),
+                              (2, -1, capi.ERR_INVALID_ARGUMENT), (0, FAKE + 1, capi.ERR_ALIGNMENT),
+                              (3, FAKE + 2, capi.ERR_ALIGNMENT), (7, 12, capi.ERR_ALIGNMENT),
+                              (4, 0, capi.OK), (5, 0, capi.OK), (6, 0, capi.OK)]:
+        changed = list(args)
+        changed[at] = value
+        assert lib.b200_align_rows(*changed) == expect, (at, value)
