@@ -371,7 +371,7 @@ int launch_stream(const Call& c, const DeviceView& v, cudaStream_t stream) {
   a.feat_blocks = (int)ceil_div(a.feat, 128);
   a.red = red;
   a.red_blocks = (int)ceil_div(red, kSlabK);
-  a.min_items = 4;
+  a.min_items = 16;
   a.out = c.u;
   a.ldo = c.ldu;
   a.status = v.status;
@@ -390,13 +390,16 @@ int launch_stream(const Call& c, const DeviceView& v, cudaStream_t stream) {
 // go round.  Measured, us, streaming / pair, for experts x N x K at rows per
 // expert: 8 x 14336 x 4096 at 2: 112 / 122, at 48: 153 / 172, at 64: 205 /
 // 175; 16 x 512 x 8192 at 16: 32 / 40; 32 x 2056 x 1032 at 16: 33 / 32, its
-// gradient in A 45 / 37; 64 x 1024 x 2048 at 16: 54 / 55, 54 / 51.
+// gradient in A 45 / 37; 64 x 1024 x 2048 at 16: 54 / 55, 54 / 51.  With more
+// rows it still is where three of four pairs would have no tile: 4 x 744 x
+// 6200 at 100: 24 / 35, at 256: 39 / 48, at 400: 50 / 45.
 bool use_stream(const Call& c, int feat, int red, int pairs) {
   const int k = g_kernel.load();
   if (k != 0) return k == 1;
   const long long groups = c.experts < c.rows ? c.experts : c.rows;
-  return c.rows <= 48ll * c.experts &&
-         (red >= 4096 || groups * ceil_div(feat, 256) < 2ll * pairs);
+  const long long tiles = groups * ceil_div(feat, 256);  // of the pair kernel, at the least
+  if (c.rows <= 48ll * c.experts) return red >= 4096 || tiles < 2ll * pairs;
+  return c.rows <= 256ll * c.experts && red >= 4096 && 4 * tiles <= pairs;
 }
 
 template <int kMode, class T>
@@ -479,7 +482,7 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   a.feat_blocks = (int)ceil_div(c.N, kW4Rows);
   a.red = c.K;
   a.red_blocks = (int)ceil_div(c.K, kW4K);
-  a.min_items = 4;
+  a.min_items = kRows ? 8 : 4;
   a.out = c.c;
   a.ldo = c.ldc;
   a.status = v.status;

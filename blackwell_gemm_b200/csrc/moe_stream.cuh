@@ -104,8 +104,9 @@ __device__ __forceinline__ void stream_groups(const StreamArgs& a, int tile, int
 // stored; a part is left in this CTA's slot, and the last contributor to
 // arrive stores the sum.  `piece` numbers the warps of a CTA that finish.
 // valid = false (a wait ran out): the part is only counted, so that the
-// counts are zero again when the launch ends.
-template <int kTok, class T, int kTile>
+// counts are zero again when the launch ends.  kParts: fewer where registers
+// are short.
+template <int kTok, class T, int kParts = 4, int kTile>
 __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamWalk<kTile>& walk,
                                               const StreamSegment& s, int quarter, int piece,
                                               int tok0, float (&acc)[kTok], bool valid) {
@@ -138,22 +139,25 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
     if (lane == 0) atomicExch(a.counts + c0 * 8 + piece, 0u);
 #pragma unroll
     for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
-    // (two parts' loads in flight at a time; added in order)
-    constexpr int kBatch = kTok < 16 ? kTok : 16;
-    for (int p = c0; p <= c1; p += 2) {
-      const float* from = slot(p);
-      const float* then = slot(p < c1 ? p + 1 : p);
+    // kParts parts' loads in flight at a time, added in order.
+    constexpr int kBatch = kTok < 16 ? kTok : kParts == 4 ? 16 : 8;
+    for (int p = c0; p <= c1; p += kParts) {
+      const float* from[kParts];
+#pragma unroll
+      for (int i = 0; i < kParts; ++i) from[i] = slot(p + i <= c1 ? p + i : c1);
 #pragma unroll
       for (int b = 0; b < kTok; b += kBatch) {
-        float v[kBatch], u[kBatch];
+        if (b >= rows) break;
+        float v[kParts][kBatch];
 #pragma unroll
-        for (int c = 0; c < kBatch; ++c) {
-          const bool in = b + c < rows;
-          v[c] = in ? __ldcg(from + (b + c) * 128) : 0.0f;
-          u[c] = in && p < c1 ? __ldcg(then + (b + c) * 128) : 0.0f;
-        }
+        for (int i = 0; i < kParts; ++i)
 #pragma unroll
-        for (int c = 0; c < kBatch; ++c) acc[b + c] = (acc[b + c] + v[c]) + u[c];
+          for (int c = 0; c < kBatch; ++c)
+            v[i][c] = b + c < rows && p + i <= c1 ? __ldcg(from[i] + (b + c) * 128) : 0.0f;
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+          for (int c = 0; c < kBatch; ++c) acc[b + c] += v[i][c];
       }
     }
   }

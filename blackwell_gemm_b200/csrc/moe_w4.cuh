@@ -717,7 +717,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
         for (int c = 0; c < 32; ++c) acc[c] *= 1.0f / U::kUnit;
         const bool valid =
             __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
-        stream_finish<32, T>(args, walk, s, quarter, (int)set * 4 + quarter, tok0, acc, valid);
+        stream_finish<32, T, 2>(args, walk, s, quarter, (int)set * 4 + quarter, tok0, acc, valid);
       }
     }
     __syncwarp();
