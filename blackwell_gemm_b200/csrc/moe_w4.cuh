@@ -65,10 +65,6 @@ struct W4Unpack<__nv_bfloat16> {
                                      *reinterpret_cast<const __nv_bfloat162*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-  static __device__ __forceinline__ uint32_t bias(uint32_t z) {
-    // -z / 64 in bf16: exact (z has four bits)
-    return pack_pair<__nv_bfloat16>(-kUnit * (float)z, -kUnit * (float)z);
-  }
   static __device__ __forceinline__ float wide(uint16_t s) {
     return __uint_as_float((uint32_t)s << 16);
   }
@@ -84,13 +80,16 @@ struct W4Unpack<__half> {
                               *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&r);
   }
-  static __device__ __forceinline__ uint32_t bias(uint32_t z) {
-    return pack_pair<__half>(-kUnit * (float)z, -kUnit * (float)z);
-  }
   static __device__ __forceinline__ float wide(uint16_t s) {
     return __half2float(*reinterpret_cast<const __half*>(&s));
   }
 };
+
+// -z kUnit twice, the same way: exact, and no conversion instruction.
+template <class T>
+__device__ __forceinline__ uint32_t w4_bias(uint32_t z) {
+  return W4Unpack<T>::fma2(z * 0x10001u, W4Unpack<T>::kLow ^ 0x80008000u, 0u);
+}
 
 // The eight weights of a word, k ascending, two to a register.
 template <class T>
@@ -349,8 +348,8 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
             z0 = ld_shared_u8(zeros);
             z1 = ld_shared_u8(zeros + 8);
           }
-          w4_pairs<T>(q[2 * m][c], U::bias(z0), lo);
-          w4_pairs<T>(q[2 * m + 1][c], U::bias(z1), hi);
+          w4_pairs<T>(q[2 * m][c], w4_bias<T>(z0), lo);
+          w4_pairs<T>(q[2 * m + 1][c], w4_bias<T>(z1), hi);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t a[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
@@ -637,7 +636,7 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
           uint32_t bias[kSub];
 #pragma unroll
           for (int g = 0; g < kSub; ++g)
-            bias[g] = U::bias(
+            bias[g] = w4_bias<T>(
                 kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
 #pragma unroll
           for (int g = 0; g < kSub; ++g)
