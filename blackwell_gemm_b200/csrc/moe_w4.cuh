@@ -211,8 +211,8 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
 // registers into warp-level MMAs.  A record then costs about 840 warp
 // instructions, where the way through TMEM takes 1780 (stores, loads and the
 // handshakes between its stages), and with so few tokens the tensor core's
-// rate does not matter.  Groups of four warps take records in turn, a warp 32
-// rows of each: four groups for up to 8 tokens, three for 16, where a fourth
+// rate does not matter.  Groups of four warps take stages in turn, a warp 32
+// rows of each record: four groups for up to 8 tokens, three for 16, where a fourth
 // would leave 96 registers to a warp, which then spills (57344 x 8192, us:
 // 8 tokens 52.8 with four groups, 55.8 with three; 16 tokens 72.8 and 66.9).
 // Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
@@ -254,7 +254,7 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(smem_u32(&bar_full[s]), 1);
-      mbar_init(smem_u32(&bar_empty[s]), 8);  // the two groups' warps
+      mbar_init(smem_u32(&bar_empty[s]), 4);  // one group's warps
     }
     abort_word = 0;
     fence_mbar_init_cluster();
@@ -294,8 +294,8 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
                     s_off[args.experts], args.rows,
                     (long long)blockIdx.x * (128 * C::kGroups) + threadIdx.x,
                     gridDim.x * (128ll * C::kGroups));
-  uint32_t stage = 0, phase = 0;
-  uint32_t turn = 0;  // group that takes the next record
+  uint32_t first_stage = 0, first_phase = 0;  // of the segment
+  uint32_t turn = 0;                          // group that takes its first stage
   bool ok = true;
   while (walk.next(&s)) {
     float acc[2][kNt][4];
@@ -305,79 +305,82 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
       for (int n = 0; n < kNt; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-    for (int kb = s.kb0; ok && kb < s.kb1; kb += 2) {
-      // a stage's records go to groups turn and turn + 1
-      const uint32_t records = kb + 1 < s.kb1 ? 2 : 1;
-      const uint32_t which = group >= turn ? group - turn : group + C::kGroups - turn;
-      const uint32_t at = stage, parity = phase;
-      turn += records;
-      if (turn >= C::kGroups) turn -= C::kGroups;
-      if (++stage == kStages) { stage = 0; phase ^= 1u; }
-      if (which >= records) continue;
-      const uint32_t bar = smem_u32(&bar_full[at]), done = smem_u32(&bar_empty[at]);
-      const uint32_t tokens = smem_base + at * R::kStageBytes + which * 2 * R::kSlab;
-      const uint32_t record =
-          smem_base + at * R::kStageBytes + R::kTokens + which * args.record_bytes;
-      if (!__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) {
+    const int stages = (s.kb1 - s.kb0 + 1) / 2;
+    const uint32_t offset = group >= turn ? group - turn : group + C::kGroups - turn;
+    uint32_t stage = first_stage + offset, phase = first_phase;
+    if (stage >= kStages) { stage -= kStages; phase ^= 1u; }
+    for (int st = (int)offset; st < stages; st += C::kGroups) {
+      const uint32_t bar = smem_u32(&bar_full[stage]);
+      if (!__all_sync(0xffffffffu, mbar_test_wait(bar, phase))) {
         int got = 0;
-        if (lane == 0) got = wait_ready(bar, parity, wctx, kErrWaitFull);
+        if (lane == 0) got = wait_ready(bar, phase, wctx, kErrWaitFull);
         ok = __shfl_sync(0xffffffffu, got, 0) != 0;
         __syncwarp();
         if (!ok) break;
       }
-      uint32_t q[4][4];  // [row][c]
+      uint32_t tokens = smem_base + stage * R::kStageBytes;
+      uint32_t record = tokens + R::kTokens;
+      const int records = min(2, s.kb1 - s.kb0 - 2 * st);
+#pragma unroll 1
+      for (int rec = 0; rec < records;
+           ++rec, tokens += 2 * R::kSlab, record += args.record_bytes) {
+        uint32_t q[4][4];  // [row][c]
 #pragma unroll
-      for (int r = 0; r < 4; ++r) ld_shared_v4_u32(record + w4_q_offset(t, row + 8 * r), q[r]);
-      float part[2][kNt][4];
+        for (int r = 0; r < 4; ++r) ld_shared_v4_u32(record + w4_q_offset(t, row + 8 * r), q[r]);
+        float part[2][kNt][4];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        constexpr int kPer = kGroup / 32;  // words to a group
-        const int sub = c / kPer;
-        uint32_t x[kNt][4];
+        for (int c = 0; c < 4; ++c) {
+          constexpr int kPer = kGroup / 32;  // words to a group
+          const int sub = c / kPer;
+          uint32_t x[kNt][4];
 #pragma unroll
-        for (int n = 0; n < kNt; ++n)
-          ld_shared_v4_u32(tokens + (c >> 1) * R::kSlab + n * 1024 + token_row +
-                               ((((c & 1) * 4 + t) ^ token) << 4),
-                           x[n]);
-#pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          uint32_t lo[4], hi[4];
-          uint32_t z0 = 8, z1 = 8;
-          if constexpr (kZeros) {
-            const uint32_t zeros = record + kW4Q + kSub * 256 + sub * 128 + row + 16 * m;
-            z0 = ld_shared_u8(zeros);
-            z1 = ld_shared_u8(zeros + 8);
-          }
-          w4_pairs<T>(q[2 * m][c], w4_bias<T>(z0), lo);
-          w4_pairs<T>(q[2 * m + 1][c], w4_bias<T>(z1), hi);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t a[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
-#pragma unroll
-            for (int n = 0; n < kNt; ++n)
-              mma_16x8x16<T>(part[m][n], a, x[n][2 * h], x[n][2 * h + 1], c % kPer == 0 && h == 0);
-          }
-        }
-        if (c % kPer == kPer - 1) {
-          const uint32_t scales = record + kW4Q + (sub * 128 + row) * 2;
+          for (int n = 0; n < kNt; ++n)
+            ld_shared_v4_u32(tokens + (c >> 1) * R::kSlab + n * 1024 + token_row +
+                                 ((((c & 1) * 4 + t) ^ token) << 4),
+                             x[n]);
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
-            const float s0 = U::wide(ld_shared_u16(scales + 32 * m));
-            const float s1 = U::wide(ld_shared_u16(scales + 32 * m + 16));
+            uint32_t lo[4], hi[4];
+            uint32_t z0 = 8, z1 = 8;
+            if constexpr (kZeros) {
+              const uint32_t zeros = record + kW4Q + kSub * 256 + sub * 128 + row + 16 * m;
+              z0 = ld_shared_u8(zeros);
+              z1 = ld_shared_u8(zeros + 8);
+            }
+            w4_pairs<T>(q[2 * m][c], w4_bias<T>(z0), lo);
+            w4_pairs<T>(q[2 * m + 1][c], w4_bias<T>(z1), hi);
 #pragma unroll
-            for (int n = 0; n < kNt; ++n)
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t a[4] = {lo[2 * h], hi[2 * h], lo[2 * h + 1], hi[2 * h + 1]};
 #pragma unroll
-              for (int i = 0; i < 4; ++i)
-                acc[m][n][i] = fmaf(i < 2 ? s0 : s1, part[m][n][i], acc[m][n][i]);
+              for (int n = 0; n < kNt; ++n)
+                mma_16x8x16<T>(part[m][n], a, x[n][2 * h], x[n][2 * h + 1], c % kPer == 0 && h == 0);
+            }
+          }
+          if (c % kPer == kPer - 1) {
+            const uint32_t scales = record + kW4Q + (sub * 128 + row) * 2;
+#pragma unroll
+            for (int m = 0; m < 2; ++m) {
+              const float s0 = U::wide(ld_shared_u16(scales + 32 * m));
+              const float s1 = U::wide(ld_shared_u16(scales + 32 * m + 16));
+#pragma unroll
+              for (int n = 0; n < kNt; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  acc[m][n][i] = fmaf(i < 2 ? s0 : s1, part[m][n][i], acc[m][n][i]);
+            }
           }
         }
       }
       __syncwarp();
-      if (lane == 0) {
-        mbar_arrive_local(done);
-        if (records == 1) mbar_arrive_local(done);  // for the record that is not there
-      }
+      if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+      stage += C::kGroups;
+      if (stage >= kStages) { stage -= kStages; phase ^= 1u; }
     }
+    const uint32_t end = first_stage + stages, laps = end / kStages;
+    first_stage = end - laps * kStages;
+    first_phase ^= laps & 1u;
+    turn = (turn + stages) % C::kGroups;
     // The groups' sums meet in shared memory; warps 0-3 finish the tile,
     // lane = row.
     float* sums = reinterpret_cast<float*>(smem_raw + (exchange - smem_u32(smem_raw)));
