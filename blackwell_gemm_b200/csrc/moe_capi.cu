@@ -77,6 +77,11 @@ bool init_stream() {
 
 template <int kGroup, bool kZeros, class T>
 bool init_w4_one() {
+  if constexpr (kGroup < 128) {
+    if (!set_smem(w4_rows_kernel<32, kGroup, kZeros, T>,
+                  W4RowsCfg<32, kGroup>::smem_bytes(kMaxExperts)))
+      return false;
+  }
   return set_smem(w4_rows_kernel<8, kGroup, kZeros, T>,
                   W4RowsCfg<8, kGroup>::smem_bytes(kMaxExperts)) &&
          set_smem(w4_rows_kernel<16, kGroup, kZeros, T>,
@@ -512,6 +517,14 @@ int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
     return launch_w4<true, 8, kGroup, kZeros, T>(c, v, stream);
   if (c.rows <= 16 || c.rows <= 8ll * c.experts)
     return launch_w4<true, 16, kGroup, kZeros, T>(c, v, stream);
+  // Small groups: warp MMAs take a tile of 32 as well, because the way through
+  // TMEM reads a product back for every group (24 rows x 14336 x 4096: groups
+  // of 32 40.2 and 30.0 us, of 64 36.1 and 31.9, of 128 26.5 and 27.2; 128
+  // rows over 8 experts, groups of 32: 200 and 122).
+  if constexpr (kGroup < 128) {
+    if (c.rows <= 32 || c.rows <= 16ll * c.experts)
+      return launch_w4<true, 32, kGroup, kZeros, T>(c, v, stream);
+  }
   return launch_w4<false, 64, kGroup, kZeros, T>(c, v, stream);
 }
 

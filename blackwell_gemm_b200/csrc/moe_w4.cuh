@@ -207,21 +207,23 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
   }
 }
 
-// Few rows (at most 16 to a tile): unpacked weights go straight from
+// Few rows (at most 32 to a tile): unpacked weights go straight from
 // registers into warp-level MMAs.  A record then costs about 840 warp
 // instructions, where the way through TMEM takes 1780 (stores, loads and the
 // handshakes between its stages), and with so few tokens the tensor core's
 // rate does not matter.  Groups of four warps take stages in turn, a warp 32
-// rows of each record: four groups for up to 8 tokens, three for 16, where a fourth
-// would leave 96 registers to a warp, which then spills (57344 x 8192, us:
-// 8 tokens 52.8 with four groups, 55.8 with three; 16 tokens 72.8 and 66.9).
+// rows of each record: four groups for up to 8 tokens, three for 16, where a
+// fourth would leave 96 registers to a warp, which then spills (57344 x 8192,
+// 16 tokens: 61.4 us with three, 71.0 with four), two for 32.
+// 57344 x 8192, groups of 128, takes 48.4 us for one token: 5.0 TB/s of
+// packed weights, 0.77 of HBM's measured rate.
 // Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
 // lets eight lanes read all banks of the swizzled token slab.
 template <int kTok, int kGroup>
 struct W4RowsCfg {
   using Ring = W4Ring<kTok, kGroup>;
   static constexpr int kPitch = 136;  // floats from token to token of the exchange
-  static constexpr int kGroups = kTok <= 8 ? 4 : 3;
+  static constexpr int kGroups = kTok <= 8 ? 4 : kTok <= 16 ? 3 : 2;
   static constexpr int kExchange = kGroups * kTok * kPitch * 4;
   static constexpr int kStages = Ring::stages(kExchange);
   static constexpr int kThreads = 32 * (4 * kGroups + 1);
