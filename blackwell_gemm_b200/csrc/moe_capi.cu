@@ -86,7 +86,8 @@ bool init_w4_one() {
                   W4RowsCfg<8, kGroup>::smem_bytes(kMaxExperts)) &&
          set_smem(w4_rows_kernel<16, kGroup, kZeros, T>,
                   W4RowsCfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
-         set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts));
+         set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts)) &&
+         set_smem(w4_wide_kernel<kGroup, kZeros, T>, W4WideCfg<kGroup>::smem_bytes(kMaxExperts));
 }
 
 template <int kGroup, class T>
@@ -465,12 +466,16 @@ int check_w4_shape(int experts, int N, int K, int group) {
              : B200_ERR_TOO_LARGE;
 }
 
-template <bool kRows, int kTok, int kGroup, bool kZeros, class T>
+enum W4Kind { kW4Few, kW4Some, kW4Wide };  // rows, stream and wide kernel
+
+template <W4Kind kKind, int kTok, int kGroup, bool kZeros, class T>
 int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   constexpr int box_rows = W4Ring<kTok, kGroup>::kSlabRows;
   CUtensorMap tt;
   int st;
-  if (c.K % kSlabK == 0) {  // (k in a slab, row, slab)
+  if (kKind == kW4Wide) {
+    st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, W4WideCfg<kGroup>::kBox);
+  } else if (c.K % kSlabK == 0) {  // (k in a slab, row, slab)
     const cuuint64_t dims[3] = {kSlabK, (cuuint64_t)c.rows, (cuuint64_t)(c.K / kSlabK)};
     const cuuint64_t strides[2] = {(cuuint64_t)c.lda * 2, kSlabK * 2};
     const cuuint32_t box[3] = {kSlabK, box_rows, 4};
@@ -487,7 +492,7 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   a.feat_blocks = (int)ceil_div(c.N, kW4Rows);
   a.red = c.K;
   a.red_blocks = (int)ceil_div(c.K, kW4K);
-  a.min_items = kRows ? 8 : 4;
+  a.min_items = kKind == kW4Few ? 8 : 4;
   a.out = c.c;
   a.ldo = c.ldc;
   a.status = v.status;
@@ -496,12 +501,16 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   a.record_bytes = w4_record_bytes(kGroup, kZeros);
   a.expert_bytes = (long long)a.feat_blocks * a.red_blocks * a.record_bytes;
   Workspace ws;
-  st = ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a);
+  st = ws.take(v, (size_t)v.sms * (kKind == kW4Wide ? 3 : 2) * kTok * 128 * sizeof(float), stream, &a);
   if (st != B200_OK) return st;
-  if constexpr (kRows) {
+  if constexpr (kKind == kW4Few) {
     using C = W4RowsCfg<kTok, kGroup>;
     return launch(w4_rows_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
                   C::smem_bytes(c.experts), stream, tt, a);
+  } else if constexpr (kKind == kW4Wide) {
+    using C = W4WideCfg<kGroup>;
+    return launch(w4_wide_kernel<kGroup, kZeros, T>, v.sms, C::kThreads, C::smem_bytes(c.experts),
+                  stream, tt, a);
   } else {
     using C = W4Cfg<kGroup>;
     return launch(w4_stream_kernel<kGroup, kZeros, T>, v.sms, C::kThreads,
@@ -514,18 +523,28 @@ int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   // A tile as wide as most experts' rows: an expert with more takes another
   // tile, that is, reads its weights again.
   if (c.rows <= 8 || c.rows <= 4ll * c.experts)
-    return launch_w4<true, 8, kGroup, kZeros, T>(c, v, stream);
+    return launch_w4<kW4Few, 8, kGroup, kZeros, T>(c, v, stream);
   if (c.rows <= 16 || c.rows <= 8ll * c.experts)
-    return launch_w4<true, 16, kGroup, kZeros, T>(c, v, stream);
+    return launch_w4<kW4Few, 16, kGroup, kZeros, T>(c, v, stream);
   // Small groups: warp MMAs take a tile of 32 as well, because the way through
   // TMEM reads a product back for every group (24 rows x 14336 x 4096: groups
   // of 32 40.2 and 30.0 us, of 64 36.1 and 31.9, of 128 26.5 and 27.2; 128
   // rows over 8 experts, groups of 32: 200 and 122).
   if constexpr (kGroup < 128) {
     if (c.rows <= 32 || c.rows <= 16ll * c.experts)
-      return launch_w4<true, 32, kGroup, kZeros, T>(c, v, stream);
+      return launch_w4<kW4Few, 32, kGroup, kZeros, T>(c, v, stream);
   }
-  return launch_w4<false, 64, kGroup, kZeros, T>(c, v, stream);
+  // Tiles of 64 rows or of 256.  One matrix: as soon as 64 do not hold them
+  // (96 rows x 14336 x 4096: 42.2 us in two tiles, 40.2 in a wide one; groups
+  // of 32 66.8 and 62.8).  A bank: a wide tile costs the same from 129 rows
+  // on, so experts must fill it by half, with small groups altogether (8
+  // experts of 14336 x 4096, groups of 128: 512 rows 153 and 184 us, 1024
+  // rows 262 and 236; groups of 32: 1024 rows 483 and 601, 2048 rows 900 and
+  // 890).
+  const long long some = c.experts == 1 ? 64 : kGroup == 32 ? 256ll * c.experts : 96ll * c.experts;
+  if (c.rows <= some)
+    return launch_w4<kW4Some, 64, kGroup, kZeros, T>(c, v, stream);
+  return launch_w4<kW4Wide, 256, kGroup, kZeros, T>(c, v, stream);
 }
 
 template <class T>

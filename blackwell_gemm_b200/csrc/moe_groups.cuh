@@ -16,6 +16,39 @@ __device__ __forceinline__ bool wait_ready(uint32_t bar, uint32_t parity, const 
   return wait_slow(bar, parity, w, code, true);
 }
 
+// The same with nothing called (a kernel that moves registers between its
+// warps may not call functions).  draining: the abort word does not end it.
+__device__ __forceinline__ bool wait_inline(uint32_t bar, uint32_t parity, const WaitCtx& w,
+                                            int code, bool draining = false) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const unsigned long long t0 = globaltimer_ns();
+  for (;;) {
+#pragma unroll 1
+    for (int i = 0; i < 32; ++i)
+      if (mbar_try_wait(bar, parity)) return true;
+    if (!draining && ld_volatile_shared(w.abort_local) != 0) return false;
+    if (globaltimer_ns() - t0 > w.timeout_ns) {
+      atomicCAS(w.status, 0, code);
+      asm volatile("st.volatile.shared.u32 [%0], %1;" :: "r"(w.abort_local), "r"(1u) : "memory");
+      return false;
+    }
+  }
+}
+
+// End of a producing thread: its last copies have landed before the CTA may
+// leave, also where a wait elsewhere ran out.  `stage` and `phase` are what
+// comes next, `full` the ring's barriers.
+template <int kStages>
+__device__ __forceinline__ void drain_copies(uint32_t full, uint32_t stage, uint32_t phase,
+                                             long long issued, const WaitCtx& w) {
+#pragma unroll 1
+  for (int i = 0; i < kStages && i < issued; ++i) {
+    if (stage == 0) { stage = kStages; phase ^= 1u; }
+    --stage;
+    wait_inline(full + stage * 8u, phase, w, kErrWaitDrain, true);
+  }
+}
+
 constexpr int kMaxExperts = 1024;
 // Device error word: offsets that fall or leave [0, rows] (they are clamped).
 constexpr int kErrOffsets = 0x100A;

@@ -30,10 +30,10 @@ struct StreamArgs {
   void* out;
   long long ldo;
   float* slots;           // [CTA][2][tok][128]
-  unsigned int* counts;   // [CTA][8], zero between launches
+  unsigned int* counts;   // [CTA][16], zero between launches
   int* status;
   unsigned long long timeout_ns;
-  const uint8_t* packed;  // 4-bit weights (w4_stream.cuh)
+  const uint8_t* packed;  // 4-bit weights (moe_w4.cuh)
   long long expert_bytes;
   int record_bytes;
 };
@@ -132,11 +132,11 @@ __device__ __forceinline__ void stream_finish(const StreamArgs& a, const StreamW
     }
     __syncwarp();
     unsigned int before = 0;
-    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 8 + piece, 1u);
+    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 16 + piece, 1u);
     before = __shfl_sync(0xffffffffu, before, 0);
     if (before != (unsigned int)(c1 - c0)) return;
     __syncwarp();
-    if (lane == 0) atomicExch(a.counts + c0 * 8 + piece, 0u);
+    if (lane == 0) atomicExch(a.counts + c0 * 16 + piece, 0u);
 #pragma unroll
     for (int c = 0; c < kTok; ++c) acc[c] = 0.0f;
     // kParts parts' loads in flight at a time, added in order.

@@ -734,6 +734,447 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
   }
 }
 
+// Many rows: 256 tokens to a tile, so that a record is unpacked once for all
+// of them.  A product is one group for one half of the tile's tokens (up to
+// 128 columns); three places for products and two for weights fill TMEM.  The
+// running sums of 128 weight rows x 256 tokens are half of the SM's registers:
+// warps 8-23 hold them, 96 registers to a thread, which warps 0-3 (0 records,
+// 1 MMA, 2 tokens) and 4-7 (unpack) leave over.
+// What bounds it: a record's tokens, 64 KiB, are written to shared memory and
+// read by the MMAs once, which takes it 1100 cycles, and an MMA of 128 columns
+// takes about 60 with its A in TMEM; the way from a product's MMAs to its
+// place's next use, about 1300 with three places, brings that to 2500
+// (2048 rows x 14336 x 4096, groups of 128: 274 us, 0.88 PFLOP/s, in tiles of
+// 64 410; groups of 32, four times the products: 605 us, in tiles of 64 802).
+template <int kGroup>
+struct W4WideCfg {
+  static constexpr int kTok = 256;
+  static constexpr int kSub = kW4K / kGroup;
+  static constexpr int kSlab = kTok * 128;     // 64 k of the tile's tokens
+  static constexpr int kBox = 128;             // rows of a token box
+  static constexpr int kTokenStages = 5;       // slabs
+  static constexpr int kPlaces = 2;            // records' weights
+  static constexpr int kProducts = 3;
+  // When record j is unpacked the MMAs of j - 2 are done, so all products
+  // but the last three before those have been taken: of j - 5 and earlier.
+  static constexpr int kScalePlaces = 5;
+  static constexpr int kScales = kScalePlaces * kSub * 128 * 2;
+  static constexpr int kRecord = (w4_record_bytes(kGroup, true) + 127) / 128 * 128;
+  static constexpr int kRoom = (214 * 1024 - kTokenStages * kSlab - kScales) / kRecord;
+  static constexpr int kStages = kRoom < 6 ? kRoom : 6;
+  static constexpr int kThreads = 768;
+  static constexpr int smem_bytes(int experts) {
+    return kTokenStages * kSlab + kStages * kRecord + kScales + group_table_bytes(experts) + 1024;
+  }
+  static_assert(kStages >= 3, "records in flight");
+  static_assert((40 + 56) * 128 + 96 * 512 <= kThreads * 80, "registers of the launch");
+};
+
+// Tokens of a tile's first half (a multiple of 16 unless it is all of them).
+__device__ __forceinline__ int w4_half(int rows) {
+  return rows <= 128 ? rows : ((rows + 1) / 2 + 15) & ~15;
+}
+
+// stream_finish for the sums that a warp of the wide kernel holds.  Whole
+// tiles pass through a slot too: code that holds the sums in registers is
+// unrolled, code cold in the instruction cache costs more than the detour
+// (a finish of 128 unrolled columns took 29,000 cycles), and what reads them
+// back is a short loop.
+template <class T>
+__device__ __forceinline__ void w4_wide_finish(const StreamArgs& a, const StreamWalk<256>& walk,
+                                               const StreamSegment& s, int quarter, int piece,
+                                               int h0, const int (&from)[2], const int (&chunks)[2],
+                                               const float (&acc)[2][32], bool valid) {
+  const int lane = threadIdx.x & 31;
+  const int f = s.block * 128 + quarter * 32 + lane;
+  const bool whole = s.kb0 == 0 && s.kb1 == walk.red_blocks;
+  int c0 = blockIdx.x, c1 = blockIdx.x;
+  if (!whole) {
+    const long long first = s.unit * walk.red_blocks;
+    c0 = sk_owner(first, walk.items, walk.ranges);
+    c1 = sk_owner(first + walk.red_blocks - 1, walk.items, walk.ranges);
+  }
+  // (slots as in stream_finish; a whole tile comes between a CTA's divided
+  // ones or instead of one, and slot 2 is its own)
+  const int own = whole ? 2 : 0;
+  auto slot = [&](int c) {
+    return a.slots + ((long long)c * 3 + (own != 0 ? own : c == c0 ? 1 : 0)) * 256 * 128 +
+           quarter * 32 + lane;
+  };
+  if (valid) {
+    float* mine = slot(blockIdx.x);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* to = mine + ((h == 0 ? 0 : h0) + from[h] * 16) * 128;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        if (c < chunks[h]) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) __stcg(to + (c * 16 + i) * 128, acc[h][c * 16 + i]);
+        }
+      }
+    }
+  }
+  __syncwarp();
+  if (!whole) {
+    unsigned int before = 0;
+    if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 16 + piece, 1u);
+    before = __shfl_sync(0xffffffffu, before, 0);
+    if (before != (unsigned int)(c1 - c0)) return;
+    __syncwarp();
+    if (lane == 0) atomicExch(a.counts + c0 * 16 + piece, 0u);
+  }
+  if (!valid || f >= a.feat) return;
+#pragma unroll 1
+  for (int j = 0; j < 4; ++j) {
+    const int h = j >> 1;
+    if ((j & 1) >= (h == 0 ? chunks[0] : chunks[1])) continue;
+    const int t0 = (h == 0 ? from[0] * 16 : h0 + from[1] * 16) + (j & 1) * 16;
+    const int rows = s.rows - t0;
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
+    // parts in range order
+#pragma unroll 1
+    for (int p = c0; p <= c1; ++p) {
+      const float* at = slot(p) + t0 * 128;
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __ldcg(at + i * 128);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[i] += v[i];
+    }
+    T* col = static_cast<T*>(a.out) + (long long)(s.row0 + t0) * a.ldo + f;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < rows) *col = round_one<T>(sum[i] * (1.0f / W4Unpack<T>::kUnit));
+      col += a.ldo;
+    }
+  }
+}
+
+// tmap_t: the token operand (k, row), box 64 x 128.
+template <int kGroup, bool kZeros, class T>
+__global__ void __launch_bounds__(W4WideCfg<kGroup>::kThreads, 1)
+w4_wide_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args) {
+  using C = W4WideCfg<kGroup>;
+  using U = W4Unpack<T>;
+  constexpr int kTok = C::kTok;
+  constexpr int kSub = C::kSub;
+  constexpr int kSteps = kGroup / kMmaK;  // MMAs to a product
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ alignas(8) uint64_t bar_full[C::kStages];
+  __shared__ alignas(8) uint64_t bar_empty[C::kStages];
+  __shared__ alignas(8) uint64_t bar_tok_full[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_tok_empty[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_unpacked[C::kPlaces];
+  __shared__ alignas(8) uint64_t bar_used[C::kPlaces];
+  __shared__ alignas(8) uint64_t bar_product[C::kProducts];
+  __shared__ alignas(8) uint64_t bar_taken[C::kProducts];
+  __shared__ alignas(8) uint64_t bar_drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_word;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
+  const int lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t records = smem_base + C::kTokenStages * C::kSlab;
+  const uint32_t scales = records + C::kStages * C::kRecord;  // [place][group][row], 16-bit
+  int* s_off = reinterpret_cast<int*>(smem_raw + (scales + C::kScales - smem_u32(smem_raw)));
+  int* s_tiles = s_off + args.experts + 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 4);
+    }
+    for (int s = 0; s < C::kTokenStages; ++s) {
+      mbar_init(smem_u32(&bar_tok_full[s]), 1);
+      mbar_init(smem_u32(&bar_tok_empty[s]), 1);
+    }
+    for (int b = 0; b < C::kPlaces; ++b) {
+      mbar_init(smem_u32(&bar_unpacked[b]), 4);
+      mbar_init(smem_u32(&bar_used[b]), 1);
+    }
+    for (int b = 0; b < C::kProducts; ++b) {
+      mbar_init(smem_u32(&bar_product[b]), 1);
+      mbar_init(smem_u32(&bar_taken[b]), 16);
+    }
+    mbar_init(smem_u32(&bar_drain), 1);
+    abort_word = 0;
+    fence_mbar_init_cluster();
+    prefetch_tmap(&tmap_t);
+  }
+  if (warp == 1) {
+    tmem_alloc_1(smem_u32(&tmem_slot), kTmemCols);
+    tmem_relinquish_1();
+  }
+  grid_wait();
+  if (warp == 2) stream_groups(args, kTok, s_off, s_tiles);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  grid_launch_next();
+  const uint32_t tmem_base = tmem_slot;
+  const uint32_t tmem_a = tmem_base + C::kProducts * 128;
+
+  WaitCtx wctx;
+  wctx.status = args.status;
+  wctx.timeout_ns = args.timeout_ns;
+  wctx.abort_local = smem_u32(&abort_word);
+  wctx.abort_peer = wctx.abort_local;
+
+  StreamWalk<kTok> walk;
+  walk.init(args, s_off, s_tiles);
+  StreamSegment s;
+
+  if (warp < 4) {
+    registers_dec<40>();
+    if (warp == 0) {
+      if (elect_one()) {
+        const uint64_t policy = l2_policy_evict_normal();
+        uint32_t stage = 0, phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        while (ok && walk.next(&s)) {
+          for (int kb = s.kb0; kb < s.kb1; ++kb) {
+            ok = wait_inline(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty);
+            if (!ok) break;
+            const uint32_t bar = smem_u32(&bar_full[stage]);
+            mbar_arrive_expect_tx(bar, args.record_bytes);
+            bulk_load_hint(records + stage * C::kRecord, w4_record(args, s, kb), args.record_bytes,
+                           bar, policy);
+            ++issued;
+            if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+          }
+        }
+        drain_copies<C::kStages>(smem_u32(&bar_full[0]), stage, phase, issued, wctx);
+      }
+    } else if (warp == 2) {
+      if (elect_one()) {
+        const uint64_t policy = l2_policy_evict_last();
+        uint32_t stage = 0, phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        while (ok && walk.next(&s)) {
+          const int boxes = s.rows > C::kBox ? 2 : 1;
+          for (int kb = 2 * s.kb0; kb < 2 * s.kb1; ++kb) {
+            ok = wait_inline(smem_u32(&bar_tok_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty);
+            if (!ok) break;
+            const uint32_t bar = smem_u32(&bar_tok_full[stage]);
+            mbar_arrive_expect_tx(bar, boxes * C::kBox * 128);
+            for (int b = 0; b < boxes; ++b)
+              tma_load_2d_hint(smem_base + stage * C::kSlab + b * C::kBox * 128, &tmap_t,
+                               kb * kSlabK, s.row0 + b * C::kBox, bar, policy);
+            ++issued;
+            if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+          }
+        }
+        drain_copies<C::kTokenStages>(smem_u32(&bar_tok_full[0]), stage, phase, issued, wctx);
+      }
+    } else if (warp == 1) {
+      if (elect_one()) {
+        uint32_t stage = 0, phase = 0;               // token slabs
+        uint32_t w = 0, wp = 0, p = 0, pp = 1;       // places in TMEM and their phases
+        bool ok = true;
+        // (looked at before the MMAs ahead of them go out)
+        bool landed = false, unpacked = false, taken = true;
+        const uint32_t tok_full = smem_u32(&bar_tok_full[0]), unpacked0 = smem_u32(&bar_unpacked[0]),
+                       taken0 = smem_u32(&bar_taken[0]);
+        const uint32_t to_empty = smem_u32(&bar_tok_empty[0]) - tok_full,
+                       to_used = smem_u32(&bar_used[0]) - unpacked0,
+                       to_product = smem_u32(&bar_product[0]) - taken0;
+        while (ok && walk.next(&s)) {
+          const int h0 = w4_half(s.rows);
+          const bool two = s.rows > h0;
+          const uint32_t idesc0 = make_idesc_16bit(128, (h0 + 15) & ~15, kFormat<T>, false, false);
+          const uint32_t idesc1 =
+              make_idesc_16bit(128, (s.rows - h0 + 15) & ~15, kFormat<T>, false, false);
+          for (int left = s.kb1 - s.kb0; left > 0; --left) {
+            const uint32_t a = tmem_a + w * 64;
+            const uint32_t my_unpacked = unpacked0 + w * 8u;
+            if (!unpacked && !wait_inline(my_unpacked, wp, wctx, kErrWaitFull)) {
+              ok = false;
+              break;
+            }
+            if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+            unpacked = mbar_test_wait(unpacked0 + w * 8u, wp);
+            uint32_t slab[2];
+#pragma unroll
+            for (int g = 0; g < kSub; ++g) {
+              // the slabs that this group begins
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (j * 4 >= g * kSteps && j * 4 < (g + 1) * kSteps) {
+                  slab[j] = stage;
+                  if (!landed && !wait_inline(tok_full + stage * 8u, phase, wctx, kErrWaitFull))
+                    ok = false;
+                  if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+                  landed = mbar_test_wait(tok_full + stage * 8u, phase);
+                }
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (h == 1 && !two) break;
+                const uint32_t my_taken = taken0 + p * 8u;
+                if (!taken && !wait_inline(my_taken, pp, wctx, kErrWaitAccEmpty)) ok = false;
+                if (!ok) break;
+                const uint32_t d = tmem_base + p * 128;
+                if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+                taken = mbar_test_wait(taken0 + p * 8u, pp);
+                tc_fence_after_sync();
+                const uint32_t first = smem_base + (h == 0 ? 0u : (uint32_t)h0 * 128u);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                  const int k = g * kSteps + i;
+                  umma_tmem_a_1(d, a + k * 8,
+                                make_sdesc_k128(first + slab[k >> 2] * C::kSlab) + (k & 3) * 2,
+                                h == 0 ? idesc0 : idesc1, i != 0 ? 1u : 0u);
+                }
+                umma_commit_1(my_taken + to_product);
+              }
+              if (!ok) break;
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                if (j * 4 + 4 > g * kSteps && j * 4 + 4 <= (g + 1) * kSteps)
+                  umma_commit_1(tok_full + to_empty + slab[j] * 8u);
+            }
+            if (!ok) break;
+            umma_commit_1(my_unpacked + to_used);
+          }
+        }
+        umma_commit_1(smem_u32(&bar_drain));
+        wait_inline(smem_u32(&bar_drain), 0, wctx, kErrWaitDrain, true);
+      }
+    }
+    __syncwarp();
+    tc_fence_before_sync();
+    named_bar_sync(1, C::kThreads);
+    if (warp == 1) {
+      tc_fence_after_sync();
+      tmem_dealloc_1(tmem_base, kTmemCols);
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int row = quarter * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) {
+      if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+      int got = 0;
+      if (lane == 0) got = wait_inline(bar, parity, wctx, code);
+      got = __shfl_sync(0xffffffffu, got, 0);
+      __syncwarp();
+      return got != 0;
+    };
+    bool ok = true;
+    if (warp < 8) {
+      // ----------------------------------------------------------- unpack
+      registers_dec<56>();
+      uint32_t stage = 0, phase = 0, w = 0, wp = 0, n = 0;
+      while (ok && walk.next(&s)) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull);
+          if (!ok) break;
+          const uint32_t record = records + stage * C::kRecord;
+          uint32_t bias[kSub], scale[kSub];
+#pragma unroll
+          for (int g = 0; g < kSub; ++g) {
+            bias[g] = w4_bias<T>(
+                kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
+            scale[g] = ld_shared_u16(record + kW4Q + (g * 128 + row) * 2);
+          }
+          uint32_t q[4][4];  // [t][c]
+#pragma unroll
+          for (int t = 0; t < 4; ++t) ld_shared_v4_u32(record + w4_q_offset(t, row), q[t]);
+          ok = wait_warp(smem_u32(&bar_used[w]), wp ^ 1u, kErrWaitAccEmpty);
+          if (!ok) break;
+          tc_fence_after_sync();
+#pragma unroll
+          for (int g = 0; g < kSub; ++g)
+            st_shared_u16(scales + ((n * kSub + g) * 128 + row) * 2, (uint16_t)scale[g]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t r[16];
+#pragma unroll
+            for (int t = 0; t < 4; ++t) w4_pairs<T>(q[t][c], bias[c * 32 / kGroup], r + t * 4);
+            tmem_st_32x32b_x16(tmem_a + w * 64 + c * 16 + lanes, r);
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+          tmem_wait_st();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_local(smem_u32(&bar_unpacked[w]));
+          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+          if (++n == C::kScalePlaces) n = 0;
+        }
+      }
+    } else {
+      // --------------------------------------------------- products, finish
+      registers_inc<96>();
+      const int set = (warp - 8) >> 2;  // takes a fourth of each product's columns
+      zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
+                        s_off[args.experts], args.rows,
+                        (long long)blockIdx.x * 512 + (threadIdx.x - 256), gridDim.x * 512ll);
+      uint32_t p = 0, pp = 0, n = 0;
+      while (walk.next(&s)) {
+        const int h0 = w4_half(s.rows);
+        // this warp's columns of a half: up to two chunks of 16 from from[h] on
+        int from[2], chunks[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int all = ((h == 0 ? h0 : s.rows - h0) + 15) >> 4;
+          from[h] = all * set >> 2;
+          chunks[h] = (all * (set + 1) >> 2) - from[h];
+        }
+        float acc[2][32];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[h][c] = 0.0f;
+        for (int kb = s.kb0; ok && kb < s.kb1; ++kb) {
+          const uint32_t mine = scales + (n * kSub * 128 + row) * 2;
+          if (++n == C::kScalePlaces) n = 0;
+#pragma unroll 1
+          for (int g = 0; g < kSub; ++g) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              if (h == 1 && s.rows <= h0) break;
+              ok = ok && wait_warp(smem_u32(&bar_product[p]), pp, kErrWaitAccFull);
+              if (!ok) break;
+              tc_fence_after_sync();
+              const float scale = U::wide(ld_shared_u16(mine + g * 256));
+              const uint32_t d = tmem_base + p * 128 + from[h] * 16 + lanes;
+              // (a second chunk that is another warp's is read and not used)
+              if (chunks[h] > 0) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                  uint32_t v[16];
+                  tmem_ld_32x32b_x16(d + c * 16, v);
+                  tmem_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i)
+                    acc[h][c * 16 + i] =
+                        fmaf(scale, __uint_as_float(v[i]), acc[h][c * 16 + i]);
+                }
+              }
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_local(smem_u32(&bar_taken[p]));
+              if (++p == C::kProducts) { p = 0; pp ^= 1u; }
+            }
+          }
+        }
+        const bool valid =
+            __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
+        w4_wide_finish<T>(args, walk, s, quarter, set * 4 + quarter, h0, from, chunks, acc, valid);
+      }
+    }
+    tc_fence_before_sync();
+    named_bar_sync(1, C::kThreads);
+  }
+}
+
 // q: experts x N x K / 2 bytes, the low nibble the even k; scales, zeros:
 // experts x N x K / group, 16-bit and 8-bit; all contiguous.  One block per
 // record; rows and k past the matrix get scale 0 and q = 8.

@@ -498,6 +498,17 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src,
                : "memory");
 }
 
+// Registers of this warpgroup's threads (all four warps together), from the
+// launch's share down or up; what goes up must have come down elsewhere.
+template <int kRegisters>
+__device__ __forceinline__ void registers_dec() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" :: "n"(kRegisters));
+}
+template <int kRegisters>
+__device__ __forceinline__ void registers_inc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" :: "n"(kRegisters));
+}
+
 // `bytes` (a multiple of 16) consecutive bytes of global memory into this
 // CTA's shared memory; both addresses 16-byte aligned.
 __device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, uint32_t bytes,
@@ -538,6 +549,16 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
          "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]),
          "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]),
          "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+      :: "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+         "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+         "r"(r[15]), "r"(taddr)
       : "memory");
 }
 

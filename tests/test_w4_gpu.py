@@ -65,6 +65,44 @@ def test_rows_groups_types(m, group, zeros, dtype):
     close(y, x, w[0], u, dtype == "fp16")
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [66, 128, 129, 145, 200, 256, 257, 700])
+def test_many_rows(m, group, dtype):
+    dt, u = DT[dtype]
+    n, k = 392, 1120 if group == 32 else 1152
+    q, s, z, w = weights(1, n, k, group, m % 2 == 1, dt, seed=m)
+    packed = bg.pack_w4(q[0], s[0], None if z is None else z[0])
+    x = rows_of(m, k, dt)
+    close(bg.matmul_b200_w4(x, packed), x, w[0], u, dtype == "fp16")
+
+
+@pytest.mark.parametrize("n,k", [(128, 32), (130, 352), (2048, 4096), (5000, 1024)])
+def test_many_rows_sizes(n, k):
+    # whole and divided contractions, weights past one record and short of one
+    q, s, z, w = weights(1, n, k, 32, True, torch.bfloat16, seed=n)
+    packed = bg.pack_w4(q[0], s[0], z[0])
+    x = rows_of(410, k, torch.bfloat16)
+    y = bg.matmul_b200_w4(x, packed)
+    close(y, x, w[0], 2.0 ** -8)
+    assert torch.equal(y, bg.matmul_b200_w4(x, packed))
+
+
+@pytest.mark.parametrize("group", [32, 128])
+def test_many_rows_of_a_bank(group):
+    # experts with none, one, a half, one and a bit and several tiles of rows
+    offsets = [3, 3, 4, 132, 393, 393, 1100]
+    q, s, z, w = weights(6, 264, 512, group, group == 32, torch.bfloat16)
+    x = rows_of(1111, 512, torch.bfloat16)
+    x[:3], x[1100:] = float("nan"), float("inf")
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    y = bg.matmul_b200_w4(x, bg.pack_w4(q, s, z), off)
+    for e in range(6):
+        a, b = offsets[e], offsets[e + 1]
+        close(y[a:b], x[a:b], w[e], 2.0 ** -8)
+    assert not y[:3].any() and not y[1100:].any()
+
+
 @pytest.mark.parametrize("n,k,group", [(1, 32, 32), (7, 64, 64), (128, 128, 128), (129, 96, 32),
                                        (1000, 160, 32), (24, 1088, 64), (130, 4096, 128),
                                        (4097, 2048, 128), (512, 14336, 128)])
