@@ -284,6 +284,8 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
+      // (the leader's barriers count both CTAs' copies)
+      if (rank == 0) drain_copies<kStages>(smem_u32(&bar_full[0]), stage, phase, filled, wctx);
     }
     __syncwarp();
   } else if (warp == 1) {

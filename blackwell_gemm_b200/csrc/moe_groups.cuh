@@ -45,7 +45,7 @@ __device__ __forceinline__ void drain_copies(uint32_t full, uint32_t stage, uint
   for (int i = 0; i < kStages && i < issued; ++i) {
     if (stage == 0) { stage = kStages; phase ^= 1u; }
     --stage;
-    wait_inline(full + stage * 8u, phase, w, kErrWaitDrain, true);
+    if (!wait_inline(full + stage * 8u, phase, w, kErrWaitDrain, true)) break;
   }
 }
 

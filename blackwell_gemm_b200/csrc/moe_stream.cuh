@@ -250,6 +250,7 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
     if (elect_one()) {
       const uint64_t once = l2_policy_evict_first(), keep = l2_policy_evict_last();
       uint32_t stage = 0, phase = 0;
+      long long issued = 0;
       bool ok = true;
       while (ok && walk.next(&s)) {
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
@@ -271,9 +272,11 @@ grouped_stream_kernel(const __grid_constant__ CUtensorMap tmap_w,
           for (int i = 0; i < boxes; ++i)
             tma_load_2d_hint(sa + C::kWeight + i * 16 * 128, &tmap_t, k0, s.row0 + i * 16, fb,
                              keep);
+          ++issued;
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
+      drain_copies<kStages>(smem_u32(&bar_full[0]), stage, phase, issued, wctx);
     }
     __syncwarp();
   } else if (warp == 1) {

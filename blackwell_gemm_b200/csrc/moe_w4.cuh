@@ -187,24 +187,28 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
   uint32_t stage = 0, phase = 0;
   // Looking at a barrier takes 100 cycles and more on a busy SM, so the next
   // stage's is looked at before this stage's copies go out.
-  bool ready = true;
+  bool ready = true, ok = true;
+  long long issued = 0;
   StreamSegment s;
-  while (walk.next(&s)) {
+  while (ok && walk.next(&s)) {
     for (int kb = s.kb0; kb < s.kb1; kb += 2) {
       const uint32_t fb = full + stage * 8u;
       const uint32_t sa = ring + stage * kBytes;
       const uint32_t bytes = kPart == kW4Tokens ? 0
                              : kb + 1 < s.kb1   ? 2 * args.record_bytes
                                                 : args.record_bytes;
-      if (!ready && !wait_ready(empty + stage * 8u, phase ^ 1u, wctx, kErrWaitEmpty)) return;
+      ok = ready || wait_ready(empty + stage * 8u, phase ^ 1u, wctx, kErrWaitEmpty);
+      if (!ok) break;
       if (++stage == kStages) { stage = 0; phase ^= 1u; }
       ready = mbar_test_wait(empty + stage * 8u, phase ^ 1u);
       mbar_arrive_expect_tx(fb, bytes + kTokenBytes);
       if (kPart != kW4Tokens)
         bulk_load_hint(sa + kTokenBytes, w4_record(args, s, kb), bytes, fb, once);
       if (kPart != kW4Weights) w4_load_tokens<R>(tmap_t, slabs, sa, kb, s.row0, fb, keep);
+      ++issued;
     }
   }
+  drain_copies<kStages>(full, stage, phase, issued, wctx);
 }
 
 // Few rows (at most 32 to a tile): unpacked weights go straight from
