@@ -25,6 +25,12 @@
 // warp of its own between the load and the MMA, cost each tile 1.3 us: 8
 // experts x 1023 rows, 14336 x 4096, took 800 us where 1024 rows took 663.)
 // An expert without rows gets zeros.
+//
+// Bound by the tensor pipe: 8 experts, 8192 rows, 4096 x 4096, bf16: forward
+// 200 us, dA 198, dB 192 (1.37 to 1.43 PFLOP/s, 0.81 to 0.84 of a large
+// library product's rate), the pipe 87, 89 and 77 % active.  What is lost is
+// the last wave of tiles, the filling of each CTA's ring and, in dB, the
+// store of a whole weight tile.
 #pragma once
 #include <cuda_fp16.h>
 
@@ -64,7 +70,8 @@ struct GroupedCfg {
 };
 
 // dB: maps[2 e] and maps[2 e + 1] are dC's and A's tensor maps, ended at the
-// last row of expert e.  One warp per expert.
+// last row of expert e.  One warp per expert, 5 us: its parts follow one
+// another (two maps read, changed in shared memory, written, fenced).
 __global__ void __launch_bounds__(32)
 grouped_maps_kernel(const __grid_constant__ CUtensorMap tmap_dc,
                     const __grid_constant__ CUtensorMap tmap_a, const int* offsets, int rows,

@@ -14,6 +14,10 @@
 // up the chunks before its own and ranks its pairs (two launches; one when a
 // single block does it all).  Moving rows is bound by memory: one block per
 // token, every row read once and written once, sums in fp32.
+// 8192 tokens, 64 experts, two each, width 4096: choose 6.6 us and rank 11.7
+// (a chain of counts, barriers and ranks over 1024 threads; 3 MB), dispatch
+// 33 (202 MB, 6.1 TB/s), combine 37 (202 MB, 5.4 TB/s), its gradient 55
+// (336 MB, 6.1 TB/s), the logits' gradient 6.4.
 #pragma once
 #include "moe_groups.cuh"
 

