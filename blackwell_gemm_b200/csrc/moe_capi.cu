@@ -75,8 +75,18 @@ bool init_stream() {
          set_smem(grouped_stream_kernel<kDA, 64, T>, StreamCfg<64>::smem_bytes(kMaxExperts));
 }
 
+template <int kGroup, class T>
+constexpr bool kSplits = kFormat<T> == 1 && kGroup < 128;  // w4_split_kernel is there
+
 template <int kGroup, bool kZeros, class T>
 bool init_w4_one() {
+  if constexpr (kSplits<kGroup, T>) {
+    if (!set_smem(w4_split_kernel<64, kGroup, kZeros>,
+                  W4SplitCfg<64, kGroup>::smem_bytes(kMaxExperts)) ||
+        !set_smem(w4_split_kernel<128, kGroup, kZeros>,
+                  W4SplitCfg<128, kGroup>::smem_bytes(kMaxExperts)))
+      return false;
+  }
   if constexpr (kGroup < 128) {
     if (!set_smem(w4_rows_kernel<32, kGroup, kZeros, T>,
                   W4RowsCfg<32, kGroup>::smem_bytes(kMaxExperts)))
@@ -466,14 +476,16 @@ int check_w4_shape(int experts, int N, int K, int group) {
              : B200_ERR_TOO_LARGE;
 }
 
-enum W4Kind { kW4Few, kW4Some, kW4Wide };  // rows, stream and wide kernel
+enum W4Kind { kW4Few, kW4Some, kW4Wide, kW4Split };  // rows, stream, wide, split kernel
 
 template <W4Kind kKind, int kTok, int kGroup, bool kZeros, class T>
 int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   constexpr int box_rows = W4Ring<kTok, kGroup>::kSlabRows;
   CUtensorMap tt;
   int st;
-  if (kKind == kW4Wide) {
+  if (kKind == kW4Split) {
+    st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, kTok);
+  } else if (kKind == kW4Wide) {
     st = map_rows(&tt, c.dtype, c.a, c.K, c.rows, c.lda, W4WideCfg<kGroup>::kBox);
   } else if (c.K % kSlabK == 0) {  // (k in a slab, row, slab)
     const cuuint64_t dims[3] = {kSlabK, (cuuint64_t)c.rows, (cuuint64_t)(c.K / kSlabK)};
@@ -507,6 +519,10 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
     using C = W4RowsCfg<kTok, kGroup>;
     return launch(w4_rows_kernel<kTok, kGroup, kZeros, T>, v.sms, C::kThreads,
                   C::smem_bytes(c.experts), stream, tt, a);
+  } else if constexpr (kKind == kW4Split) {
+    using C = W4SplitCfg<kTok, kGroup>;
+    return launch(w4_split_kernel<kTok, kGroup, kZeros>, v.sms, C::kThreads,
+                  C::smem_bytes(c.experts), stream, tt, a);
   } else if constexpr (kKind == kW4Wide) {
     using C = W4WideCfg<kGroup>;
     return launch(w4_wide_kernel<kGroup, kZeros, T>, v.sms, C::kThreads, C::smem_bytes(c.experts),
@@ -533,6 +549,19 @@ int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   if constexpr (kGroup < 128) {
     if (c.rows <= 32 || c.rows <= 16ll * c.experts)
       return launch_w4<kW4Few, 32, kGroup, kZeros, T>(c, v, stream);
+  }
+  // bf16, small groups: weights as the sum of two bf16, so that no group's sums
+  // are read back (one matrix of 14336 x 4096, groups of 32: 64 rows 44 and 35
+  // us, 128 rows 63 and 46, 2048 rows 606 and 390; 8 experts, groups of 64: 256
+  // rows 164 and 131, 1024 rows 344 and 253).  One matrix in groups of 64 is
+  // better off without (2048 rows 358 and 390), as are groups of 128 (276 and
+  // 389).
+  if constexpr (kSplits<kGroup, T>) {
+    if (kGroup == 32 || c.experts > 1) {
+      if (c.rows <= 64ll * c.experts)
+        return launch_w4<kW4Split, 64, kGroup, kZeros, T>(c, v, stream);
+      return launch_w4<kW4Split, 128, kGroup, kZeros, T>(c, v, stream);
+    }
   }
   // Tiles of 64 rows or of 256.  One matrix: as soon as 64 do not hold them
   // (96 rows x 14336 x 4096: 42.2 us in two tiles, 40.2 in a wide one; groups

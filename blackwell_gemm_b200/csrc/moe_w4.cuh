@@ -8,9 +8,10 @@
 // bound by the 4-bit stream from HBM and, close behind, by the integer work of
 // unpacking it.  The tensor core takes the rest: warps unpack q - z -- small
 // integers, exact in 16 bits -- and these are the MMA's A operand (128 weight
-// rows), with the tokens as its N.  A group's product leaves the tensor core as fp32 and is multiplied by its scale
-// there, in fp32, on the way into the running sum: no weight is ever rounded
-// to 16 bits.
+// rows), with the tokens as its N.  A group's product leaves the tensor core as
+// fp32 and is multiplied by its scale there, in fp32, on the way into the
+// running sum: no weight is ever rounded to 16 bits.  (w4_split_kernel has
+// another way to the same end.)
 //
 // Weights are laid out once (w4_pack_kernel) in records of 128 rows x 128 k,
 // in the order a CTA walks them, so a record is one bulk copy and a CTA's
@@ -22,9 +23,10 @@
 //   scales  [128 / G][128 rows], 16-bit
 //   zeros   [128 / G][128 rows], 8-bit, when there are any
 //
-// Work is divided as in moe_stream.cuh (items are records).  Three kernels
-// by the rows of a tile: up to 32 with warp-level MMAs (w4_rows_kernel), 64
-// and 256 through TMEM (w4_stream_kernel, w4_wide_kernel).
+// Work is divided as in moe_stream.cuh (items are records).  Kernels by the
+// rows of a tile: up to 32 with warp-level MMAs (w4_rows_kernel), 64 and 256
+// through TMEM (w4_stream_kernel, w4_wide_kernel), 64 and 128 for small groups
+// of bf16 (w4_split_kernel).
 #pragma once
 #include "moe_stream.cuh"
 
@@ -725,6 +727,399 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
         const bool valid =
             __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
         stream_finish<32, T, 2>(args, walk, s, quarter, (int)set * 4 + quarter, tok0, acc, valid);
+      }
+    }
+    __syncwarp();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after_sync();
+    tmem_dealloc_1(tmem_base, kTmemCols);
+  }
+}
+
+// More rows, bf16: scaled weights as the sum of two bf16.  w = s (q - z) has 8
+// + 4 significant bits.  hi = bf16((q - z) bf16(31/32 s)) is w (1 - 1/32) but
+// for two roundings, so lo = w - hi lies between 2^-6 and 2^-3 of w's first
+// bit: its bits down to w's last are at most eight, and it is exact.  The sum of
+// the two products is the weight's, unrounded; and as lo has w's sign and is
+// zero only where w is, a token's infinity comes out as one, not as the NaN of
+// inf - inf or inf x 0.  The tensor core works twice, but no group's sums are read back: the running sum
+// stays in TMEM to the end of the tile.  (fp16 scales have 11 bits, which two
+// fp16 hold as well, but not their range: a weight past 65504, or its low part
+// below 2^-24, would be lost.  fp16 takes the kernels above and below.)
+// (q - z) carries kUnit here too, which the finished sum gives back; scales
+// below 2^-100 lose low bits to it.
+//
+// Warps: 0 records, 1 MMA, 2 tokens, 4-11 two sets that take records in turn
+// to unpack, 12-15 finish tiles.  kTok 128: two buffers of sums and two
+// records' weights fill TMEM; 64: two and three.
+//
+// What bounds it: up to 64 rows a record's unpacking, 1050 cycles (twelve
+// packed multiply-adds for eight weights keep their pipe full; a third
+// set of warps changed nothing); 128 rows, 16 MMAs with their A in TMEM, 1700.
+// 2048 rows x 14336 x 4096, groups of 32: 390 us (0.62 PFLOP/s), where reading
+// back each group's sums takes 600.
+template <int kTok_, int kGroup>
+struct W4SplitCfg {
+  static constexpr int kTok = kTok_;
+  static constexpr int kSub = kW4K / kGroup;
+  static constexpr int kSlab = kTok * 128;
+  static constexpr int kTokens = 2 * kSlab;  // a record's
+  static constexpr int kTokenStages = 4;
+  static constexpr int kPlaces = (kTmemCols - 2 * kTok) / 128;
+  static constexpr int kRecord = (w4_record_bytes(kGroup, true) + 127) / 128 * 128;
+  static constexpr int kRoom = (214 * 1024 - kTokenStages * kTokens) / kRecord;
+  static constexpr int kStages = kRoom < 12 ? kRoom : 12;
+  // Sets of unpacking warps, a record each in turn: no more than places, so
+  // that two sets never wait for one place, whose phases they could confuse.
+  static constexpr int kSets = 2;
+  static_assert(kSets <= kPlaces, "one set to a place at a time");
+  static constexpr int kThreads = 32 * (8 + 4 * kSets);
+  static constexpr int smem_bytes(int experts) {
+    return kTokenStages * kTokens + kStages * kRecord + group_table_bytes(experts) + 1024;
+  }
+};
+
+// hi + lo = p s, two weights at a time; `less`: 31/32 s.
+__device__ __forceinline__ void w4_split(uint32_t p, uint32_t s, uint32_t less, uint32_t* hi,
+                                         uint32_t* lo) {
+  const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&p);
+  const __nv_bfloat162 b = *reinterpret_cast<const __nv_bfloat162*>(&s);
+  const __nv_bfloat162 h = __hmul2_rn(a, *reinterpret_cast<const __nv_bfloat162*>(&less));
+  const __nv_bfloat162 l = __hfma2(a, b, __hneg2(h));
+  *hi = *reinterpret_cast<const uint32_t*>(&h);
+  *lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+
+// stream_finish for sums that are still in TMEM (`acc`: this warp's lanes,
+// first column), 16 columns at a time; `freed` is told when they are read.
+template <int kTok>
+__device__ __forceinline__ void w4_split_finish(const StreamArgs& a, const StreamWalk<kTok>& walk,
+                                                const StreamSegment& s, int quarter, uint32_t acc,
+                                                uint32_t freed, bool valid) {
+  using T = __nv_bfloat16;
+  constexpr float kScale = 1.0f / W4Unpack<T>::kUnit;
+  const int lane = threadIdx.x & 31;
+  const int f = s.block * 128 + quarter * 32 + lane;
+  const bool whole = s.kb0 == 0 && s.kb1 == walk.red_blocks;
+  int c0 = blockIdx.x, c1 = blockIdx.x;
+  if (!whole) {
+    const long long first = s.unit * walk.red_blocks;
+    c0 = sk_owner(first, walk.items, walk.ranges);
+    c1 = sk_owner(first + walk.red_blocks - 1, walk.items, walk.ranges);
+  }
+  auto slot = [&](int c) {
+    return a.slots + ((long long)c * 2 + (c == c0 ? 1 : 0)) * kTok * 128 + quarter * 32 + lane;
+  };
+  auto store = [&](int t0, const float (&v)[16]) {
+    T* col = static_cast<T*>(a.out) + (long long)(s.row0 + t0) * a.ldo + f;
+    const int rows = s.rows - t0;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      if (i < rows && f < a.feat) *col = round_one<T>(v[i] * kScale);
+      col += a.ldo;
+    }
+  };
+  tc_fence_after_sync();
+  if (valid) {
+#pragma unroll 1
+    for (int t0 = 0; t0 < s.rows; t0 += 16) {
+      uint32_t r[16];
+      tmem_ld_32x32b_x16(acc + t0, r);
+      tmem_wait_ld();
+      float v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+      if (whole) {
+        store(t0, v);
+      } else {
+        float* to = slot(blockIdx.x) + t0 * 128;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) __stcg(to + i * 128, v[i]);
+      }
+    }
+  }
+  tc_fence_before_sync();
+  __syncwarp();
+  if (lane == 0) mbar_arrive_local(freed);
+  if (whole) return;
+  unsigned int before = 0;
+  if (lane == 0) before = atomic_add_acq_rel(a.counts + c0 * 16 + quarter, 1u);
+  before = __shfl_sync(0xffffffffu, before, 0);
+  if (before != (unsigned int)(c1 - c0)) return;
+  __syncwarp();
+  if (lane == 0) atomicExch(a.counts + c0 * 16 + quarter, 0u);
+  if (!valid) return;
+#pragma unroll 1
+  for (int t0 = 0; t0 < s.rows; t0 += 16) {
+    float sum[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) sum[i] = 0.0f;
+    // parts in range order, two parts' loads in flight
+#pragma unroll 1
+    for (int p = c0; p <= c1; p += 2) {
+      const float* at = slot(p) + t0 * 128;
+      const float* bt = slot(p < c1 ? p + 1 : p) + t0 * 128;
+      float v[2][16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[0][i] = __ldcg(at + i * 128);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) v[1][i] = p < c1 ? __ldcg(bt + i * 128) : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[i] += v[0][i];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) sum[i] += v[1][i];
+    }
+    store(t0, sum);
+  }
+}
+
+// tmap_t: the token operand (k, row), box 64 x kTok.
+template <int kTok, int kGroup, bool kZeros>
+__global__ void __launch_bounds__(W4SplitCfg<kTok, kGroup>::kThreads, 1)
+w4_split_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args) {
+  using T = __nv_bfloat16;
+  using C = W4SplitCfg<kTok, kGroup>;
+  using U = W4Unpack<T>;
+  constexpr int kSub = C::kSub;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ alignas(8) uint64_t bar_full[C::kStages];
+  __shared__ alignas(8) uint64_t bar_empty[C::kStages];
+  __shared__ alignas(8) uint64_t bar_tok_full[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_tok_empty[C::kTokenStages];
+  __shared__ alignas(8) uint64_t bar_unpacked[C::kPlaces];
+  __shared__ alignas(8) uint64_t bar_used[C::kPlaces];
+  __shared__ alignas(8) uint64_t bar_acc_full[2];
+  __shared__ alignas(8) uint64_t bar_acc_empty[2];
+  __shared__ alignas(8) uint64_t bar_drain;
+  __shared__ uint32_t tmem_slot;
+  __shared__ uint32_t abort_word;
+
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
+  const int lane = threadIdx.x & 31;
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  const uint32_t records = smem_base + C::kTokenStages * C::kTokens;
+  int* s_off = reinterpret_cast<int*>(
+      smem_raw + (records + C::kStages * C::kRecord - smem_u32(smem_raw)));
+  int* s_tiles = s_off + args.experts + 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kStages; ++s) {
+      mbar_init(smem_u32(&bar_full[s]), 1);
+      mbar_init(smem_u32(&bar_empty[s]), 4);
+    }
+    for (int s = 0; s < C::kTokenStages; ++s) {
+      mbar_init(smem_u32(&bar_tok_full[s]), 1);
+      mbar_init(smem_u32(&bar_tok_empty[s]), 1);
+    }
+    for (int b = 0; b < C::kPlaces; ++b) {
+      mbar_init(smem_u32(&bar_unpacked[b]), 4);
+      mbar_init(smem_u32(&bar_used[b]), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(smem_u32(&bar_acc_full[b]), 1);
+      mbar_init(smem_u32(&bar_acc_empty[b]), 4);
+    }
+    mbar_init(smem_u32(&bar_drain), 1);
+    abort_word = 0;
+    fence_mbar_init_cluster();
+    prefetch_tmap(&tmap_t);
+  }
+  if (warp == 1) {
+    tmem_alloc_1(smem_u32(&tmem_slot), kTmemCols);
+    tmem_relinquish_1();
+  }
+  grid_wait();
+  if (warp == 2) stream_groups(args, kTok, s_off, s_tiles);
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  grid_launch_next();
+  const uint32_t tmem_base = tmem_slot;
+  const uint32_t tmem_a = tmem_base + 2 * kTok;
+
+  WaitCtx wctx;
+  wctx.status = args.status;
+  wctx.timeout_ns = args.timeout_ns;
+  wctx.abort_local = smem_u32(&abort_word);
+  wctx.abort_peer = cluster_map(smem_u32(&abort_word), 0);
+
+  StreamWalk<kTok> walk;
+  walk.init(args, s_off, s_tiles);
+  StreamSegment s;
+
+  if (warp == 0) {
+    if (elect_one()) {
+      // (weights of a single tile are read once; several tiles come back to them)
+      const uint64_t policy =
+          s_tiles[args.experts] <= args.experts ? l2_policy_evict_first() : l2_policy_evict_normal();
+      uint32_t stage = 0, phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      while (ok && walk.next(&s)) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          ok = wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&bar_full[stage]);
+          mbar_arrive_expect_tx(bar, args.record_bytes);
+          bulk_load_hint(records + stage * C::kRecord, w4_record(args, s, kb), args.record_bytes,
+                         bar, policy);
+          ++issued;
+          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      drain_copies<C::kStages>(smem_u32(&bar_full[0]), stage, phase, issued, wctx);
+    }
+    __syncwarp();
+  } else if (warp == 2) {
+    if (elect_one()) {
+      const uint64_t policy = l2_policy_evict_last();
+      uint32_t stage = 0, phase = 0;
+      long long issued = 0;
+      bool ok = true;
+      while (ok && walk.next(&s)) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          ok = wait_ready(smem_u32(&bar_tok_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty);
+          if (!ok) break;
+          const uint32_t bar = smem_u32(&bar_tok_full[stage]);
+          mbar_arrive_expect_tx(bar, C::kTokens);
+          for (int b = 0; b < 2; ++b)
+            tma_load_2d_hint(smem_base + stage * C::kTokens + b * C::kSlab, &tmap_t,
+                             kb * kW4K + b * kSlabK, s.row0, bar, policy);
+          ++issued;
+          if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+        }
+      }
+      drain_copies<C::kTokenStages>(smem_u32(&bar_tok_full[0]), stage, phase, issued, wctx);
+    }
+    __syncwarp();
+  } else if (warp == 1) {
+    if (elect_one()) {
+      uint32_t stage = 0, phase = 0, w = 0, wp = 0, buf = 0, bp = 1;
+      bool ok = true;
+      // (looked at before the MMAs ahead of them go out)
+      bool landed = false, unpacked = false;
+      const uint32_t tok_full = smem_u32(&bar_tok_full[0]), tok_empty = smem_u32(&bar_tok_empty[0]),
+                     unpacked0 = smem_u32(&bar_unpacked[0]), used0 = smem_u32(&bar_used[0]);
+      while (ok && walk.next(&s)) {
+        const uint32_t idesc = make_idesc_16bit(128, (s.rows + 15) & ~15, kFormat<T>, false, false);
+        ok = wait_ready(smem_u32(&bar_acc_empty[buf]), bp, wctx, kErrWaitAccEmpty);
+        if (!ok) break;
+        const uint32_t d = tmem_base + buf * kTok;
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          if (!(unpacked || wait_ready(unpacked0 + w * 8u, wp, wctx, kErrWaitFull)) ||
+              !(landed || wait_ready(tok_full + stage * 8u, phase, wctx, kErrWaitFull))) {
+            ok = false;
+            break;
+          }
+          const uint64_t bdesc = make_sdesc_k128(smem_base + stage * C::kTokens);
+          const uint32_t a = tmem_a + w * 128;
+          const uint32_t my_tokens = tok_empty + stage * 8u, my_used = used0 + w * 8u;
+          if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
+          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+          landed = mbar_test_wait(tok_full + stage * 8u, phase);
+          unpacked = mbar_test_wait(unpacked0 + w * 8u, wp);
+          tc_fence_after_sync();
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t b = bdesc + ((k >> 2) * C::kSlab + (k & 3) * 32) / 16;
+            umma_tmem_a_1(d, a + k * 8, b, idesc, k != 0 || kb != s.kb0 ? 1u : 0u);
+            umma_tmem_a_1(d, a + 64 + k * 8, b, idesc, 1u);
+          }
+          umma_commit_1(my_used);
+          umma_commit_1(my_tokens);
+        }
+        if (!ok) break;
+        umma_commit_1(smem_u32(&bar_acc_full[buf]));
+        buf ^= 1u;
+        if (buf == 0) bp ^= 1u;
+      }
+      umma_commit_1(smem_u32(&bar_drain));
+      if (!mbar_try_wait(smem_u32(&bar_drain), 0))
+        wait_slow(smem_u32(&bar_drain), 0, wctx, kErrWaitDrain, false);
+    }
+    __syncwarp();
+  } else if (warp >= 4) {
+    const int quarter = warp & 3;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    auto wait_warp = [&](uint32_t bar, uint32_t parity, int code) {
+      if (__all_sync(0xffffffffu, mbar_test_wait(bar, parity))) return true;
+      int got = 0;
+      if (lane == 0) got = wait_ready(bar, parity, wctx, code);
+      got = __shfl_sync(0xffffffffu, got, 0);
+      __syncwarp();
+      return got != 0;
+    };
+    bool ok = true;
+    if (warp < 4 + 4 * C::kSets) {
+      // ----------------------------------------------------------- unpack
+      const int row = quarter * 32 + lane;
+      const uint32_t set = (uint32_t)(warp - 4) >> 2;
+      uint32_t stage = 0, phase = 0, w = 0, wp = 0, turn = 0;
+      while (ok && walk.next(&s)) {
+        for (int kb = s.kb0; kb < s.kb1; ++kb) {
+          if (turn == set) {
+            ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull);
+            if (!ok) break;
+            const uint32_t record = records + stage * C::kRecord;
+            uint32_t bias[kSub], scale[kSub], less[kSub];
+#pragma unroll
+            for (int g = 0; g < kSub; ++g) {
+              bias[g] = w4_bias<T>(
+                  kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
+              scale[g] = ld_shared_u16(record + kW4Q + (g * 128 + row) * 2) * 0x10001u;
+              less[g] = U::fma2(scale[g], 0x3F783F78u, 0u);
+            }
+            uint32_t q[4][4];  // [t][c]
+#pragma unroll
+            for (int t = 0; t < 4; ++t) ld_shared_v4_u32(record + w4_q_offset(t, row), q[t]);
+            ok = wait_warp(smem_u32(&bar_used[w]), wp ^ 1u, kErrWaitAccEmpty);
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint32_t a = tmem_a + w * 128 + lanes;
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              uint32_t hi[16], lo[16];
+#pragma unroll
+              for (int t = 0; t < 4; ++t) {
+                uint32_t v[4];
+                w4_pairs<T>(q[t][c], bias[c * 32 / kGroup], v);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  w4_split(v[i], scale[c * 32 / kGroup], less[c * 32 / kGroup], &hi[t * 4 + i],
+                           &lo[t * 4 + i]);
+              }
+              tmem_st_32x32b_x16(a + c * 16, hi);
+              tmem_st_32x32b_x16(a + 64 + c * 16, lo);
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+            tmem_wait_st();
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_local(smem_u32(&bar_unpacked[w]));
+          }
+          if (++turn == C::kSets) turn = 0;
+          if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
+          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+        }
+      }
+    } else {
+      // ----------------------------------------------------------- finish
+      zero_unowned_rows(static_cast<T*>(args.out), args.ldo, args.feat, s_off[0],
+                        s_off[args.experts], args.rows,
+                        (long long)blockIdx.x * 128 + (threadIdx.x & 127), gridDim.x * 128ll);
+      uint32_t buf = 0, bp = 0;
+      while (walk.next(&s)) {
+        ok = ok && wait_warp(smem_u32(&bar_acc_full[buf]), bp, kErrWaitAccFull);
+        const bool valid =
+            __all_sync(0xffffffffu, ok && ld_volatile_shared(wctx.abort_local) == 0);
+        w4_split_finish<kTok>(args, walk, s, quarter, tmem_base + buf * kTok + lanes,
+                              smem_u32(&bar_acc_empty[buf]), valid);
+        buf ^= 1u;
+        if (buf == 0) bp ^= 1u;
       }
     }
     __syncwarp();

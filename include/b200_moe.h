@@ -126,8 +126,9 @@ int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* pac
 /* C[r, :] = A[r, :] W[e]^T with packed weights.  offsets as for
  * b200_grouped_gemm, or NULL for experts = 1: every row takes the one matrix.
  * A: rows x K, stride lda; C: rows x N, stride ldc; alignment as there.  The
- * weights enter as exact integers, the scales multiply fp32 sums.  Any number
- * of rows; made for few (the weights are read once per 64 rows of an expert). */
+ * weights enter unrounded: as exact integers whose fp32 sums the scales
+ * multiply, or as the sum of two bf16.  Any number of rows (the weights are
+ * read once per 8 to 256 rows of an expert). */
 int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets, int rows,
                  int experts, int N, int K, int group, int zeros, int lda, int ldc, int dtype,
                  void* stream);

@@ -133,6 +133,48 @@ def test_bank(offsets, rows, group):
     assert not y[~owned].any()
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("experts,m", [(1, 2), (1, 20), (1, 50), (1, 140), (1, 300), (2, 100),
+                                       (2, 700)])
+def test_infinities_and_nan_in_tokens(experts, m, group, dtype):
+    # one inf, -inf or NaN in a row: inf with the weight's sign, NaN where it is 0
+    dt, _ = DT[dtype]
+    n, k = 136, 256
+    q, s, z, w = weights(experts, n, k, group, True, dt, seed=m)
+    x = rows_of(m, k, dt)
+    odd = torch.arange(0, m, 3, device="cuda")
+    x[odd, (7 * odd) % k] = float("inf")
+    x[odd[1::3], (7 * odd[1::3]) % k] = float("-inf")
+    x[odd[2::3], (7 * odd[2::3]) % k] = float("nan")
+    off = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    if experts == 1:
+        y, want = bg.matmul_b200_w4(x, bg.pack_w4(q[0], s[0], z[0])), x.double() @ w[0].T
+    else:
+        y = bg.matmul_b200_w4(x, bg.pack_w4(q, s, z), off)
+        want = torch.cat([x[:m // 2].double() @ w[0].T, x[m // 2:].double() @ w[1].T])
+    assert torch.equal(y.isnan(), want.isnan())
+    assert torch.equal(y.isposinf(), want.isposinf())
+    assert torch.equal(y.isneginf(), want.isneginf())
+
+
+@pytest.mark.parametrize("group", [32, 64])
+def test_every_scale_keeps_its_bits(group):
+    # weights m 2^e (q - z) for all 128 significands, in units fp32 sums hold:
+    # tokens of one 1 each return the weights themselves
+    n, k, m = 128, 512, 512
+    s = (1 + torch.arange(n, device="cuda") / 128).bfloat16().repeat_interleave(k // group).view(n, -1)
+    q = torch.arange(n * k // 2, device="cuda").mul(73).remainder(256).to(torch.uint8).view(n, -1)
+    z = torch.arange(n * k // group, device="cuda").mul(5).remainder(16).to(torch.uint8).view(n, -1)
+    wide = torch.stack((q & 15, q >> 4), -1).view(n, k).double()
+    w = (wide - z.double().repeat_interleave(group, 1)) * s.double().repeat_interleave(group, 1)
+    x = torch.eye(m, device="cuda").bfloat16()
+    y = bg.matmul_b200_w4(torch.cat([x, x]), bg.pack_w4(torch.stack([q, q]), torch.stack([s, s]),
+                                                        torch.stack([z, z])),
+                          torch.tensor([0, m, 2 * m], dtype=torch.int32, device="cuda"))
+    assert torch.equal(y[:m], w.T.bfloat16()) and torch.equal(y[m:], w.T.bfloat16())
+
+
 def test_every_nibble_and_exact_bits():
     # weights, rows and scales whose products and sums fp32 holds exactly
     n, k = 256, 256
