@@ -229,6 +229,7 @@ struct W4RowsCfg {
   static constexpr int kGroups = kTok <= 8 ? 4 : kTok <= 16 ? 3 : 2;
   static constexpr int kExchange = kGroups * kTok * kPitch * 4;
   static constexpr int kStages = Ring::stages(kExchange);
+  static_assert(kGroups <= kStages, "one group to a stage at a time");
   static constexpr int kThreads = 32 * (4 * kGroups + 1);
   static constexpr int smem_bytes(int experts) {
     return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;
