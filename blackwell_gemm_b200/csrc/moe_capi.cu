@@ -76,7 +76,9 @@ bool init_stream() {
 }
 
 template <int kGroup, class T>
-constexpr bool kSplits = kFormat<T> == 1 && kGroup < 128;  // w4_split_kernel is there
+constexpr bool kSplits = kFormat<T> == 1 && kGroup < 128;  // w4_split_kernel is used
+template <int kGroup, class T>
+constexpr bool kOnlySplits = kSplits<kGroup, T> && kGroup == 32;  // ... for all many-row calls
 
 template <int kGroup, bool kZeros, class T>
 bool init_w4_one() {
@@ -92,12 +94,15 @@ bool init_w4_one() {
                   W4RowsCfg<32, kGroup>::smem_bytes(kMaxExperts)))
       return false;
   }
+  if constexpr (!kOnlySplits<kGroup, T>) {
+    if (!set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts)) ||
+        !set_smem(w4_wide_kernel<kGroup, kZeros, T>, W4WideCfg<kGroup>::smem_bytes(kMaxExperts)))
+      return false;
+  }
   return set_smem(w4_rows_kernel<8, kGroup, kZeros, T>,
                   W4RowsCfg<8, kGroup>::smem_bytes(kMaxExperts)) &&
          set_smem(w4_rows_kernel<16, kGroup, kZeros, T>,
-                  W4RowsCfg<16, kGroup>::smem_bytes(kMaxExperts)) &&
-         set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts)) &&
-         set_smem(w4_wide_kernel<kGroup, kZeros, T>, W4WideCfg<kGroup>::smem_bytes(kMaxExperts));
+                  W4RowsCfg<16, kGroup>::smem_bytes(kMaxExperts));
 }
 
 template <int kGroup, class T>
@@ -535,6 +540,13 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
 }
 
 template <int kGroup, bool kZeros, class T>
+int run_w4_split(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
+  if (c.rows <= 64ll * c.experts)
+    return launch_w4<kW4Split, 64, kGroup, kZeros, T>(c, v, stream);
+  return launch_w4<kW4Split, 128, kGroup, kZeros, T>(c, v, stream);
+}
+
+template <int kGroup, bool kZeros, class T>
 int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   // A tile as wide as most experts' rows: an expert with more takes another
   // tile, that is, reads its weights again.
@@ -556,24 +568,24 @@ int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   // rows 164 and 131, 1024 rows 344 and 253).  One matrix in groups of 64 is
   // better off without (2048 rows 358 and 390), as are groups of 128 (276 and
   // 389).
-  if constexpr (kSplits<kGroup, T>) {
-    if (kGroup == 32 || c.experts > 1) {
-      if (c.rows <= 64ll * c.experts)
-        return launch_w4<kW4Split, 64, kGroup, kZeros, T>(c, v, stream);
-      return launch_w4<kW4Split, 128, kGroup, kZeros, T>(c, v, stream);
+  if constexpr (kOnlySplits<kGroup, T>) {
+    return run_w4_split<kGroup, kZeros, T>(c, v, stream);
+  } else {
+    if constexpr (kSplits<kGroup, T>) {
+      if (c.experts > 1) return run_w4_split<kGroup, kZeros, T>(c, v, stream);
     }
+    // Tiles of 64 rows or of 256.  One matrix: as soon as 64 do not hold them
+    // (96 rows x 14336 x 4096: 42.2 us in two tiles, 40.2 in a wide one; groups
+    // of 32 66.8 and 62.8).  A bank: a wide tile costs the same from 129 rows
+    // on, so experts must fill it by half, in groups of 32 altogether (8
+    // experts of 14336 x 4096, groups of 128: 512 rows 153 and 184 us, 1024
+    // rows 262 and 236; groups of 32: 1024 rows 483 and 601, 2048 rows 900 and
+    // 890).
+    const long long some = c.experts == 1 ? 64 : kGroup == 32 ? 256ll * c.experts : 96ll * c.experts;
+    if (c.rows <= some)
+      return launch_w4<kW4Some, 64, kGroup, kZeros, T>(c, v, stream);
+    return launch_w4<kW4Wide, 256, kGroup, kZeros, T>(c, v, stream);
   }
-  // Tiles of 64 rows or of 256.  One matrix: as soon as 64 do not hold them
-  // (96 rows x 14336 x 4096: 42.2 us in two tiles, 40.2 in a wide one; groups
-  // of 32 66.8 and 62.8).  A bank: a wide tile costs the same from 129 rows
-  // on, so experts must fill it by half, with small groups altogether (8
-  // experts of 14336 x 4096, groups of 128: 512 rows 153 and 184 us, 1024
-  // rows 262 and 236; groups of 32: 1024 rows 483 and 601, 2048 rows 900 and
-  // 890).
-  const long long some = c.experts == 1 ? 64 : kGroup == 32 ? 256ll * c.experts : 96ll * c.experts;
-  if (c.rows <= some)
-    return launch_w4<kW4Some, 64, kGroup, kZeros, T>(c, v, stream);
-  return launch_w4<kW4Wide, 256, kGroup, kZeros, T>(c, v, stream);
 }
 
 template <class T>

@@ -204,6 +204,45 @@ def test_strided_rows_and_repeatable_bits():
         assert torch.equal(first, bg.matmul_b200_w4(x, packed))
 
 
+@pytest.mark.parametrize("m", [5, 25, 60, 150, 400])
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_scales_over_the_range(m, group):
+    # a power of two in the scales is one in the answer, bit by bit
+    q, s, z, _ = weights(2, 136, 256, group, True, torch.bfloat16)
+    off = torch.tensor([0, m // 3, m], dtype=torch.int32, device="cuda")
+    x = rows_of(m, 256, torch.bfloat16)
+    y = bg.matmul_b200_w4(x, bg.pack_w4(q, s, z), off)
+    for p in (-80, 80):
+        scaled = bg.matmul_b200_w4(x, bg.pack_w4(q, (s.double() * 2.0 ** p).bfloat16(), z), off)
+        assert torch.equal(scaled.double(), y.double() * 2.0 ** p)
+
+
+@pytest.mark.parametrize("group,dtype", [(32, "bf16"), (32, "fp16"), (128, "bf16")])
+def test_many_rows_on_other_streams_and_in_graphs(group, dtype):
+    dt, u = DT[dtype]
+    n, k, m = 640, 2048, 300
+    q, s, _, w = weights(1, n, k, group, False, dt)
+    packed = bg.pack_w4(q[0], s[0])
+    odd = torch.zeros(m, k + 8, dtype=dt, device="cuda")
+    odd[:, 8:] = rows_of(m, k, dt)
+    x = odd[:, 8:]
+    first = bg.matmul_b200_w4(x, packed)
+    close(first, x, w[0], u, dtype == "fp16")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = bg.matmul_b200_w4(x, packed)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(first, again)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = bg.matmul_b200_w4(x, packed)
+    for _ in range(2):
+        y.zero_()
+        graph.replay()
+        assert torch.equal(first, y)
+
+
 def test_infinities_follow_the_product():
     n, k = 128, 256
     q, s, _, w = weights(1, n, k, 128, False, torch.bfloat16)
