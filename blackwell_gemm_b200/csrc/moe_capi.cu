@@ -76,9 +76,7 @@ bool init_stream() {
 }
 
 template <int kGroup, class T>
-constexpr bool kSplits = kFormat<T> == 1 && kGroup < 128;  // w4_split_kernel is used
-template <int kGroup, class T>
-constexpr bool kOnlySplits = kSplits<kGroup, T> && kGroup == 32;  // ... for all many-row calls
+constexpr bool kSplits = kFormat<T> == 1 && kGroup < 128;  // many rows: w4_split_kernel
 
 template <int kGroup, bool kZeros, class T>
 bool init_w4_one() {
@@ -88,15 +86,14 @@ bool init_w4_one() {
         !set_smem(w4_split_kernel<128, kGroup, kZeros>,
                   W4SplitCfg<128, kGroup>::smem_bytes(kMaxExperts)))
       return false;
+  } else {
+    if (!set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts)) ||
+        !set_smem(w4_wide_kernel<kGroup, kZeros, T>, W4WideCfg<kGroup>::smem_bytes(kMaxExperts)))
+      return false;
   }
   if constexpr (kGroup < 128) {
     if (!set_smem(w4_rows_kernel<32, kGroup, kZeros, T>,
                   W4RowsCfg<32, kGroup>::smem_bytes(kMaxExperts)))
-      return false;
-  }
-  if constexpr (!kOnlySplits<kGroup, T>) {
-    if (!set_smem(w4_stream_kernel<kGroup, kZeros, T>, W4Cfg<kGroup>::smem_bytes(kMaxExperts)) ||
-        !set_smem(w4_wide_kernel<kGroup, kZeros, T>, W4WideCfg<kGroup>::smem_bytes(kMaxExperts)))
       return false;
   }
   return set_smem(w4_rows_kernel<8, kGroup, kZeros, T>,
@@ -540,13 +537,6 @@ int launch_w4(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
 }
 
 template <int kGroup, bool kZeros, class T>
-int run_w4_split(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
-  if (c.rows <= 64ll * c.experts)
-    return launch_w4<kW4Split, 64, kGroup, kZeros, T>(c, v, stream);
-  return launch_w4<kW4Split, 128, kGroup, kZeros, T>(c, v, stream);
-}
-
-template <int kGroup, bool kZeros, class T>
 int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
   // A tile as wide as most experts' rows: an expert with more takes another
   // tile, that is, reads its weights again.
@@ -563,17 +553,15 @@ int run_w4_group(const W4Call& c, const DeviceView& v, cudaStream_t stream) {
       return launch_w4<kW4Few, 32, kGroup, kZeros, T>(c, v, stream);
   }
   // bf16, small groups: weights as the sum of two bf16, so that no group's sums
-  // are read back (one matrix of 14336 x 4096, groups of 32: 64 rows 44 and 35
-  // us, 128 rows 63 and 46, 2048 rows 606 and 390; 8 experts, groups of 64: 256
-  // rows 164 and 131, 1024 rows 344 and 253).  One matrix in groups of 64 is
-  // better off without (2048 rows 358 and 390), as are groups of 128 (276 and
-  // 389).
-  if constexpr (kOnlySplits<kGroup, T>) {
-    return run_w4_split<kGroup, kZeros, T>(c, v, stream);
+  // are read back (one matrix of 14336 x 4096, groups of 32: 64 rows 43 and 34
+  // us, 2048 rows 602 and 333; of 64: 37 and 34, 354 and 333; 1024 rows over 8
+  // experts 520 and 251, 345 and 237).  Groups of 128 are better off without
+  // (2048 rows 272 and 333).
+  if constexpr (kSplits<kGroup, T>) {
+    if (c.rows <= 64ll * c.experts)
+      return launch_w4<kW4Split, 64, kGroup, kZeros, T>(c, v, stream);
+    return launch_w4<kW4Split, 128, kGroup, kZeros, T>(c, v, stream);
   } else {
-    if constexpr (kSplits<kGroup, T>) {
-      if (c.experts > 1) return run_w4_split<kGroup, kZeros, T>(c, v, stream);
-    }
     // Tiles of 64 rows or of 256.  One matrix: as soon as 64 do not hold them
     // (96 rows x 14336 x 4096: 42.2 us in two tiles, 40.2 in a wide one; groups
     // of 32 66.8 and 62.8).  A bank: a wide tile costs the same from 129 rows

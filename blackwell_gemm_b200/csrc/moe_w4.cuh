@@ -754,13 +754,15 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
 // below 2^-100 lose low bits to it.
 //
 // Warps: 0 records, 1 MMA, 2 tokens, 4-11 two sets that take records in turn
-// to unpack, 12-15 finish tiles.  kTok 128: two buffers of sums and two
-// records' weights fill TMEM; 64: two and three.
+// to unpack, 12-15 finish tiles.  kTok 128: two buffers of sums and four half
+// records' weights fill TMEM; 64: two and three whole records'.
 //
 // What bounds it: up to 64 rows a record's unpacking, 1050 cycles (twelve
-// packed multiply-adds for eight weights keep their pipe full; a third
-// set of warps changed nothing); 128 rows, 16 MMAs with their A in TMEM, 1700.
-// 2048 rows x 14336 x 4096, groups of 32: 390 us (0.62 PFLOP/s), where reading
+// packed multiply-adds for eight weights keep their pipe full; a third set of
+// warps changed nothing); 128 rows, 1400, the way from unpacked weights
+// through the MMAs to a free place (with two places of whole records 1700;
+// with half of the MMAs left out only a tenth less).
+// 2048 rows x 14336 x 4096, groups of 32: 333 us (0.72 PFLOP/s), where reading
 // back each group's sums takes 600.
 template <int kTok_, int kGroup>
 struct W4SplitCfg {
@@ -769,14 +771,18 @@ struct W4SplitCfg {
   static constexpr int kSlab = kTok * 128;
   static constexpr int kTokens = 2 * kSlab;  // a record's
   static constexpr int kTokenStages = 4;
-  static constexpr int kPlaces = (kTmemCols - 2 * kTok) / 128;
+  // A place holds a record's weights or, with fewer columns left, half of
+  // them (hi, then lo), so that unpacking and MMAs take turns more finely.
+  static constexpr int kParts = kTok == 128 ? 2 : 1;
+  static constexpr int kPlace = 128 / kParts;  // columns
+  static constexpr int kPlaces = (kTmemCols - 2 * kTok) / kPlace;
   static constexpr int kRecord = (w4_record_bytes(kGroup, true) + 127) / 128 * 128;
   static constexpr int kRoom = (214 * 1024 - kTokenStages * kTokens) / kRecord;
   static constexpr int kStages = kRoom < 12 ? kRoom : 12;
   // Sets of unpacking warps, a record each in turn: no more than places, so
   // that two sets never wait for one place, whose phases they could confuse.
   static constexpr int kSets = 2;
-  static_assert(kSets <= kPlaces, "one set to a place at a time");
+  static_assert(kSets * kParts <= kPlaces && kPlaces % kParts == 0, "one set to a place at a time");
   static constexpr int kThreads = 32 * (8 + 4 * kSets);
   static constexpr int smem_bytes(int experts) {
     return kTokenStages * kTokens + kStages * kRecord + group_table_bytes(experts) + 1024;
@@ -1010,26 +1016,35 @@ w4_split_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs arg
         if (!ok) break;
         const uint32_t d = tmem_base + buf * kTok;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
-          if (!(unpacked || wait_ready(unpacked0 + w * 8u, wp, wctx, kErrWaitFull)) ||
-              !(landed || wait_ready(tok_full + stage * 8u, phase, wctx, kErrWaitFull))) {
+          if (!(landed || wait_ready(tok_full + stage * 8u, phase, wctx, kErrWaitFull))) {
             ok = false;
             break;
           }
           const uint64_t bdesc = make_sdesc_k128(smem_base + stage * C::kTokens);
-          const uint32_t a = tmem_a + w * 128;
-          const uint32_t my_tokens = tok_empty + stage * 8u, my_used = used0 + w * 8u;
+          const uint32_t my_tokens = tok_empty + stage * 8u;
           if (++stage == C::kTokenStages) { stage = 0; phase ^= 1u; }
-          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
           landed = mbar_test_wait(tok_full + stage * 8u, phase);
-          unpacked = mbar_test_wait(unpacked0 + w * 8u, wp);
-          tc_fence_after_sync();
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t b = bdesc + ((k >> 2) * C::kSlab + (k & 3) * 32) / 16;
-            umma_tmem_a_1(d, a + k * 8, b, idesc, k != 0 || kb != s.kb0 ? 1u : 0u);
-            umma_tmem_a_1(d, a + 64 + k * 8, b, idesc, 1u);
+          for (int h = 0; h < C::kParts; ++h) {
+            if (!(unpacked || wait_ready(unpacked0 + w * 8u, wp, wctx, kErrWaitFull))) {
+              ok = false;
+              break;
+            }
+            const uint32_t a = tmem_a + w * C::kPlace;
+            const uint32_t my_used = used0 + w * 8u;
+            if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+            unpacked = mbar_test_wait(unpacked0 + w * 8u, wp);
+            tc_fence_after_sync();
+#pragma unroll
+            for (int i = 0; i < 8 / C::kParts; ++i) {
+              const int k = h * (8 / C::kParts) + i;
+              const uint64_t b = bdesc + ((k >> 2) * C::kSlab + (k & 3) * 32) / 16;
+              umma_tmem_a_1(d, a + i * 8, b, idesc, k != 0 || kb != s.kb0 ? 1u : 0u);
+              umma_tmem_a_1(d, a + C::kPlace / 2 + i * 8, b, idesc, 1u);
+            }
+            umma_commit_1(my_used);
           }
-          umma_commit_1(my_used);
+          if (!ok) break;
           umma_commit_1(my_tokens);
         }
         if (!ok) break;
@@ -1076,35 +1091,42 @@ w4_split_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs arg
             uint32_t q[4][4];  // [t][c]
 #pragma unroll
             for (int t = 0; t < 4; ++t) ld_shared_v4_u32(record + w4_q_offset(t, row), q[t]);
-            ok = wait_warp(smem_u32(&bar_used[w]), wp ^ 1u, kErrWaitAccEmpty);
-            if (!ok) break;
-            tc_fence_after_sync();
-            const uint32_t a = tmem_a + w * 128 + lanes;
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              uint32_t hi[16], lo[16];
+            for (int h = 0; h < C::kParts; ++h) {
+              ok = ok && wait_warp(smem_u32(&bar_used[w + h]), wp ^ 1u, kErrWaitAccEmpty);
+              if (!ok) break;
+              tc_fence_after_sync();
+              const uint32_t a = tmem_a + (w + h) * C::kPlace + lanes;
 #pragma unroll
-              for (int t = 0; t < 4; ++t) {
-                uint32_t v[4];
-                w4_pairs<T>(q[t][c], bias[c * 32 / kGroup], v);
+              for (int j = 0; j < 4 / C::kParts; ++j) {
+                const int c = h * (4 / C::kParts) + j;
+                uint32_t hi[16], lo[16];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  w4_split(v[i], scale[c * 32 / kGroup], less[c * 32 / kGroup], &hi[t * 4 + i],
-                           &lo[t * 4 + i]);
+                for (int t = 0; t < 4; ++t) {
+                  uint32_t v[4];
+                  w4_pairs<T>(q[t][c], bias[c * 32 / kGroup], v);
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    w4_split(v[i], scale[c * 32 / kGroup], less[c * 32 / kGroup], &hi[t * 4 + i],
+                             &lo[t * 4 + i]);
+                }
+                tmem_st_32x32b_x16(a + j * 16, hi);
+                tmem_st_32x32b_x16(a + C::kPlace / 2 + j * 16, lo);
               }
-              tmem_st_32x32b_x16(a + c * 16, hi);
-              tmem_st_32x32b_x16(a + 64 + c * 16, lo);
+              tmem_wait_st();
+              tc_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) {
+                mbar_arrive_local(smem_u32(&bar_unpacked[w + h]));
+                if (h == C::kParts - 1) mbar_arrive_local(smem_u32(&bar_empty[stage]));
+              }
             }
-            __syncwarp();
-            if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
-            tmem_wait_st();
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_local(smem_u32(&bar_unpacked[w]));
+            if (!ok) break;
           }
           if (++turn == C::kSets) turn = 0;
           if (++stage == C::kStages) { stage = 0; phase ^= 1u; }
-          if (++w == C::kPlaces) { w = 0; wp ^= 1u; }
+          w += C::kParts;
+          if (w == C::kPlaces) { w = 0; wp ^= 1u; }
         }
       }
     } else {
