@@ -759,9 +759,9 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
 //
 // What bounds it: up to 64 rows a record's unpacking, 1050 cycles (twelve
 // packed multiply-adds for eight weights keep their pipe full; a third set of
-// warps changed nothing); 128 rows, 1400, the way from unpacked weights
-// through the MMAs to a free place (with two places of whole records 1700;
-// with half of the MMAs left out only a tenth less).
+// warps changed nothing); 128 rows, 1400 to 1600, the tensor pipe 74 % active
+// (75 cycles for an MMA of 128 columns with its A in TMEM) and the rest the way
+// from unpacked weights to a free place (1700 with two places of whole records).
 // 2048 rows x 14336 x 4096, groups of 32: 333 us (0.72 PFLOP/s), where reading
 // back each group's sums takes 600.
 template <int kTok_, int kGroup>
