@@ -632,7 +632,12 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
           const bool pair = kb + 1 < s.kb1;
           if (set == 1) {
             next_place();
-            if (!pair) {  // nothing to unpack; the stage still counts this warp
+            if (!pair) {
+              // Nothing to unpack; the stage still counts this warp.  It waits
+              // for the record all the same: a set that did not could come
+              // round to the stage again and release it for the other.
+              ok = wait_warp(smem_u32(&bar_full[stage]), phase, kErrWaitFull);
+              if (!ok) break;
               if (lane == 0) mbar_arrive_local(smem_u32(&bar_empty[stage]));
               continue;
             }

@@ -1,0 +1,40 @@
+"""4-bit products where the kernels' rings, scales and arguments meet their ends.
+
+Tolerances are those of test_w4_gpu.py."""
+import pytest
+import torch
+
+import blackwell_gemm_b200 as bg
+from blackwell_gemm_b200 import capi
+from test_w4_gpu import DT, close, rows_of, weights
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _clean():
+    capi.device_status(True)
+    yield
+    assert capi.device_status(True) == 0
+
+
+@pytest.mark.parametrize("dtype,k,group", [
+    ("fp16", 32, 32), ("fp16", 64, 32), ("fp16", 64, 64), ("fp16", 96, 32), ("fp16", 128, 32),
+    ("fp16", 128, 64), ("fp16", 128, 128), ("bf16", 128, 128), ("bf16", 384, 128),
+    ("bf16", 96, 32), ("bf16", 128, 64)])
+def test_short_contractions_through_many_tiles(dtype, k, group):
+    # one or three records to a tile, several laps of every ring in each CTA
+    dt, u = DT[dtype]
+    experts, n = 64, 5504
+    q, s, z, w = weights(experts, n, k, group, group != 64, dt, seed=k)
+    counts = [33 + (7 * e) % 32 for e in range(experts)]
+    offsets = [sum(counts[:e]) for e in range(experts + 1)]
+    x = rows_of(offsets[-1], k, dt)
+    off = torch.tensor(offsets, dtype=torch.int32, device="cuda")
+    packed = bg.pack_w4(q, s, z)
+    y = bg.matmul_b200_w4(x, packed, off)
+    for e in range(experts):
+        a, b = offsets[e], offsets[e + 1]
+        close(y[a:b], x[a:b], w[e], u, dtype == "fp16")
+    for _ in range(3):
+        assert torch.equal(y, bg.matmul_b200_w4(x, packed, off))
