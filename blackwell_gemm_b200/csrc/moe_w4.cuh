@@ -228,8 +228,11 @@ struct W4RowsCfg {
   static constexpr int kPitch = 136;  // floats from token to token of the exchange
   static constexpr int kGroups = kTok <= 8 ? 4 : kTok <= 16 ? 3 : 2;
   static constexpr int kExchange = kGroups * kTok * kPitch * 4;
-  static constexpr int kStages = Ring::stages(kExchange);
-  static_assert(kGroups <= kStages, "one group to a stage at a time");
+  // Whole turns to a ring, so that a stage is always the same group's: a group
+  // tells the laps of a stage apart by one bit, which it can only while it
+  // sees every lap (copies may land out of order).
+  static constexpr int kStages = Ring::stages(kExchange) / kGroups * kGroups;
+  static_assert(kStages >= kGroups, "a stage for each group");
   static constexpr int kThreads = 32 * (4 * kGroups + 1);
   static constexpr int smem_bytes(int experts) {
     return kStages * Ring::kStageBytes + kExchange + group_table_bytes(experts) + 1024;

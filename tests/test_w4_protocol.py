@@ -178,3 +178,93 @@ def test_release_without_waiting_is_caught(stages):
             return True
         return False
     assert any(fails(seed) for seed in range(40))
+
+
+# ---------------------------------------- up to 32 rows (w4_rows_kernel)
+def rows_kernel(segments, groups, stages, rng):
+    """Groups of warps take stages in turn; a barrier of them all ends a segment."""
+    items = [min(2, length - kb) for length in segments for kb in range(0, length, 2)]
+    ends, at = [], 0
+    for length in segments:
+        at += (length + 1) // 2
+        ends.append(at)
+    ring = Ring(stages, WARPS, rng)
+    arrived = [0] * len(ends)
+
+    def take(group):
+        begin = 0
+        for segment, end in enumerate(ends):
+            for i in range(begin, end):
+                if i % groups != group:
+                    continue
+                yield from ring.wait(i)
+                for _ in range(items[i]):
+                    ring.read(i)
+                    yield
+                ring.release(i)
+                yield
+            arrived[segment] += 1
+            while arrived[segment] < groups * WARPS:
+                yield
+            begin = end
+
+    tasks = [ring.produce([WARPS * r for r in items])]
+    tasks += [take(g) for g in range(groups) for _ in range(WARPS)]
+    run(tasks, [ring.land()], rng)
+    assert all(u == 0 for u in ring.unread)
+
+
+def _fails(*args):
+    for seed in range(30):
+        try:
+            rows_kernel(*args, random.Random(seed))
+        except AssertionError:
+            return True
+    return False
+
+
+@pytest.mark.parametrize("groups,stages", [(4, 8), (3, 6), (2, 4)])
+def test_groups_of_warps_hold(groups, stages):
+    for segments in ([64], [1, 32, 32, 9], [3, 3, 3, 3, 3, 3, 3], [1] * 30):
+        for seed in range(10):
+            rows_kernel(segments, groups, stages, random.Random(seed))
+
+
+@pytest.mark.parametrize("groups,stages", [(3, 7), (2, 5)])
+def test_stages_that_change_groups_are_caught(groups, stages):
+    # a group that comes to a stage must have seen its last lap's copy land
+    assert _fails([64], groups, stages)
+
+
+def test_ring_depths_of_the_kernels(tmp_path):
+    """What is compiled has a whole number of turns to a ring."""
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from blackwell_gemm_b200 import build
+    if shutil.which("nvcc") is None and not Path("/usr/local/cuda/bin/nvcc").exists():
+        pytest.skip("no nvcc")
+    source = tmp_path / "rings.cu"
+    source.write_text("""
+#include <cstdio>
+#include "moe_w4.cuh"
+using namespace b200;
+template <int kTok, int kGroup> void show() {
+  using C = W4RowsCfg<kTok, kGroup>;
+  std::printf("%d %d %d %d\\n", kTok, kGroup, C::kGroups, C::kStages);
+}
+int main() {
+  show<8, 32>(), show<8, 64>(), show<8, 128>(), show<16, 32>(), show<16, 64>(), show<16, 128>();
+  show<32, 32>(), show<32, 64>();
+}
+""")
+    exe = tmp_path / "rings"
+    subprocess.run([build._nvcc(), "-std=c++17", *build.ARCH_FLAGS, "-I", str(build.INCLUDE), "-I",
+                    str(build.CSRC), "-o", str(exe), str(source)], check=True)
+    rows = [tuple(map(int, line.split())) for line in
+            subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout.split("\n")
+            if line]
+    assert len(rows) == 8
+    for tok, group, groups, stages in rows:
+        assert stages % groups == 0, (tok, group, groups, stages)
+        assert not _fails([64], groups, stages)
