@@ -17,6 +17,11 @@ struct DeviceView {
 // The current device, set up on its first call.  Returns a status code.
 int device_view(DeviceView* out);
 
+// What names a stream among all that the program ever has: a handle may come
+// back after its stream is destroyed, and cudaStreamPerThread is one handle
+// for another stream in each thread.  False where the stream has none.
+bool stream_id(cudaStream_t stream, unsigned long long* id);
+
 // A tiled tensor map of rank 2 or 3 over 1-, 2- or 4-byte elements, 128-byte
 // swizzle, zero fill out of bounds.  strides_bytes: rank - 1 strides of the
 // outer dimensions.  Returns a status code.

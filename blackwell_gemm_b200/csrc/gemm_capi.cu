@@ -562,7 +562,7 @@ int choose_splits(int M, int N, int k_blocks, int pairs) {
 // (cudaMalloc, cleared on the stream itself); null when none can be made.
 struct StreamSched {
   int device;
-  cudaStream_t stream;
+  unsigned long long stream;  // stream_id
   unsigned int* words;
 };
 constexpr int kMaxStreamScheds = 256;
@@ -571,13 +571,15 @@ int g_num_stream_sched = 0;
 
 unsigned int* stream_sched(cudaStream_t stream) {
   int dev = -1;
+  unsigned long long id = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
+  if (!stream_id(stream, &id)) return nullptr;
   std::lock_guard<std::mutex> lock(g_mu);
   for (int i = 0; i < g_num_stream_sched; ++i)
-    if (g_stream_sched[i].device == dev && g_stream_sched[i].stream == stream)
+    if (g_stream_sched[i].device == dev && g_stream_sched[i].stream == id)
       return g_stream_sched[i].words;
   if (g_num_stream_sched == kMaxStreamScheds) return nullptr;
   unsigned int* p = nullptr;
@@ -586,7 +588,7 @@ unsigned int* stream_sched(cudaStream_t stream) {
     if (p) cudaFree(p);
     return nullptr;
   }
-  g_stream_sched[g_num_stream_sched++] = {dev, stream, p};
+  g_stream_sched[g_num_stream_sched++] = {dev, id, p};
   return p;
 }
 
@@ -646,7 +648,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
 // its own).  Arrays live until exit.
 struct StreamFlags {
   int device;
-  cudaStream_t stream;
+  unsigned long long stream;  // stream_id
   unsigned int* flags;
   size_t count;
   unsigned int epoch;
@@ -657,14 +659,16 @@ int g_num_stream_flags = 0;
 
 unsigned int* stream_flags(cudaStream_t stream, size_t count, unsigned int* epoch) {
   int dev = -1;
+  unsigned long long id = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
     cudaGetLastError();
     return nullptr;
   }
+  if (!stream_id(stream, &id)) return nullptr;
   std::lock_guard<std::mutex> lock(g_mu);
   for (int i = 0; i < g_num_stream_flags; ++i) {
     StreamFlags& f = g_stream_flags[i];
-    if (f.device == dev && f.stream == stream && f.count >= count) {
+    if (f.device == dev && f.stream == id && f.count >= count) {
       if (++f.epoch == 0) return nullptr;  // 2^32 calls: fall back to cleared flags
       *epoch = f.epoch;
       return f.flags;
@@ -682,7 +686,7 @@ unsigned int* stream_flags(cudaStream_t stream, size_t count, unsigned int* epoc
     if (p) cudaFree(p);
     return nullptr;
   }
-  g_stream_flags[g_num_stream_flags++] = {dev, stream, p, n, 1u};
+  g_stream_flags[g_num_stream_flags++] = {dev, id, p, n, 1u};
   *epoch = 1u;
   return p;
 }
@@ -2214,6 +2218,12 @@ int device_view(DeviceView* out) {
   out->pool = d->pool;
   out->timeout_ns = g_timeout_ns.load();
   return B200_OK;
+}
+
+bool stream_id(cudaStream_t stream, unsigned long long* id) {
+  if (cudaStreamGetId(stream, id) == cudaSuccess) return true;
+  cudaGetLastError();
+  return false;
 }
 
 int encode_tensor(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base,

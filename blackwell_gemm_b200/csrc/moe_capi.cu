@@ -151,7 +151,7 @@ int moe_device(DeviceView* v, MoeDevice** out) {
 constexpr size_t kCountBytes = 4096 * sizeof(unsigned int);
 struct StreamCounts {
   int device;
-  cudaStream_t stream;
+  unsigned long long stream;  // stream_id
   unsigned int* counts;
 };
 constexpr int kMaxStreamCounts = 256;
@@ -159,9 +159,11 @@ StreamCounts g_counts[kMaxStreamCounts];
 int g_num_counts = 0;
 
 unsigned int* stream_counts(int device, cudaStream_t stream) {
+  unsigned long long id = 0;
+  if (!stream_id(stream, &id)) return nullptr;
   std::lock_guard<std::mutex> lock(g_mu);
   for (int i = 0; i < g_num_counts; ++i)
-    if (g_counts[i].device == device && g_counts[i].stream == stream) return g_counts[i].counts;
+    if (g_counts[i].device == device && g_counts[i].stream == id) return g_counts[i].counts;
   if (g_num_counts == kMaxStreamCounts) return nullptr;
   unsigned int* p = nullptr;
   if (cudaMalloc(&p, kCountBytes) != cudaSuccess ||
@@ -170,7 +172,7 @@ unsigned int* stream_counts(int device, cudaStream_t stream) {
     if (p) cudaFree(p);
     return nullptr;
   }
-  g_counts[g_num_counts++] = {device, stream, p};
+  g_counts[g_num_counts++] = {device, id, p};
   return p;
 }
 

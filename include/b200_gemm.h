@@ -13,7 +13,10 @@
  * stream, where the reference launches) and a status code instead of silent
  * garbage on unsupported input.
  *
- * All pointers are device pointers.  Calls are asynchronous on `stream`.
+ * All pointers are device pointers.  Calls are asynchronous on `stream`, which
+ * may be cudaStreamPerThread: what the library keeps per stream is told apart
+ * by cudaStreamGetId.  A thread synchronizes that stream before it ends (with
+ * work still on it, a later cudaDeviceSynchronize was seen not to return).
  * Plain C types only; no torch types cross this boundary.
  */
 #ifndef B200_GEMM_H_
