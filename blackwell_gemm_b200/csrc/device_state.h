@@ -14,6 +14,34 @@ struct DeviceView {
   unsigned long long timeout_ns = 0; // bound on any single pipeline wait
 };
 
+// While it lives, this thread's calls leave captures of other threads alone: in
+// CUDA's default capture mode any allocation, also one in the order of a
+// stream that nobody captures, is refused and ends every capture under way.
+struct RelaxedCapture {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  ~RelaxedCapture() { cudaThreadExchangeStreamCaptureMode(&mode); }
+  RelaxedCapture(const RelaxedCapture&) = delete;
+  RelaxedCapture& operator=(const RelaxedCapture&) = delete;
+};
+
+// Memory of a pool, taken and given back in the order of `stream`.
+template <class T>
+inline bool pool_take(T** p, size_t bytes, cudaMemPool_t pool, cudaStream_t stream) {
+  const RelaxedCapture relaxed;
+  void* got = nullptr;
+  if (pool == nullptr || cudaMallocFromPoolAsync(&got, bytes, pool, stream) != cudaSuccess) {
+    cudaGetLastError();
+    return false;
+  }
+  *p = static_cast<T*>(got);
+  return true;
+}
+inline bool pool_give(void* p, cudaStream_t stream) {
+  const RelaxedCapture relaxed;
+  return cudaFreeAsync(p, stream) == cudaSuccess;
+}
+
 // The current device, set up on its first call.  Returns a status code.
 int device_view(DeviceView* out);
 

@@ -378,6 +378,7 @@ int init_device(DeviceState& d, int dev) {
   const int vst = init_variants(d.sms, d.max_pairs);
   if (vst != B200_OK) return vst;
   if (!skc_init_all(d)) return B200_ERR_LAUNCH;
+  const RelaxedCapture relaxed;  // another thread may be capturing
   if (cudaMalloc(&d.status, sizeof(int)) != cudaSuccess ||
       cudaMemset(d.status, 0, sizeof(int)) != cudaSuccess)
     return B200_ERR_LAUNCH;
@@ -558,8 +559,8 @@ int choose_splits(int M, int N, int k_blocks, int pairs) {
 // Per-(device, stream) counters of the dynamic dealing (GemmArgs::sched):
 // two words, zero at every launch -- each launch's last pair sets them back
 // to zero -- so consecutive launches on one stream share them and launches
-// on different streams never do.  Created on a stream's first call
-// (cudaMalloc, cleared on the stream itself); null when none can be made.
+// on different streams never do.  Created on a stream's first call (from the
+// pool, cleared on the stream itself); null when none can be made.
 struct StreamSched {
   int device;
   unsigned long long stream;  // stream_id
@@ -569,7 +570,7 @@ constexpr int kMaxStreamScheds = 256;
 StreamSched g_stream_sched[kMaxStreamScheds];
 int g_num_stream_sched = 0;
 
-unsigned int* stream_sched(cudaStream_t stream) {
+unsigned int* stream_sched(cudaMemPool_t pool, cudaStream_t stream) {
   int dev = -1;
   unsigned long long id = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -583,9 +584,10 @@ unsigned int* stream_sched(cudaStream_t stream) {
       return g_stream_sched[i].words;
   if (g_num_stream_sched == kMaxStreamScheds) return nullptr;
   unsigned int* p = nullptr;
-  if (cudaMalloc(&p, 256) != cudaSuccess || cudaMemsetAsync(p, 0, 256, stream) != cudaSuccess) {
+  if (!pool_take(&p, 256, pool, stream)) return nullptr;
+  if (cudaMemsetAsync(p, 0, 256, stream) != cudaSuccess) {
     cudaGetLastError();
-    if (p) cudaFree(p);
+    pool_give(p, stream);
     return nullptr;
   }
   g_stream_sched[g_num_stream_sched++] = {dev, id, p};
@@ -620,10 +622,9 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
       cap = cudaStreamCaptureStatusActive;
     }
     if (cap == cudaStreamCaptureStatusNone) {
-      args.sched = stream_sched(stream);
+      args.sched = stream_sched(d.pool, stream);
     } else if (d.pool != nullptr) {
-      if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&sched_ws), 256, d.pool, stream) ==
-              cudaSuccess &&
+      if (pool_take(&sched_ws, 256, d.pool, stream) &&
           cudaMemsetAsync(sched_ws, 0, 256, stream) == cudaSuccess) {
         args.sched = reinterpret_cast<unsigned int*>(sched_ws);
       } else {
@@ -635,7 +636,7 @@ int launch(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorMap& tc, 
   pair_kernel<kProfile, V, kOut, kSK><<<2 * pairs, C::kThreads, C::kSmemBytes, stream>>>(
       ta, tb, tc, args);
   const int st = cudaGetLastError() == cudaSuccess ? B200_OK : B200_ERR_LAUNCH;
-  if (sched_ws != nullptr) cudaFreeAsync(sched_ws, stream);
+  if (sched_ws != nullptr) pool_give(sched_ws, stream);
   return st;
 }
 
@@ -657,7 +658,8 @@ constexpr int kMaxStreamFlags = 256;
 StreamFlags g_stream_flags[kMaxStreamFlags];
 int g_num_stream_flags = 0;
 
-unsigned int* stream_flags(cudaStream_t stream, size_t count, unsigned int* epoch) {
+unsigned int* stream_flags(cudaMemPool_t pool, cudaStream_t stream, size_t count,
+                           unsigned int* epoch) {
   int dev = -1;
   unsigned long long id = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) {
@@ -677,13 +679,13 @@ unsigned int* stream_flags(cudaStream_t stream, size_t count, unsigned int* epoc
   if (g_num_stream_flags == kMaxStreamFlags) return nullptr;
   const size_t n = count < 4096 ? 4096 : count;
   unsigned int* p = nullptr;
-  // Once per (device, stream): cudaMalloc, then a clear queued on the stream
-  // itself -- every kernel that reads the array runs on that stream, after
-  // the clear, so nothing waits on the host or on other streams.
-  if (cudaMalloc(&p, n * sizeof(unsigned int)) != cudaSuccess ||
-      cudaMemsetAsync(p, 0, n * sizeof(unsigned int), stream) != cudaSuccess) {
+  // Once per (device, stream): allocated from the pool and cleared in the
+  // order of the stream itself -- every kernel that reads the array runs on
+  // that stream, so nothing waits on the host or on other streams.
+  if (!pool_take(&p, n * sizeof(unsigned int), pool, stream)) return nullptr;
+  if (cudaMemsetAsync(p, 0, n * sizeof(unsigned int), stream) != cudaSuccess) {
     cudaGetLastError();
-    if (p) cudaFree(p);
+    pool_give(p, stream);
     return nullptr;
   }
   g_stream_flags[g_num_stream_flags++] = {dev, id, p, n, 1u};
@@ -717,11 +719,7 @@ int launch_streamk(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
   const size_t flag_bytes = (size_t)ceil_div(slots * 4, 256) * 256;
   const size_t slot_bytes = (size_t)slots * kPieceFloats * sizeof(float);
   char* ws = nullptr;
-  if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), flag_bytes + slot_bytes, d.pool,
-                              stream) != cudaSuccess) {
-    cudaGetLastError();
-    return B200_ERR_LAUNCH;
-  }
+  if (!pool_take(&ws, flag_bytes + slot_bytes, d.pool, stream)) return B200_ERR_LAUNCH;
   args.sk_slots = reinterpret_cast<float*>(ws + flag_bytes);
   // Flags: outside stream capture, a per-(device, stream) array that keeps
   // its values between calls, each call raising flags to a new epoch (stale
@@ -738,7 +736,7 @@ int launch_streamk(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
   }
   unsigned int* persistent = nullptr;
   if (cap == cudaStreamCaptureStatusNone)
-    persistent = stream_flags(stream, (size_t)slots, &args.sk_epoch);
+    persistent = stream_flags(d.pool, stream, (size_t)slots, &args.sk_epoch);
   if (persistent != nullptr) {
     args.sk_flags = persistent;
   } else {
@@ -747,7 +745,7 @@ int launch_streamk(const CUtensorMap& ta, const CUtensorMap& tb, const CUtensorM
     if (cudaMemsetAsync(ws, 0, flag_bytes, stream) != cudaSuccess) st = B200_ERR_LAUNCH;
   }
   if (st == B200_OK) st = launch<false, V, kOutBf16, true>(ta, tb, tc, args, 1, d, stream);
-  cudaFreeAsync(ws, stream);
+  pool_give(ws, stream);
   *used = true;
   return st;
 }
@@ -930,9 +928,7 @@ int launch_skinny(const void* A, const void* B, void* C, int M, int N, int K, in
   if (scratch != nullptr) {
     if (bytes > scratch->work_bytes) return B200_ERR_TOO_LARGE;
     W = reinterpret_cast<float*>(scratch->work);
-  } else if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&W), bytes, d.pool, stream) !=
-             cudaSuccess) {
-    cudaGetLastError();
+  } else if (!pool_take(&W, bytes, d.pool, stream)) {
     return B200_ERR_LAUNCH;
   }
   int st = encode_2d(&tw, W, N, M, ldw, 32, P::kChunk, true, false);
@@ -945,7 +941,7 @@ int launch_skinny(const void* A, const void* B, void* C, int M, int N, int K, in
     if (cudaGetLastError() != cudaSuccess) st = B200_ERR_LAUNCH;
   }
   if (st == B200_OK) st = cast_to_bf16(W, ldw, C, ldc, M, N, d.sms, stream, epi);
-  if (scratch == nullptr) cudaFreeAsync(W, stream);
+  if (scratch == nullptr) pool_give(W, stream);
   return st;
 }
 
@@ -1008,11 +1004,7 @@ int launch_skinny_stream(const void* A, const void* B, void* C, int M, int N, in
         st = B200_ERR_LAUNCH;
     }
   } else {
-    if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), flag_bytes + slot_bytes, d.pool,
-                                stream) != cudaSuccess) {
-      cudaGetLastError();
-      return B200_ERR_LAUNCH;
-    }
+    if (!pool_take(&ws, flag_bytes + slot_bytes, d.pool, stream)) return B200_ERR_LAUNCH;
     args.slots = reinterpret_cast<float*>(ws + flag_bytes);
     // Flags: the stream's epoch-numbered array outside capture (no clearing
     // operation before the kernel), cleared workspace flags under capture.
@@ -1023,7 +1015,7 @@ int launch_skinny_stream(const void* A, const void* B, void* C, int M, int N, in
     }
     unsigned int* persistent = nullptr;
     if (cap == cudaStreamCaptureStatusNone)
-      persistent = stream_flags(stream, nflags, &args.epoch);
+      persistent = stream_flags(d.pool, stream, nflags, &args.epoch);
     if (persistent != nullptr) {
       args.flags = persistent;
     } else {
@@ -1055,7 +1047,7 @@ int launch_skinny_stream(const void* A, const void* B, void* C, int M, int N, in
       st = B200_ERR_LAUNCH;
     }
   }
-  if (ws != nullptr) cudaFreeAsync(ws, stream);
+  if (ws != nullptr) pool_give(ws, stream);
   return st;
 }
 
@@ -1351,18 +1343,14 @@ int run_gemm(const void* A, const void* B, void* C, int M, int N, int K, int lda
       const int ldw = (int)ceil_div(N, 8) * 8;
       const size_t bytes = (size_t)M * ldw * sizeof(float);
       float* W = nullptr;
-      if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&W), bytes, d->pool, stream) !=
-          cudaSuccess) {
-        cudaGetLastError();
-        return B200_ERR_LAUNCH;
-      }
+      if (!pool_take(&W, bytes, d->pool, stream)) return B200_ERR_LAUNCH;
       st = encode_2d(&tc, W, N, M, ldw, 32, 32, true);
       if (st == B200_OK && cudaMemsetAsync(W, 0, bytes, stream) != cudaSuccess)
         st = B200_ERR_LAUNCH;
       if (st == B200_OK) st = launch<false, kV256x64, kOutF32Add>(ta, tb, tc, args, splits, *d,
                                                                    stream);
       if (st == B200_OK) st = cast_to_bf16(W, ldw, C, ldc, M, N, d->sms, stream, epi);
-      cudaFreeAsync(W, stream);
+      pool_give(W, stream);
       return st;
     }
   }
@@ -1492,8 +1480,7 @@ int run_gemm_host(const void* A, const void* B, void* C, int M, int N, int K, in
             cudaStreamWaitEvent(p->mm, ev_start, 0) == cudaSuccess &&
             cudaStreamWaitEvent(p->down, ev_start, 0) == cudaSuccess;
   char* ws = nullptr;
-  if (ok) ok = cudaMallocFromPoolAsync(reinterpret_cast<void**>(&ws), total, d->pool, p->up) ==
-               cudaSuccess;
+  if (ok) ok = pool_take(&ws, total, d->pool, p->up);
   if (!ok) return finish(B200_ERR_LAUNCH);
   char* dA = ws;
   char* dB = ws + a_bytes;
@@ -1555,7 +1542,7 @@ int run_gemm_host(const void* A, const void* B, void* C, int M, int N, int K, in
     cudaStreamSynchronize(p->up);
     cudaStreamSynchronize(p->mm);
   }
-  cudaFreeAsync(ws, p->down);
+  pool_give(ws, p->down);
   const bool released = cudaEventRecord(ev_end, p->down) == cudaSuccess &&
                         cudaStreamWaitEvent(stream, ev_end, 0) == cudaSuccess;
   if (!released) {

@@ -158,21 +158,21 @@ constexpr int kMaxStreamCounts = 256;
 StreamCounts g_counts[kMaxStreamCounts];
 int g_num_counts = 0;
 
-unsigned int* stream_counts(int device, cudaStream_t stream) {
+unsigned int* stream_counts(const DeviceView& v, cudaStream_t stream) {
   unsigned long long id = 0;
   if (!stream_id(stream, &id)) return nullptr;
   std::lock_guard<std::mutex> lock(g_mu);
   for (int i = 0; i < g_num_counts; ++i)
-    if (g_counts[i].device == device && g_counts[i].stream == id) return g_counts[i].counts;
+    if (g_counts[i].device == v.device && g_counts[i].stream == id) return g_counts[i].counts;
   if (g_num_counts == kMaxStreamCounts) return nullptr;
   unsigned int* p = nullptr;
-  if (cudaMalloc(&p, kCountBytes) != cudaSuccess ||
-      cudaMemsetAsync(p, 0, kCountBytes, stream) != cudaSuccess) {
+  if (!pool_take(&p, kCountBytes, v.pool, stream)) return nullptr;
+  if (cudaMemsetAsync(p, 0, kCountBytes, stream) != cudaSuccess) {
     cudaGetLastError();
-    if (p) cudaFree(p);
+    pool_give(p, stream);
     return nullptr;
   }
-  g_counts[g_num_counts++] = {device, id, p};
+  g_counts[g_num_counts++] = {v.device, id, p};
   return p;
 }
 
@@ -189,13 +189,8 @@ struct Workspace {
       cudaGetLastError();
       cap = cudaStreamCaptureStatusActive;
     }
-    args->counts = cap == cudaStreamCaptureStatusNone ? stream_counts(v.device, s) : nullptr;
-    if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&base), kCountBytes + slot_bytes, v.pool,
-                                s) != cudaSuccess) {
-      cudaGetLastError();
-      base = nullptr;
-      return B200_ERR_LAUNCH;
-    }
+    args->counts = cap == cudaStreamCaptureStatusNone ? stream_counts(v, s) : nullptr;
+    if (!pool_take(&base, kCountBytes + slot_bytes, v.pool, s)) return B200_ERR_LAUNCH;
     args->slots = reinterpret_cast<float*>(base + kCountBytes);
     if (args->counts == nullptr) {
       args->counts = reinterpret_cast<unsigned int*>(base);
@@ -207,23 +202,20 @@ struct Workspace {
     return B200_OK;
   }
   ~Workspace() {
-    if (base) cudaFreeAsync(base, stream);
+    if (base) pool_give(base, stream);
   }
 };
 
 // A buffer of the device's pool for one call, freed in stream order.
 struct PoolBuffer {
-  void* p = nullptr;
+  char* p = nullptr;
   cudaStream_t stream = nullptr;
   int take(const DeviceView& v, size_t bytes, cudaStream_t s) {
     stream = s;
-    if (cudaMallocFromPoolAsync(&p, bytes, v.pool, s) == cudaSuccess) return B200_OK;
-    cudaGetLastError();
-    p = nullptr;
-    return B200_ERR_LAUNCH;
+    return pool_take(&p, bytes, v.pool, s) ? B200_OK : B200_ERR_LAUNCH;
   }
   ~PoolBuffer() {
-    if (p) cudaFreeAsync(p, stream);
+    if (p) pool_give(p, stream);
   }
 };
 
@@ -348,7 +340,7 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
     st = maps.take(v, (size_t)c.experts * 2 * sizeof(CUtensorMap), stream);
     if (st == B200_OK)
       st = launch(grouped_maps_kernel, c.experts, 32, 0, stream, tw, tt, c.offsets, c.rows,
-                  static_cast<CUtensorMap*>(maps.p));
+                  reinterpret_cast<CUtensorMap*>(maps.p));
     if (st != B200_OK) return st;
   }
   GroupedArgs a = {};
@@ -362,7 +354,7 @@ int launch_pair(const Call& c, const DeviceView& v, const MoeDevice& m, cudaStre
   a.ldo = kMode == kGroupedDB ? c.ldb : c.ldu;
   a.expert_stride = c.expert_stride;
   a.group = 8;
-  a.maps = static_cast<const CUtensorMap*>(maps.p);
+  a.maps = reinterpret_cast<const CUtensorMap*>(maps.p);
   a.status = v.status;
   a.timeout_ns = v.timeout_ns;
   const long long tf = ceil_div(a.feat, 256);
@@ -648,12 +640,8 @@ int run_route(RouteArgs a, const DeviceView& v, cudaStream_t stream) {
   const size_t smem = (size_t)(1 + kRouteWarps) * a.experts * sizeof(int);
   int* counts = nullptr;
   if (blocks > 1) {
-    if (cudaMallocFromPoolAsync(reinterpret_cast<void**>(&counts),
-                                (size_t)blocks * a.experts * sizeof(int), v.pool,
-                                stream) != cudaSuccess) {
-      cudaGetLastError();
+    if (!pool_take(&counts, (size_t)blocks * a.experts * sizeof(int), v.pool, stream))
       return B200_ERR_LAUNCH;
-    }
     a.counts = counts;
   }
   int st = a.experts <= 32    ? launch_choose<1>(a, blocks, smem, stream)
@@ -664,7 +652,7 @@ int run_route(RouteArgs a, const DeviceView& v, cudaStream_t stream) {
   if (st == B200_OK && blocks > 1) {
     st = launch(route_rank_kernel, blocks, kRouteThreads, smem, stream, a);
   }
-  if (counts) cudaFreeAsync(counts, stream);
+  if (counts) pool_give(counts, stream);
   return st;
 }
 

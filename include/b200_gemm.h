@@ -123,9 +123,9 @@ int b200_gemm_set_skinny_tiles(int tiles);
  * the pair-slots and K >= 4096 (default; B200_GEMM_STREAMK overrides), 2 =
  * whenever the last wave is partial, at any K.  The first stream-K call (pair tail or skinny
  * stream-K kernel) on each (device, stream) allocates that stream's flag
- * array with cudaMalloc, which may synchronise the device; it is cleared on
- * the stream itself.  No reference counterpart (the reference deals whole
- * tiles with cluster launch control). */
+ * array from the pool and clears it, both in the order of that stream.  No
+ * reference counterpart (the reference deals whole tiles with cluster launch
+ * control). */
 int b200_gemm_set_stream_k(int mode);
 
 /* Dealing of whole tiles to the persistent pairs: 0 = static (default;
@@ -135,7 +135,7 @@ int b200_gemm_set_stream_k(int mode);
  * compact window of the raster and no pair idles while another has tiles
  * queued (measured no faster on the configuration shapes, slower on some:
  * the static deal stays the default).  The counters are two words per (device,
- * stream), made on the stream's first call (cudaMalloc) and left at zero by
+ * stream), made on the stream's first call (from the pool) and left at zero by
  * every launch.  No reference counterpart (the reference steals work with
  * cluster launch control, src/kernels/kernel_v8.cu:608-653). */
 int b200_gemm_set_dynamic(int mode);

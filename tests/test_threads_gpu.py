@@ -120,3 +120,53 @@ def test_streams_made_and_destroyed():
         assert runtime.cudaStreamDestroy(stream) == 0
     torch.cuda.synchronize()
     assert all(torch.equal(out[r], want) for r in range(300))
+
+
+@pytest.mark.parametrize("what", ["grouped", "w4", "stream-K", "dealing"])
+def test_calls_while_another_thread_captures(what):
+    # nothing that a call allocates may end a capture (global mode) elsewhere
+    rows, n, k = 4, 640, 4096
+    x, w = whole(rows, k), whole(2, n, k, seed=1)
+    off = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    weight = bg.pack_w4(*bg.quantize_w4(w[0]))
+    a, b = whole(2048, 512), whole(6400, 512, seed=1)
+    x16, wide = whole(16, k), whole(1280, k, seed=1)
+    side = torch.cuda.Stream()
+    stream = side.cuda_stream
+    out = {"grouped": (rows, n), "w4": (rows, n), "stream-K": (16, 1280), "dealing": (2048, 6400)}[what]
+    out = torch.zeros(*out, dtype=torch.bfloat16, device="cuda")
+    lib = capi.lib()
+    capi.set_dynamic(1 if what == "dealing" else 0)
+    call = {
+        "grouped": lambda: lib.b200_grouped_gemm(x.data_ptr(), w.data_ptr(), out.data_ptr(),
+                                                 off.data_ptr(), rows, 2, n, k, k, k, n * k, n,
+                                                 capi.BF16, stream),
+        "w4": lambda: lib.b200_w4_gemm(x.data_ptr(), weight.data.data_ptr(), out.data_ptr(), None,
+                                       rows, 1, n, k, 128, 0, k, n, capi.BF16, stream),
+        "stream-K": lambda: capi.gemm_bf16(x16.data_ptr(), wide.data_ptr(), out.data_ptr(), 16, 1280,
+                                           k, k, k, 1280, stream),
+        "dealing": lambda: capi.gemm_bf16(a.data_ptr(), b.data_ptr(), out.data_ptr(), 2048, 6400, 512,
+                                          512, 512, 6400, stream),
+    }[what]
+    want = {"grouped": lambda: bg.matmul_b200_grouped(x, w.transpose(1, 2), off),
+            "w4": lambda: bg.matmul_b200_w4(x, weight),
+            "stream-K": lambda: (x16.double() @ wide.double().T).bfloat16(),
+            "dealing": lambda: (a.double() @ b.double().T).bfloat16()}[what]()
+    if what == "stream-K":
+        capi.set_skinny_mode(3)
+    got = []
+    team = threading.Thread(target=lambda: got.extend([call(), call()]))
+    static = torch.ones(8, device="cuda")
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    try:
+        with torch.cuda.graph(graph, capture_error_mode="global"):
+            doubled = static * 2
+            team.start()
+            team.join()
+    finally:
+        capi.set_skinny_mode(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert got == [capi.OK, capi.OK] and bool((doubled == 2).all())
+    assert torch.equal(out, want)
