@@ -436,6 +436,16 @@ at::Tensor w4_matmul(const at::Tensor& A, const at::Tensor& packed, int64_t expe
   TORCH_CHECK(A.device() == packed.device(), kW4, ": A and the weight are on different devices");
   TORCH_CHECK(A.size(1) == K, kW4, ": inner dimensions differ (A has K = ", A.size(1),
               ", the weight has K = ", K, ")");
+  TORCH_CHECK(experts >= 0 && N >= 0 && K >= 0 && group >= 0, kW4,
+              ": the weight's sizes must not be negative");
+  TORCH_CHECK(experts <= B200_MAX_EXPERTS, kW4, ": more than ", B200_MAX_EXPERTS, " experts");
+  check_sizes({N, K, group}, kW4);
+  size_t bytes = 0;
+  check_status(b200_w4_packed_bytes((int)experts, (int)N, (int)K, (int)group, zeros, &bytes), kW4);
+  TORCH_CHECK(packed.scalar_type() == at::kByte && packed.is_contiguous() &&
+                  packed.numel() == (int64_t)bytes,
+              kW4, ": the weight's data must be pack_w4's, ", bytes,
+              " contiguous bytes (uint8) for its sizes");
   TORCH_CHECK(!(at::GradMode::is_enabled() && A.requires_grad()), kW4,
               ": no gradient is defined (4-bit weights serve); use torch.no_grad()");
   check_sizes({A.size(0)}, kW4);

@@ -38,3 +38,30 @@ def test_short_contractions_through_many_tiles(dtype, k, group):
         close(y[a:b], x[a:b], w[e], u, dtype == "fp16")
     for _ in range(3):
         assert torch.equal(y, bg.matmul_b200_w4(x, packed, off))
+
+
+def test_weights_that_do_not_hold_what_they_say():
+    q, s, z, _ = weights(2, 264, 512, 64, True, torch.bfloat16)
+    good = bg.pack_w4(q, s, z)
+    off = torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda")
+    x = rows_of(4, 512, torch.bfloat16)
+    bg.matmul_b200_w4(x, good, off)
+    for change, match in [
+            (dict(N=512), "contiguous bytes"), (dict(K=1024), "inner dimensions"),
+            (dict(zeros=False), "contiguous bytes"), (dict(experts=1, bank=False), "contiguous"),
+            (dict(group=32), "contiguous bytes"), (dict(group=48), "status 1"),
+            (dict(group=0), "status 1"), (dict(N=264 + 2 ** 32), "2\\^31"),
+            (dict(N=-1), "negative"), (dict(experts=3), "contiguous bytes"),
+            (dict(experts=2 ** 32 + 2), "1024 experts"),
+            (dict(data=good.data[:-1]), "contiguous bytes"),
+            (dict(data=good.data.view(torch.int16)), "contiguous bytes"),
+            (dict(data=good.data.repeat_interleave(2)[::2]), "contiguous bytes")]:
+        bad = good._replace(**change)
+        experts = min(bad.experts, 3)
+        ends = None if bad.experts == 1 else torch.arange(experts + 1, dtype=torch.int32,
+                                                          device="cuda")
+        with pytest.raises(RuntimeError, match=match):
+            bg.matmul_b200_w4(x, bad, ends)
+    # a copy of it, as a checkpoint gives back, is as good
+    again = bg.W4Weight(*[t.clone() if isinstance(t, torch.Tensor) else t for t in good])
+    assert torch.equal(bg.matmul_b200_w4(x, again, off), bg.matmul_b200_w4(x, good, off))
