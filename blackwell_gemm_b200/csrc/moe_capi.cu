@@ -669,7 +669,7 @@ int launch_move(Move what, const MoveArgs& a, cudaStream_t stream) {
   }
 }
 
-int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
+int run_move(Move what, MoveArgs a, const int* total, int dtype, cudaStream_t stream) {
   if (a.tokens < 0 || a.top_k < 0 || a.width < 0 || a.top_k > kMaxTopK ||
       (dtype != B200_BF16 && dtype != B200_FP16))
     return B200_ERR_INVALID_ARGUMENT;
@@ -679,7 +679,7 @@ int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
   if (a.width == 0 && what != kCombineGrad) return B200_OK;
   const bool any = a.top_k > 0, wide = a.width > 0;
   if ((any && !a.rows) || (wide && (!a.out || (any && !a.in))) ||
-      (what != kCombine && !a.total) ||
+      (what != kCombine && !total) ||
       (what == kCombineGrad && ((wide && !a.in2) || !a.weights)))
     return B200_ERR_INVALID_ARGUMENT;
   if (wide && (a.ld_in < a.width || a.ld_out < a.width ||
@@ -687,7 +687,7 @@ int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
     return B200_ERR_INVALID_ARGUMENT;
   if (((reinterpret_cast<uintptr_t>(a.in) | reinterpret_cast<uintptr_t>(a.in2) |
         reinterpret_cast<uintptr_t>(a.out)) & 1u) ||
-      ((reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(a.total) |
+      ((reinterpret_cast<uintptr_t>(a.rows) | reinterpret_cast<uintptr_t>(total) |
         reinterpret_cast<uintptr_t>(a.weights) | reinterpret_cast<uintptr_t>(a.dweights)) & 3u))
     return B200_ERR_ALIGNMENT;
   DeviceView v;
@@ -696,6 +696,17 @@ int run_move(Move what, const MoveArgs& a, int dtype, cudaStream_t stream) {
   if (st != B200_OK) return st;
   const bool vec = aligned16(a.in) && aligned16(a.out) && aligned16(a.in2) &&
                    ((a.width | a.ld_in | a.ld_out | a.ld_in2) & 7) == 0;
+  const int pairs = a.tokens * a.top_k;
+  PoolBuffer named;
+  if (what != kCombine && pairs > kScanPairs) {
+    int got = named.take(v, (size_t)pairs * sizeof(int), stream);
+    const int blocks = (int)ceil_div(pairs, 256);
+    if (got == B200_OK)
+      got = launch(mark_rows_kernel, blocks < 8 * v.sms ? blocks : 8 * v.sms, 256, 0, stream, a.rows,
+                   reinterpret_cast<int*>(named.p), pairs);
+    if (got != B200_OK) return got;
+    a.named = reinterpret_cast<const int*>(named.p);
+  }
   if (dtype == B200_FP16)
     return vec ? launch_move<__half, 8>(what, a, stream) : launch_move<__half, 1>(what, a, stream);
   return vec ? launch_move<__nv_bfloat16, 8>(what, a, stream)
@@ -857,11 +868,10 @@ int b200_dispatch(const void* x, const int* rows, const int* total, void* xs, in
   a.out = xs;
   a.ld_out = ldxs;
   a.rows = rows;
-  a.total = total;
   a.tokens = tokens;
   a.top_k = top_k;
   a.width = width;
-  return run_move(kDispatch, a, dtype, static_cast<cudaStream_t>(stream));
+  return run_move(kDispatch, a, total, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int b200_combine(const void* y, const float* weights, const int* rows, void* out, int tokens,
@@ -876,7 +886,7 @@ int b200_combine(const void* y, const float* weights, const int* rows, void* out
   a.tokens = tokens;
   a.top_k = top_k;
   a.width = width;
-  return run_move(kCombine, a, dtype, static_cast<cudaStream_t>(stream));
+  return run_move(kCombine, a, nullptr, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int b200_combine_grad(const void* dout, const void* y, const float* weights, const int* rows,
@@ -892,11 +902,10 @@ int b200_combine_grad(const void* dout, const void* y, const float* weights, con
   a.weights = weights;
   a.dweights = dweights;
   a.rows = rows;
-  a.total = total;
   a.tokens = tokens;
   a.top_k = top_k;
   a.width = width;
-  return run_move(kCombineGrad, a, dtype, static_cast<cudaStream_t>(stream));
+  return run_move(kCombineGrad, a, total, dtype, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

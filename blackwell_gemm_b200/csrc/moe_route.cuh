@@ -16,8 +16,9 @@
 // token, every row read once and written once, sums in fp32.
 // 8192 tokens, 64 experts, two each, width 4096: choose 6.6 us and rank 11.7
 // (a chain of counts, barriers and ranks over 1024 threads; 3 MB), dispatch
-// 33 (202 MB, 6.1 TB/s), combine 37 (202 MB, 5.4 TB/s), its gradient 55
-// (336 MB, 6.1 TB/s), the logits' gradient 6.4.
+// 36 (202 MB, 5.6 TB/s, 2 us of it the search for rows without a slot), combine
+// 37 (202 MB, 5.4 TB/s), its gradient 59 (336 MB, 5.7 TB/s, the same), the
+// logits' gradient 6.4.
 #pragma once
 #include "moe_groups.cuh"
 
@@ -372,7 +373,7 @@ struct MoveArgs {
   const float* weights;   // tokens x top_k, or null: 1
   float* dweights;        // combine's gradient
   const int* rows;        // tokens x top_k
-  const int* total;       // rows that have an expert
+  const int* named;       // per sorted row a slot that may name it, or null
   int tokens, top_k, width;
 };
 
@@ -401,10 +402,9 @@ __device__ __forceinline__ void store_pack(void* base, long long i, const Pack<T
 __device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
 __device__ __forceinline__ float widen(__half v) { return __half2float(v); }
 
-// A token's rows and weights into shared memory, and the number of owned rows
-// behind the rows; a row that is no row of the operand is treated as none.
+// A token's rows and weights into shared memory; a row that is no row of the
+// operand is treated as none.
 __device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* s_row, float* s_w) {
-  if (threadIdx.x == kMaxTopK - 1 && a.total != nullptr) s_row[kMaxTopK] = *a.total;
   if ((int)threadIdx.x < a.top_k) {
     const long long at = t * a.top_k + threadIdx.x;
     const int r = a.rows[at];
@@ -414,18 +414,53 @@ __device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* 
   __syncthreads();
 }
 
-// Rows t * top_k .. of the sorted operand that no expert owns are zeroed by
-// token t's block.
+// Sorted rows that no slot names -- past the owned ones or, where slots were
+// taken out of a routing, among them -- are zero.  named[r] is a slot that
+// names row r, if there is any: memory that nobody cleared, so an entry counts
+// only where that slot's row is r.
+__global__ void __launch_bounds__(256)
+mark_rows_kernel(const int* __restrict__ rows, int* __restrict__ named, int pairs) {
+  grid_wait();
+  grid_launch_next();
+  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pairs; i += gridDim.x * 256ll) {
+    const int r = rows[i];
+    if (r >= 0 && r < pairs) named[r] = (int)i;
+  }
+}
+
+// Token t's block zeroes those of rows t * top_k .. that no slot names.  Up to
+// kScanPairs slots it looks through all of them itself; beyond, mark_rows_kernel
+// has been there (a launch more, but no work that grows with the square).
+// Dispatch, us, looking through / marked: 32 slots 2.5 / 5.1, 2048 4.8 / 5.2,
+// 4096 7.8 / 6.5, 65532 691 / 57; with rows left as they are 2.3, 3.2, 4.6, 54.
+constexpr int kScanPairs = 2048;
 template <class T, int kVec>
-__device__ __forceinline__ void zero_tail(const MoveArgs& a, long long t, int total) {
+__device__ __forceinline__ void zero_unnamed(const MoveArgs& a, long long t) {
+  __shared__ uint32_t s_named[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pairs = a.tokens * a.top_k, first = (int)t * a.top_k;
+  uint32_t bits = 0;
+  if (a.named == nullptr) {
+    for (int i = threadIdx.x; i < pairs; i += blockDim.x) {
+      const uint32_t r = (uint32_t)(a.rows[i] - first);
+      if (r < (uint32_t)a.top_k) bits |= 1u << r;
+    }
+    bits = __reduce_or_sync(0xffffffffu, bits);
+  } else if (warp == 0) {
+    const int at = lane < a.top_k ? a.named[first + lane] : -1;
+    bits = __ballot_sync(0xffffffffu, (uint32_t)at < (uint32_t)pairs && a.rows[at] == first + lane);
+  }
+  if (lane == 0) s_named[warp] = bits;
+  __syncthreads();
+  bits = 0;
+  for (int w = 0; w < (int)(blockDim.x >> 5); ++w) bits |= s_named[w];
   for (int j = 0; j < a.top_k; ++j) {
-    const long long r = t * a.top_k + j;
-    if (r < total) continue;
+    if (bits >> j & 1u) continue;
     Pack<T, kVec> z;
 #pragma unroll
     for (int i = 0; i < kVec; ++i) z.v[i] = round_one<T>(0.0f);
     for (int c = threadIdx.x * kVec; c < a.width; c += blockDim.x * kVec)
-      store_pack<T, kVec>(a.out, r * a.ld_out + c, z);
+      store_pack<T, kVec>(a.out, (long long)(first + j) * a.ld_out + c, z);
   }
 }
 
@@ -433,7 +468,7 @@ template <class T, int kVec>
 __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK + 1];
+  __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
   load_slots(a, t, s_row, s_w);
@@ -442,14 +477,14 @@ __global__ void __launch_bounds__(256) dispatch_kernel(const MoveArgs a) {
     for (int j = 0; j < a.top_k; ++j)
       if (s_row[j] >= 0) store_pack<T, kVec>(a.out, (long long)s_row[j] * a.ld_out + c, p);
   }
-  zero_tail<T, kVec>(a, t, s_row[kMaxTopK]);
+  zero_unnamed<T, kVec>(a, t);
 }
 
 template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK + 1];
+  __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   const long long t = blockIdx.x;
   load_slots(a, t, s_row, s_w);
@@ -480,7 +515,7 @@ template <class T, int kVec>
 __global__ void __launch_bounds__(256) combine_grad_kernel(const MoveArgs a) {
   grid_wait();
   grid_launch_next();
-  __shared__ int s_row[kMaxTopK + 1];
+  __shared__ int s_row[kMaxTopK];
   __shared__ float s_w[kMaxTopK];
   __shared__ float s_part[8][kMaxTopK];
   const long long t = blockIdx.x;
@@ -507,10 +542,9 @@ __global__ void __launch_bounds__(256) combine_grad_kernel(const MoveArgs a) {
     dot = warp_sum(dot);
     if ((threadIdx.x & 31) == 0) s_part[threadIdx.x >> 5][j] = dot;
   }
-  zero_tail<T, kVec>(a, t, s_row[kMaxTopK]);
-  if (a.dweights == nullptr) return;
-  __syncthreads();
-  if ((int)threadIdx.x < a.top_k) {
+  zero_unnamed<T, kVec>(a, t);
+  // (zero_unnamed's barrier lies between the parts and their sum)
+  if (a.dweights != nullptr && (int)threadIdx.x < a.top_k) {
     float all = 0.0f;
     for (int w = 0; w < (int)(blockDim.x >> 5); ++w) all += s_part[w][threadIdx.x];
     a.dweights[t * a.top_k + threadIdx.x] = all;

@@ -48,7 +48,8 @@ def route_b200(logits, top_k: int, *, normalize: bool = True) -> Routing:
 
 def dispatch_b200(x, routing: Routing):
     """xs[row] = x[token of row]: (tokens, width) bf16 or fp16 to (tokens *
-    top_k, width), sorted by expert; rows of no expert are zero.
+    top_k, width), sorted by expert; rows that no slot names are zero.  Slots may
+    be taken out of a routing: ``routing._replace(rows=...)`` with -1 there.
     Differentiable: a token's gradient is its rows' sum, in fp32, rounded once."""
     return _ext().dispatch_b200(x, routing.rows, routing.offsets)
 

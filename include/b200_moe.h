@@ -89,10 +89,13 @@ int b200_route_grad(const void* logits, int tokens, int experts, long long ld, i
                     int normalize, const int* chosen, const float* weights, const float* dweights,
                     void* dlogits, void* stream);
 
-/* xs[rows[t][j], :] = x[t, :]; rows of xs from *total on (the last entry of
- * offsets) are zero.  xs: tokens * top_k rows.  16-bit elements; strides in
- * elements; 16-byte aligned rows of a multiple of 8 elements move fastest,
- * any others work. */
+/* xs[rows[t][j], :] = x[t, :]; rows of xs that no slot names are zero (of a
+ * routing as b200_route makes it those from the last entry of offsets on; of one
+ * that slots were taken out of, theirs too).  A row outside 0 .. tokens * top_k
+ * - 1 is an empty slot; no two slots name the same row.  total: the last entry
+ * of offsets, not null (its value is not needed).  xs: tokens * top_k rows.
+ * 16-bit elements; strides in elements; 16-byte aligned rows of a multiple of 8
+ * elements move fastest, any others work. */
 int b200_dispatch(const void* x, const int* rows, const int* total, void* xs, int tokens, int top_k,
                   int width, long long ldx, long long ldxs, int dtype, void* stream);
 
@@ -103,7 +106,7 @@ int b200_combine(const void* y, const float* weights, const int* rows, void* out
                  int top_k, int width, long long ldy, long long ldo, int dtype, void* stream);
 
 /* Gradients of b200_combine: dy[rows[t][j], :] = weights[t][j] dout[t, :] (rows
- * from *total on zero), dweights[t][j] = <dout[t, :], y[rows[t][j], :]> (0 at
+ * that no slot names zero; total as above), dweights[t][j] = <dout[t, :], y[rows[t][j], :]> (0 at
  * empty slots; dweights may be NULL). */
 int b200_combine_grad(const void* dout, const void* y, const float* weights, const int* rows,
                       const int* total, void* dy, float* dweights, int tokens, int top_k, int width,
