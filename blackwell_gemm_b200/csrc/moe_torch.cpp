@@ -8,6 +8,7 @@
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
 #include "b200_moe.h"
@@ -49,6 +50,25 @@ void check_16bit(const at::Tensor& t, const char* who, const char* name) {
 void check_same(const at::Tensor& t, const at::Tensor& like, const char* who, const char* name) {
   TORCH_CHECK(t.device() == like.device(), who, ": ", name, " is on another device");
   TORCH_CHECK(t.scalar_type() == like.scalar_type(), who, ": ", name, " has another dtype");
+}
+
+// There are no forward-mode derivatives: a tangent would be lost.
+void check_no_tangent(std::initializer_list<at::Tensor> operands, const char* who) {
+  for (const at::Tensor& t : operands)
+    TORCH_CHECK(!t._fw_grad(0).defined(), who,
+                ": forward-mode derivatives are not defined; use the backward pass");
+}
+
+// Nor second ones: where a backward pass is itself recorded and its results
+// depend on something differentiable, walking through them is an error.
+variable_list differentiable_once(variable_list grads, bool depends, const char* who) {
+  if (!depends || !at::GradMode::is_enabled()) return grads;
+  for (at::Tensor& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  torch::autograd::DelayedError error(
+      std::string(who) + ": second derivatives are not defined (trying to differentiate twice)",
+      (int64_t)grads.size());
+  return error.apply(std::move(grads));
 }
 
 // A rows x cols operand as the kernels read it (unit column stride, rows and
@@ -161,6 +181,7 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
     const Rows ra = as_rows(a);
     const Bank rb = as_bank(b.transpose(1, 2));
     ctx->save_for_backward({ra.t, rb.t, offsets});
+    ctx->saved_data["both"] = a.requires_grad() && b.requires_grad();
     return grouped_forward(ra, rb, offsets);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -175,7 +196,10 @@ struct GroupedMatmul : torch::autograd::Function<GroupedMatmul> {
       if (ctx->needs_input_grad(0)) da = grouped_da(dc, as_bank(bank), offsets);
       if (ctx->needs_input_grad(1)) db = grouped_db(dc, as_rows(a), offsets).transpose(1, 2);
     }
-    return {da, db, at::Tensor()};
+    // (linear in each operand: a gradient is constant unless both are variables)
+    return differentiable_once({da, db, at::Tensor()},
+                               ctx->saved_data["both"].toBool() || grads[0].requires_grad(),
+                               kGrouped);
   }
 };
 
@@ -183,6 +207,7 @@ at::Tensor matmul_b200_grouped(const at::Tensor& A, const at::Tensor& B,
                                const at::Tensor& offsets) {
   TORCH_CHECK(A.dim() == 2 && B.dim() == 3, kGrouped,
               ": A must be (rows, K) and B (experts, K, N)");
+  check_no_tangent({A, B}, kGrouped);
   check_16bit(A, kGrouped, "A");
   check_16bit(B, kGrouped, "B");
   check_same(B, A, kGrouped, "B");
@@ -256,12 +281,13 @@ struct Route : torch::autograd::Function<Route> {
                                    dlogits.data_ptr(), current_stream()),
                    "route_b200 backward");
     }
-    return {dlogits, at::Tensor(), at::Tensor()};
+    return differentiable_once({dlogits, at::Tensor(), at::Tensor()}, true, kRoute);
   }
 };
 
 std::vector<at::Tensor> route_b200(const at::Tensor& logits, int64_t top_k, bool normalize) {
   TORCH_CHECK(logits.dim() == 2, kRoute, ": logits must be (tokens, experts)");
+  check_no_tangent({logits}, kRoute);
   TORCH_CHECK(logits.is_cuda(), kRoute, ": logits must be a CUDA tensor");
   TORCH_CHECK(logits.scalar_type() == at::kFloat || logits.scalar_type() == at::kBFloat16 ||
                   logits.scalar_type() == at::kHalf,
@@ -280,6 +306,7 @@ std::vector<at::Tensor> route_b200(const at::Tensor& logits, int64_t top_k, bool
 void check_routing(const at::Tensor& t, const at::Tensor& rows, const at::Tensor& offsets,
                    bool sorted, const char* who, const char* name) {
   TORCH_CHECK(t.dim() == 2, who, ": ", name, " must be 2-D");
+  check_no_tangent({t}, who);
   check_16bit(t, who, name);
   TORCH_CHECK(rows.dim() == 2 && rows.is_contiguous() && rows.scalar_type() == at::kInt &&
                   offsets.dim() == 1 && offsets.size(0) >= 1 && offsets.is_contiguous() &&
@@ -333,7 +360,8 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     if (grads[0].defined())
       dx = combine_forward(grads[0].to(ctx->saved_data["dtype"].toScalarType()), nullptr,
                            ctx->get_saved_variables()[0], "dispatch_b200 backward");
-    return {dx, at::Tensor(), at::Tensor()};
+    return differentiable_once({dx, at::Tensor(), at::Tensor()}, grads[0].requires_grad(),
+                               kDispatch);
   }
 };
 
@@ -347,6 +375,7 @@ struct Combine : torch::autograd::Function<Combine> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& y, const at::Tensor& weights,
                             const at::Tensor& rows, const at::Tensor& offsets) {
     ctx->save_for_backward({y, weights, rows, offsets});
+    ctx->saved_data["both"] = y.requires_grad() && weights.requires_grad();
     return combine_forward(y, weights.data_ptr<float>(), rows, kCombine);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
@@ -367,12 +396,15 @@ struct Combine : torch::autograd::Function<Combine> {
                             row_stride(in), y.size(1), dtype_code(y), current_stream()),
           "combine_b200 backward");
     }
-    return {dy, dweights, at::Tensor(), at::Tensor()};
+    return differentiable_once({dy, dweights, at::Tensor(), at::Tensor()},
+                               ctx->saved_data["both"].toBool() || grads[0].requires_grad(),
+                               kCombine);
   }
 };
 
 at::Tensor combine_b200(const at::Tensor& y, const at::Tensor& weights, const at::Tensor& rows,
                         const at::Tensor& offsets) {
+  check_no_tangent({weights}, kCombine);
   check_routing(y, rows, offsets, true, kCombine, "y");
   TORCH_CHECK(weights.sizes() == rows.sizes() && weights.scalar_type() == at::kFloat &&
                   weights.device() == y.device(),
@@ -430,6 +462,7 @@ at::Tensor w4_matmul(const at::Tensor& A, const at::Tensor& packed, int64_t expe
                      int64_t K, int64_t group, bool zeros, bool half,
                      const std::optional<at::Tensor>& offsets) {
   TORCH_CHECK(A.dim() == 2, kW4, ": A must be (rows, K)");
+  check_no_tangent({A}, kW4);
   check_16bit(A, kW4, "A");
   TORCH_CHECK(A.scalar_type() == (half ? at::kHalf : at::kBFloat16), kW4,
               ": A and the scales must have the same dtype");

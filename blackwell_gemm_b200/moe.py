@@ -4,6 +4,8 @@ Rows are sorted by expert: expert e owns rows ``offsets[e] .. offsets[e+1]-1``.
 ``offsets`` stays on the device; no call here waits for the GPU.  Everything
 runs on the current stream and is computed by libb200gemm.so
 (include/b200_moe.h); there is no fallback.
+Gradients are first derivatives by the backward pass; forward-mode derivatives
+raise at the call, second ones where they are taken.
 """
 from __future__ import annotations
 
