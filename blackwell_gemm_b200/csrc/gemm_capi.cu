@@ -34,17 +34,26 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t
                                    const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                    CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
 
+template <class Fn>
+Fn driver_entry(const char* name) {
+  void* p = nullptr;
+  cudaDriverEntryPointQueryResult q;
+  if (cudaGetDriverEntryPoint(name, &p, cudaEnableDefault, &q) != cudaSuccess ||
+      q != cudaDriverEntryPointSuccess)
+    return nullptr;
+  return reinterpret_cast<Fn>(p);
+}
+
 EncodeTiledFn encode_tiled() {
-  static EncodeTiledFn fn = []() -> EncodeTiledFn {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) !=
-            cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      return nullptr;
-    return reinterpret_cast<EncodeTiledFn>(p);
-  }();
+  static EncodeTiledFn fn = driver_entry<EncodeTiledFn>("cuTensorMapEncodeTiled");
   return fn;
+}
+
+// Whether this thread has a context: the device's own or one that the caller made.
+bool has_context() {
+  static auto fn = driver_entry<CUresult (*)(CUcontext*)>("cuCtxGetCurrent");
+  CUcontext c = nullptr;
+  return fn != nullptr && fn(&c) == CUDA_SUCCESS && c != nullptr;
 }
 
 // Kernel configurations, named pair-tile width x stage K: {K slabs per
@@ -406,7 +415,8 @@ int device_state(DeviceState** out) {
   if (dev < 0 || dev >= kMaxDevices) return B200_ERR_UNSUPPORTED_DEVICE;
   // A thread that has not used this runtime yet (an autograd thread) has no
   // current context, and the tensor-map encoder refuses to work without one.
-  if (cudaSetDevice(dev) != cudaSuccess) {
+  // A context that the caller made stays as it is: its operands lie there.
+  if (!has_context() && cudaSetDevice(dev) != cudaSuccess) {
     cudaGetLastError();
     return B200_ERR_UNSUPPORTED_DEVICE;
   }
