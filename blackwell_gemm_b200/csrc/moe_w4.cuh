@@ -754,12 +754,13 @@ w4_stream_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs ar
 // bit: its bits down to w's last are at most eight, and it is exact.  The sum of
 // the two products is the weight's, unrounded; and as lo has w's sign and is
 // zero only where w is, a token's infinity comes out as one, not as the NaN of
-// inf - inf or inf x 0.  The tensor core works twice, but no group's sums are read back: the running sum
-// stays in TMEM to the end of the tile.  (fp16 scales have 11 bits, which two
+// inf - inf or inf x 0.  An infinite scale has hi = +-(q - z) and lo = w: their
+// sum is w again.  The tensor core works twice, but no group's sums are read
+// back: the running sum stays in TMEM to the end of the tile.  (fp16 scales have 11 bits, which two
 // fp16 hold as well, but not their range: a weight past 65504, or its low part
 // below 2^-24, would be lost.  fp16 takes the kernels above and below.)
-// (q - z) carries kUnit here too, which the finished sum gives back; scales
-// below 2^-100 lose low bits to it.
+// (q - z) carries kUnit here too, which the finished sum gives back; hi + lo is
+// w down to scales of 2^-120, below which it loses low bits to bf16's range.
 //
 // Warps: 0 records, 1 MMA, 2 tokens, 4-11 two sets that take records in turn
 // to unpack, 12-15 finish tiles.  kTok 128: two buffers of sums and four half
@@ -797,7 +798,7 @@ struct W4SplitCfg {
   }
 };
 
-// hi + lo = p s, two weights at a time; `less`: 31/32 s.
+// hi + lo = p s, two weights at a time; `less`: 31/32 s, or s's sign if that is infinite.
 __device__ __forceinline__ void w4_split(uint32_t p, uint32_t s, uint32_t less, uint32_t* hi,
                                          uint32_t* lo) {
   const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(&p);
@@ -1094,7 +1095,8 @@ w4_split_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs arg
               bias[g] = w4_bias<T>(
                   kZeros ? ld_shared_u8(record + kW4Q + kSub * 256 + g * 128 + row) : 8u);
               scale[g] = ld_shared_u16(record + kW4Q + (g * 128 + row) * 2) * 0x10001u;
-              less[g] = U::fma2(scale[g], 0x3F783F78u, 0u);
+              less[g] = (scale[g] & 0x7F80u) == 0x7F80u ? (scale[g] & 0x80008000u) | 0x3F803F80u
+                                                        : U::fma2(scale[g], 0x3F783F78u, 0u);
             }
             uint32_t q[4][4];  // [t][c]
 #pragma unroll

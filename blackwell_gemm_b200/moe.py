@@ -143,10 +143,13 @@ def matmul_b200_w4(A, weight: W4Weight, offsets=None):
 
     A: (rows, K) CUDA, bf16 or fp16 like the weight's scales.  offsets:
     (experts + 1,) int32 or int64 on the device, for a bank.  Returns
-    (rows, N).  The 4-bit integers enter the product exactly, the scales
-    multiply fp32 sums, and the result is rounded once.  Made for few rows (the
-    weights are read once per 64 rows of an expert); correct for any number.
-    No gradient."""
+    (rows, N).  The weights enter unrounded, and the result is rounded once:
+    either as 4-bit integers, exact, whose fp32 sums the scales multiply, or (bf16
+    in groups of 32 and 64 with more than 32 rows, in a bank with more than 16 to an
+    expert) as the sum of two bf16, exact for scales of 2^-120 and more.  An
+    infinite scale gives a result that is not finite; where its weights differ in
+    sign or are zero the first way may say inf and the second NaN.  The weights are
+    read once per 8 to 256 rows of an expert.  No gradient."""
     if offsets is None and weight.bank and weight.experts != 1:
         raise RuntimeError("matmul_b200_w4: a bank of experts needs offsets")
     return _ext().w4_matmul(A, weight.data, weight.experts, weight.N, weight.K, weight.group,

@@ -130,8 +130,12 @@ int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* pac
  * b200_grouped_gemm, or NULL for experts = 1: every row takes the one matrix.
  * A: rows x K, stride lda; C: rows x N, stride ldc; alignment as there.  The
  * weights enter unrounded: as exact integers whose fp32 sums the scales
- * multiply, or as the sum of two bf16.  Any number of rows (the weights are
- * read once per 8 to 256 rows of an expert). */
+ * multiply, or (bf16 in groups of 32 and 64, from 33 rows on, a bank from 17 rows
+ * an expert on average) as the sum of two bf16, exact for scales of 2^-120 and
+ * more.  The result is then rounded once.  With an infinite scale the first way
+ * gives the sum's sign times infinity, the second the sum of infinite weights,
+ * NaN where their signs differ or q = z.  Any number of rows (the weights are read
+ * once per 8 to 256 rows of an expert). */
 int b200_w4_gemm(const void* A, const void* packed, void* C, const int* offsets, int rows,
                  int experts, int N, int K, int group, int zeros, int lda, int ldc, int dtype,
                  void* stream);

@@ -65,3 +65,54 @@ def test_weights_that_do_not_hold_what_they_say():
     # a copy of it, as a checkpoint gives back, is as good
     again = bg.W4Weight(*[t.clone() if isinstance(t, torch.Tensor) else t for t in good])
     assert torch.equal(bg.matmul_b200_w4(x, again, off), bg.matmul_b200_w4(x, good, off))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("experts,m", [(1, 1), (1, 12), (1, 30), (1, 33), (1, 64), (1, 100), (1, 300),
+                                       (2, 90), (2, 700)])
+def test_infinite_and_nan_scales(experts, m, group, dtype):
+    # an infinite scale makes infinite weights, in kernels for few rows and for many
+    dt, u = DT[dtype]
+    n, k = 136, 256
+    q, s, z, w = weights(experts, n, k, group, True, dt, seed=m)
+    nibbles = torch.stack((q & 15, q >> 4), -1).reshape(experts, n, k)
+    for row, low in ((3, False), (40, True), (77, False), (135, True)):
+        # every weight of this row's first group above its zero point, or below
+        nibbles[:, row, :group] = nibbles[:, row, :group] % 7 + (0 if low else 9)
+        z[:, row, 0] = 8
+    q = (nibbles[..., 0::2] | nibbles[..., 1::2] << 4).contiguous()
+    w = (nibbles.double() - z.double().repeat_interleave(group, -1)) * \
+        s.double().repeat_interleave(group, -1)
+    inf = float("inf")
+    for row, scale in ((3, inf), (40, inf), (77, -inf), (135, float("nan"))):
+        s[:, row, 0] = scale
+    x = rows_of(m, k, dt).abs() + 0.25
+    off = torch.tensor([0, m // 2, m], dtype=torch.int32, device="cuda")
+    if experts == 1:
+        y = bg.matmul_b200_w4(x, bg.pack_w4(q[0], s[0], z[0]))
+    else:
+        y = bg.matmul_b200_w4(x, bg.pack_w4(q, s, z), off)
+    assert bool((y[:, 3] == inf).all()) and bool((y[:, 40] == -inf).all())
+    assert bool((y[:, 77] == -inf).all()) and bool(y[:, 135].isnan().all())
+    rest = torch.ones(n, dtype=torch.bool, device="cuda")
+    rest[[3, 40, 77, 135]] = False
+    for e in range(experts):
+        a, b = (0, m) if experts == 1 else (off[e].item(), off[e + 1].item())
+        close(y[a:b, rest], x[a:b], w[e][rest], u, dtype == "fp16")
+
+
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("m", [8, 32, 64, 512])
+@pytest.mark.parametrize("power", [-120, -110, 119])
+def test_small_and_large_scales_keep_their_bits(power, m, group):
+    # tokens of one 1 each return the weights themselves
+    n, k = 128, 512
+    s = (1 + torch.arange(n, device="cuda") / 128).double() * 2.0 ** power
+    s = s.bfloat16().repeat_interleave(k // group).view(n, -1)
+    q = torch.arange(n * k // 2, device="cuda").mul(73).remainder(256).to(torch.uint8).view(n, -1)
+    z = torch.arange(n * k // group, device="cuda").mul(5).remainder(16).to(torch.uint8).view(n, -1)
+    wide = torch.stack((q & 15, q >> 4), -1).view(n, k).double()
+    w = (wide - z.double().repeat_interleave(group, 1)) * s.double().repeat_interleave(group, 1)
+    x = torch.eye(k, device="cuda").bfloat16()[:m]
+    assert torch.equal(bg.matmul_b200_w4(x, bg.pack_w4(q, s, z)), w.T[:m].bfloat16())
