@@ -33,6 +33,7 @@ DEVICE_WAIT_CODES = {
     0x1008: "stream-K: an earlier CTA's partial tile never arrived",
     0x1009: "dynamic dealing: a slot of the pair's unit ring",
     0x100A: "grouped rows: offsets that decrease or leave the rows (clamped)",
+    0x100B: "4-bit weights: a zero point above 15 (its low four bits were taken)",
 }
 
 KSPLIT_HANDLE_BYTES = 128

@@ -622,7 +622,7 @@ int run_w4_pack(const void* q, const void* scales, const void* zeros, void* pack
   return launch(w4_pack_kernel, (int)records, 256, 0, stream, static_cast<const uint8_t*>(q),
                 static_cast<const uint16_t*>(scales), static_cast<const uint8_t*>(zeros),
                 static_cast<uint8_t*>(packed), N, K, group, blocks, red,
-                w4_record_bytes(group, zeros != nullptr));
+                w4_record_bytes(group, zeros != nullptr), v.status);
 }
 
 // -------------------------------------------------------------------- routing

@@ -52,6 +52,8 @@ __device__ __forceinline__ void drain_copies(uint32_t full, uint32_t stage, uint
 constexpr int kMaxExperts = 1024;
 // Device error word: offsets that fall or leave [0, rows] (they are clamped).
 constexpr int kErrOffsets = 0x100A;
+// The same: 4-bit zero points above 15 (their low four bits were packed).
+constexpr int kErrZeroPoint = 0x100B;
 
 __host__ __device__ constexpr int group_table_bytes(int experts) {
   return ((2 * (experts + 1) * 4 + 15) / 16) * 16;

@@ -7,6 +7,7 @@
 // step pays no Python call per node.
 #include <ATen/cuda/CUDAContext.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -446,6 +447,11 @@ at::Tensor w4_pack(const at::Tensor& q, const at::Tensor& scales,
     z = zeros->contiguous();
   }
   const c10::cuda::CUDAGuard guard(q.device());
+  // (the one wait for the device here, once per weight; in a capture the
+  // packing kernel alone reports it)
+  if (z.defined() && z.numel() > 0 &&
+      c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None)
+    TORCH_CHECK(z.max().item<int64_t>() <= 15, kPack, ": zeros must be 0 .. 15");
   size_t bytes = 0;
   check_status(b200_w4_packed_bytes((int)e, (int)n, (int)k, (int)group, z.defined(), &bytes),
                kPack);

@@ -1608,11 +1608,12 @@ w4_wide_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
 
 // q: experts x N x K / 2 bytes, the low nibble the even k; scales, zeros:
 // experts x N x K / group, 16-bit and 8-bit; all contiguous.  One block per
-// record; rows and k past the matrix get scale 0 and q = 8.
+// record; rows and k past the matrix get scale 0 and q = 8.  A zero point above
+// 15 is reported in the device's error word.
 __global__ void __launch_bounds__(256)
 w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scales,
                const uint8_t* __restrict__ zeros, uint8_t* __restrict__ out, int N, int K, int group,
-               int blocks, int red_blocks, int record_bytes) {
+               int blocks, int red_blocks, int record_bytes, int* status) {
   grid_wait();
   grid_launch_next();
   const long long rec = blockIdx.x;
@@ -1645,7 +1646,11 @@ w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scale
     const bool in = n < N && kg < groups;
     const long long at = (e * N + n) * (long long)groups + kg;
     reinterpret_cast<uint16_t*>(dst + kW4Q)[g * 128 + row] = in ? scales[at] : (uint16_t)0;
-    if (zeros != nullptr) dst[kW4Q + sub * 256 + g * 128 + row] = in ? zeros[at] & 15u : 8u;
+    if (zeros != nullptr) {
+      const uint32_t z = in ? zeros[at] : 8u;
+      if (z > 15u) atomicCAS(status, 0, kErrZeroPoint);
+      dst[kW4Q + sub * 256 + g * 128 + row] = z & 15u;
+    }
   }
 }
 

@@ -1,9 +1,10 @@
 """Mixture-of-experts operators: products whose weight is a bank of experts.
 
 Rows are sorted by expert: expert e owns rows ``offsets[e] .. offsets[e+1]-1``.
-``offsets`` stays on the device; no call here waits for the GPU.  Everything
-runs on the current stream and is computed by libb200gemm.so
-(include/b200_moe.h); there is no fallback.
+``offsets`` stays on the device; no call here waits for the GPU, but for
+``pack_w4``, once per weight, to look at zero points.  Everything runs on the
+current stream and is computed by libb200gemm.so (include/b200_moe.h); there is
+no fallback.
 Gradients are first derivatives by the backward pass; forward-mode derivatives
 raise at the call, second ones where they are taken.
 """
@@ -101,7 +102,8 @@ def pack_w4(q, scales, zeros=None) -> W4Weight:
     one zero point per group of 32, 64 or 128 consecutive k.  q: uint8
     (N, K/2) or (experts, N, K/2), the low nibble the even k.  scales: bf16 or
     fp16, (.., N, K/group); the rows multiplied later must have the same dtype.
-    zeros: uint8 0..15 of scales' shape, or None for 8 everywhere."""
+    zeros: uint8 0..15 of scales' shape, or None for 8 everywhere; larger ones
+    raise, for which the call waits for the device."""
     bank = q.dim() == 3
     if not bank:
         if q.dim() != 2:

@@ -121,7 +121,8 @@ int b200_combine_grad(const void* dout, const void* y, const float* weights, con
  * kernel reads it.  q: experts x N x K/2 bytes, the low nibble the even k;
  * scales: experts x N x K/group; zeros: the same shape, one byte each, or
  * NULL; all contiguous.  packed: b200_w4_packed_bytes bytes, 16-byte aligned
- * (zeros != 0 when zero points are given). */
+ * (zeros != 0 when zero points are given).  Of a zero point above 15 the low four
+ * bits are taken and device error word 0x100B is set. */
 int b200_w4_packed_bytes(int experts, int N, int K, int group, int zeros, size_t* bytes);
 int b200_w4_pack(const void* q, const void* scales, const void* zeros, void* packed, int experts,
                  int N, int K, int group, void* stream);

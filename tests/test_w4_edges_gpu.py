@@ -116,3 +116,40 @@ def test_small_and_large_scales_keep_their_bits(power, m, group):
     w = (wide - z.double().repeat_interleave(group, 1)) * s.double().repeat_interleave(group, 1)
     x = torch.eye(k, device="cuda").bfloat16()[:m]
     assert torch.equal(bg.matmul_b200_w4(x, bg.pack_w4(q, s, z)), w.T[:m].bfloat16())
+
+
+def test_zero_points_above_15_are_not_taken_silently():
+    q, s, z, w = weights(2, 130, 192, 64, True, torch.bfloat16)
+    x = rows_of(8, 192, torch.bfloat16)
+    off = torch.tensor([0, 4, 8], dtype=torch.int32, device="cuda")
+    z[0, 0, 0] = 15
+    bg.pack_w4(q, s, z)
+    bad = z.clone()
+    bad[1, 129, 2] = 16
+    with pytest.raises(RuntimeError, match="0 .. 15"):
+        bg.pack_w4(q, s, bad)
+    with pytest.raises(RuntimeError, match="0 .. 15"):
+        bg.pack_w4(q[1], s[1], bad[1])
+    # through the C ABI, and in a capture, the device's error word says so
+    packed = bg.pack_w4(q, s, z)
+    out = torch.empty_like(packed.data)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def pack(zeros, stream):
+        return capi.lib().b200_w4_pack(q.data_ptr(), s.data_ptr(), zeros.data_ptr(), out.data_ptr(),
+                                       2, 130, 192, 64, stream)
+    assert pack(z, stream) == capi.OK and capi.device_status(True) == 0
+    assert torch.equal(out, packed.data)
+    assert pack(bad, stream) == capi.OK and capi.device_status(True) == 0x100B
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = bg.pack_w4(q, s, z)
+        y = bg.matmul_b200_w4(x, again, off)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(again.data, packed.data)
+    assert torch.equal(y, bg.matmul_b200_w4(x, packed, off))
+    z.copy_(bad)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert capi.device_status(True) == 0x100B
