@@ -88,6 +88,7 @@ SIGNATURES = {
     "b200_grouped_gemm_db": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _ll, _i, _vp]),
     "b200_grouped_set_kernel": (_i, [_i]),
     "b200_align_rows": (_i, [_vp, _ll, _ll, _vp, _i, _i, _i, _i, _vp]),
+    "b200_narrow_offsets": (_i, [_vp, _ll, _i, _vp, _vp]),
     "b200_route": (_i, [_vp, _i, _i, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp, _vp]),
     "b200_route_grad": (_i, [_vp, _i, _i, _ll, _i, _i, _i, _vp, _vp, _vp, _vp, _vp]),
     "b200_dispatch": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _ll, _ll, _i, _vp]),

@@ -758,6 +758,21 @@ int b200_align_rows(const void* src, long long matrix_stride, long long row_stri
                 matrix_stride, row_stride, static_cast<uint16_t*>(dst), matrices, rows, cols, ld);
 }
 
+int b200_narrow_offsets(const void* offsets, long long stride, int count, int* out, void* stream) {
+  if (count < 0 || stride < 0) return B200_ERR_INVALID_ARGUMENT;
+  if (count == 0) return B200_OK;
+  if (count > kMaxExperts + 1) return B200_ERR_TOO_LARGE;
+  if (!offsets || !out) return B200_ERR_INVALID_ARGUMENT;
+  if ((reinterpret_cast<uintptr_t>(offsets) & 7u) || (reinterpret_cast<uintptr_t>(out) & 3u))
+    return B200_ERR_ALIGNMENT;
+  DeviceView v;
+  MoeDevice* m = nullptr;
+  const int st = moe_device(&v, &m);
+  if (st != B200_OK) return st;
+  return launch(narrow_offsets_kernel, 1, 256, 0, static_cast<cudaStream_t>(stream),
+                static_cast<const long long*>(offsets), stride, count, out);
+}
+
 int b200_grouped_set_kernel(int kernel) {
   if (kernel < 0 || kernel > 2) return B200_ERR_INVALID_ARGUMENT;
   g_kernel.store(kernel);

@@ -102,6 +102,17 @@ __device__ __forceinline__ bool build_groups(const int* offsets, int experts, in
   return __any_sync(0xffffffffu, bad);
 }
 
+// 64-bit offsets as the kernels read them: what 32 bits do not hold becomes
+// something outside the rows, which build_groups clamps and reports.
+__global__ void __launch_bounds__(256)
+narrow_offsets_kernel(const long long* __restrict__ offsets, long long stride, int count,
+                      int* __restrict__ out) {
+  grid_wait();
+  grid_launch_next();
+  for (int i = threadIdx.x; i < count; i += 256)
+    out[i] = (int)min(max(offsets[i * stride], -1ll), 0x7FFFFFFFll);
+}
+
 // The 16-bit output formats: round to nearest even, two at a time or one.
 template <class T>
 __device__ __forceinline__ uint32_t pack_pair(float lo, float hi);

@@ -129,8 +129,13 @@ at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::T
   TORCH_CHECK(offsets.device() == like.device(), who, ": offsets must be on the operands' device");
   TORCH_CHECK(offsets.scalar_type() == at::kInt || offsets.scalar_type() == at::kLong, who,
               ": offsets must be int32 or int64");
-  if (offsets.scalar_type() == at::kInt && offsets.is_contiguous()) return offsets;
-  return offsets.to(at::kInt).contiguous();
+  if (offsets.scalar_type() == at::kInt) return offsets.contiguous();
+  const c10::cuda::CUDAGuard guard(offsets.device());
+  auto narrow = fresh({offsets.size(0)}, at::kInt, offsets);
+  check_status(b200_narrow_offsets(offsets.data_ptr(), offsets.stride(0), (int)offsets.size(0),
+                                   narrow.data_ptr<int>(), current_stream()),
+               who);
+  return narrow;
 }
 
 void check_sizes(std::initializer_list<int64_t> sizes, const char* who) {

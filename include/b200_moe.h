@@ -64,6 +64,11 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
 int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
                     int matrices, int rows, int cols, int ld, void* stream);
 
+/* int64 offsets as the calls here take them: `count` values, `stride` elements
+ * apart, to int32.  One that 32 bits do not hold becomes -1 or 2^31 - 1: outside
+ * the rows, as it was, and so clamped and reported. */
+int b200_narrow_offsets(const void* offsets, long long stride, int count, int* out, void* stream);
+
 /* Kernel for b200_grouped_gemm and _da: 0 = chosen by rows per expert
  * (default), 1 = the streaming kernel (few rows), 2 = the pair kernel. */
 int b200_grouped_set_kernel(int kernel);
