@@ -852,6 +852,11 @@ int b200_route_grad(const void* logits, int tokens, int experts, long long ld, i
   if (tokens == 0 || experts == 0) return B200_OK;
   if (!logits || ld < experts || !dlogits || (top_k > 0 && (!chosen || !weights || !dweights)))
     return B200_ERR_INVALID_ARGUMENT;
+  if (((reinterpret_cast<uintptr_t>(logits) | reinterpret_cast<uintptr_t>(dlogits)) &
+       (type == B200_FP32 ? 3u : 1u)) ||
+      ((reinterpret_cast<uintptr_t>(chosen) | reinterpret_cast<uintptr_t>(weights) |
+        reinterpret_cast<uintptr_t>(dweights)) & 3u))
+    return B200_ERR_ALIGNMENT;
   DeviceView v;
   MoeDevice* m = nullptr;
   const int st = moe_device(&v, &m);

@@ -15,3 +15,13 @@ def test_narrow_offsets():
     assert call(FAKE, 1, 3, FAKE + 2, None) == capi.ERR_ALIGNMENT
     assert call(FAKE, 1, 1026, FAKE, None) == capi.ERR_TOO_LARGE
     assert call(None, 1, 0, None, None) == capi.OK
+
+
+def test_route_gradient_alignment():
+    call = capi.lib().b200_route_grad
+    for type, size in ((capi.FP32, 4), (capi.BF16, 2), (capi.FP16, 2)):
+        good = [FAKE, 4, 8, 8, type, 2, 1, FAKE, FAKE, FAKE, FAKE, None]
+        for at, by in ((0, size // 2), (7, 2), (8, 2), (9, 2), (10, size // 2)):
+            args = list(good)
+            args[at] += by
+            assert call(*args) == capi.ERR_ALIGNMENT, (type, at)
