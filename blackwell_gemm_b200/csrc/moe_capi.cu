@@ -21,6 +21,9 @@ using namespace b200;
 namespace {
 
 constexpr int kMaxDevices = 64;
+// The kernels index an extent in 32 bits and may look a tile, a block's step or
+// a block's chunk of tokens past its end.
+constexpr int kMaxExtent = 0x7FFFFFFF - (1 << 25) + 1;
 
 struct MoeDevice {
   bool ready = false;
@@ -279,6 +282,7 @@ int check_call(const Call& c, int mode) {
       (has_bank && (bank_in ? !tma_bank(c) : (reinterpret_cast<uintptr_t>(c.bank) & 1u) != 0)) ||
       (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
     return B200_ERR_ALIGNMENT;
+  if (c.rows > kMaxExtent || c.N > kMaxExtent || c.K > kMaxExtent) return B200_ERR_TOO_LARGE;
   // unit numbers are 32-bit
   const int feat = mode == kGroupedDA ? c.K : c.N;
   const long long units = mode == kGroupedDB
@@ -465,7 +469,7 @@ int check_w4_shape(int experts, int N, int K, int group) {
   if (experts < 0 || N < 0 || K < 0) return B200_ERR_INVALID_ARGUMENT;
   if ((group != 32 && group != 64 && group != 128) || K % group != 0)
     return B200_ERR_INVALID_ARGUMENT;
-  if (experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  if (experts > kMaxExperts || N > kMaxExtent || K > kMaxExtent) return B200_ERR_TOO_LARGE;
   // record numbers are launch indexes
   return (long long)experts * ceil_div(N, kW4Rows) * ceil_div(K, kW4K) < (1ll << 31)
              ? B200_OK
@@ -595,7 +599,8 @@ int run_w4(const W4Call& c, cudaStream_t stream) {
       (!empty && (!tma_rows(c.a, c.lda) || !aligned16(c.packed))) ||
       (reinterpret_cast<uintptr_t>(c.offsets) & 3u))
     return B200_ERR_ALIGNMENT;
-  if ((ceil_div(c.rows, 16) + c.experts) * ceil_div(c.N, kW4Rows) >= (1ll << 30))
+  if (c.rows > kMaxExtent ||
+      (ceil_div(c.rows, 16) + c.experts) * ceil_div(c.N, kW4Rows) >= (1ll << 30))
     return B200_ERR_TOO_LARGE;
   DeviceView v;
   MoeDevice* m = nullptr;
@@ -673,7 +678,9 @@ int run_move(Move what, MoveArgs a, const int* total, int dtype, cudaStream_t st
   if (a.tokens < 0 || a.top_k < 0 || a.width < 0 || a.top_k > kMaxTopK ||
       (dtype != B200_BF16 && dtype != B200_FP16))
     return B200_ERR_INVALID_ARGUMENT;
-  if ((long long)a.tokens * a.top_k >= (1ll << 31)) return B200_ERR_TOO_LARGE;
+  if ((long long)a.tokens * a.top_k >= (1ll << 31) || a.tokens > kMaxExtent ||
+      a.width > kMaxExtent)
+    return B200_ERR_TOO_LARGE;
   // no slots: dispatch and the gradient write nothing, combine writes zeros
   if (a.tokens == 0 || (a.top_k == 0 && what != kCombine)) return B200_OK;
   if (a.width == 0 && what != kCombineGrad) return B200_OK;
@@ -747,6 +754,7 @@ int b200_align_rows(const void* src, long long matrix_stride, long long row_stri
   if (matrices == 0 || rows == 0 || cols == 0) return B200_OK;
   if (!src || !dst || row_stride < 0 || matrix_stride < 0) return B200_ERR_INVALID_ARGUMENT;
   if (!tma_rows(dst, ld) || (reinterpret_cast<uintptr_t>(src) & 1u)) return B200_ERR_ALIGNMENT;
+  if (ld > kMaxExtent) return B200_ERR_TOO_LARGE;
   DeviceView v;
   MoeDevice* m = nullptr;
   const int st = moe_device(&v, &m);
@@ -807,7 +815,8 @@ int b200_route(const void* logits, int tokens, int experts, long long ld, int ty
   if (tokens < 0 || experts < 0 || top_k < 0 || top_k > experts || top_k > kMaxTopK ||
       type < B200_BF16 || type > B200_FP32)
     return B200_ERR_INVALID_ARGUMENT;
-  if (experts > kMaxExperts || (long long)tokens * top_k >= (1ll << 31)) return B200_ERR_TOO_LARGE;
+  if (experts > kMaxExperts || tokens > kMaxExtent || (long long)tokens * top_k >= (1ll << 31))
+    return B200_ERR_TOO_LARGE;
   if (!offsets) return B200_ERR_INVALID_ARGUMENT;
   const bool any = tokens > 0 && top_k > 0;
   if (any && (!logits || ld < experts || !weights || !chosen || !rows || !sources))
@@ -848,7 +857,7 @@ int b200_route_grad(const void* logits, int tokens, int experts, long long ld, i
   if (tokens < 0 || experts < 0 || top_k < 0 || top_k > experts || top_k > kMaxTopK ||
       type < B200_BF16 || type > B200_FP32)
     return B200_ERR_INVALID_ARGUMENT;
-  if (experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  if (experts > kMaxExperts || tokens > kMaxExtent) return B200_ERR_TOO_LARGE;
   if (tokens == 0 || experts == 0) return B200_OK;
   if (!logits || ld < experts || !dlogits || (top_k > 0 && (!chosen || !weights || !dweights)))
     return B200_ERR_INVALID_ARGUMENT;

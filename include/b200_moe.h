@@ -12,6 +12,7 @@
  * row.  Rows before offsets[0] or from offsets[experts] on belong to no
  * expert.  Offsets that decrease or leave [0, rows] are clamped, and device
  * error word 0x100A is set (b200_gemm_device_status).
+ * Rows, columns, tokens and widths are at most 2^31 - 2^25 (B200_ERR_TOO_LARGE).
  * Element types: dtype = B200_BF16 or B200_FP16, for every 16-bit operand of
  * a call; sums are fp32, rounded to the output once. */
 #ifndef B200_MOE_H_

@@ -25,3 +25,38 @@ def test_route_gradient_alignment():
             args = list(good)
             args[at] += by
             assert call(*args) == capi.ERR_ALIGNMENT, (type, at)
+
+
+def test_extents_that_32_bit_indexes_could_pass():
+    # a tile, a chunk or a block's step more must not leave 32 bits
+    lib, most = capi.lib(), 2 ** 31 - 2 ** 25
+    for big in (most + 1, 2 ** 31 - 8):
+        ld, far = big // 8 * 8 + 8 if big + 8 < 2 ** 31 else 2 ** 31 - 8, 2 ** 40
+
+        def grouped(rows=8, n=8, k=8, ldn=8, ldk=8):
+            return (lib.b200_grouped_gemm(FAKE, FAKE, FAKE, FAKE, rows, 2, n, k, ldk, ldk, far, ldn,
+                                          capi.BF16, None),
+                    lib.b200_grouped_gemm_da(FAKE, FAKE, FAKE, FAKE, rows, 2, n, k, ldn, ldk, far, ldk,
+                                             capi.BF16, None),
+                    lib.b200_grouped_gemm_db(FAKE, FAKE, FAKE, FAKE, rows, 2, n, k, ldn, ldk, ldk, far,
+                                             capi.BF16, None))
+        for change in (dict(rows=big), dict(n=big, ldn=ld)):
+            assert grouped(**change) == (capi.ERR_TOO_LARGE,) * 3, change
+        if ld >= big:
+            assert grouped(k=big, ldk=ld) == (capi.ERR_TOO_LARGE,) * 3
+        for rows, n in ((big, 8), (8, big)):
+            assert lib.b200_w4_gemm(FAKE, FAKE, FAKE, None, rows, 1, n, 64, 64, 0, 64, max(n, 8),
+                                    capi.BF16, None) == capi.ERR_TOO_LARGE
+        assert lib.b200_route(FAKE, big, 8, 8, capi.FP32, 1, 1, FAKE, FAKE, FAKE, FAKE, FAKE,
+                              None) == capi.ERR_TOO_LARGE
+        assert lib.b200_route_grad(FAKE, big, 8, 8, capi.FP32, 1, 1, FAKE, FAKE, FAKE, FAKE,
+                                   None) == capi.ERR_TOO_LARGE
+        for tokens, width in ((big, 16), (4, big)):
+            assert lib.b200_dispatch(FAKE, FAKE, FAKE, FAKE, tokens, 1, width, big, big, capi.BF16,
+                                     None) == capi.ERR_TOO_LARGE
+            assert lib.b200_combine(FAKE, FAKE, FAKE, FAKE, tokens, 1, width, big, big, capi.BF16,
+                                    None) == capi.ERR_TOO_LARGE
+            assert lib.b200_combine_grad(FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, FAKE, tokens, 1, width,
+                                         big, big, big, capi.BF16, None) == capi.ERR_TOO_LARGE
+        assert lib.b200_align_rows(FAKE, 0, 8, FAKE, 1, 8, big, ld if ld >= big else 2 ** 31 - 8,
+                                   None) == capi.ERR_TOO_LARGE
