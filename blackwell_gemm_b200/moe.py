@@ -129,7 +129,7 @@ def quantize_w4(w, group: int = 128):
         raise RuntimeError(f"quantize_w4: K = {k} is not a multiple of group = {group}")
     parts = w.float().reshape(*lead, n, k // group, group)
     scales = (parts.abs().amax(-1) / 7).to(w.dtype)
-    step = scales.float().clamp(min=1e-30)[..., None]
+    step = scales.float().masked_fill(scales == 0, 1.0)[..., None]
     q = ((parts / step).round().clamp(-8, 7) + 8).to(dtype=_uint8()).reshape(*lead, n, k)
     return q[..., 0::2] | (q[..., 1::2] << 4), scales
 

@@ -60,3 +60,20 @@ def test_extents_that_32_bit_indexes_could_pass():
                                          big, big, big, capi.BF16, None) == capi.ERR_TOO_LARGE
         assert lib.b200_align_rows(FAKE, 0, 8, FAKE, 1, 8, big, ld if ld >= big else 2 ** 31 - 8,
                                    None) == capi.ERR_TOO_LARGE
+
+
+def test_quantize_tiny_weights():
+    # nearest multiple of the scale, however small that is; zeros stay zero
+    import torch
+    import blackwell_gemm_b200 as bg
+    g = torch.Generator().manual_seed(0)
+    for power in (0, -60, -110):
+        w = (torch.randn(16, 256, generator=g).double() * 2.0 ** power).bfloat16()
+        w[3, :64] = 0
+        q, s = bg.quantize_w4(w, 64)
+        nibbles = torch.stack((q & 15, q >> 4), -1).view(16, 256).double()
+        back = (nibbles - 8) * s.double().repeat_interleave(64, 1)
+        # half a step; the largest may stand 7 (1 + 2^-8) steps out
+        assert bool(((back - w.double()).abs() <=
+                     s.double().repeat_interleave(64, 1) * (0.5 + 2.0 ** -20)).all()), power
+        assert not back[3, :64].any()
