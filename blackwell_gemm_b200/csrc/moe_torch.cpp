@@ -72,6 +72,12 @@ variable_list differentiable_once(variable_list grads, bool depends, const char*
   return error.apply(std::move(grads));
 }
 
+// A copy that no graph records (a backward pass may itself be recorded).
+void copy_plain(const at::Tensor& to, const at::Tensor& from) {
+  const at::NoGradGuard plain;
+  to.copy_(from);
+}
+
 // A rows x cols operand as the kernels read it (unit column stride, rows and
 // base on 16 bytes): `t` itself where it is one, else a copy.
 struct Rows {
@@ -87,14 +93,14 @@ Rows as_rows(const at::Tensor& t) {
       aligned16(t))
     return {t, (int)ld};
   auto buf = fresh({rows, pad}, t.scalar_type(), t);
-  // (an expanded or transposed operand is made contiguous first)
-  const at::Tensor src = (cols == 1 || t.stride(1) == 1) && (rows == 1 || t.stride(0) >= 0)
-                             ? t
-                             : t.contiguous();
-  check_status(b200_align_rows(src.data_ptr(), 0, rows > 1 ? src.stride(0) : cols, buf.data_ptr(), 1,
-                               (int)rows, (int)cols, (int)pad, current_stream()),
-               "aligning rows");
-  return {buf.narrow(1, 0, cols), (int)pad};
+  const at::Tensor to = buf.narrow(1, 0, cols);
+  if (cols == 1 || t.stride(1) == 1)
+    check_status(b200_align_rows(t.data_ptr(), 0, rows > 1 ? t.stride(0) : cols, buf.data_ptr(), 1,
+                                 (int)rows, (int)cols, (int)pad, current_stream()),
+                 "aligning rows");
+  else
+    copy_plain(to, t);  // (transposed: what lies past cols is never read)
+  return {to, (int)pad};
 }
 
 // The same for a bank of matrices, given as (experts, N, K).
@@ -114,12 +120,14 @@ Bank as_bank(const at::Tensor& t) {
       stride % 8 == 0 && stride >= n * ld && aligned16(t))
     return {t, (int)ld, stride};
   auto buf = fresh({e, n, pad}, t.scalar_type(), t);
-  const at::Tensor src =
-      (k == 1 || t.stride(2) == 1) && t.stride(1) >= 0 && t.stride(0) >= 0 ? t : t.contiguous();
-  check_status(b200_align_rows(src.data_ptr(), src.stride(0), src.stride(1), buf.data_ptr(), (int)e,
-                               (int)n, (int)k, (int)pad, current_stream()),
-               "aligning a bank");
-  return {buf.narrow(2, 0, k), (int)pad, n * pad};
+  const at::Tensor to = buf.narrow(2, 0, k);
+  if (k == 1 || t.stride(2) == 1)
+    check_status(b200_align_rows(t.data_ptr(), t.stride(0), t.stride(1), buf.data_ptr(), (int)e,
+                                 (int)n, (int)k, (int)pad, current_stream()),
+                 "aligning a bank");
+  else
+    copy_plain(to, t);
+  return {to, (int)pad, n * pad};
 }
 
 at::Tensor check_offsets(const at::Tensor& offsets, int64_t experts, const at::Tensor& like,

@@ -77,8 +77,9 @@ def matmul_b200_grouped(A, B, offsets):
     its gradient is zero.  Sums are fp32, rounded once.
 
     The gradient of B is an (experts, K, N) view of (experts, N, K) memory, the
-    layout of W.  K not a multiple of 8 (or operands otherwise not on 16-byte
-    rows) costs a copy of that operand per call.  Offsets that decrease or
+    layout of W.  An operand that is not read as it lies costs a copy of it per
+    call (with gradients: per training step): rows of W or A not on 16 bytes, as
+    with K no multiple of 8, or a bank that lies as (experts, K, N).  Offsets that decrease or
     leave [0, rows] are clamped and reported by ``capi.device_status``."""
     return _ext().matmul_b200_grouped(A, B, offsets)
 

@@ -31,3 +31,26 @@ def test_offsets_past_32_bits_are_clamped_and_reported(bad, seen):
     strided = torch.stack((good, good), 1)[:, 0]
     assert torch.equal(bg.matmul_b200_grouped(x, w, strided), bg.matmul_b200_grouped(x, w, good))
     assert capi.device_status(True) == 0
+
+
+@pytest.mark.parametrize("n,k", [(512, 1024), (512, 1021), (509, 1024)])
+def test_one_copy_of_an_operand_that_is_not_read_as_it_lies(n, k):
+    # a bank that lies as (experts, K, N), rows that lie as (K, rows)
+    g = torch.Generator(device="cuda").manual_seed(0)
+    w = torch.randn(8, k, n, generator=g, device="cuda").bfloat16()
+    x = torch.randn(k, 640, generator=g, device="cuda").bfloat16().t()
+    off = torch.arange(9, dtype=torch.int32, device="cuda") * 80
+    want = torch.cat([x[80 * e:80 * e + 80].double() @ w[e].double() for e in range(8)])
+    bg.matmul_b200_grouped(x, w, off)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y = bg.matmul_b200_grouped(x, w, off)
+    extra = torch.cuda.max_memory_allocated() - before
+    pad = (k + 7) // 8 * 8
+    copies = 8 * n * pad * 2 + 640 * pad * 2
+    # (the allocator leaves up to 1 MB of a cached block with an allocation)
+    assert extra <= copies + 640 * n * 2 + 3 * 2 ** 20 < copies + 8 * n * k * 2, (extra, copies)
+    size = torch.cat([x[80 * e:80 * e + 80].double().abs() @ w[e].double().abs() for e in range(8)])
+    bound = 1.0001 * 2.0 ** -8 * want.abs() + 2.0 ** -23 * (k + 2) * size
+    assert bool(((y.double() - want).abs() <= bound).all())
