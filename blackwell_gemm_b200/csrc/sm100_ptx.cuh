@@ -520,11 +520,6 @@ __device__ __forceinline__ void bulk_load_hint(uint32_t dst, const void* src, ui
       : "memory");
 }
 
-// Make generic-proxy writes visible to the async proxy, all state spaces.
-__device__ __forceinline__ void fence_proxy_async_all() {
-  asm volatile("fence.proxy.async;" ::: "memory");
-}
-
 // ------------------------------------------------ an MMA operand held in TMEM
 // D[tmem] (+)= A[tmem] * B[smem]^T; A: 128 lanes (rows) x 8 columns of two
 // 16-bit K elements each.
