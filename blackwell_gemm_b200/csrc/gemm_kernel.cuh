@@ -579,6 +579,7 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
+  cluster_arrive_started();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -619,10 +620,9 @@ gemm_bf16_pair_kernel(const __grid_constant__ CUtensorMap tmap_a,
     prefetch_tmap(&tmap_b);
     prefetch_tmap(&tmap_c);
   }
-  if (warp == 1) {
-    tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
-    tmem_relinquish_pair();
-  }
+  __syncwarp();
+  cluster_wait_started();
+  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
   tc_fence_before_sync();
   cluster_sync_all();
   tc_fence_after_sync();

@@ -455,6 +455,7 @@ gemm_skinny_cluster_kernel(const __grid_constant__ CUtensorMap tmap_b,   // N x 
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
+  if constexpr (kPair) cluster_arrive_started();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -480,10 +481,13 @@ gemm_skinny_cluster_kernel(const __grid_constant__ CUtensorMap tmap_b,   // N x 
     prefetch_tmap(&tmap_b);
     prefetch_tmap(&tmap_a);
   }
+  if constexpr (kPair) {
+    __syncwarp();
+    cluster_wait_started();
+  }
   if (warp == 1) {
     if constexpr (kPair) {
       tmem_alloc_pair(smem_u32(&tmem_slot), P::kTmemAlloc);
-      tmem_relinquish_pair();
     } else {
       tmem_alloc_1(smem_u32(&tmem_slot), P::kTmemAlloc);
       tmem_relinquish_1();
@@ -731,6 +735,7 @@ gemm_skinny_stream_kernel(const __grid_constant__ CUtensorMap tmap_b,   // N x K
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
+  if constexpr (kPair) cluster_arrive_started();
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const uint32_t rank = kPair ? cluster_ctarank() : 0u;
@@ -758,10 +763,13 @@ gemm_skinny_stream_kernel(const __grid_constant__ CUtensorMap tmap_b,   // N x K
     prefetch_tmap(&tmap_a);
     prefetch_tmap(&tmap_c);
   }
+  if constexpr (kPair) {
+    __syncwarp();
+    cluster_wait_started();
+  }
   if (warp == 1) {
     if constexpr (kPair) {
       tmem_alloc_pair(smem_u32(&tmem_slot), P::kTmemAlloc);
-      tmem_relinquish_pair();
     } else {
       tmem_alloc_1(smem_u32(&tmem_slot), P::kTmemAlloc);
       tmem_relinquish_1();

@@ -178,6 +178,7 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
 
+  cluster_arrive_started();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -206,10 +207,9 @@ grouped_pair_kernel(const __grid_constant__ CUtensorMap tmap_w,
     }
     prefetch_tmap(&tmap_s);
   }
-  if (warp == 1) {
-    tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
-    tmem_relinquish_pair();
-  }
+  __syncwarp();
+  cluster_wait_started();
+  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot), kTmemCols);
   grid_wait();
   if (warp == 2) {
     const bool bad = build_groups(args.offsets, args.experts, args.rows, 256, s_off, s_tiles);

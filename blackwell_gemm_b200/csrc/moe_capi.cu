@@ -150,7 +150,8 @@ int moe_device(DeviceView* v, MoeDevice** out) {
 
 // Arrival counts of the streaming kernels: one array per (device, stream),
 // made on the stream's first call; every launch leaves it at zero.  Null when
-// none can be made (the caller then clears counts of its own).
+// none can be made, as for streams after the first 256 (the caller then clears
+// counts of its own).
 constexpr size_t kCountBytes = 4096 * sizeof(unsigned int);
 struct StreamCounts {
   int device;

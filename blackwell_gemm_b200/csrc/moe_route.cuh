@@ -9,7 +9,8 @@
 //              that chose e too: the order does not depend on timing
 //   dispatch   xs[row(t, j)] = x[t]          combine  out[t] = sum_j w y[row]
 //
-// A warp holds a token's logits in registers.  The tokens are cut into one
+// A warp holds a token's logits in registers (with more than 256 experts not all
+// of them: 1 KB a thread is spilled there).  The tokens are cut into one
 // chunk per block: counts per (chunk, expert) first, then every block adds
 // up the chunks before its own and ranks its pairs (two launches; one when a
 // single block does it all).  Moving rows is bound by memory: one block per

@@ -214,12 +214,16 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
 // Few rows (at most 32 to a tile): unpacked weights go straight from
 // registers into warp-level MMAs, without the stores, loads and handshakes of
 // the way through TMEM (about half the instructions a record), and with so few
-// tokens the tensor core's rate does not matter.  Groups of four warps take stages in turn, a warp 32
-// rows of each record: four groups for up to 8 tokens, three for 16, where a
-// fourth would leave 96 registers to a warp, which then spills (57344 x 8192,
-// 16 tokens: 61.4 us with three, 71.0 with four), two for 32.
+// tokens the tensor core's rate does not matter.  Groups of four warps take
+// stages in turn, a warp 32 rows of each record: four groups for up to 8
+// tokens, three for 16 (57344 x 8192, 16 tokens: 61.4 us, with four 71.0: a
+// thread has 96 registers then, not 128), two for 32.  Some registers are
+// spilled in all of them: 24 to 80 bytes stored with 8 tokens, 16 to 108 with
+// 16, 68 to 284 with 32.
 // 57344 x 8192, groups of 128, takes 48.4 us for one token: 5.0 TB/s of
-// packed weights, 0.77 of HBM's measured rate.
+// packed weights, 0.77 of HBM's measured rate.  Smaller weights take 8 to 14 us
+// more than their bytes; no unit is full then (28672 x 8192, 16 tokens: issue
+// slots 41 %, tensor pipe 35 %).
 // Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
 // lets eight lanes read all banks of the swizzled token slab.
 template <int kTok, int kGroup>
@@ -1170,7 +1174,8 @@ w4_split_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs arg
 // 128 columns); three places for products and two for weights fill TMEM.  The
 // running sums of 128 weight rows x 256 tokens are half of the SM's registers:
 // warps 8-23 hold them, 96 registers to a thread, which warps 0-3 (0 records,
-// 1 MMA, 2 tokens) and 4-7 (unpack) leave over.
+// 1 MMA, 2 tokens) and 4-7 (unpack) leave over; about 100 bytes a thread are
+// spilled at the launch's 80.
 // What bounds it: a record's tokens, 64 KiB, are written to shared memory and
 // read by the MMAs once, which takes it 1100 cycles, and an MMA of 128 columns
 // takes about 60 with its A in TMEM; the way from a product's MMAs to its

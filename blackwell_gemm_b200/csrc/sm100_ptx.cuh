@@ -56,6 +56,16 @@ __device__ __forceinline__ void cluster_sync_all() {
                "barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
+// The two halves of a cluster barrier, for a first one at a kernel's start:
+// arrive at once, wait where the other CTAs have to be running.  (Nothing
+// written before is published: a cluster_sync_all follows the set-up.)
+__device__ __forceinline__ void cluster_arrive_started() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait_started() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 __device__ __forceinline__ void st_cluster_u32(uint32_t cluster_addr, uint32_t v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" :: "r"(cluster_addr), "r"(v) : "memory");
 }
@@ -212,16 +222,19 @@ __device__ __forceinline__ void fence_proxy_async_smem() {
 }
 
 // ---------------------------------------------------------------- tcgen05
+// Allocation for a CTA pair is a request to both SMs, made by a warp of either
+// CTA.  The peer has to be running by then (cluster_wait_started): a CTA that
+// asks earlier gets its columns and may leave the peer in its own request for
+// good.  That happened where CTAs start beside the end of another kernel, a pair
+// in some 100,000 (74 pairs, 1444 launches).  The permit goes back with the
+// columns, not before the peer has its own.
 __device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem, uint32_t ncols) {
   asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;"
                :: "r"(dst_smem), "r"(ncols) : "memory");
 }
 
-__device__ __forceinline__ void tmem_relinquish_pair() {
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-
 __device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;"
                :: "r"(taddr), "r"(ncols) : "memory");
 }
