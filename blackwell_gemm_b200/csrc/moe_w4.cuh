@@ -216,14 +216,14 @@ __device__ __forceinline__ void w4_produce(const StreamArgs& args, StreamWalk<kT
 // the way through TMEM (about half the instructions a record), and with so few
 // tokens the tensor core's rate does not matter.  Groups of four warps take
 // stages in turn, a warp 32 rows of each record: four groups for up to 8
-// tokens, three for 16 (57344 x 8192, 16 tokens: 61.4 us, with four 71.0: a
+// tokens, three for 16 (57344 x 8192, 16 tokens: 62.0 us, with four 71.0: a
 // thread has 96 registers then, not 128), two for 32.  Some registers are
 // spilled in all of them: 24 to 80 bytes stored with 8 tokens, 16 to 108 with
 // 16, 68 to 284 with 32.
-// 57344 x 8192, groups of 128, takes 48.4 us for one token: 5.0 TB/s of
-// packed weights, 0.77 of HBM's measured rate.  Smaller weights take 8 to 14 us
+// 57344 x 8192, groups of 128, takes 48.7 us for one token: 4.9 TB/s of
+// packed weights, 0.76 of HBM's measured rate.  Smaller weights take 8 to 14 us
 // more than their bytes; no unit is full then (28672 x 8192, 16 tokens: issue
-// slots 41 %, tensor pipe 35 %).
+// slots 42 %, tensor pipe 35 %).
 // Column n of the products is token (n >> 1) + 4 (n & 1) of its eight, which
 // lets eight lanes read all banks of the swizzled token slab.
 template <int kTok, int kGroup>
