@@ -170,3 +170,23 @@ def test_calls_while_another_thread_captures(what):
     torch.cuda.synchronize()
     assert got == [capi.OK, capi.OK] and bool((doubled == 2).all())
     assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("rows,experts", [(12, 4), (50, 1), (300, 1)])
+def test_two_streams_at_once(rows, experts):
+    # nothing orders the streams: each has counts and slots of its own
+    n, k = 640, 4096
+    x, w = whole(rows, k), whole(experts, n, k, seed=1)
+    off = (torch.arange(experts + 1, device="cuda") * rows // experts).int()
+    weight = bg.pack_w4(*bg.quantize_w4(w, 32))
+    calls = (lambda: bg.matmul_b200_grouped(x, w.transpose(1, 2), off),
+             lambda: bg.matmul_b200_w4(x, weight, off))
+    want = [call() for call in calls]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for r in range(60):
+        with torch.cuda.stream(streams[r % 3]):
+            got.append((r % 2, calls[r % 2]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, want[which]) for which, y in got)
