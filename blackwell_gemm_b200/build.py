@@ -4,7 +4,7 @@ Two artefacts, both written next to this file so they travel with the source
 tree and are found without installation:
 
 * ``libb200gemm.so`` -- the sm_100a kernels and the C ABI of
-  ``include/b200_gemm.h`` and ``include/b200_moe.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
+  ``include/b200_*.h`` (nvcc, ``-gencode arch=compute_100a,code=sm_100a``,
   static CUDA runtime, the driver's tensor-map encoder looked up at run time so
   no ``-lcuda`` is needed);
 * ``_C<ext-suffix>`` -- the torch extension with the reference-compatible
@@ -70,7 +70,10 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
     units = {  # source -> what else it includes
         "gemm_capi.cu": [CSRC / "gemm_skinny.cuh"],
         "moe_capi.cu": [*sorted(CSRC.glob("grouped_*.cuh")), *sorted(CSRC.glob("moe_*.cuh")),
-                        INCLUDE / "b200_moe.h"],
+                        CSRC / "launch.h", INCLUDE / "b200_moe.h"],
+        "ffn_capi.cu": [*sorted(CSRC.glob("ffn_*.cuh")), CSRC / "grad_norm.cuh",
+                        CSRC / "moe_groups.cuh", CSRC / "moe_stream.cuh", CSRC / "launch.h",
+                        INCLUDE / "b200_moe.h", INCLUDE / "b200_ffn.h"],
     }
     OBJ.mkdir(exist_ok=True)
     stale = [name for name, more in units.items()
@@ -98,8 +101,9 @@ def build_lib(force: bool = False, verbose: bool = False) -> Path:
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
-    srcs = [CSRC / "matmul.cpp", CSRC / "moe_torch.cpp", CSRC / "moe_torch.h",
-            INCLUDE / "b200_gemm.h", INCLUDE / "b200_moe.h"]
+    units = [CSRC / "matmul.cpp", CSRC / "moe_torch.cpp", CSRC / "ffn_torch.cpp"]
+    srcs = [*units, CSRC / "moe_torch.h", CSRC / "ffn_torch.h", CSRC / "torch_operands.h",
+            INCLUDE / "b200_gemm.h", INCLUDE / "b200_moe.h", INCLUDE / "b200_ffn.h"]
     if not force and not _stale(EXT, srcs):
         return EXT
     import torch
@@ -114,7 +118,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-shared", "-fPIC",
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_EXTENSION_NAME=_C",
            "-DTORCH_API_INCLUDE_EXTENSION_H", *[f"-I{i}" for i in incs],
-           CSRC / "matmul.cpp", CSRC / "moe_torch.cpp", "-o", tmp,
+           *units, "-o", tmp,
            f"-L{PKG}", "-lb200gemm", f"-L{torch_lib}", "-lc10", "-lc10_cuda", "-ltorch",
            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", STDCXX,
            "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]

@@ -43,6 +43,13 @@ _vp, _i, _u32, _u64, _ull = ctypes.c_void_p, ctypes.c_int, ctypes.c_uint32, ctyp
     ctypes.c_ulonglong
 _ll = ctypes.c_longlong
 _ip = ctypes.POINTER(ctypes.c_int)
+
+
+class Tensor(ctypes.Structure):
+    """b200_tensor: `count` elements of `type` (BF16, FP16, FP32) from `data` on."""
+    _fields_ = [("data", _vp), ("count", _ll), ("type", _i)]
+
+
 SIGNATURES = {
     "b200_gemm_bf16": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp]),
     "b200_gemm_bf16_profile": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp]),
@@ -98,6 +105,16 @@ SIGNATURES = {
     "b200_w4_packed_bytes": (_i, [_i, _i, _i, _i, _i, ctypes.POINTER(ctypes.c_size_t)]),
     "b200_w4_pack": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "b200_w4_gemm": (_i, [_vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp]),
+    # include/b200_ffn.h
+    "b200_ffn_act": (_i, [_vp] * 6 + [_i] * 10 + [_vp]),
+    "b200_ffn_gated": (_i, [_vp] * 6 + [_i] * 6 + [_ll, _i, _ll, _i, _i, _i, _i, _vp]),
+    "b200_ffn_act_grad": (_i, [_vp] * 4 + [_i] * 7 + [_vp]),
+    "b200_ffn_gated_grad": (_i, [_vp] * 4 + [_i] * 8 + [_vp]),
+    "b200_ffn_da": (_i, [_vp] * 5 + [_i] * 7 + [_ll, _i, _ll, _i, _i, _vp]),
+    "b200_ffn_dw": (_i, [_vp] * 4 + [_i] * 8 + [_vp]),
+    "b200_ffn_set_kernel": (_i, [_i]),
+    "b200_grad_norm": (_i, [ctypes.POINTER(Tensor), _i, _vp, _vp]),
+    "b200_clip_grads": (_i, [ctypes.POINTER(Tensor), _i, ctypes.c_float, _vp, _vp]),
 }
 
 _lib = None
@@ -310,6 +327,15 @@ BF16, FP16, FP32 = 0, 1, 2
 def grouped_set_kernel(kernel: int) -> None:
     """0 chosen by rows per expert (default), 1 streaming kernel, 2 pair kernel."""
     check(lib().b200_grouped_set_kernel(int(kernel)), "b200_grouped_set_kernel")
+
+
+# ---------------------------------------------------------------- feed-forward
+ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid")  # by code
+
+
+def ffn_set_kernel(kernel: int) -> None:
+    """0 chosen by sizes (default), 1 streaming kernel, 2 pair kernel."""
+    check(lib().b200_ffn_set_kernel(int(kernel)), "b200_ffn_set_kernel")
 
 
 # ------------------------------------------------- fused K-split over NVLink

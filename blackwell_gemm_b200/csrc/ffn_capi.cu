@@ -1,0 +1,595 @@
+// C-ABI launchers of the feed-forward operators (include/b200_ffn.h).
+//
+// Per call: check the arguments, encode the tensor maps, choose a kernel and
+// launch it on the caller's stream.  Per device, once: shared-memory limits
+// and the number of 2-CTA clusters that can be resident.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <mutex>
+
+#include "b200_ffn.h"
+#include "device_state.h"
+#include "ffn_gemm.cuh"
+#include "ffn_grad.cuh"
+#include "ffn_stream.cuh"
+#include "grad_norm.cuh"
+#include "launch.h"
+
+using namespace b200;
+
+namespace {
+
+struct FfnDevice {
+  bool ready = false;
+  int init_status = B200_OK;
+  int pairs[4] = {};  // resident clusters per FfnMode
+};
+
+std::mutex g_mu;
+FfnDevice g_ffn[kMaxDevices];
+std::atomic<int> g_kernel{0};
+
+// dW: experts whose table fits beside six stages.
+constexpr int kFewExperts = 128;
+
+template <int kMode, bool kMany, class T>
+bool init_pair(int sms, int* pairs) {
+  using C = FfnCfg<kMode, kMany>;
+  constexpr int experts = kMode == kFfnDW && !kMany ? kFewExperts : kMaxExperts;
+  // (512 B: more than the kernel's static shared memory)
+  static_assert(C::smem_bytes(experts) <= 227 * 1024 - 512, "shared memory of one CTA");
+  auto* fn = ffn_pair_kernel<kMode, kMany, T>;
+  if (!set_smem(fn, C::smem_bytes(experts))) return false;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * sms);
+  cfg.blockDim = dim3(C::kThreads);
+  cfg.dynamicSmemBytes = C::smem_bytes(experts);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n < 1) return false;
+  if (*pairs == 0 || n < *pairs) *pairs = n;
+  return true;
+}
+
+template <bool kGated, int kTok, class T>
+bool init_stream() {
+  using C = FfnStreamCfg<kTok>;
+  static_assert(C::smem_bytes(kMaxExperts) <= 227 * 1024 - 512, "shared memory of one CTA");
+  return set_smem(ffn_stream_kernel<kGated, kTok, T>, C::smem_bytes(kMaxExperts));
+}
+
+template <class T>
+bool init_type(FfnDevice& d, int sms) {
+  return init_pair<kFfnGated, false, T>(sms, &d.pairs[0]) &&
+         init_pair<kFfnAct, false, T>(sms, &d.pairs[1]) &&
+         init_pair<kFfnDA, false, T>(sms, &d.pairs[2]) &&
+         init_pair<kFfnDW, false, T>(sms, &d.pairs[3]) &&
+         init_pair<kFfnDW, true, T>(sms, &d.pairs[3]) && init_stream<true, 16, T>() &&
+         init_stream<true, 64, T>() && init_stream<true, 256, T>() &&
+         init_stream<false, 16, T>() && init_stream<false, 64, T>() &&
+         init_stream<false, 256, T>();
+}
+
+int ffn_device(DeviceView* v, FfnDevice** out) {
+  const int st = device_view(v);
+  if (st != B200_OK) return st;
+  std::lock_guard<std::mutex> lock(g_mu);
+  FfnDevice& d = g_ffn[v->device];
+  if (!d.ready) {
+    d.ready = true;
+    d.init_status = init_type<__nv_bfloat16>(d, v->sms) && init_type<__half>(d, v->sms)
+                        ? B200_OK
+                        : B200_ERR_LAUNCH;
+    if (d.init_status != B200_OK) cudaGetLastError();
+  }
+  if (d.init_status != B200_OK) return d.init_status;
+  *out = &d;
+  return B200_OK;
+}
+
+// A bank of matrices, or one: read by TMA.
+struct Bank {
+  const void* p;
+  int ld;
+  long long stride;
+};
+
+// One product.  t: the token operand read; out: what is written.
+struct FfnCall {
+  const void* t;
+  Bank w[2];
+  int weights;  // 1 or 2
+  const int* offsets;
+  int rows, experts, N, K;
+  int ldt;
+  FfnOut o;
+  int dtype;
+};
+
+bool on(const void* p, unsigned bytes) {
+  return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+}
+
+// What all the operators' sizes have to be; experts counts matrices.
+int check_sizes(int rows, int experts, int N, int K, const int* offsets, int dtype) {
+  if (rows < 0 || experts < 0 || N < 0 || K < 0) return B200_ERR_INVALID_ARGUMENT;
+  if (dtype != B200_BF16 && dtype != B200_FP16) return B200_ERR_INVALID_ARGUMENT;
+  if (offsets == nullptr && experts != 1) return B200_ERR_INVALID_ARGUMENT;
+  if (experts > kMaxExperts) return B200_ERR_TOO_LARGE;
+  if (!on(offsets, 4)) return B200_ERR_ALIGNMENT;
+  if (rows > kMaxExtent || N > kMaxExtent || K > kMaxExtent) return B200_ERR_TOO_LARGE;
+  return B200_OK;
+}
+
+// A matrix (or bank) that TMA reads; null is allowed where it is empty.
+int check_bank(const Bank& w, int experts, int N, int K) {
+  if (experts == 0 || N == 0 || K == 0) return B200_OK;
+  if (!w.p || w.ld < K || (experts > 1 && w.stride < (long long)N * w.ld))
+    return B200_ERR_INVALID_ARGUMENT;
+  return tma_rows(w.p, w.ld) && (experts <= 1 || (w.stride & 7) == 0) ? B200_OK
+                                                                       : B200_ERR_ALIGNMENT;
+}
+
+int check_rows(const void* p, int ld, int rows, int cols) {
+  if (rows == 0 || cols == 0) return B200_OK;
+  if (!p || ld < cols) return B200_ERR_INVALID_ARGUMENT;
+  return tma_rows(p, ld) ? B200_OK : B200_ERR_ALIGNMENT;
+}
+
+// A row operand that kernels read or write element by element.
+int check_plain(const void* p, int ld, int rows, int cols, bool may_be_null) {
+  if (rows == 0 || cols == 0 || (p == nullptr && may_be_null)) return B200_OK;
+  if (!p || ld < cols) return B200_ERR_INVALID_ARGUMENT;
+  return on(p, 2) ? B200_OK : B200_ERR_ALIGNMENT;
+}
+
+int check_z(const float* z, int ldz, int rows, int cols) {
+  if (z == nullptr || rows == 0 || cols == 0) return B200_OK;
+  if (ldz < cols) return B200_ERR_INVALID_ARGUMENT;
+  return on(z, 16) && (ldz & 3) == 0 ? B200_OK : B200_ERR_ALIGNMENT;
+}
+
+// unit numbers are 32-bit
+int check_units(long long row_tiles, long long experts, long long feat, long long times) {
+  return (row_tiles + experts) * ceil_div(feat, 64) * times < (1ll << 30) ? B200_OK
+                                                                         : B200_ERR_TOO_LARGE;
+}
+
+#define CHECK(x)                     \
+  do {                               \
+    const int st_ = (x);             \
+    if (st_ != B200_OK) return st_;  \
+  } while (0)
+
+// (columns, rows, halves), the halves rows * ld apart.
+int map_halves(CUtensorMap* m, int dtype, const void* p, int cols, int rows, int halves, int ld,
+               int box_rows) {
+  return map_bank(m, dtype, p, cols, rows, halves, ld, (long long)rows * ld, box_rows);
+}
+
+template <int kMode, bool kMany, class T>
+int launch_pair(FfnArgs& a, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& t,
+                const CUtensorMap& s, const DeviceView& v, const FfnDevice& d,
+                cudaStream_t stream) {
+  using C = FfnCfg<kMode, kMany>;
+  a.group = 8;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  const long long tf = ceil_div(a.feat, C::kFeat);
+  const long long most =
+      kMode == kFfnDW ? tf * ceil_div(a.cols, 256) * a.halves * a.experts
+                      : tf * (ceil_div(a.rows, 256) + (a.experts < a.rows ? a.experts : a.rows));
+  const int pairs = (int)(most < d.pairs[kMode] ? most : d.pairs[kMode]);
+  return launch(ffn_pair_kernel<kMode, kMany, T>, 2 * pairs, C::kThreads,
+                C::smem_bytes(a.experts), stream, w0, w1, t, s, a);
+}
+
+// The forward products and dA: a bank of matrices times rows.
+template <int kMode, class T>
+int run_pair(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStream_t stream) {
+  constexpr bool kDA = kMode == kFfnDA;
+  const int red = kDA ? c.N : c.K;
+  CUtensorMap w[2], t, s;
+  for (int i = 0; i < c.weights; ++i)
+    CHECK(map_bank(&w[i], c.dtype, c.w[i].p, c.K, c.N, c.experts, c.w[i].ld, c.w[i].stride,
+                   kMode == kFfnAct ? 128 : 64));
+  if (c.weights == 1) w[1] = w[0];
+  const int halves = kDA ? c.weights : 1;
+  CHECK(map_halves(&t, c.dtype, c.t, red, c.rows, halves, c.ldt, 128));
+  CHECK(map_halves(&s, c.dtype, c.t, red, c.rows, halves, c.ldt, 16));
+  FfnArgs a = {};
+  a.offsets = c.offsets;
+  a.experts = c.experts;
+  a.rows = c.rows;
+  a.feat = c.o.feat;
+  a.red = red;
+  a.halves = halves;
+  a.o = c.o;
+  return launch_pair<kMode, false, T>(a, w[0], w[1], t, s, v, d, stream);
+}
+
+template <bool kGated, int kTok, class T>
+int run_stream(const FfnCall& c, const DeviceView& v, cudaStream_t stream) {
+  using C = FfnStreamCfg<kTok>;
+  CUtensorMap w[2], t;
+  for (int i = 0; i < c.weights; ++i)
+    CHECK(map_bank(&w[i], c.dtype, c.w[i].p, c.K, c.N, c.experts, c.w[i].ld, c.w[i].stride,
+                   kGated ? 64 : 128));
+  if (c.weights == 1) w[1] = w[0];
+  CHECK(map_rows(&t, c.dtype, c.t, c.K, c.rows, c.ldt, 16));
+  StreamArgs a = {};
+  a.offsets = c.offsets;
+  a.experts = c.experts;
+  a.rows = c.rows;
+  a.feat = c.N;
+  a.feat_blocks = (int)ceil_div(c.N, kGated ? 64 : 128);
+  a.red = c.K;
+  a.red_blocks = (int)ceil_div(c.K, kSlabK);
+  a.min_items = 16;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  Workspace ws;
+  CHECK(ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a));
+  return launch(ffn_stream_kernel<kGated, kTok, T>, v.sms, C::kThreads, C::smem_bytes(c.experts),
+                stream, w[0], w[1], t, a, c.o);
+}
+
+bool use_stream(const FfnCall& c) {
+  const int k = g_kernel.load();
+  if (k != 0) return k == 1;
+  return c.rows <= 64ll * c.experts;
+}
+
+template <bool kGated, class T>
+int run_forward(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStream_t stream) {
+  if (!use_stream(c)) return run_pair<kGated ? kFfnGated : kFfnAct, T>(c, v, d, stream);
+  if (c.rows <= 16) return run_stream<kGated, 16, T>(c, v, stream);
+  if (c.rows <= 64ll * c.experts) return run_stream<kGated, 64, T>(c, v, stream);
+  return run_stream<kGated, 256, T>(c, v, stream);
+}
+
+template <bool kGated>
+int run_product(FfnCall& c, cudaStream_t stream) {
+  if (c.rows == 0 || c.N == 0) return B200_OK;
+  DeviceView v;
+  FfnDevice* d = nullptr;
+  CHECK(ffn_device(&v, &d));
+  if (c.experts == 0 || c.K == 0) {
+    if (kGated) {  // act(0) * 0
+      if (c.o.z != nullptr &&
+          cudaMemsetAsync(c.o.z, 0, (size_t)2 * c.rows * c.o.ldz * sizeof(float), stream) !=
+              cudaSuccess)
+        return B200_ERR_LAUNCH;
+      return zero_rows(c.o.out, (int)c.o.ldo, c.N, c.rows, stream);
+    }
+    const int blocks = (int)std::min(ceil_div((long long)c.rows * c.N, 256), 8ll * v.sms);
+    return c.dtype == B200_FP16
+               ? launch(ffn_empty_kernel<__half>, blocks, 256, 0, stream, c.o, c.rows)
+               : launch(ffn_empty_kernel<__nv_bfloat16>, blocks, 256, 0, stream, c.o, c.rows);
+  }
+  c.o.vec_out = on(c.o.out, 8) && (c.o.ldo & 3) == 0;
+  c.o.vec_res = on(c.o.residual, 8) && (c.o.ldr & 3) == 0;
+  return c.dtype == B200_FP16 ? run_forward<kGated, __half>(c, v, *d, stream)
+                              : run_forward<kGated, __nv_bfloat16>(c, v, *d, stream);
+}
+
+int check_act(int act) {
+  return act >= B200_ACT_NONE && act <= B200_ACT_SIGMOID ? B200_OK : B200_ERR_INVALID_ARGUMENT;
+}
+
+int run_grad(FfnGradArgs a, bool gated, void* dbias, int dtype, cudaStream_t stream) {
+  DeviceView v;
+  FfnDevice* d = nullptr;
+  CHECK(ffn_device(&v, &d));
+  a.strips = (int)ceil_div(a.feat, 256);
+  // About eight blocks to an SM, of 32 rows at least.
+  const long long want = std::max(1ll, 8ll * v.sms / a.strips);
+  a.block_rows = (int)std::max(32ll, ceil_div(ceil_div(a.rows, want), 8) * 8);
+  const int row_blocks = (int)ceil_div(a.rows, a.block_rows);
+  PoolBuffer partial;
+  if (dbias != nullptr) {
+    CHECK(partial.take(v, (size_t)row_blocks * a.feat * sizeof(float), stream));
+    a.partial = reinterpret_cast<float*>(partial.p);
+  }
+  const int blocks = a.strips * row_blocks;
+  const bool half = dtype == B200_FP16;
+  if (gated)
+    return half ? launch(ffn_grad_kernel<true, __half>, blocks, 256, 0, stream, a)
+                : launch(ffn_grad_kernel<true, __nv_bfloat16>, blocks, 256, 0, stream, a);
+  CHECK(half ? launch(ffn_grad_kernel<false, __half>, blocks, 256, 0, stream, a)
+             : launch(ffn_grad_kernel<false, __nv_bfloat16>, blocks, 256, 0, stream, a));
+  if (dbias == nullptr) return B200_OK;
+  return half ? launch(ffn_bias_kernel<__half>, a.strips, 256, 0, stream, a.partial, row_blocks,
+                       a.feat, static_cast<__half*>(dbias))
+              : launch(ffn_bias_kernel<__nv_bfloat16>, a.strips, 256, 0, stream, a.partial,
+                       row_blocks, a.feat, static_cast<__nv_bfloat16*>(dbias));
+}
+
+// ------------------------------------------------------------ norm, clipping
+constexpr int kNormBlocks = 4;  // per SM
+
+// The tables of one call: tensors in launches of up to kNormTensors.
+int norm_tables(const b200_tensor* tensors, int n, int* at, NormTable* table) {
+  table->tensors = table->chunks = 0;
+  long long chunks = 0;
+  while (*at < n && table->tensors < kNormTensors) {
+    const b200_tensor& t = tensors[*at];
+    const long long more = ceil_div(t.count, kNormChunk);
+    if (chunks + more > 0x7FFFFFFFll - (1 << 20)) {
+      if (table->tensors == 0) return B200_ERR_TOO_LARGE;
+      break;
+    }
+    ++*at;
+    if (t.count == 0) continue;
+    table->t[table->tensors++] = {t.data, t.count, (int)chunks, t.type};
+    chunks += more;
+  }
+  table->chunks = (int)chunks;
+  return B200_OK;
+}
+
+int run_norm(const b200_tensor* tensors, int n, bool clip, float max_norm, float* norm,
+             cudaStream_t stream) {
+  if (n < 0 || (n > 0 && !tensors) || !norm) return B200_ERR_INVALID_ARGUMENT;
+  if (clip && !(max_norm >= 0.0f)) return B200_ERR_INVALID_ARGUMENT;
+  if (!on(norm, 4)) return B200_ERR_ALIGNMENT;
+  for (int i = 0; i < n; ++i) {
+    const b200_tensor& t = tensors[i];
+    if (t.type != B200_BF16 && t.type != B200_FP16 && t.type != B200_FP32)
+      return B200_ERR_INVALID_ARGUMENT;
+    if (t.count < 0 || (t.count > 0 && !t.data)) return B200_ERR_INVALID_ARGUMENT;
+    if (!on(t.data, t.type == B200_FP32 ? 4 : 2)) return B200_ERR_ALIGNMENT;
+  }
+  DeviceView v;
+  FfnDevice* d = nullptr;
+  CHECK(ffn_device(&v, &d));
+  const int most = kNormBlocks * v.sms;
+  // (a table holds kNormTensors tensors, or all the chunks that 31 bits count)
+  NormTable table;
+  int launches = 0, partials = 0;
+  for (int at = 0; at < n; ++launches) CHECK(norm_tables(tensors, n, &at, &table));
+  PoolBuffer sums;
+  CHECK(sums.take(v, (size_t)std::max(launches, 1) * most * sizeof(double), stream));
+  double* partial = reinterpret_cast<double*>(sums.p);
+  for (int at = 0; at < n;) {
+    CHECK(norm_tables(tensors, n, &at, &table));
+    const int blocks = std::min(table.chunks, most);
+    if (blocks == 0) continue;
+    CHECK(launch(norm_kernel<>, blocks, kNormThreads, 0, stream, table, partial + partials));
+    partials += blocks;
+  }
+  if (!clip || partials == 0)
+    return launch(norm_finish_kernel<>, 1, kNormThreads, 0, stream, partial, partials, norm);
+  for (int at = 0; at < n;) {
+    CHECK(norm_tables(tensors, n, &at, &table));
+    const int blocks = std::min(table.chunks, most);
+    if (blocks == 0) continue;
+    CHECK(launch(clip_kernel<>, blocks, kNormThreads, 0, stream, table, partial, partials,
+                 max_norm, norm));
+    norm = nullptr;  // (the first of them writes it)
+  }
+  return B200_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_ffn_act(const void* A, const void* W, const void* bias, const void* residual, void* C,
+                 float* z, int rows, int N, int K, int lda, int ldw, int ldr, int ldc, int ldz,
+                 int act, int dtype, void* stream) {
+  CHECK(check_sizes(rows, 1, N, K, nullptr, dtype));
+  CHECK(check_act(act));
+  FfnCall c = {A, {{W, ldw, 0}, {}}, 1, nullptr, rows, 1, N, K, lda, {}, dtype};
+  if (N > 0) CHECK(check_bank(c.w[0], rows > 0, N, K));
+  CHECK(check_rows(A, lda, N > 0 ? rows : 0, K));
+  CHECK(check_plain(C, ldc, rows, N, false));
+  CHECK(check_plain(residual, ldr, rows, N, true));
+  CHECK(check_plain(bias, N, 1, N, true));
+  CHECK(check_z(z, ldz, rows, N));
+  CHECK(check_units(ceil_div(rows, 16), 1, N, 1));
+  c.o.out = C;
+  c.o.ldo = ldc;
+  c.o.z = z;
+  c.o.ldz = ldz;
+  c.o.bias = bias;
+  c.o.residual = residual;
+  c.o.ldr = ldr;
+  c.o.feat = N;
+  c.o.act = act;
+  return run_product<false>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_ffn_gated(const void* A, const void* Wg, const void* Wu, const int* offsets, void* H,
+                   float* z, int rows, int experts, int N, int K, int lda, int ldg,
+                   long long stride_g, int ldu, long long stride_u, int ldh, int ldz, int act,
+                   int dtype, void* stream) {
+  CHECK(check_sizes(rows, experts, N, K, offsets, dtype));
+  CHECK(check_act(act));
+  FfnCall c = {A, {{Wg, ldg, stride_g}, {Wu, ldu, stride_u}}, 2, offsets, rows, experts, N, K,
+               lda, {}, dtype};
+  if (rows > 0) {
+    CHECK(check_bank(c.w[0], experts, N, K));
+    CHECK(check_bank(c.w[1], experts, N, K));
+  }
+  CHECK(check_rows(A, lda, N > 0 && experts > 0 ? rows : 0, K));
+  CHECK(check_plain(H, ldh, rows, N, false));
+  CHECK(check_z(z, ldz, rows, N));
+  CHECK(check_units(ceil_div(rows, 16), experts, N, 1));
+  c.o.out = H;
+  c.o.ldo = ldh;
+  c.o.z = z;
+  c.o.ldz = ldz;
+  c.o.z_half = (long long)rows * ldz;
+  c.o.feat = N;
+  c.o.act = act;
+  return run_product<true>(c, static_cast<cudaStream_t>(stream));
+}
+
+int b200_ffn_act_grad(const void* dC, const float* z, void* dz, void* dbias, int rows, int N,
+                      int ldc, int ldz, int lddz, int act, int dtype, void* stream) {
+  CHECK(check_sizes(rows, 1, N, 0, nullptr, dtype));
+  CHECK(check_act(act));
+  CHECK(check_rows(dC, ldc, rows, N));
+  if (act != B200_ACT_NONE && !z && rows > 0 && N > 0) return B200_ERR_INVALID_ARGUMENT;
+  CHECK(check_z(act != B200_ACT_NONE ? z : nullptr, ldz, rows, N));
+  if (dz) CHECK(check_rows(dz, lddz, rows, N));
+  CHECK(check_plain(dbias, N, 1, N, true));
+  CHECK(check_units(ceil_div(rows, 32), 1, N, 1));
+  if (N == 0 || (!dz && !dbias) || (rows == 0 && !dbias)) return B200_OK;
+  if (rows == 0) return zero_rows(dbias, N, N, 1, static_cast<cudaStream_t>(stream));
+  FfnGradArgs a = {};
+  a.dout = dC;
+  a.ldd = ldc;
+  a.z = z;
+  a.ldz = ldz;
+  a.dz = dz;
+  a.lddz = lddz;
+  a.experts = 1;
+  a.rows = rows;
+  a.feat = N;
+  a.act = act;
+  return run_grad(a, false, dbias, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200_ffn_gated_grad(const void* dH, const float* z, const int* offsets, void* dz, int rows,
+                        int experts, int N, int ldh, int ldz, int lddz, int act, int dtype,
+                        void* stream) {
+  CHECK(check_sizes(rows, experts, N, 0, offsets, dtype));
+  CHECK(check_act(act));
+  CHECK(check_rows(dH, ldh, rows, N));
+  CHECK(check_rows(dz, lddz, rows, N));
+  if (!z && rows > 0 && N > 0) return B200_ERR_INVALID_ARGUMENT;
+  CHECK(check_z(z, ldz, rows, N));
+  CHECK(check_units(ceil_div(rows, 32), experts, N, 1));
+  if (rows == 0 || N == 0 || experts == 0) return B200_OK;
+  FfnGradArgs a = {};
+  a.dout = dH;
+  a.ldd = ldh;
+  a.z = z;
+  a.ldz = ldz;
+  a.z_half = (long long)rows * ldz;
+  a.dz = dz;
+  a.lddz = lddz;
+  a.dz_half = (long long)rows * lddz;
+  a.offsets = offsets;
+  a.experts = experts;
+  a.rows = rows;
+  a.feat = N;
+  a.act = act;
+  return run_grad(a, true, nullptr, dtype, static_cast<cudaStream_t>(stream));
+}
+
+int b200_ffn_da(const void* dz, const void* W0, const void* W1, const int* offsets, void* dA,
+                int halves, int rows, int experts, int N, int K, int lddz, int ld0,
+                long long stride0, int ld1, long long stride1, int lda, int dtype, void* stream) {
+  CHECK(check_sizes(rows, experts, N, K, offsets, dtype));
+  if (halves != 1 && halves != 2) return B200_ERR_INVALID_ARGUMENT;
+  FfnCall c = {dz, {{W0, ld0, stride0}, {W1, ld1, stride1}}, halves, offsets, rows, experts, N, K,
+               lddz, {}, dtype};
+  for (int i = 0; i < halves && rows > 0; ++i) CHECK(check_bank(c.w[i], experts, N, K));
+  CHECK(check_rows(dz, lddz, K > 0 && experts > 0 ? rows : 0, N));
+  CHECK(check_plain(dA, lda, rows, K, false));
+  CHECK(check_units(ceil_div(rows, 16), experts, K, 1));
+  if (rows == 0 || K == 0) return B200_OK;
+  DeviceView v;
+  FfnDevice* d = nullptr;
+  CHECK(ffn_device(&v, &d));
+  if (experts == 0 || N == 0) return zero_rows(dA, lda, K, rows, static_cast<cudaStream_t>(stream));
+  c.o.out = dA;
+  c.o.ldo = lda;
+  c.o.feat = K;
+  c.o.act = B200_ACT_NONE;
+  c.o.vec_out = on(dA, 8) && (lda & 3) == 0;
+  return dtype == B200_FP16
+             ? run_pair<kFfnDA, __half>(c, v, *d, static_cast<cudaStream_t>(stream))
+             : run_pair<kFfnDA, __nv_bfloat16>(c, v, *d, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"
+
+namespace {
+
+template <class T>
+int run_dw(const void* dz, const void* A, const int* offsets, void* dW, int halves, int rows,
+           int experts, int N, int K, int lddz, int lda, int dtype, cudaStream_t stream) {
+  DeviceView v;
+  FfnDevice* d = nullptr;
+  CHECK(ffn_device(&v, &d));
+  CUtensorMap tz, ta, ts;
+  CHECK(map_halves(&tz, dtype, dz, N, rows, halves, lddz, 64));
+  CHECK(map_rows(&ta, dtype, A, K, rows, lda, 64));
+  const bool tma = tma_rows(dW, K);
+  if (tma)
+    CHECK(map_bank(&ts, dtype, dW, K, N, halves * experts, K, (long long)N * K, 32));
+  else
+    ts = ta;  // (not used: the kernel stores to `out`)
+  FfnArgs a = {};
+  PoolBuffer maps;
+  if (offsets != nullptr) {
+    CHECK(maps.take(v, (size_t)experts * 2 * sizeof(CUtensorMap), stream));
+    CHECK(launch(ffn_maps_kernel<>, experts, 32, 0, stream, tz, ta, offsets, rows,
+                 reinterpret_cast<CUtensorMap*>(maps.p)));
+    a.maps = reinterpret_cast<const CUtensorMap*>(maps.p);
+  }
+  a.offsets = offsets;
+  a.experts = experts;
+  a.rows = rows;
+  a.feat = N;
+  a.cols = K;
+  a.halves = halves;
+  a.o.out = tma ? nullptr : dW;
+  return experts > kFewExperts ? launch_pair<kFfnDW, true, T>(a, tz, ta, tz, ts, v, *d, stream)
+                               : launch_pair<kFfnDW, false, T>(a, tz, ta, tz, ts, v, *d, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int b200_ffn_dw(const void* dz, const void* A, const int* offsets, void* dW, int halves, int rows,
+                int experts, int N, int K, int lddz, int lda, int dtype, void* stream) {
+  CHECK(check_sizes(rows, experts, N, K, offsets, dtype));
+  if (halves != 1 && halves != 2) return B200_ERR_INVALID_ARGUMENT;
+  const bool any = experts > 0 && N > 0 && K > 0;
+  if (!any) return B200_OK;
+  CHECK(check_rows(dz, lddz, rows, N));
+  CHECK(check_rows(A, lda, rows, K));
+  if (!dW) return B200_ERR_INVALID_ARGUMENT;
+  if (!on(dW, 2)) return B200_ERR_ALIGNMENT;
+  CHECK(check_units(ceil_div(N, 256), 0, K, (long long)halves * experts));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0)
+    return cudaMemsetAsync(dW, 0, (size_t)2 * halves * experts * N * K, s) == cudaSuccess
+               ? B200_OK
+               : B200_ERR_LAUNCH;
+  return dtype == B200_FP16 ? run_dw<__half>(dz, A, offsets, dW, halves, rows, experts, N, K, lddz,
+                                             lda, dtype, s)
+                            : run_dw<__nv_bfloat16>(dz, A, offsets, dW, halves, rows, experts, N,
+                                                    K, lddz, lda, dtype, s);
+}
+
+int b200_ffn_set_kernel(int kernel) {
+  if (kernel < 0 || kernel > 2) return B200_ERR_INVALID_ARGUMENT;
+  g_kernel.store(kernel);
+  return B200_OK;
+}
+
+int b200_grad_norm(const b200_tensor* tensors, int n, float* norm, void* stream) {
+  return run_norm(tensors, n, false, 0.0f, norm, static_cast<cudaStream_t>(stream));
+}
+
+int b200_clip_grads(const b200_tensor* tensors, int n, float max_norm, float* norm, void* stream) {
+  return run_norm(tensors, n, true, max_norm, norm, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

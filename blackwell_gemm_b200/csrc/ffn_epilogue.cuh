@@ -1,0 +1,177 @@
+// The end of a feed-forward product, shared by its kernels: 16 tokens x 128
+// accumulator rows, staged in shared memory so that a thread finds what belongs
+// together (a feature's gate and up product lie in different TMEM lanes) and
+// rows are written in long pieces.
+//
+//   gated: rows 0..63 are gate products, 64..127 the up products of the same 64
+//          features; h = act(g) * u
+//   else:  128 features; y = act(acc + bias) + residual
+//
+// All of it in fp32, rounded once.  With z the pre-activations are kept in fp32:
+// rounding them to 16 bits would put errors as large as the result's own
+// rounding into the gradient two more times.
+#pragma once
+#include "ffn_act.cuh"
+#include "moe_groups.cuh"
+
+namespace b200 {
+
+struct FfnOut {
+  void* out;
+  long long ldo;
+  float* z;               // null: not kept
+  long long ldz, z_half;  // z_half: from the gate's to the up products'
+  const void* bias;
+  const void* residual;
+  long long ldr;
+  int feat;  // output columns
+  int act;
+  int vec_out, vec_res;  // rows on 8 bytes
+};
+
+constexpr int kStageTokens = 16;
+constexpr int kFfnStageBytes = kStageTokens * 128 * 4;
+
+template <class T>
+__device__ __forceinline__ float widen(uint16_t bits);
+template <>
+__device__ __forceinline__ float widen<__nv_bfloat16>(uint16_t bits) {
+  return __uint_as_float((uint32_t)bits << 16);
+}
+template <>
+__device__ __forceinline__ float widen<__half>(uint16_t bits) {
+  return __half2float(__ushort_as_half(bits));
+}
+
+// Up to four elements of a row from `p`, of which the first `n` are there.
+template <class T>
+__device__ __forceinline__ void load_four(const T* p, int n, bool vec, float (&v)[4]) {
+  const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
+  if (vec && n >= 4) {
+    const uint2 w = *reinterpret_cast<const uint2*>(h);
+    v[0] = widen<T>((uint16_t)w.x);
+    v[1] = widen<T>((uint16_t)(w.x >> 16));
+    v[2] = widen<T>((uint16_t)w.y);
+    v[3] = widen<T>((uint16_t)(w.y >> 16));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = i < n ? widen<T>(h[i]) : 0.0f;
+  }
+}
+
+template <class T>
+__device__ __forceinline__ void store_four(T* p, int n, bool vec, const float (&v)[4]) {
+  if (vec && n >= 4) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(pack_pair<T>(v[0], v[1]), pack_pair<T>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = round_one<T>(v[i]);
+  }
+}
+
+// (z's rows are always on 16 bytes)
+__device__ __forceinline__ void store_z(float* p, int n, const float (&v)[4]) {
+  if (n >= 4) {
+    *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (i < n) p[i] = v[i];
+  }
+}
+
+// One warp's part of the staging: lane's accumulator row `quarter * 32 + lane`
+// of 16 tokens.
+__device__ __forceinline__ void stage_put(uint32_t stage, int quarter, const float (&v)[16]) {
+  const uint32_t at = stage + (uint32_t)(quarter * 32 + (threadIdx.x & 31)) * 4u;
+#pragma unroll
+  for (int t = 0; t < kStageTokens; ++t) st_shared_u32(at + t * 512u, __float_as_uint(v[t]));
+}
+
+// What a thread keeps over a tile: its features' bias.
+template <bool kGated>
+struct FfnTile {
+  float bias[kGated ? 1 : 8];
+};
+
+// feat0: the first feature of the 64 or 128; tid: 0..127 of the group of warps.
+template <bool kGated, class T>
+__device__ __forceinline__ void ffn_tile(const FfnOut& o, int feat0, int tid, FfnTile<kGated>& s) {
+  if constexpr (!kGated) {
+    const int f = feat0 + (tid & 15) * 4;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float b[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if (o.bias != nullptr)
+        load_four<T>(static_cast<const T*>(o.bias) + f + h * 64, o.feat - f - h * 64, false, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s.bias[h * 4 + i] = b[i];
+    }
+  }
+}
+
+// 16 staged tokens, of which the first `tokens` are written, to rows row0 on.
+template <bool kGated, class T>
+__device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long long row0,
+                                         int tokens, int feat0, int tid,
+                                         const FfnTile<kGated>& s) {
+  const int f = feat0 + (tid & 15) * 4;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int t = (tid >> 4) + 8 * j;
+    if (t >= tokens) break;
+    const long long row = row0 + t;
+    T* out = static_cast<T*>(o.out) + row * o.ldo + f;
+    const uint32_t at = stage + (uint32_t)t * 512u + (uint32_t)(tid & 15) * 16u;
+    float a[4], b[4];
+    ld_shared_v4_f32(at, a[0], a[1], a[2], a[3]);
+    ld_shared_v4_f32(at + 256u, b[0], b[1], b[2], b[3]);
+    if constexpr (kGated) {
+      const int n = o.feat - f;
+      if (n <= 0) continue;
+      if (o.z != nullptr) {
+        store_z(o.z + row * o.ldz + f, n, a);
+        store_z(o.z + o.z_half + row * o.ldz + f, n, b);
+      }
+      activate(o.act, a);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] *= b[i];
+      store_four(out, n, o.vec_out, a);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float(&v)[4] = h ? b : a;
+        const int n = o.feat - f - h * 64;
+        if (n <= 0) continue;
+        float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (o.residual != nullptr)
+          load_four<T>(static_cast<const T*>(o.residual) + row * o.ldr + f + h * 64, n, o.vec_res,
+                       r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] += s.bias[h * 4 + i];
+        if (o.z != nullptr) store_z(o.z + row * o.ldz + f + h * 64, n, v);
+        activate(o.act, v);
+        if (o.residual != nullptr) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) v[i] += r[i];
+        }
+        store_four(out + h * 64, n, o.vec_out, v);
+      }
+    }
+  }
+}
+
+// A group of four warps: `v` staged, finished and the staging free again.
+template <bool kGated, class T>
+__device__ __forceinline__ void ffn_finish(const FfnOut& o, uint32_t stage, uint32_t bar,
+                                           int quarter, const float (&v)[16], long long row0,
+                                           int tokens, int feat0, int tid,
+                                           const FfnTile<kGated>& s) {
+  stage_put(stage, quarter, v);
+  named_bar_sync(bar, 128);
+  ffn_rows<kGated, T>(o, stage, row0, tokens, feat0, tid, s);
+  named_bar_sync(bar, 128);
+}
+
+}  // namespace b200

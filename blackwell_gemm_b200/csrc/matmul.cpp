@@ -16,6 +16,7 @@
 #include <torch/extension.h>
 
 #include "b200_gemm.h"
+#include "ffn_torch.h"
 #include "moe_torch.h"
 
 namespace {
@@ -131,4 +132,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         "matmul_b200 with the intra-kernel profiler writing into `profiler`");
   m.def("profile_rows", &profile_rows, "profiler rows needed for an M x N x K call on this device");
   register_moe(m);
+  register_ffn(m);
 }

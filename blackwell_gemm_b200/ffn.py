@@ -1,0 +1,83 @@
+"""Feed-forward operators: products with the activation, gate, bias and residual
+of a feed-forward layer in their epilogue, and the norm and clipping of a training
+step's gradients.
+
+Everything runs on the current stream and is computed by libb200gemm.so
+(include/b200_ffn.h); there is no fallback, and no call waits for the GPU.
+Gradients are first derivatives by the backward pass; forward-mode derivatives
+raise at the call, second ones where they are taken.
+
+Activations: "none", "relu", "silu" (z s(z)), "gelu" (z Phi(z)), "gelu_tanh" (its
+tanh form) and "sigmoid" (s(z)), with s the logistic function and Phi the normal
+distribution's.
+"""
+from __future__ import annotations
+
+__all__ = ["matmul_b200_act", "matmul_b200_gated", "grad_norm_b200", "clip_grads_b200"]
+
+
+_loaded = None
+
+
+def _ext():
+    global _loaded
+    if _loaded is None:
+        from . import load
+        _loaded = load()
+    return _loaded
+
+
+def matmul_b200_act(A, B, bias=None, residual=None, *, activation: str = "none"):
+    """C = act(A @ B + bias) + residual in one pass; differentiable in all four.
+
+    A: (M, K) bf16 or fp16 CUDA; B: (K, N), normally the .T of an (N, K) weight;
+    bias: (N,) or None; residual: (M, N) or None; all of A's dtype.  Sums and the
+    epilogue are fp32, rounded once.
+
+    With gradients, and an activation, its argument is kept in fp32 (4 bytes an
+    element).  Its gradient is rounded to A's dtype before the products that make A's
+    and B's; the bias' is summed before that.  The gradient of B is a (K, N) view of
+    (N, K) memory, the layout of the weight.  An operand whose rows are not on 16 bytes
+    (K no multiple of 8) costs a copy of it per call, with gradients per training
+    step."""
+    return _ext().matmul_b200_act(A, B, bias, residual, activation)
+
+
+def matmul_b200_gated(A, B_gate, B_up, offsets=None, *, activation: str = "silu"):
+    """H = act(A @ B_gate) * (A @ B_up) in one pass; differentiable in all three.
+
+    A: (rows, K) bf16 or fp16 CUDA; B_gate, B_up: (K, N), normally the .T of (N, K)
+    weights, which may be halves of one matrix.  With offsets, banks (experts, K, N)
+    of which row r takes its expert's, as in matmul_b200_grouped: rows sorted by
+    expert, (experts + 1,) int32 or int64 on the device, clamped where they decrease
+    or leave [0, rows]; rows of no expert are zero in H and in A's gradient and take
+    no part in the weights'.  Sums and the gate are fp32, rounded once.
+
+    With gradients both products are kept in fp32 (8 bytes an element of H), and
+    their gradients are rounded to A's dtype before the products that follow.  Weight
+    gradients have the layout of the (N, K) weights and share one allocation.  Operands
+    that are not read as they lie cost a copy, as there."""
+    return _ext().matmul_b200_gated(A, B_gate, B_up, offsets, activation)
+
+
+def grad_norm_b200(grads):
+    """The 2-norm of all elements of `grads` together, a 0-d float32 tensor.
+
+    grads: tensors (at least one) of float32, bf16 and fp16 on one CUDA device, of
+    any shapes, empty ones among them.  Summed in fp64, the same bits every time."""
+    return _ext().grad_norm_b200(_list(grads))
+
+
+def clip_grads_b200(grads, max_norm: float):
+    """Scale `grads` in place by min(1, max_norm / (norm + 1e-6)) and return their norm
+    before that, a 0-d float32 tensor: grad_norm_b200 and the scaling in two launches
+    (for each 320 tensors), without a wait for the device.  Nothing is written where
+    the norm is within max_norm.  A norm that is NaN makes every gradient NaN, an
+    infinite one zero, and NaN where it was infinite.  Tensors must not share memory;
+    one with gaps between its elements goes through a copy."""
+    return _ext().clip_grads_b200(_list(grads), max_norm)
+
+
+def _list(grads):
+    import torch
+    return [grads] if isinstance(grads, torch.Tensor) else list(grads)
