@@ -334,7 +334,7 @@ ACTIVATIONS = ("none", "relu", "silu", "gelu", "gelu_tanh", "sigmoid")  # by cod
 
 
 def ffn_set_kernel(kernel: int) -> None:
-    """0 chosen by sizes (default), 1 streaming kernel, 2 pair kernel."""
+    """0 chosen by sizes (default), 1 streaming kernel, 2 pair kernel, 3 cluster kernel."""
     check(lib().b200_ffn_set_kernel(int(kernel)), "b200_ffn_set_kernel")
 
 

@@ -12,6 +12,7 @@
 
 #include "b200_ffn.h"
 #include "device_state.h"
+#include "ffn_cluster.cuh"
 #include "ffn_gemm.cuh"
 #include "ffn_grad.cuh"
 #include "ffn_stream.cuh"
@@ -26,6 +27,7 @@ struct FfnDevice {
   bool ready = false;
   int init_status = B200_OK;
   int pairs[4] = {};  // resident clusters per FfnMode
+  int clusters[2][4] = {};  // resident clusters of parts of 1 or 2 CTAs, 1, 2, 4 or 8 parts
 };
 
 std::mutex g_mu;
@@ -67,9 +69,42 @@ bool init_stream() {
   return set_smem(ffn_stream_kernel<kGated, kTok, T>, C::smem_bytes(kMaxExperts));
 }
 
+template <int kMode, bool kPair, class T>
+bool init_cluster(int sms, int* clusters) {
+  using C = FfnClusterCfg<kPair>;
+  static_assert(C::kSmem <= 227 * 1024 - 512, "shared memory of one CTA");
+  auto* fn = ffn_cluster_kernel<kMode, kPair, T>;
+  if (!set_smem(fn, C::kSmem)) return false;
+  for (int i = 0; i < (kPair ? 3 : 4); ++i) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    const int ctas = (kPair ? 2 : 1) << i;
+    cfg.gridDim = dim3((unsigned)(sms / ctas * ctas));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ctas;
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess || n < 1) return false;
+    if (clusters[i] == 0 || n < clusters[i]) clusters[i] = n;
+  }
+  return true;
+}
+
+template <int kMode, class T>
+bool init_clusters(FfnDevice& d, int sms) {
+  return init_cluster<kMode, false, T>(sms, d.clusters[0]) &&
+         init_cluster<kMode, true, T>(sms, d.clusters[1]);
+}
+
 template <class T>
 bool init_type(FfnDevice& d, int sms) {
-  return init_pair<kFfnGated, false, T>(sms, &d.pairs[0]) &&
+  return init_clusters<kFfnGated, T>(d, sms) && init_clusters<kFfnAct, T>(d, sms) &&
+         init_clusters<kFfnDA, T>(d, sms) &&
+         init_pair<kFfnGated, false, T>(sms, &d.pairs[0]) &&
          init_pair<kFfnAct, false, T>(sms, &d.pairs[1]) &&
          init_pair<kFfnDA, false, T>(sms, &d.pairs[2]) &&
          init_pair<kFfnDW, false, T>(sms, &d.pairs[3]) &&
@@ -178,8 +213,8 @@ int map_halves(CUtensorMap* m, int dtype, const void* p, int cols, int rows, int
 
 template <int kMode, bool kMany, class T>
 int launch_pair(FfnArgs& a, const CUtensorMap& w0, const CUtensorMap& w1, const CUtensorMap& t,
-                const CUtensorMap& s, const DeviceView& v, const FfnDevice& d,
-                cudaStream_t stream) {
+                const CUtensorMap& h, const CUtensorMap& s, const DeviceView& v,
+                const FfnDevice& d, cudaStream_t stream) {
   using C = FfnCfg<kMode, kMany>;
   a.group = 8;
   a.status = v.status;
@@ -187,10 +222,24 @@ int launch_pair(FfnArgs& a, const CUtensorMap& w0, const CUtensorMap& w1, const 
   const long long tf = ceil_div(a.feat, C::kFeat);
   const long long most =
       kMode == kFfnDW ? tf * ceil_div(a.cols, 256) * a.halves * a.experts
-                      : tf * (ceil_div(a.rows, 256) + (a.experts < a.rows ? a.experts : a.rows));
+      : a.offsets == nullptr
+          ? tf * ceil_div(a.rows, 256)
+          : tf * (ceil_div(a.rows, 256) + (a.experts < a.rows ? a.experts : a.rows));
+  // Tiles of equal contractions may be divided, where some are left over: the kernel
+  // sees whether that pays.
+  const int blocks = (int)ceil_div(kMode == kFfnDW ? a.rows : a.red, kSlabK) *
+                     (kMode == kFfnDA ? a.halves : 1);
+  const bool divide = (kMode != kFfnDW || a.offsets == nullptr) &&
+                      blocks > FfnWalk<kMode>::kJoinBlocks && most > d.pairs[kMode] &&
+                      (a.offsets != nullptr || most % d.pairs[kMode] != 0);
+  a.tile_n = kMode == kFfnDW || a.offsets != nullptr
+                 ? 256
+                 : (int)ceil_div(ceil_div(a.rows, ceil_div(a.rows, 256)), 32) * 32;
   const int pairs = (int)(most < d.pairs[kMode] ? most : d.pairs[kMode]);
+  Workspace ws;
+  if (divide) CHECK(ws.take(v, (size_t)2 * pairs * 2 * 256 * 128 * sizeof(float), stream, &a));
   return launch(ffn_pair_kernel<kMode, kMany, T>, 2 * pairs, C::kThreads,
-                C::smem_bytes(a.experts), stream, w0, w1, t, s, a);
+                C::smem_bytes(a.experts), stream, w0, w1, t, h, s, a);
 }
 
 // The forward products and dA: a bank of matrices times rows.
@@ -198,13 +247,14 @@ template <int kMode, class T>
 int run_pair(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStream_t stream) {
   constexpr bool kDA = kMode == kFfnDA;
   const int red = kDA ? c.N : c.K;
-  CUtensorMap w[2], t, s;
+  CUtensorMap w[2], t, h, s;
   for (int i = 0; i < c.weights; ++i)
     CHECK(map_bank(&w[i], c.dtype, c.w[i].p, c.K, c.N, c.experts, c.w[i].ld, c.w[i].stride,
                    kMode == kFfnAct ? 128 : 64));
   if (c.weights == 1) w[1] = w[0];
   const int halves = kDA ? c.weights : 1;
   CHECK(map_halves(&t, c.dtype, c.t, red, c.rows, halves, c.ldt, 128));
+  CHECK(map_halves(&h, c.dtype, c.t, red, c.rows, halves, c.ldt, 64));
   CHECK(map_halves(&s, c.dtype, c.t, red, c.rows, halves, c.ldt, 16));
   FfnArgs a = {};
   a.offsets = c.offsets;
@@ -214,7 +264,99 @@ int run_pair(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStre
   a.red = red;
   a.halves = halves;
   a.o = c.o;
-  return launch_pair<kMode, false, T>(a, w[0], w[1], t, s, v, d, stream);
+  return launch_pair<kMode, false, T>(a, w[0], w[1], t, h, s, v, d, stream);
+}
+
+// How the cluster kernel would take a product, and about how long, in us.
+struct ClusterPlan {
+  bool pair = false;
+  int splits = 0, tokens = 0;  // splits 0: it cannot
+  double us = 1e30;
+};
+
+// Every way that fits one wave, by what was measured: 6.5 us for the launch, the ring's
+// first loads and the last barrier; a stage's 16 KiB of weights and box of tokens at 95
+// GB/s to a CTA, 70 in a pair, or the weights at HBM's 6.3 TB/s; 16 tokens of the
+// epilogue 0.55 us to a group of warps, of the exchange 0.25.  (2048 x 8192 at 256
+// rows: 22.9 us in 64 CTAs, 22.1 in 32 pairs, where the persistent pairs took 48; 4096
+// x 14336 at 128 rows 27.0, 44 through slots in L2.)
+ClusterPlan plan_cluster(int rows, int feat, int blocks, int feat_cta, const FfnDevice& d) {
+  ClusterPlan best;
+  for (int pair = 0; pair < 2; ++pair) {
+    const int step = pair ? 32 : 16;
+    int last = 0;
+    for (int most = 256; most >= step; most /= 2) {
+      const long long tt = ceil_div(rows, most);
+      const int tokens = (int)(ceil_div(ceil_div(rows, tt), step) * step);
+      if (tokens == last) continue;
+      last = tokens;
+      const long long tiles = ceil_div(feat, feat_cta << pair) * ceil_div(rows, tokens);
+      for (int i = 0; i < (pair ? 3 : 4); ++i) {
+        const int splits = 1 << i;
+        if (tiles > d.clusters[pair][i] || splits > blocks) continue;
+        const double share = (double)ceil_div(blocks, splits);
+        const double load = (16384.0 + (pair ? tokens / 2 : tokens) * 128) / (pair ? 70e3 : 95e3);
+        const double hbm = 16384.0 * (double)(tiles / ceil_div(rows, tokens) * splits) *
+                           (pair ? 2 : 1) / 6.3e6;
+        const double chunks = tokens / 32.0;  // to a group of warps
+        const double us = 6.5 + share * std::max(load, hbm) + 0.55 * chunks / splits +
+                          (splits > 1 ? 0.7 + 0.25 * chunks * (1.0 - 1.0 / splits) : 0.0);
+        if (us < best.us) best = {pair != 0, splits, tokens, us};
+      }
+    }
+  }
+  return best;
+}
+
+// One tile to a cluster, its contraction over `splits` parts of one CTA or two.
+template <int kMode, bool kPair, class T>
+int run_cluster(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
+                cudaStream_t stream) {
+  using C = FfnClusterCfg<kPair>;
+  constexpr bool kDA = kMode == kFfnDA;
+  const int red = kDA ? c.N : c.K, halves = kDA ? c.weights : 1;
+  FfnClusterArgs a = {};
+  a.rows = c.rows;
+  a.feat = c.o.feat;
+  a.red = red;
+  a.halves = halves;
+  a.splits = plan.splits;
+  a.tokens = plan.tokens;
+  a.tiles_t = (int)ceil_div(c.rows, a.tokens);
+  a.box = kPair ? a.tokens / 2 : a.tokens;
+  a.stage_bytes = C::kWeight + a.box * 128;
+  a.stages = std::min(C::kMaxStages, C::kRing / a.stage_bytes);
+  a.o = c.o;
+  a.status = v.status;
+  a.timeout_ns = v.timeout_ns;
+  CUtensorMap w[2], t;
+  for (int i = 0; i < c.weights; ++i)
+    CHECK(map_bank(&w[i], c.dtype, c.w[i].p, c.K, c.N, 1, c.w[i].ld, 0,
+                   kMode == kFfnAct ? 128 : 64));
+  if (c.weights == 1) w[1] = w[0];
+  CHECK(map_halves(&t, c.dtype, c.t, red, c.rows, halves, c.ldt, a.box));
+  const int feat = (kPair ? 2 : 1) * (kMode == kFfnGated ? 64 : 128);
+  const int ctas = a.splits * (kPair ? 2 : 1);
+  return launch_clusters(ffn_cluster_kernel<kMode, kPair, T>,
+                         (int)ceil_div(c.o.feat, feat) * a.tiles_t * ctas, ctas, C::kThreads,
+                         C::kSmem, stream, w[0], w[1], t, a);
+}
+
+// The cluster kernel's plan for a call, if it has one.
+template <int kMode>
+ClusterPlan cluster_plan(const FfnCall& c, const FfnDevice& d) {
+  constexpr bool kDA = kMode == kFfnDA;
+  const int k = g_kernel.load();
+  if (c.offsets != nullptr || (k != 0 && k != 3)) return {};
+  const int blocks = (int)ceil_div(kDA ? c.N : c.K, kSlabK) * (kDA ? c.weights : 1);
+  return plan_cluster(c.rows, c.o.feat, blocks, kMode == kFfnGated ? 64 : 128, d);
+}
+
+template <int kMode, class T>
+int run_plan(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
+             cudaStream_t stream) {
+  return plan.pair ? run_cluster<kMode, true, T>(c, plan, v, stream)
+                   : run_cluster<kMode, false, T>(c, plan, v, stream);
 }
 
 template <bool kGated, int kTok, class T>
@@ -243,18 +385,54 @@ int run_stream(const FfnCall& c, const DeviceView& v, cudaStream_t stream) {
                 stream, w[0], w[1], t, a, c.o);
 }
 
-bool use_stream(const FfnCall& c) {
+// f with the activation as a constant.
+template <class F>
+void by_act(int act, F&& f) {
+  switch (act) {
+    case B200_ACT_RELU: f(ActCode<B200_ACT_RELU>()); break;
+    case B200_ACT_SILU: f(ActCode<B200_ACT_SILU>()); break;
+    case B200_ACT_GELU: f(ActCode<B200_ACT_GELU>()); break;
+    case B200_ACT_GELU_TANH: f(ActCode<B200_ACT_GELU_TANH>()); break;
+    case B200_ACT_SIGMOID: f(ActCode<B200_ACT_SIGMOID>()); break;
+    default: f(ActCode<B200_ACT_NONE>()); break;
+  }
+}
+
+// The streaming kernel spreads any number of tiles over the SMs, but takes 64 rows of an
+// expert at a time and joins divided tiles through L2.  One matrix: where no cluster
+// fits or is estimated slower (14336 x 4096 gated, 1 row: 41.0 us, pairs 45.3; 64 rows
+// 45.6 and 47.2, 96 rows 53.4 and 48.5).  A bank: up to 64 rows an expert on average, and
+// up to 256 where half of the pairs would have no tile (8 x 14336 x 4096 gated, 512 rows:
+// 297 us, pairs 330; 1024 rows 361 and 332; 4 x 744 x 6200, 400 rows: 29 and 36).
+template <bool kGated>
+bool use_stream(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
+                const FfnDevice& d) {
   const int k = g_kernel.load();
   if (k != 0) return k == 1;
-  return c.rows <= 64ll * c.experts;
+  if (c.offsets != nullptr) {
+    if (c.rows <= 64ll * c.experts) return true;
+    return c.rows <= 256ll * c.experts &&
+           2 * c.experts * ceil_div(c.N, kGated ? 128 : 256) <= d.pairs[kFfnAct];
+  }
+  if (c.rows > 64) return false;
+  const long long units = ceil_div(c.N, kGated ? 64 : 128), items = units * ceil_div(c.K, kSlabK);
+  const double box = (double)ceil_div(c.rows, 16) * 16 * 128;
+  const double us = 7.7 + 0.15 * c.rows +
+                    (double)items * std::max((16384 + box) / 95e3 / v.sms, 16384 / 6.3e6);
+  return us < plan.us;
 }
 
 template <bool kGated, class T>
 int run_forward(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStream_t stream) {
-  if (!use_stream(c)) return run_pair<kGated ? kFfnGated : kFfnAct, T>(c, v, d, stream);
-  if (c.rows <= 16) return run_stream<kGated, 16, T>(c, v, stream);
-  if (c.rows <= 64ll * c.experts) return run_stream<kGated, 64, T>(c, v, stream);
-  return run_stream<kGated, 256, T>(c, v, stream);
+  constexpr int kMode = kGated ? kFfnGated : kFfnAct;
+  const ClusterPlan plan = cluster_plan<kMode>(c, d);
+  if (use_stream<kGated>(c, plan, v, d)) {
+    if (c.rows <= 16) return run_stream<kGated, 16, T>(c, v, stream);
+    if (c.rows <= 64ll * c.experts) return run_stream<kGated, 64, T>(c, v, stream);
+    return run_stream<kGated, 256, T>(c, v, stream);
+  }
+  if (plan.splits > 0) return run_plan<kMode, T>(c, plan, v, stream);
+  return run_pair<kMode, T>(c, v, d, stream);
 }
 
 template <bool kGated>
@@ -272,9 +450,14 @@ int run_product(FfnCall& c, cudaStream_t stream) {
       return zero_rows(c.o.out, (int)c.o.ldo, c.N, c.rows, stream);
     }
     const int blocks = (int)std::min(ceil_div((long long)c.rows * c.N, 256), 8ll * v.sms);
-    return c.dtype == B200_FP16
-               ? launch(ffn_empty_kernel<__half>, blocks, 256, 0, stream, c.o, c.rows)
-               : launch(ffn_empty_kernel<__nv_bfloat16>, blocks, 256, 0, stream, c.o, c.rows);
+    int st = B200_OK;
+    by_act(c.o.act, [&](auto code) {
+      constexpr int kAct = decltype(code)::value;
+      st = c.dtype == B200_FP16
+               ? launch(ffn_empty_kernel<kAct, __half>, blocks, 256, 0, stream, c.o, c.rows)
+               : launch(ffn_empty_kernel<kAct, __nv_bfloat16>, blocks, 256, 0, stream, c.o, c.rows);
+    });
+    return st;
   }
   c.o.vec_out = on(c.o.out, 8) && (c.o.ldo & 3) == 0;
   c.o.vec_res = on(c.o.residual, 8) && (c.o.ldr & 3) == 0;
@@ -286,7 +469,18 @@ int check_act(int act) {
   return act >= B200_ACT_NONE && act <= B200_ACT_SIGMOID ? B200_OK : B200_ERR_INVALID_ARGUMENT;
 }
 
-int run_grad(FfnGradArgs a, bool gated, void* dbias, int dtype, cudaStream_t stream) {
+template <class T>
+int launch_grad(const FfnGradArgs& a, bool gated, int act, int blocks, cudaStream_t stream) {
+  int st = B200_OK;
+  by_act(act, [&](auto code) {
+    constexpr int kAct = decltype(code)::value;
+    st = gated ? launch(ffn_grad_kernel<true, kAct, T>, blocks, 256, 0, stream, a)
+               : launch(ffn_grad_kernel<false, kAct, T>, blocks, 256, 0, stream, a);
+  });
+  return st;
+}
+
+int run_grad(FfnGradArgs a, bool gated, int act, void* dbias, int dtype, cudaStream_t stream) {
   DeviceView v;
   FfnDevice* d = nullptr;
   CHECK(ffn_device(&v, &d));
@@ -302,11 +496,8 @@ int run_grad(FfnGradArgs a, bool gated, void* dbias, int dtype, cudaStream_t str
   }
   const int blocks = a.strips * row_blocks;
   const bool half = dtype == B200_FP16;
-  if (gated)
-    return half ? launch(ffn_grad_kernel<true, __half>, blocks, 256, 0, stream, a)
-                : launch(ffn_grad_kernel<true, __nv_bfloat16>, blocks, 256, 0, stream, a);
-  CHECK(half ? launch(ffn_grad_kernel<false, __half>, blocks, 256, 0, stream, a)
-             : launch(ffn_grad_kernel<false, __nv_bfloat16>, blocks, 256, 0, stream, a));
+  CHECK(half ? launch_grad<__half>(a, gated, act, blocks, stream)
+             : launch_grad<__nv_bfloat16>(a, gated, act, blocks, stream));
   if (dbias == nullptr) return B200_OK;
   return half ? launch(ffn_bias_kernel<__half>, a.strips, 256, 0, stream, a.partial, row_blocks,
                        a.feat, static_cast<__half*>(dbias))
@@ -457,8 +648,7 @@ int b200_ffn_act_grad(const void* dC, const float* z, void* dz, void* dbias, int
   a.experts = 1;
   a.rows = rows;
   a.feat = N;
-  a.act = act;
-  return run_grad(a, false, dbias, dtype, static_cast<cudaStream_t>(stream));
+  return run_grad(a, false, act, dbias, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int b200_ffn_gated_grad(const void* dH, const float* z, const int* offsets, void* dz, int rows,
@@ -485,8 +675,7 @@ int b200_ffn_gated_grad(const void* dH, const float* z, const int* offsets, void
   a.experts = experts;
   a.rows = rows;
   a.feat = N;
-  a.act = act;
-  return run_grad(a, true, nullptr, dtype, static_cast<cudaStream_t>(stream));
+  return run_grad(a, true, act, nullptr, dtype, static_cast<cudaStream_t>(stream));
 }
 
 int b200_ffn_da(const void* dz, const void* W0, const void* W1, const int* offsets, void* dA,
@@ -510,9 +699,13 @@ int b200_ffn_da(const void* dz, const void* W0, const void* W1, const int* offse
   c.o.feat = K;
   c.o.act = B200_ACT_NONE;
   c.o.vec_out = on(dA, 8) && (lda & 3) == 0;
-  return dtype == B200_FP16
-             ? run_pair<kFfnDA, __half>(c, v, *d, static_cast<cudaStream_t>(stream))
-             : run_pair<kFfnDA, __nv_bfloat16>(c, v, *d, static_cast<cudaStream_t>(stream));
+  const ClusterPlan plan = cluster_plan<kFfnDA>(c, *d);
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (plan.splits > 0)
+    return dtype == B200_FP16 ? run_plan<kFfnDA, __half>(c, plan, v, s)
+                              : run_plan<kFfnDA, __nv_bfloat16>(c, plan, v, s);
+  return dtype == B200_FP16 ? run_pair<kFfnDA, __half>(c, v, *d, s)
+                            : run_pair<kFfnDA, __nv_bfloat16>(c, v, *d, s);
 }
 
 }  // extern "C"
@@ -548,8 +741,8 @@ int run_dw(const void* dz, const void* A, const int* offsets, void* dW, int halv
   a.cols = K;
   a.halves = halves;
   a.o.out = tma ? nullptr : dW;
-  return experts > kFewExperts ? launch_pair<kFfnDW, true, T>(a, tz, ta, tz, ts, v, *d, stream)
-                               : launch_pair<kFfnDW, false, T>(a, tz, ta, tz, ts, v, *d, stream);
+  return experts > kFewExperts ? launch_pair<kFfnDW, true, T>(a, tz, ta, tz, tz, ts, v, *d, stream)
+                               : launch_pair<kFfnDW, false, T>(a, tz, ta, tz, tz, ts, v, *d, stream);
 }
 
 }  // namespace
@@ -579,7 +772,7 @@ int b200_ffn_dw(const void* dz, const void* A, const int* offsets, void* dW, int
 }
 
 int b200_ffn_set_kernel(int kernel) {
-  if (kernel < 0 || kernel > 2) return B200_ERR_INVALID_ARGUMENT;
+  if (kernel < 0 || kernel > 3) return B200_ERR_INVALID_ARGUMENT;
   g_kernel.store(kernel);
   return B200_OK;
 }

@@ -89,15 +89,19 @@ __device__ __forceinline__ void stage_put(uint32_t stage, int quarter, const flo
   for (int t = 0; t < kStageTokens; ++t) st_shared_u32(at + t * 512u, __float_as_uint(v[t]));
 }
 
-// What a thread keeps over a tile: its features' bias.
+// What a thread keeps over a tile: its features' bias, and whether all of the tile's
+// features are there, in rows that it reads and writes four at a time.
 template <bool kGated>
 struct FfnTile {
   float bias[kGated ? 1 : 8];
+  bool whole;
 };
 
 // feat0: the first feature of the 64 or 128; tid: 0..127 of the group of warps.
 template <bool kGated, class T>
 __device__ __forceinline__ void ffn_tile(const FfnOut& o, int feat0, int tid, FfnTile<kGated>& s) {
+  s.whole = feat0 + (kGated ? 64 : 128) <= o.feat && o.vec_out &&
+            (kGated || o.residual == nullptr || o.vec_res);
   if constexpr (!kGated) {
     const int f = feat0 + (tid & 15) * 4;
 #pragma unroll
@@ -111,13 +115,94 @@ __device__ __forceinline__ void ffn_tile(const FfnOut& o, int feat0, int tid, Ff
   }
 }
 
-// 16 staged tokens, of which the first `tokens` are written, to rows row0 on.
-template <bool kGated, class T>
-__device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long long row0,
-                                         int tokens, int feat0, int tid,
-                                         const FfnTile<kGated>& s) {
+// A thread's part of 16 staged tokens: token tid / 16 and eight further, features
+// 4 (tid % 16) on and, not gated, 64 further.  All of it is there (FfnTile::whole, 16
+// tokens), so the loads and the arithmetic of all values run side by side.  The residual
+// is asked for before the barrier that the staged values wait at.
+template <bool kGated, int kAct, class T>
+__device__ __forceinline__ void ffn_rows_whole(const FfnOut& o, uint32_t stage, uint32_t bar,
+                                               int quarter, const float (&acc)[16],
+                                               long long row0, int feat0, int tid,
+                                               const FfnTile<kGated>& s) {
   const int f = feat0 + (tid & 15) * 4;
+  const long long row = row0 + (tid >> 4);
+  uint2 res[2][2];
+  const bool add = !kGated && o.residual != nullptr;
+  if constexpr (!kGated) {
+    const T* r = static_cast<const T*>(o.residual) + row * o.ldr + f;
 #pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        res[j][h] = add ? *reinterpret_cast<const uint2*>(r + j * 8 * o.ldr + h * 64)
+                        : make_uint2(0, 0);
+  }
+  stage_put(stage, quarter, acc);
+  named_bar_sync(bar, 128);
+  const uint32_t at = stage + (uint32_t)(tid >> 4) * 512u + (uint32_t)(tid & 15) * 16u;
+  float v[2][2][4];
+#pragma unroll
+  for (int j = 0; j < 2; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      ld_shared_v4_f32(at + j * 8u * 512u + h * 256u, v[j][h][0], v[j][h][1], v[j][h][2],
+                       v[j][h][3]);
+  T* out = static_cast<T*>(o.out) + row * o.ldo + f;
+  if constexpr (!kGated) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[j][h][i] += s.bias[h * 4 + i];
+  }
+  if (o.z != nullptr) {
+    float* z = o.z + row * o.ldz + f;
+    const long long second = kGated ? o.z_half : 64;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float(&w)[4] = v[j][h];
+        *reinterpret_cast<float4*>(z + j * 8 * o.ldz + h * second) =
+            make_float4(w[0], w[1], w[2], w[3]);
+      }
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    activate<kAct>(v[j][0]);
+    if constexpr (!kGated) activate<kAct>(v[j][1]);
+  }
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    T* to = out + j * 8 * o.ldo;
+    if constexpr (kGated) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[j][0][i] *= v[j][1][i];
+      store_four(to, 4, true, v[j][0]);
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float(&w)[4] = v[j][h];
+        w[0] += widen<T>((uint16_t)res[j][h].x);
+        w[1] += widen<T>((uint16_t)(res[j][h].x >> 16));
+        w[2] += widen<T>((uint16_t)res[j][h].y);
+        w[3] += widen<T>((uint16_t)(res[j][h].y >> 16));
+        store_four(to + h * 64, 4, true, w);
+      }
+    }
+  }
+  named_bar_sync(bar, 128);
+}
+
+// The same where features or tokens (of which `tokens` are there) end, or rows lie on
+// odd addresses.
+template <bool kGated, int kAct, class T>
+__device__ __forceinline__ void ffn_rows_ragged(const FfnOut& o, uint32_t stage, long long row0,
+                                                int tokens, int feat0, int tid,
+                                                const FfnTile<kGated>& s) {
+  const int f = feat0 + (tid & 15) * 4;
+#pragma unroll 1
   for (int j = 0; j < 2; ++j) {
     const int t = (tid >> 4) + 8 * j;
     if (t >= tokens) break;
@@ -129,12 +214,12 @@ __device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long l
     ld_shared_v4_f32(at + 256u, b[0], b[1], b[2], b[3]);
     if constexpr (kGated) {
       const int n = o.feat - f;
-      if (n <= 0) continue;
+      if (n <= 0) break;
       if (o.z != nullptr) {
         store_z(o.z + row * o.ldz + f, n, a);
         store_z(o.z + o.z_half + row * o.ldz + f, n, b);
       }
-      activate(o.act, a);
+      activate<kAct>(a);
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] *= b[i];
       store_four(out, n, o.vec_out, a);
@@ -143,7 +228,7 @@ __device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long l
       for (int h = 0; h < 2; ++h) {
         float(&v)[4] = h ? b : a;
         const int n = o.feat - f - h * 64;
-        if (n <= 0) continue;
+        if (n <= 0) break;
         float r[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (o.residual != nullptr)
           load_four<T>(static_cast<const T*>(o.residual) + row * o.ldr + f + h * 64, n, o.vec_res,
@@ -151,11 +236,9 @@ __device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long l
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] += s.bias[h * 4 + i];
         if (o.z != nullptr) store_z(o.z + row * o.ldz + f + h * 64, n, v);
-        activate(o.act, v);
-        if (o.residual != nullptr) {
+        activate<kAct>(v);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) v[i] += r[i];
-        }
+        for (int i = 0; i < 4; ++i) v[i] += r[i];
         store_four(out + h * 64, n, o.vec_out, v);
       }
     }
@@ -163,15 +246,19 @@ __device__ __forceinline__ void ffn_rows(const FfnOut& o, uint32_t stage, long l
 }
 
 // A group of four warps: `v` staged, finished and the staging free again.
-template <bool kGated, class T>
+template <bool kGated, int kAct, class T>
 __device__ __forceinline__ void ffn_finish(const FfnOut& o, uint32_t stage, uint32_t bar,
                                            int quarter, const float (&v)[16], long long row0,
                                            int tokens, int feat0, int tid,
                                            const FfnTile<kGated>& s) {
-  stage_put(stage, quarter, v);
-  named_bar_sync(bar, 128);
-  ffn_rows<kGated, T>(o, stage, row0, tokens, feat0, tid, s);
-  named_bar_sync(bar, 128);
+  if (s.whole && tokens >= kStageTokens) {
+    ffn_rows_whole<kGated, kAct, T>(o, stage, bar, quarter, v, row0, feat0, tid, s);
+  } else {
+    stage_put(stage, quarter, v);
+    named_bar_sync(bar, 128);
+    ffn_rows_ragged<kGated, kAct, T>(o, stage, row0, tokens, feat0, tid, s);
+    named_bar_sync(bar, 128);
+  }
 }
 
 }  // namespace b200

@@ -17,6 +17,11 @@
 // shared memory (ffn_epilogue.cuh).  dA takes both weights in one contraction of
 // 2N, so the sum over the halves is made in TMEM.
 //
+// Tiles that would leave pairs idle in a last wave are divided along the contraction
+// into equal ranges, one per pair, and come first, so that joining them hides behind
+// the others' products.  Whichever CTA arrives last adds the parts up in their order:
+// the sums do not depend on which one it was, and nobody waits for another.
+//
 // Eight epilogue warps, two groups of four: a group takes every other 16 tokens of
 // a tile, so one group's staging barriers overlap the other's arithmetic.
 #pragma once
@@ -34,7 +39,10 @@ struct FfnArgs {
   int cols;    // dW: extent of the MMA's N axis, K
   int halves;  // dA, dW: 1 or 2
   int group;   // raster band
+  int tile_n;  // tokens (dW: columns) of a tile, at the most
   FfnOut o;    // dW: out where TMA cannot write it (contiguous), else null
+  float* slots;          // [CTA][2][256][128] partial sums, or null: no tile is divided
+  unsigned int* counts;  // [pair][16], zero between launches
   const CUtensorMap* maps;  // dW with offsets: dz's and A's map of each expert
   int* status;
   unsigned long long timeout_ns;
@@ -107,13 +115,27 @@ struct FfnUnit {
   int mma_n;
 };
 
-// Units in order; the expert of the last one found is remembered.
+// What a pair does of a unit: contraction blocks [kb0, kb1).
+struct FfnSegment : FfnUnit {
+  int kb0, kb1;
+  int c0, c1;  // the first and last pair with a part of it
+  __device__ __forceinline__ bool whole() const { return kb0 == 0 && kb1 == blocks; }
+};
+
+// A pair's parts of the divided units, then its whole ones.  The expert of the last
+// unit found is remembered, so a walk over increasing units costs one pass over the table.
 template <int kMode>
 struct FfnWalk {
+  static constexpr int kLeastBlocks = 8;  // of a part
+  static constexpr int kJoinBlocks = 12;
   const int* off;
   const int* tiles;
   int tf, tc;  // feature tiles; dW: column tiles
   int e;
+  int next_unit, pairs, undivided;  // units [0, undivided) are dealt whole
+  int blocks;                       // of a divided unit
+  long long items, pos, hi;
+  int ranges;
   __device__ __forceinline__ void init(const FfnArgs& a, const int* s_off, const int* s_tiles) {
     constexpr int kFeat = FfnCfg<kMode>::kFeat;
     off = s_off;
@@ -121,40 +143,82 @@ struct FfnWalk {
     tf = (a.feat + kFeat - 1) / kFeat;
     tc = (a.cols + 255) / 256;
     e = 0;
+    const int total = kMode == kFfnDW ? a.experts * a.halves * tf * tc : tiles[a.experts] * tf;
+    const int pair = blockIdx.x >> 1;
+    pairs = gridDim.x >> 1;
+    next_unit = pair;
+    undivided = total;
+    pos = hi = 0;
+    ranges = 0;
+    if (a.slots == nullptr) return;
+    const int rest = total % pairs;
+    blocks = ((kMode == kFfnDW ? a.rows : a.red) + kSlabK - 1) / kSlabK *
+             (kMode == kFfnDA ? a.halves : 1);
+    items = (long long)rest * blocks;
+    ranges = (int)min(items / kLeastBlocks, (long long)pairs);
+    undivided = total - rest;
+    // Joining costs, in contraction blocks, what the parts' way through L2 takes (there
+    // are about ranges + rest of them): dividing has to save more, and whole tiles must
+    // follow that hide it.  Measured, us, divided / not: 28672 x 4096 gated, 96 rows (38
+    // tiles left of 112) 48 / 51, 384 rows (2 of 224) 79 / 87; 8192 x 8192, 1024 rows (54 of
+    // 128, not divided by this) 105 / 100, 2048 rows (34 of 256) 189 / 193.
+    const long long join = kJoinBlocks + (ranges + rest) * a.tile_n / 896ll;
+    if (ranges == 0 || undivided == 0 || (items + ranges - 1) / ranges + join >= blocks) {
+      ranges = 0;
+      undivided = total;
+      return;
+    }
+    if (pair < ranges) sk_range(pair, items, ranges, &pos, &hi);
   }
-  __device__ __forceinline__ int total(const FfnArgs& a) const {
-    return kMode == kFfnDW ? a.experts * a.halves * tf * tc : tiles[a.experts] * tf;
-  }
-  __device__ __forceinline__ FfnUnit unit(const FfnArgs& a, int u) {
-    FfnUnit r;
+
+  __device__ __forceinline__ void unit(const FfnArgs& a, int u, FfnUnit* r) {
     int x, y;
     if constexpr (kMode == kFfnDW) {
       const int per = a.halves * tf * tc;
-      r.e = u / per;
-      tile_coord(u - r.e * per, a.halves * tf, tc, a.group, &x, &y);
-      r.half = x >= tf;
-      r.row0 = off[r.e];
-      r.rows = off[r.e + 1] - r.row0;
-      r.feat0 = (x - r.half * tf) * 256;
-      r.col0 = y * 256;
-      r.blocks = (r.rows + kSlabK - 1) / kSlabK;
-      r.mma_n = 256;
+      r->e = u / per;
+      tile_coord(u - r->e * per, a.halves * tf, tc, a.group, &x, &y);
+      r->half = x >= tf;
+      r->row0 = off[r->e];
+      r->rows = off[r->e + 1] - r->row0;
+      r->feat0 = (x - r->half * tf) * 256;
+      r->col0 = y * 256;
+      r->blocks = (r->rows + kSlabK - 1) / kSlabK;
+      r->mma_n = 256;
     } else {
       while (u >= tiles[e + 1] * tf) ++e;
-      r.e = e;
-      r.half = 0;
+      r->e = e;
+      r->half = 0;
       const int first = off[e], count = off[e + 1] - first;
       const int tt = tiles[e + 1] - tiles[e];
       const int size = ((count + tt - 1) / tt + 31) & ~31;
       tile_coord(u - tiles[e] * tf, tt, tf, a.group, &x, &y);
-      r.row0 = first + x * size;
-      r.rows = min(size, count - x * size);
-      r.feat0 = y * FfnCfg<kMode>::kFeat;
-      r.col0 = 0;
-      r.blocks = (a.red + kSlabK - 1) / kSlabK * (kMode == kFfnDA ? a.halves : 1);
-      r.mma_n = (r.rows + 31) & ~31;
+      r->row0 = first + x * size;
+      r->rows = min(size, count - x * size);
+      r->feat0 = y * FfnCfg<kMode>::kFeat;
+      r->col0 = 0;
+      r->blocks = (a.red + kSlabK - 1) / kSlabK * (kMode == kFfnDA ? a.halves : 1);
+      r->mma_n = (r->rows + 31) & ~31;
     }
-    return r;
+  }
+  __device__ __forceinline__ bool next(const FfnArgs& a, FfnSegment* s) {
+    if (pos < hi) {
+      const int v = (int)(pos / blocks);
+      const long long first = (long long)v * blocks;
+      unit(a, undivided + v, s);
+      s->kb0 = (int)(pos - first);
+      s->kb1 = (int)min((long long)blocks, hi - first);
+      s->c0 = sk_owner(first, items, ranges);
+      s->c1 = sk_owner(first + blocks - 1, items, ranges);
+      pos = first + s->kb1;
+      if (pos >= hi) e = 0;  // (the whole units come before these)
+      return true;
+    }
+    if (next_unit >= undivided) return false;
+    unit(a, next_unit, s);
+    next_unit += pairs;
+    s->kb0 = 0;
+    s->kb1 = s->blocks;
+    return true;
   }
 };
 
@@ -162,12 +226,14 @@ struct FfnWalk {
 // 64 x 128 (w1 unused); dA: box 64 x 64, w1 the second half's.  dW: dz (n, r, half)
 // and A (k, r), boxes 64 x 64, without offsets.
 // tmap_t: the token operand (gated, act A, dA dz: columns, rows, half), box 64 x 128;
+// tmap_h: the same with box 64 x 64 (unused in dW);
 // tmap_s: the same with box 64 x 16; dW: dW (k, n, half * experts + e), box 64 x 32.
 template <int kMode, bool kMany, class T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(FfnCfg<kMode>::kThreads, 1)
 ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                 const __grid_constant__ CUtensorMap tmap_w1,
                 const __grid_constant__ CUtensorMap tmap_t,
+                const __grid_constant__ CUtensorMap tmap_h,
                 const __grid_constant__ CUtensorMap tmap_s, const FfnArgs args) {
   using C = FfnCfg<kMode, kMany>;
   constexpr int kStages = C::kStages;
@@ -182,13 +248,12 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   __shared__ alignas(8) uint64_t bar_drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
+  __shared__ uint32_t last_word[2];
 
   cluster_arrive_started();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
-  const int pair = blockIdx.x >> 1;
-  const int npairs = gridDim.x >> 1;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t store_base = smem_base + kStages * C::kStageBytes;
   int* s_off = reinterpret_cast<int*>(smem_raw + (store_base + C::kStaging - smem_u32(smem_raw)));
@@ -208,7 +273,10 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     fence_mbar_init_cluster();
     prefetch_tmap(&tmap_w0);
     prefetch_tmap(&tmap_w1);
-    if (kMode != kFfnDW) prefetch_tmap(&tmap_t);
+    if (kMode != kFfnDW) {
+      prefetch_tmap(&tmap_t);
+      prefetch_tmap(&tmap_h);
+    }
     prefetch_tmap(&tmap_s);
   }
   __syncwarp();
@@ -231,7 +299,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
 
   FfnWalk<kMode> walk;
   walk.init(args, s_off, s_tiles);
-  const int total = walk.total(args);
+  FfnSegment w;
   if (warp == 0) {
     // ------------------------------------------------------------ producer
     if (elect_one()) {
@@ -241,31 +309,36 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       uint32_t stage = 0, phase = 0, filled = 0;
       int last_e = -1;
       bool ok = true;
-      for (int u = pair; ok && u < total; u += npairs) {
-        const FfnUnit w = walk.unit(args, u);
+      while (ok && walk.next(args, &w)) {
         const int f0 = w.feat0 + (int)rank * (C::kFeat / 2);
         const int half = w.mma_n / 2;
         const int t0 = kMode == kFfnDW ? w.col0 + (int)rank * 128 : w.row0 + (int)rank * half;
-        const uint32_t bytes = C::kOperand + (half == 128 ? C::kOperand : half * 128);
+        // Few large boxes: past the tile's rows they bring the next ones, or zeros.
+        const int box = half > 64 ? 128 : half > 32 ? 64 : 16;
+        const uint32_t bytes = C::kOperand + (box == 16 ? half : box) * 128;
         const int per_half = kMode == kFfnDA && args.halves == 2 ? w.blocks / 2 : w.blocks;
         const CUtensorMap *dz = &tmap_w0, *a = &tmap_w1;
         if constexpr (kMode == kFfnDW) {
           if (args.maps != nullptr) {
             // A new expert's maps are fetched a unit ahead of their use.
-            for (int v = u; v < total && v <= u + npairs; v += npairs) {
-              const int e = v == u ? w.e : walk.unit(args, v).e;
-              if (e <= last_e) continue;
-              tmap_acquire(args.maps + 2 * e);
-              tmap_acquire(args.maps + 2 * e + 1);
-              prefetch_tmap(args.maps + 2 * e);
-              prefetch_tmap(args.maps + 2 * e + 1);
-              last_e = e;
+            for (int i = 0; i < 2; ++i) {
+              FfnUnit v = w;
+              if (i == 1) {
+                if (walk.next_unit >= walk.undivided) break;
+                walk.unit(args, walk.next_unit, &v);
+              }
+              if (v.e <= last_e) continue;
+              tmap_acquire(args.maps + 2 * v.e);
+              tmap_acquire(args.maps + 2 * v.e + 1);
+              prefetch_tmap(args.maps + 2 * v.e);
+              prefetch_tmap(args.maps + 2 * v.e + 1);
+              last_e = v.e;
             }
             dz = args.maps + 2 * w.e;
             a = dz + 1;
           }
         }
-        for (int kb = 0; kb < w.blocks; ++kb) {
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
             ok = false;
             break;
@@ -294,8 +367,10 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           if constexpr (kMode == kFfnDW) {
             tma_load_2d_pair_hint(sb, a, t0, w.row0 + k0, fb, keep);
             tma_load_2d_pair_hint(sb + C::kOperand / 2, a, t0 + 64, w.row0 + k0, fb, keep);
-          } else if (half == 128) {
+          } else if (box == 128) {
             tma_load_3d_pair_hint(sb, &tmap_t, k0, t0, second, fb, keep);
+          } else if (box == 64) {
+            tma_load_3d_pair_hint(sb, &tmap_h, k0, t0, second, fb, keep);
           } else {
             for (int r = 0; r < half; r += 16)
               tma_load_3d_pair_hint(sb + r * 128, &tmap_s, k0, t0 + r, second, fb, keep);
@@ -316,8 +391,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       uint32_t stage = 0, phase = 0;
       int it = 0;
       bool ok = true;
-      for (int u = pair; ok && u < total; u += npairs) {
-        const FfnUnit w = walk.unit(args, u);
+      while (ok && walk.next(args, &w)) {
         if (w.blocks == 0) continue;
         const int red = kMode == kFfnDW ? w.rows : args.red;
         const int per_half = kMode == kFfnDA && args.halves == 2 ? w.blocks / 2 : w.blocks;
@@ -328,7 +402,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + buf * 256;
-        for (int kb = 0; kb < w.blocks; ++kb) {
+        for (int kb = w.kb0; kb < w.kb1; ++kb) {
           if (!wait_ready(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitFull)) {
             ok = false;
             break;
@@ -347,7 +421,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
             if (k < steps)
               umma_bf16_pair(d_tmem, adesc + (kMnA ? 128ull : 2ull) * k,
                              bdesc + (kMnB ? 128ull : 2ull) * k, idesc,
-                             (kb != 0 || k != 0) ? 1u : 0u);
+                             (kb != w.kb0 || k != 0) ? 1u : 0u);
           }
           umma_commit_pair(empty_self + stage * 8u);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
@@ -374,8 +448,48 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     const uint32_t staging = store_base + (uint32_t)group * kFfnStageBytes;
     int it = 0;
     int ok = 1;
-    for (int u = pair; u < total; u += npairs) {
-      const FfnUnit w = walk.unit(args, u);
+    const int cta = blockIdx.x;
+    // What the groups of all the CTAs with a part of a divided tile count in at: true
+    // for the last, who takes the sum.
+    auto joined = [&]() {
+      named_bar_sync(1 + group, 128);
+      if (tid == 0) {
+        unsigned int* count = args.counts + w.c0 * 16 + (int)rank * 2 + group;
+        const bool last = atomic_add_acq_rel(count, 1u) == (unsigned int)(w.c1 - w.c0);
+        if (last) atomicExch(count, 0u);
+        last_word[group] = last;
+      }
+      named_bar_sync(1 + group, 128);
+      return last_word[group] != 0;
+    };
+    // Column `col` of this lane's accumulator row in the slot of pair c: a pair begins at
+    // most one divided tile (slot 1) and ends or crosses at most one that an
+    // earlier pair began (slot 0).
+    auto slot = [&](int c, int col) {
+      return args.slots + (((long long)(2 * c + (int)rank) * 2 + (c == w.c0 ? 1 : 0)) * 256 + col) *
+                              128 + quarter * 32 + lane;
+    };
+    // acc = the parts' sum, `kN` columns from col on, 64 loads in flight, added in order.
+    auto add_parts = [&](int col, auto& acc) {
+      constexpr int kN = sizeof(acc) / sizeof(float), kParts = 64 / kN;
+#pragma unroll
+      for (int j = 0; j < kN; ++j) acc[j] = 0.0f;
+#pragma unroll 1
+      for (int c = w.c0; c <= w.c1; c += kParts) {
+        float v[kParts][kN];
+#pragma unroll
+        for (int i = 0; i < kParts; ++i) {
+          const float* from = slot(c + i <= w.c1 ? c + i : c, col);
+#pragma unroll
+          for (int j = 0; j < kN; ++j) v[i][j] = c + i <= w.c1 ? __ldcg(from + j * 128) : 0.0f;
+        }
+#pragma unroll
+        for (int i = 0; i < kParts; ++i)
+#pragma unroll
+          for (int j = 0; j < kN; ++j) acc[j] += v[i][j];
+      }
+    };
+    while (walk.next(args, &w)) {
       const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
       const bool any = w.blocks != 0;
       if (any) {
@@ -388,37 +502,61 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         tc_fence_after_sync();
       }
       const uint32_t tbase = tmem_base + buf * 256 + ((uint32_t)(quarter * 32) << 16);
+      const bool whole = w.whole();
       if constexpr (kMode == kFfnDW) {
-        if (!ok) break;
         // Lane = n, 64 columns of k at a time through a swizzled 32 x 64 box.
         const int f0 = w.feat0 + (int)rank * kCtaM + quarter * 32;
-#pragma unroll 1
-        for (int c = 2 * group; c < 2 * group + 2; ++c) {
-          uint32_t v0[32], v1[32];
+        auto load = [&](int c, int h, uint32_t (&v)[32]) {
           if (any) {
-            tmem_ld_32x32b_x32(tbase + c * kStoreCols, v0);
-            tmem_ld_32x32b_x32(tbase + c * kStoreCols + 32, v1);
+            tmem_ld_32x32b_x32(tbase + c * kStoreCols + 32 * h, v);
             tmem_wait_ld();
-            if (c & 1) {
+            if ((c & 1) && h) {
               tc_fence_before_sync();
               __syncwarp();
               if (lane == 0) mbar_arrive_cluster(acc_empty_leader + buf * 8u);
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v0[j] = v1[j] = 0;
+            for (int j = 0; j < 32; ++j) v[j] = 0;
+          }
+        };
+        if (!whole) {
+#pragma unroll 1
+          for (int c = 4 * group; c < 4 * group + 4; ++c) {
+            uint32_t v[32];
+            load(c >> 1, c & 1, v);
+            float* to = slot(cta >> 1, c * 32);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) __stcg(to + j * 128, __uint_as_float(v[j]));
+          }
+          if (!joined()) continue;
+        }
+        if (!ok) continue;
+#pragma unroll 1
+        for (int c = 2 * group; c < 2 * group + 2; ++c) {
+          uint32_t p[2][16];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (whole) {
+              uint32_t v[32];
+              load(c, h, v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j)
+                p[h][j] = pack_pair<T>(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+            } else {
+              float v[32];
+              add_parts(c * kStoreCols + 32 * h, v);
+#pragma unroll
+              for (int j = 0; j < 16; ++j) p[h][j] = pack_pair<T>(v[2 * j], v[2 * j + 1]);
+            }
           }
           if (lane == 0) bulk_wait_group_read<0>();  // the store before has read the box
           __syncwarp();
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const uint32_t* v = j < 4 ? v0 + 8 * j : v1 + 8 * (j - 4);
-            uint32_t p[4];
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              p[q] = pack_pair<T>(__uint_as_float(v[2 * q]), __uint_as_float(v[2 * q + 1]));
-            st_shared_v4(box + lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), p[0], p[1], p[2],
-                         p[3]);
+            const uint32_t* q = p[j >> 2] + 4 * (j & 3);
+            st_shared_v4(box + lane * 128u + ((uint32_t)(j ^ (lane & 7)) << 4), q[0], q[1], q[2],
+                         q[3]);
           }
           const int z = w.half * args.experts + w.e;
           if (out == nullptr) {
@@ -453,27 +591,46 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         const int f0 = w.feat0 + (int)rank * (C::kFeat / 2);
         FfnTile<kGated> tile;
         ffn_tile<kGated, T>(args.o, f0, tid, tile);
-#pragma unroll 1
-        for (int c = group * kStageTokens; c < w.mma_n; c += 2 * kStageTokens) {
-          float acc[kStageTokens];
-          if (any) {
-            uint32_t v[16];
-            tmem_ld_32x32b_x16(tbase + c, v);
-            tmem_wait_ld();
-            if (c + 2 * kStageTokens >= w.mma_n) {
-              tc_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(acc_empty_leader + buf * 8u);
-            }
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[j] = __uint_as_float(v[j]);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
+        auto load = [&](int c, float (&acc)[kStageTokens]) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(tbase + c, v);
+          tmem_wait_ld();
+          if (c + 2 * kStageTokens >= w.mma_n) {
+            tc_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(acc_empty_leader + buf * 8u);
           }
-          ffn_finish<kGated, T>(args.o, staging, 1 + group, quarter, acc, w.row0 + c,
-                                ok ? w.rows - c : 0, f0, tid, tile);
+#pragma unroll
+          for (int j = 0; j < 16; ++j) acc[j] = __uint_as_float(v[j]);
+        };
+        if (!whole) {
+#pragma unroll 1
+          for (int c = group * kStageTokens; c < w.mma_n; c += 2 * kStageTokens) {
+            float acc[kStageTokens];
+            load(c, acc);
+            float* to = slot(cta >> 1, c);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) __stcg(to + j * 128, acc[j]);
+          }
+          if (!joined()) continue;
         }
+        auto finish = [&](auto code) {
+          constexpr int kAct = decltype(code)::value;
+#pragma unroll 1
+          for (int c = group * kStageTokens; c < w.mma_n; c += 2 * kStageTokens) {
+            float acc[kStageTokens];
+            if (whole)
+              load(c, acc);
+            else
+              add_parts(c, acc);
+            ffn_finish<kGated, kAct, T>(args.o, staging, 1 + group, quarter, acc, w.row0 + c,
+                                        ok ? w.rows - c : 0, f0, tid, tile);
+          }
+        };
+        if constexpr (kMode == kFfnDA)
+          finish(ActCode<B200_ACT_NONE>());
+        else
+          with_act(args.o.act, finish);
       }
     }
     if (kMode == kFfnDW && lane == 0) bulk_wait_group_read<0>();

@@ -27,7 +27,6 @@ struct FfnGradArgs {
   int experts, rows, feat;
   int strips;      // blocks along a row; the rest of the grid goes over the rows
   int block_rows;
-  int act;
 };
 
 __device__ __forceinline__ void load_eight(const float* p, int n, float (&v)[8]) {
@@ -72,7 +71,7 @@ __device__ __forceinline__ void store_eight(T* p, int n, const float (&v)[8]) {
 }
 
 // dout, z and dz have rows on 16 bytes.
-template <bool kGated, class T>
+template <bool kGated, int kAct, class T>
 __global__ void __launch_bounds__(256)
 ffn_grad_kernel(const FfnGradArgs a) {
   __shared__ float sums[kGated ? 1 : 8][256];
@@ -101,7 +100,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
         float u[8], g[8], slope[8];
         load_eight(a.z + r * a.ldz + f, n, z);
         load_eight(a.z + a.z_half + r * a.ldz + f, n, u);
-        activate_slope(a.act, z, g, slope);
+        activate_slope<kAct>(z, g, slope);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           slope[i] = d[i] * u[i] * slope[i];
@@ -111,10 +110,10 @@ ffn_grad_kernel(const FfnGradArgs a) {
         store_eight(to, n, slope);
         store_eight(to + a.dz_half, n, g);
       } else {
-        if (a.act != B200_ACT_NONE) {
+        if constexpr (kAct != B200_ACT_NONE) {
           float y[8], slope[8];
           load_eight(a.z + r * a.ldz + f, n, z);
-          activate_slope(a.act, z, y, slope);
+          activate_slope<kAct>(z, y, slope);
 #pragma unroll
           for (int i = 0; i < 8; ++i) d[i] *= slope[i];
         }
@@ -154,7 +153,7 @@ ffn_bias_kernel(const float* __restrict__ partial, int blocks, int feat, T* __re
 }
 
 // C = act(bias) + residual, and z = bias: a product with an empty contraction.
-template <class T>
+template <int kAct, class T>
 __global__ void __launch_bounds__(256)
 ffn_empty_kernel(const FfnOut o, int rows) {
   grid_wait();
@@ -166,7 +165,7 @@ ffn_empty_kernel(const FfnOut o, int rows) {
     float v[1] = {o.bias != nullptr
                       ? widen<T>(static_cast<const uint16_t*>(o.bias)[f]) : 0.0f};
     if (o.z != nullptr) o.z[r * o.ldz + f] = v[0];
-    activate(o.act, v);
+    activate<kAct>(v);
     if (o.residual != nullptr)
       v[0] += widen<T>(static_cast<const uint16_t*>(o.residual)[r * o.ldr + f]);
     static_cast<T*>(o.out)[r * o.ldo + f] = round_one<T>(v[0]);

@@ -189,9 +189,8 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                lane;
       };
       FfnTile<kGated> tile;
-      if (whole) ffn_tile<kGated, T>(o, f0, tid, tile);
-#pragma unroll 1
-      for (int c = 0; c < s.rows; c += kStageTokens) {
+      ffn_tile<kGated, T>(o, f0, tid, tile);
+      auto load = [&](int c, float (&acc)[kStageTokens]) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tbase + c, v);
         tmem_wait_ld();
@@ -200,53 +199,60 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           __syncwarp();
           if (lane == 0) mbar_arrive_local(smem_u32(&bar_acc_empty[buf]));
         }
-        float acc[kStageTokens];
 #pragma unroll
         for (int j = 0; j < 16; ++j) acc[j] = __uint_as_float(v[j]);
-        if (whole) {
-          ffn_finish<kGated, T>(o, staging, 1, quarter, acc, s.row0 + c, ok ? s.rows - c : 0, f0,
-                                tid, tile);
-        } else {
-          float* mine = slot(blockIdx.x) + c * 128;
+      };
+      if (!whole) {
+        float* mine = slot(blockIdx.x);
+#pragma unroll 1
+        for (int c = 0; c < s.rows; c += kStageTokens) {
+          float acc[kStageTokens];
+          load(c, acc);
 #pragma unroll
           for (int j = 0; j < 16; ++j)
-            if (c + j < s.rows) __stcg(mine + j * 128, acc[j]);
+            if (c + j < s.rows) __stcg(mine + (c + j) * 128, acc[j]);
         }
+        named_bar_sync(1, 128);
+        if (tid == 0) {
+          const bool last =
+              atomic_add_acq_rel(args.counts + c0 * 16, 1u) == (unsigned int)(c1 - c0);
+          if (last) atomicExch(args.counts + c0 * 16, 0u);
+          last_word = last;
+        }
+        named_bar_sync(1, 128);
+        if (last_word == 0) continue;
       }
-      if (whole) continue;
-      named_bar_sync(1, 128);
-      if (tid == 0) {
-        const bool last = atomic_add_acq_rel(args.counts + c0 * 16, 1u) == (unsigned int)(c1 - c0);
-        if (last) atomicExch(args.counts + c0 * 16, 0u);
-        last_word = last;
-      }
-      named_bar_sync(1, 128);
-      if (last_word == 0) continue;
-      ffn_tile<kGated, T>(o, f0, tid, tile);
+      with_act(o.act, [&](auto code) {
+        constexpr int kAct = decltype(code)::value;
 #pragma unroll 1
-      for (int c = 0; c < s.rows; c += kStageTokens) {
-        float acc[kStageTokens];
+        for (int c = 0; c < s.rows; c += kStageTokens) {
+          float acc[kStageTokens];
+          if (whole) {
+            load(c, acc);
+          } else {
+            // Four parts' loads in flight at a time, added in order.
 #pragma unroll
-        for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
-        // Four parts' loads in flight at a time, added in order.
+            for (int j = 0; j < 16; ++j) acc[j] = 0.0f;
 #pragma unroll 1
-        for (int p = c0; p <= c1; p += 4) {
-          float v[4][16];
+            for (int p = c0; p <= c1; p += 4) {
+              float v[4][16];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float* from = slot(p + i <= c1 ? p + i : c1) + c * 128;
+              for (int i = 0; i < 4; ++i) {
+                const float* from = slot(p + i <= c1 ? p + i : c1) + c * 128;
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              v[i][j] = c + j < s.rows && p + i <= c1 ? __ldcg(from + j * 128) : 0.0f;
+                for (int j = 0; j < 16; ++j)
+                  v[i][j] = c + j < s.rows && p + i <= c1 ? __ldcg(from + j * 128) : 0.0f;
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) acc[j] += v[i][j];
+            }
           }
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) acc[j] += v[i][j];
+          ffn_finish<kGated, kAct, T>(o, staging, 1, quarter, acc, s.row0 + c,
+                                      ok ? s.rows - c : 0, f0, tid, tile);
         }
-        ffn_finish<kGated, T>(o, staging, 1, quarter, acc, s.row0 + c, ok ? s.rows - c : 0, f0,
-                              tid, tile);
-      }
+      });
     }
     __syncwarp();
   }

@@ -110,21 +110,31 @@ inline int zero_rows(void* p, int ld, int width, int rows, cudaStream_t stream) 
 // the end of the one before it (every kernel launched so waits, grid_wait,
 // before it touches global memory).
 template <class... P, class... A>
-int launch(void (*fn)(P...), int blocks, int threads, size_t smem, cudaStream_t stream,
-           A&&... args) {
+int launch_clusters(void (*fn)(P...), int blocks, int cluster, int threads, size_t smem,
+                    cudaStream_t stream, A&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)blocks);
   cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = cluster > 0 ? 2 : 1;
   if (cudaLaunchKernelEx(&cfg, fn, static_cast<P>(args)...) == cudaSuccess) return B200_OK;
   cudaGetLastError();
   return B200_ERR_LAUNCH;
+}
+
+// (clusters as the kernel itself says)
+template <class... P, class... A>
+int launch(void (*fn)(P...), int blocks, int threads, size_t smem, cudaStream_t stream,
+           A&&... args) {
+  return launch_clusters(fn, blocks, 0, threads, smem, stream, static_cast<A&&>(args)...);
 }
 
 }  // namespace b200

@@ -78,8 +78,9 @@ int b200_ffn_da(const void* dz, const void* W0, const void* W1, const int* offse
 int b200_ffn_dw(const void* dz, const void* A, const int* offsets, void* dW, int halves, int rows,
                 int experts, int N, int K, int lddz, int lda, int dtype, void* stream);
 
-/* Kernel for b200_ffn_act and b200_ffn_gated: 0 = chosen by sizes (default),
- * 1 = the streaming kernel (few rows), 2 = the pair kernel. */
+/* Kernel for b200_ffn_act, b200_ffn_gated and b200_ffn_da: 0 = chosen by sizes
+ * (default), 1 = the streaming kernel (few rows; b200_ffn_da has none), 2 = the pair
+ * kernel, 3 = the cluster kernel (one matrix, where its tiles fit the device; else pairs). */
 int b200_ffn_set_kernel(int kernel);
 
 /* ---- Norm of many gradients, clipping -----------------------------------------

@@ -90,7 +90,7 @@ def test_sizes(m, n, k, dtype, kernel):
     check(m, n, k, dtype)
 
 
-@pytest.mark.parametrize("kernel", ["stream", "pair"])
+@pytest.mark.parametrize("kernel", ["stream", "pair", "cluster"])
 @pytest.mark.parametrize("act", capi.ACTIVATIONS)
 def test_activations(act, kernel):
     capi.ffn_set_kernel(KERNELS[kernel])
@@ -100,7 +100,7 @@ def test_activations(act, kernel):
                 check(70, 136, 264, dtype, act, bias, residual)
 
 
-@pytest.mark.parametrize("kernel", ["stream", "pair"])
+@pytest.mark.parametrize("kernel", ["stream", "pair", "cluster"])
 @pytest.mark.parametrize("n,k", [(1, 1), (1, 64), (7, 9), (65, 33), (127, 515), (257, 100), (130, 6)])
 def test_odd_sizes(n, k, kernel):
     capi.ffn_set_kernel(KERNELS[kernel])
@@ -126,3 +126,14 @@ def test_bias_of_many_rows(m, n):
     check(m, n, 16, train=("b",))
     first = check(m, n, 16, train=("b",))[1]["b"]
     assert torch.equal(first, check(m, n, 16, train=("b",))[1]["b"])
+
+
+# few tiles with long contractions, divided over a cluster, in each of the three products
+@pytest.mark.parametrize("m,n,k", [(70, 136, 5000), (300, 520, 2056), (257, 3208, 1608),
+                                   (2000, 264, 136), (4100, 136, 72), (1, 256, 8192)])
+@pytest.mark.parametrize("kernel", [2, 3])
+def test_divided(m, n, k, kernel):
+    capi.ffn_set_kernel(kernel)
+    y, g = check(m, n, k)
+    y2, g2 = check(m, n, k)
+    assert torch.equal(y, y2) and all(torch.equal(g[v], g2[v]) for v in g)

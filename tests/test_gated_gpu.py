@@ -23,7 +23,7 @@ from blackwell_gemm_b200 import capi
 pytestmark = pytest.mark.gpu
 
 DT = {"bf16": (torch.bfloat16, 2.0 ** -8, 0.0), "fp16": (torch.float16, 2.0 ** -11, 2.0 ** -25)}
-KERNELS = {"chosen": 0, "stream": 1, "pair": 2}
+KERNELS = {"chosen": 0, "stream": 1, "pair": 2, "cluster": 3}
 E = 2.0 ** -24
 BEND = 1.13  # the largest slope of the activations, and of their slopes
 
@@ -138,7 +138,7 @@ def test_layouts(layout, dtype, kernel):
     check(*LAYOUTS[layout], 136, 200, dtype)
 
 
-@pytest.mark.parametrize("kernel", ["stream", "pair"])
+@pytest.mark.parametrize("kernel", ["stream", "pair", "cluster"])
 @pytest.mark.parametrize("act", capi.ACTIVATIONS)
 def test_activations(act, kernel):
     capi.ffn_set_kernel(KERNELS[kernel])
@@ -148,7 +148,7 @@ def test_activations(act, kernel):
 
 
 # odd widths: rows that TMA and vector stores cannot take
-@pytest.mark.parametrize("kernel", ["stream", "pair"])
+@pytest.mark.parametrize("kernel", ["stream", "pair", "cluster"])
 @pytest.mark.parametrize("n,k", [(1, 1), (1, 64), (7, 9), (65, 33), (127, 515), (257, 100), (130, 6)])
 def test_odd_sizes(n, k, kernel):
     capi.ffn_set_kernel(KERNELS[kernel])
@@ -160,3 +160,32 @@ def test_odd_sizes(n, k, kernel):
 def test_empty(rows, n, k):
     check(None, rows, n, k)
     check([0, 0, rows], rows, n, k)
+
+
+# few tiles with long contractions, divided over a cluster, in each of the three products
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("rows,n,k", [(70, 136, 5000), (300, 520, 2056), (257, 1601, 1608),
+                                      (2000, 264, 136), (4100, 136, 72), (1, 256, 8192)])
+@pytest.mark.parametrize("kernel", [2, 3])
+def test_divided(rows, n, k, dtype, kernel):
+    capi.ffn_set_kernel(kernel)
+    first = check(None, rows, n, k, dtype)
+    again = check(None, rows, n, k, dtype)
+    assert torch.equal(first[0], again[0])     # joined in one order
+    assert all(torch.equal(a, b) for a, b in zip(first[1], again[1]))
+
+
+@pytest.mark.parametrize("layout", list(LAYOUTS))
+def test_divided_layouts(layout):
+    capi.ffn_set_kernel(2)
+    check(*LAYOUTS[layout], 1608, 2056)
+
+
+# tiles left over after whole waves: their contractions divided over all pairs
+@pytest.mark.parametrize("rows,n,k", [(600, 3300, 1608), (1500, 1601, 1608), (7000, 1280, 2560)])
+def test_left_over(rows, n, k):
+    capi.ffn_set_kernel(2)
+    first = check(None, rows, n, k)
+    again = check(None, rows, n, k)
+    assert torch.equal(first[0], again[0])     # joined in one order
+    assert all(torch.equal(a, b) for a, b in zip(first[1], again[1]))
