@@ -401,16 +401,18 @@ void by_act(int act, F&& f) {
 // The streaming kernel spreads any number of tiles over the SMs, but takes 64 rows of an
 // expert at a time and joins divided tiles through L2.  One matrix: where no cluster
 // fits or is estimated slower (14336 x 4096 gated, 1 row: 41.0 us, pairs 45.3; 64 rows
-// 45.6 and 47.2, 96 rows 53.4 and 48.5).  A bank: up to 64 rows an expert on average, and
-// up to 256 where half of the pairs would have no tile (8 x 14336 x 4096 gated, 512 rows:
-// 297 us, pairs 330; 1024 rows 361 and 332; 4 x 744 x 6200, 400 rows: 29 and 36).
+// 45.6 and 47.2, 96 rows 53.4 and 48.5).  A bank: up to 64 rows an expert on average, 48
+// in short contractions, and up to 256 where half of the pairs would have no tile (8 x
+// 14336 x 4096 gated, 512 rows: 297 us, pairs 330; 1024 rows 361 and 332; 32 x 1032 x
+// 1032, 1024 rows 30.5 and 31.9, 2048 rows 34.8 and 33.4; 4 x 744 x 6200, 400 rows 29
+// and 36).
 template <bool kGated>
 bool use_stream(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
                 const FfnDevice& d) {
   const int k = g_kernel.load();
   if (k != 0) return k == 1;
   if (c.offsets != nullptr) {
-    if (c.rows <= 64ll * c.experts) return true;
+    if (c.rows <= (c.K >= 4096 ? 64ll : 48ll) * c.experts) return true;
     return c.rows <= 256ll * c.experts &&
            2 * c.experts * ceil_div(c.N, kGated ? 128 : 256) <= d.pairs[kFfnAct];
   }
@@ -444,8 +446,8 @@ int run_product(FfnCall& c, cudaStream_t stream) {
   if (c.experts == 0 || c.K == 0) {
     if (kGated) {  // act(0) * 0
       if (c.o.z != nullptr &&
-          cudaMemsetAsync(c.o.z, 0, (size_t)2 * c.rows * c.o.ldz * sizeof(float), stream) !=
-              cudaSuccess)
+          cudaMemset2DAsync(c.o.z, c.o.ldz * sizeof(float), 0, c.N * sizeof(float), 2ll * c.rows,
+                            stream) != cudaSuccess)
         return B200_ERR_LAUNCH;
       return zero_rows(c.o.out, (int)c.o.ldo, c.N, c.rows, stream);
     }

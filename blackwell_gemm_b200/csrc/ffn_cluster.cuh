@@ -123,7 +123,6 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   if (warp == 0) {
     if (elect_one()) {
       const uint32_t full_leader = cluster_map(smem_u32(&bar_full[0]), leader);
-      const uint32_t empty_peer = cluster_map(smem_u32(&bar_empty[0]), leader + (kPair ? 1 : 0));
       // (weights that another token tile reads as well stay)
       const uint64_t once = args.tiles_t > 1 ? l2_policy_evict_normal() : l2_policy_evict_first();
       const uint64_t keep = l2_policy_evict_last();
@@ -132,7 +131,6 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       uint32_t stage = 0, phase = 0, filled = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
         if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) break;
-        if (kPair && rank == 0 && filled >= stages) mbar_arrive_cluster(empty_peer + stage * 8u);
         ++filled;
         const uint32_t sa = smem_base + stage * stage_bytes, sb = sa + C::kWeight;
         const int second = kb >= per_half;  // dA: which weight
@@ -167,22 +165,20 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         }
         if (++stage == stages) { stage = 0; phase ^= 1u; }
       }
-      // Its copies have landed before the ring is written by others (the leader's
-      // barriers count both CTAs').
-      if (rank == 0) {
+      // Before the ring is written by others: its copies have landed (the leader's barriers
+      // count both CTAs'), and the leader's last arrivals on the other's barriers.
+      const uint32_t last = smem_u32(rank == 0 ? &bar_full[0] : &bar_empty[0]);
 #pragma unroll 1
-        for (uint32_t i = 0; i < stages && i < filled; ++i) {
-          if (stage == 0) { stage = stages; phase ^= 1u; }
-          --stage;
-          if (!wait_inline(smem_u32(&bar_full[stage]), phase, wctx, kErrWaitDrain, true)) break;
-        }
+      for (uint32_t i = 0; i < stages && i < filled; ++i) {
+        if (stage == 0) { stage = stages; phase ^= 1u; }
+        --stage;
+        if (!wait_inline(last + stage * 8u, phase, wctx, kErrWaitDrain, true)) break;
       }
     }
     __syncwarp();
   } else if (warp == 1) {
     if (rank == 0 && elect_one()) {
       const uint32_t idesc = make_idesc_16bit(kPair ? 256 : 128, mma_n, kFormat<T>, kMnA, false);
-      const uint32_t empty_self = cluster_map(smem_u32(&bar_empty[0]), leader);
       uint32_t stage = 0, phase = 0;
       bool ok = true;
       for (int kb = kb0; kb < kb1; ++kb) {
@@ -204,7 +200,7 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
             umma_bf16_1(tmem_base, a, b, idesc, add);
         }
         if constexpr (kPair)
-          umma_commit_pair(empty_self + stage * 8u);
+          umma_commit_both(smem_u32(&bar_empty[0]) + stage * 8u, (uint16_t)(3u << leader));
         else
           umma_commit_1(smem_u32(&bar_empty[stage]));
         if (++stage == stages) { stage = 0; phase ^= 1u; }

@@ -304,7 +304,6 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     // ------------------------------------------------------------ producer
     if (elect_one()) {
       const uint32_t full_leader = cluster_map(smem_u32(&bar_full[0]), 0);
-      const uint32_t empty_peer = cluster_map(smem_u32(&bar_empty[0]), 1);
       const uint64_t keep = l2_policy_evict_last();
       uint32_t stage = 0, phase = 0, filled = 0;
       int last_e = -1;
@@ -343,7 +342,6 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
             ok = false;
             break;
           }
-          if (rank == 0 && filled >= (uint32_t)kStages) mbar_arrive_cluster(empty_peer + stage * 8u);
           ++filled;
           const uint32_t fb = full_leader + stage * 8u;
           const uint32_t sa = smem_base + stage * C::kStageBytes;
@@ -378,14 +376,15 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
       }
-      // (the leader's barriers count both CTAs' copies)
-      if (rank == 0) drain_copies<kStages>(smem_u32(&bar_full[0]), stage, phase, filled, wctx);
+      // Before a CTA leaves: its copies have landed (the leader's barriers count both
+      // CTAs'), and the leader's last arrivals on the other's barriers.
+      drain_copies<kStages>(smem_u32(rank == 0 ? &bar_full[0] : &bar_empty[0]), stage, phase,
+                            filled, wctx);
     }
     __syncwarp();
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMA
     if (rank == 0 && elect_one()) {
-      const uint32_t empty_self = cluster_map(smem_u32(&bar_empty[0]), 0);
       const uint32_t accf_self = cluster_map(smem_u32(&bar_acc_full[0]), 0);
       const uint32_t accf_peer = cluster_map(smem_u32(&bar_acc_full[0]), 1);
       uint32_t stage = 0, phase = 0;
@@ -423,7 +422,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                              bdesc + (kMnB ? 128ull : 2ull) * k, idesc,
                              (kb != w.kb0 || k != 0) ? 1u : 0u);
           }
-          umma_commit_pair(empty_self + stage * 8u);
+          umma_commit_both(smem_u32(&bar_empty[0]) + stage * 8u, 3);
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;

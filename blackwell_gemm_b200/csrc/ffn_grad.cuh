@@ -92,7 +92,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
   }
   float total[8] = {};
   if (n > 0) {
-#pragma unroll 2
+#pragma unroll(kGated ? 2 : 4)
     for (int r = lo + part; r < hi; r += 8) {
       float d[8], z[8];
       load_eight<T>(static_cast<const T*>(a.dout) + r * a.ldd + f, n, d);

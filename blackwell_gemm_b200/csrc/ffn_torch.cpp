@@ -78,7 +78,8 @@ struct ActMatmul : torch::autograd::Function<ActMatmul> {
                                through && act != B200_ACT_NONE ? &z : nullptr);
     // What a gradient that nobody asks for would need is not kept.
     const bool keep_a = b.requires_grad(), keep_w = a.requires_grad();
-    ctx->save_for_backward({keep_a ? ra.t : at::Tensor(), keep_w ? rw.t : at::Tensor(), z});
+    // (detached: a view made here would answer for a weight changed meanwhile in its words)
+    ctx->save_for_backward({keep_a ? ra.t : at::Tensor(), keep_w ? rw.t.detach() : at::Tensor(), z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = bias.defined();
     ctx->saved_data["residual"] = residual.defined();
@@ -152,6 +153,8 @@ at::Tensor matmul_b200_act(const at::Tensor& A, const at::Tensor& B, const OptTe
   TORCH_CHECK(A.dim() == 2 && B.dim() == 2, kAct, ": A must be (M, K) and B (K, N)");
   const int act = act_code(activation, kAct);
   check_no_tangent({A, B}, kAct);
+  if (bias.defined()) check_no_tangent({bias}, kAct);
+  if (residual.defined()) check_no_tangent({residual}, kAct);
   check_16bit(A, kAct, "A");
   check_16bit(B, kAct, "B");
   check_same(B, A, kAct, "B");
@@ -161,13 +164,11 @@ at::Tensor matmul_b200_act(const at::Tensor& A, const at::Tensor& B, const OptTe
   check_sizes({m, n, A.size(1)}, kAct);
   bool any = A.requires_grad() || B.requires_grad();
   if (bias.defined()) {
-    check_no_tangent({bias}, kAct);
     check_same(bias, A, kAct, "bias");
     TORCH_CHECK(bias.dim() == 1 && bias.size(0) == n, kAct, ": bias must have shape (", n, ",)");
     any = any || bias.requires_grad();
   }
   if (residual.defined()) {
-    check_no_tangent({residual}, kAct);
     check_same(residual, A, kAct, "residual");
     TORCH_CHECK(residual.dim() == 2 && residual.size(0) == m && residual.size(1) == n, kAct,
                 ": residual must have shape (", m, ", ", n, ")");
@@ -209,8 +210,8 @@ struct GatedMatmul : torch::autograd::Function<GatedMatmul> {
     at::Tensor z;
     at::Tensor h = gated_forward(ra, g, u, offsets, (int)act, &z);
     const bool keep_a = gate.requires_grad() || up.requires_grad(), keep_w = a.requires_grad();
-    ctx->save_for_backward({keep_a ? ra.t : at::Tensor(), keep_w ? g.t : at::Tensor(),
-                            keep_w ? u.t : at::Tensor(), offsets, z});
+    ctx->save_for_backward({keep_a ? ra.t : at::Tensor(), keep_w ? g.t.detach() : at::Tensor(),
+                            keep_w ? u.t.detach() : at::Tensor(), offsets, z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["experts"] = g.t.size(0);
     ctx->saved_data["n"] = g.t.size(1);
@@ -310,65 +311,81 @@ struct Flat {
 };
 
 Flat flatten(const std::vector<at::Tensor>& grads, bool written, const char* who) {
+  TORCH_CHECK(!grads.empty(), who, ": needs at least one gradient");
+  for (const at::Tensor& g : grads)
+    TORCH_CHECK(g.defined() && !g._fw_grad(0).defined(), who,
+                ": forward-mode derivatives are not defined; use the backward pass");
+  const c10::Device device = grads[0].device();
+  const bool recording = at::GradMode::is_enabled();
   Flat f;
   f.list.reserve(grads.size());
   for (const at::Tensor& g : grads) {
-    TORCH_CHECK(g.defined() && g.layout() == at::kStrided && g.is_cuda(), who,
+    TORCH_CHECK(g.layout() == at::kStrided && g.is_cuda(), who,
                 ": gradients must be dense CUDA tensors");
-    TORCH_CHECK(g.device() == grads[0].device(), who, ": gradients are on different devices");
+    TORCH_CHECK(g.device() == device, who, ": gradients are on different devices");
     const at::ScalarType type = g.scalar_type();
     TORCH_CHECK(type == at::kFloat || type == at::kBFloat16 || type == at::kHalf, who,
                 ": gradients must be float32, bfloat16 or float16");
-    TORCH_CHECK(!(at::GradMode::is_enabled() && g.requires_grad()), who,
+    TORCH_CHECK(!(recording && g.requires_grad()), who,
                 ": no gradient is defined for it; use torch.no_grad()");
-    check_no_tangent({g}, who);
-  }
-  const at::NoGradGuard plain;
-  for (const at::Tensor& g : grads) {
-    if (g.numel() == 0) continue;
-    at::Tensor t = g;
-    if (!g.is_non_overlapping_and_dense() || g.is_neg()) {
-      if (written)
-        for (int64_t i = 0; i < g.dim(); ++i)
-          TORCH_CHECK(g.size(i) <= 1 || g.stride(i) != 0, who,
-                      ": an expanded tensor cannot be scaled in place");
-      t = g.clone(at::MemoryFormat::Contiguous);
-      f.back.emplace_back(g, t);
+    const int64_t n = g.numel();
+    if (n == 0) continue;
+    const int code = type == at::kFloat ? B200_FP32 : dtype_code(g);
+    if (g.is_non_overlapping_and_dense() && !g.is_neg()) {
+      f.list.push_back({g.data_ptr(), n, code});
+      continue;
     }
-    f.list.push_back({t.data_ptr(), t.numel(),
-                      t.scalar_type() == at::kFloat ? B200_FP32 : dtype_code(t)});
+    if (written)
+      for (int64_t i = 0; i < g.dim(); ++i)
+        TORCH_CHECK(g.size(i) <= 1 || g.stride(i) != 0, who,
+                    ": an expanded tensor cannot be scaled in place");
+    const at::NoGradGuard plain;
+    f.back.emplace_back(g, g.clone(at::MemoryFormat::Contiguous));
+    f.list.push_back({f.back.back().second.data_ptr(), n, code});
   }
   return f;
 }
 
 // No element may be scaled twice: seen where tensors without gaps overlap and where
-// two begin at the same element.  (Tensors with gaps may interleave, as columns do.)
-void check_apart(const std::vector<at::Tensor>& grads, const char* who) {
+// two with gaps begin at the same element.  (These may interleave, as columns do.)
+void check_apart(const Flat& f, const char* who) {
   struct Span {
     const char *begin, *end;
   };
-  std::vector<Span> dense, all;
-  for (const at::Tensor& g : grads) {
-    if (g.numel() == 0) continue;
-    const char* p = static_cast<const char*>(g.data_ptr());
-    all.push_back({p, p});
-    if (g.is_non_overlapping_and_dense()) dense.push_back({p, p + g.numel() * g.element_size()});
+  std::vector<Span> spans;
+  spans.reserve(f.list.size());
+  auto apart = [&]() {
+    auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
+    if (!std::is_sorted(spans.begin(), spans.end(), before))
+      std::sort(spans.begin(), spans.end(), before);
+    for (size_t i = 1; i < spans.size(); ++i)
+      TORCH_CHECK(spans[i].begin >= spans[i - 1].end && spans[i].begin != spans[i - 1].begin, who,
+                  ": gradients must not share memory");
+  };
+  // (the copies are memory of their own)
+  for (const b200_tensor& t : f.list) {
+    const char* p = static_cast<const char*>(t.data);
+    spans.push_back({p, p + t.count * (t.type == B200_FP32 ? 4 : 2)});
   }
-  for (std::vector<Span>* list : {&dense, &all}) {
-    std::sort(list->begin(), list->end(),
-              [](const Span& a, const Span& b) { return a.begin < b.begin; });
-    for (size_t i = 1; i < list->size(); ++i)
-      TORCH_CHECK((*list)[i].begin >= (*list)[i - 1].end &&
-                      (*list)[i].begin != (*list)[i - 1].begin,
-                  who, ": gradients must not share memory");
+  apart();
+  if (f.back.empty()) return;
+  spans.clear();
+  for (const auto& [to, from] : f.back) {
+    const char* p = static_cast<const char*>(to.data_ptr());
+    spans.push_back({p, p});
   }
+  apart();
+}
+
+// Where the work goes; nowhere yet if the checks are going to refuse it.
+std::optional<c10::Device> device_of(const std::vector<at::Tensor>& grads) {
+  return !grads.empty() && grads[0].defined() && grads[0].is_cuda()
+             ? std::optional<c10::Device>(grads[0].device())
+             : std::nullopt;
 }
 
 at::Tensor grad_norm_b200(const std::vector<at::Tensor>& grads) {
-  TORCH_CHECK(!grads.empty(), kNorm, ": needs at least one gradient");
-  TORCH_CHECK(grads[0].defined() && grads[0].is_cuda(), kNorm,
-              ": gradients must be dense CUDA tensors");
-  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const c10::cuda::OptionalCUDAGuard guard(device_of(grads));
   const Flat f = flatten(grads, false, kNorm);
   auto norm = fresh({}, at::kFloat, grads[0]);
   check_status(b200_grad_norm(f.list.data(), (int)f.list.size(), norm.data_ptr<float>(),
@@ -379,12 +396,9 @@ at::Tensor grad_norm_b200(const std::vector<at::Tensor>& grads) {
 
 at::Tensor clip_grads_b200(const std::vector<at::Tensor>& grads, double max_norm) {
   TORCH_CHECK(max_norm >= 0, kClip, ": max_norm must not be negative");
-  TORCH_CHECK(!grads.empty(), kClip, ": needs at least one gradient");
-  TORCH_CHECK(grads[0].defined() && grads[0].is_cuda(), kClip,
-              ": gradients must be dense CUDA tensors");
-  const c10::cuda::CUDAGuard guard(grads[0].device());
+  const c10::cuda::OptionalCUDAGuard guard(device_of(grads));
   const Flat f = flatten(grads, true, kClip);
-  check_apart(grads, kClip);
+  check_apart(f, kClip);
   auto norm = fresh({}, at::kFloat, grads[0]);
   check_status(b200_clip_grads(f.list.data(), (int)f.list.size(), (float)max_norm,
                                norm.data_ptr<float>(), current_stream()),

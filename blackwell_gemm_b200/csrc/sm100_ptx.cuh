@@ -265,6 +265,15 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
                :: "r"(bar) : "memory");
 }
 
+// The same on the barriers at this shared-memory address of every CTA of the cluster
+// whose rank's bit is set in `ctas`.
+__device__ __forceinline__ void umma_commit_both(uint32_t bar, uint16_t ctas) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+      " [%0], %1;"
+      :: "r"(bar), "h"(ctas) : "memory");
+}
+
 // 32 lanes x 32 consecutive 32-bit columns: thread i receives lane (base+i).
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
