@@ -216,7 +216,11 @@ int launch_pair(FfnArgs& a, const CUtensorMap& w0, const CUtensorMap& w1, const 
                 const CUtensorMap& h, const CUtensorMap& s, const DeviceView& v,
                 const FfnDevice& d, cudaStream_t stream) {
   using C = FfnCfg<kMode, kMany>;
-  a.group = 8;
+  // Bands of token tiles: wide ones read the weights less often, narrow ones the tokens.
+  // (8, 16 and 32 wide, us: gated 8192 x 28672 x 4096 1190, 1180, 1308; its dA 1254, 1288,
+  // 1366 and dW 1247, 1290, 1355; dA of 4095 rows, all in one band of 16, 697 and 679.)
+  const bool few = ceil_div(a.rows, 256) <= 16;
+  a.group = kMode == kFfnDW || (kMode == kFfnDA && !few) ? 8 : 16;
   a.status = v.status;
   a.timeout_ns = v.timeout_ns;
   const long long tf = ceil_div(a.feat, C::kFeat);

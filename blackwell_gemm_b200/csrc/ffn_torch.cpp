@@ -206,7 +206,7 @@ struct GatedMatmul : torch::autograd::Function<GatedMatmul> {
     const at::Tensor offsets = defined_or_empty(offsets_);
     const c10::cuda::CUDAGuard guard(a.device());
     const Rows ra = as_rows(a);
-    const Bank g = as_bank(bank_of(gate)), u = as_bank(bank_of(up));
+    const Bank g = as_bank(bank_of(gate), offsets), u = as_bank(bank_of(up), offsets);
     at::Tensor z;
     at::Tensor h = gated_forward(ra, g, u, offsets, (int)act, &z);
     const bool keep_a = gate.requires_grad() || up.requires_grad(), keep_w = a.requires_grad();
@@ -239,7 +239,7 @@ struct GatedMatmul : torch::autograd::Function<GatedMatmul> {
                                        (int)padded(n), act, dtype_code(dz), current_stream()),
                    "matmul_b200_gated backward");
       if (ctx->needs_input_grad(0)) {
-        const Bank g = as_bank(saved[1]), u = as_bank(saved[2]);
+        const Bank g = as_bank(saved[1], offsets), u = as_bank(saved[2], offsets);
         da = fresh({m, k}, type, z);
         check_status(b200_ffn_da(dz.data_ptr(), g.t.data_ptr(), u.t.data_ptr(), off, da.data_ptr(),
                                  2, (int)m, (int)e, (int)n, (int)k, (int)padded(n), g.ld, g.stride,
@@ -298,8 +298,8 @@ at::Tensor matmul_b200_gated(const at::Tensor& A, const at::Tensor& gate, const 
     return GatedMatmul::apply(A, gate, up, offsets.defined() ? OptTensor(offsets) : OptTensor(),
                               act);
   const c10::cuda::CUDAGuard guard(A.device());
-  return gated_forward(as_rows(A), as_bank(bank_of(gate)), as_bank(bank_of(up)), offsets, act,
-                       nullptr);
+  return gated_forward(as_rows(A), as_bank(bank_of(gate), offsets),
+                       as_bank(bank_of(up), offsets), offsets, act, nullptr);
 }
 
 // -------------------------------------------------------- gradient norm, clipping

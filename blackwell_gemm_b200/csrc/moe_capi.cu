@@ -643,12 +643,13 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
   return run_grouped<kGroupedDB>(c, static_cast<cudaStream_t>(stream));
 }
 
-int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
-                    int matrices, int rows, int cols, int ld, void* stream) {
+int b200_align_bank(const void* src, long long matrix_stride, long long row_stride, void* dst,
+                    const int* offsets, int matrices, int rows, int cols, int ld, void* stream) {
   if (matrices < 0 || rows < 0 || cols < 0 || ld < cols) return B200_ERR_INVALID_ARGUMENT;
   if (matrices == 0 || rows == 0 || cols == 0) return B200_OK;
   if (!src || !dst || row_stride < 0 || matrix_stride < 0) return B200_ERR_INVALID_ARGUMENT;
   if (!tma_rows(dst, ld) || (reinterpret_cast<uintptr_t>(src) & 1u)) return B200_ERR_ALIGNMENT;
+  if (reinterpret_cast<uintptr_t>(offsets) & 3u) return B200_ERR_ALIGNMENT;
   if (ld > kMaxExtent) return B200_ERR_TOO_LARGE;
   DeviceView v;
   MoeDevice* m = nullptr;
@@ -658,7 +659,14 @@ int b200_align_rows(const void* src, long long matrix_stride, long long row_stri
   const long long most = 16ll * v.sms;
   return launch(align_rows_kernel, (int)(blocks < most ? blocks : most), 256, 0,
                 static_cast<cudaStream_t>(stream), static_cast<const uint16_t*>(src),
-                matrix_stride, row_stride, static_cast<uint16_t*>(dst), matrices, rows, cols, ld);
+                matrix_stride, row_stride, static_cast<uint16_t*>(dst), matrices, rows, cols, ld,
+                offsets);
+}
+
+int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
+                    int matrices, int rows, int cols, int ld, void* stream) {
+  return b200_align_bank(src, matrix_stride, row_stride, dst, nullptr, matrices, rows, cols, ld,
+                         stream);
 }
 
 int b200_narrow_offsets(const void* offsets, long long stride, int count, int* out, void* stream) {

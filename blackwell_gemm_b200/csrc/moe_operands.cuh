@@ -23,10 +23,12 @@ narrow_offsets_kernel(const long long* __restrict__ offsets, long long stride, i
 // x cols 16-bit elements with unit column stride into rows of ld (a multiple
 // of 8).  A thread makes 16 bytes of a row from the five words that hold them
 // -- a row may start on any 2 bytes -- so loads and stores stay wide.  Bound
-// by memory: each element read and written once.
+// by memory: each element read and written once.  With offsets, a bank: the
+// matrices of experts without rows are left out.
 __global__ void __launch_bounds__(256)
 align_rows_kernel(const uint16_t* __restrict__ src, long long matrix_stride, long long row_stride,
-                  uint16_t* __restrict__ dst, int matrices, int rows, int cols, int ld) {
+                  uint16_t* __restrict__ dst, int matrices, int rows, int cols, int ld,
+                  const int* __restrict__ offsets) {
   grid_wait();
   grid_launch_next();
   const int groups = ld / 8;
@@ -36,6 +38,7 @@ align_rows_kernel(const uint16_t* __restrict__ src, long long matrix_stride, lon
     const long long r = i / groups;
     const int c = (int)(i - r * groups) * 8;
     const int m = (int)(r / rows);
+    if (offsets != nullptr && offsets[m + 1] <= offsets[m]) continue;
     const uint16_t* from = src + m * matrix_stride + (r - (long long)m * rows) * row_stride + c;
     const uintptr_t at = reinterpret_cast<uintptr_t>(from);
     uint32_t w[4];

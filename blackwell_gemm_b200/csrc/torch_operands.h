@@ -104,7 +104,8 @@ struct Bank {
   int64_t stride;
 };
 
-inline Bank as_bank(const at::Tensor& t) {
+// With offsets only the matrices of experts with rows are copied.
+inline Bank as_bank(const at::Tensor& t, const at::Tensor& offsets = {}) {
   const int64_t e = t.size(0), n = t.size(1), k = t.size(2);
   const int64_t pad = std::max<int64_t>(round_up8(k), 8);
   if (t.numel() == 0) return {t, (int)pad, n * pad};
@@ -116,7 +117,8 @@ inline Bank as_bank(const at::Tensor& t) {
   auto buf = fresh({e, n, pad}, t.scalar_type(), t);
   const at::Tensor to = buf.narrow(2, 0, k);
   if (k == 1 || t.stride(2) == 1)
-    check_status(b200_align_rows(t.data_ptr(), t.stride(0), t.stride(1), buf.data_ptr(), (int)e,
+    check_status(b200_align_bank(t.data_ptr(), t.stride(0), t.stride(1), buf.data_ptr(),
+                                 offsets.defined() ? offsets.data_ptr<int>() : nullptr, (int)e,
                                  (int)n, (int)k, (int)pad, current_stream()),
                  "aligning a bank");
   else

@@ -65,6 +65,11 @@ int b200_grouped_gemm_db(const void* dC, const void* A, void* dB, const int* off
 int b200_align_rows(const void* src, long long matrix_stride, long long row_stride, void* dst,
                     int matrices, int rows, int cols, int ld, void* stream);
 
+/* The same for a bank whose offsets say which experts own rows (or NULL): the
+ * matrices of the others are not copied, and what dst holds of them is left. */
+int b200_align_bank(const void* src, long long matrix_stride, long long row_stride, void* dst,
+                    const int* offsets, int matrices, int rows, int cols, int ld, void* stream);
+
 /* int64 offsets as the calls here take them: `count` values, `stride` elements
  * apart, to int32.  One that 32 bits do not hold becomes -1 or 2^31 - 1: outside
  * the rows, as it was, and so clamped and reported. */
