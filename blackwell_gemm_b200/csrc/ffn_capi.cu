@@ -366,12 +366,14 @@ int run_plan(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
 template <bool kGated, int kTok, class T>
 int run_stream(const FfnCall& c, const DeviceView& v, cudaStream_t stream) {
   using C = FfnStreamCfg<kTok>;
-  CUtensorMap w[2], t;
+  CUtensorMap w[2], t, h;
   for (int i = 0; i < c.weights; ++i)
     CHECK(map_bank(&w[i], c.dtype, c.w[i].p, c.K, c.N, c.experts, c.w[i].ld, c.w[i].stride,
                    kGated ? 64 : 128));
   if (c.weights == 1) w[1] = w[0];
   CHECK(map_rows(&t, c.dtype, c.t, c.K, c.rows, c.ldt, 16));
+  h = t;
+  if (kTok > 16) CHECK(map_rows(&h, c.dtype, c.t, c.K, c.rows, c.ldt, 64));
   StreamArgs a = {};
   a.offsets = c.offsets;
   a.experts = c.experts;
@@ -386,7 +388,7 @@ int run_stream(const FfnCall& c, const DeviceView& v, cudaStream_t stream) {
   Workspace ws;
   CHECK(ws.take(v, (size_t)v.sms * 2 * kTok * 128 * sizeof(float), stream, &a));
   return launch(ffn_stream_kernel<kGated, kTok, T>, v.sms, C::kThreads, C::smem_bytes(c.experts),
-                stream, w[0], w[1], t, a, c.o);
+                stream, w[0], w[1], t, h, a, c.o);
 }
 
 // f with the activation as a constant.

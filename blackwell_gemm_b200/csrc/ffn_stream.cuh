@@ -6,9 +6,10 @@
 // gated: a block is 64 gate rows and the same 64 rows of the up weight.  A tile
 // whose contraction falls into several ranges is joined by whichever of its CTAs
 // finishes last, in range order, so sums do not depend on which one that was, and no
-// CTA waits for another.  Here a CTA's four epilogue warps count in together,
-// because the activation needs a feature's both products; the end is the pair
-// kernel's (ffn_epilogue.cuh).
+// CTA waits for another.  Here four epilogue warps count in together, because the
+// activation needs a feature's both products; two such groups take every other 16 tokens
+// (one alone: 64 rows x 28672 x 4096 gated 45 us).  The end is the pair kernel's
+// (ffn_epilogue.cuh).
 #pragma once
 #include "ffn_epilogue.cuh"
 #include "moe_stream.cuh"
@@ -20,10 +21,11 @@ struct FfnStreamCfg {
   static constexpr int kWeight = 128 * kSlabK * 2;  // 16 KiB per item
   static constexpr int kTokens = kTok * kSlabK * 2;
   static constexpr int kStageBytes = kWeight + kTokens;
-  static constexpr int kStages = (200 * 1024) / kStageBytes;
-  static constexpr int kThreads = 192;
+  static constexpr int kStages = (196 * 1024) / kStageBytes;
+  static constexpr int kEpiWarps = 8;
+  static constexpr int kThreads = 32 * (2 + kEpiWarps);
   static constexpr int smem_bytes(int experts) {
-    return kStages * kStageBytes + kFfnStageBytes + group_table_bytes(experts) + 1024;
+    return kStages * kStageBytes + 2 * kFfnStageBytes + group_table_bytes(experts) + 1024;
   }
 };
 
@@ -33,7 +35,8 @@ template <bool kGated, int kTok, class T>
 __global__ void __launch_bounds__(FfnStreamCfg<kTok>::kThreads, 1)
 ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                   const __grid_constant__ CUtensorMap tmap_w1,
-                  const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args,
+                  const __grid_constant__ CUtensorMap tmap_t,
+                  const __grid_constant__ CUtensorMap tmap_h, const StreamArgs args,
                   const FfnOut o) {
   using C = FfnStreamCfg<kTok>;
   constexpr int kStages = C::kStages;
@@ -46,14 +49,14 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   __shared__ alignas(8) uint64_t bar_drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
-  __shared__ uint32_t last_word;
+  __shared__ uint32_t last_word[2];
   constexpr uint32_t kCols = 2 * kTok < 32 ? 32 : 2 * kTok;  // two accumulators
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t staging = smem_base + kStages * C::kStageBytes;
-  int* s_off = reinterpret_cast<int*>(smem_raw + (staging + kFfnStageBytes - smem_u32(smem_raw)));
+  const uint32_t staging_base = smem_base + kStages * C::kStageBytes;
+  int* s_off = reinterpret_cast<int*>(smem_raw + (staging_base + 2 * kFfnStageBytes - smem_u32(smem_raw)));
   int* s_tiles = s_off + args.experts + 1;
 
   if (threadIdx.x == 0) {
@@ -63,7 +66,7 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bar_acc_full[b]), 1);
-      mbar_init(smem_u32(&bar_acc_empty[b]), 4);
+      mbar_init(smem_u32(&bar_acc_empty[b]), C::kEpiWarps);
     }
     mbar_init(smem_u32(&bar_drain), 1);
     abort_word = 0;
@@ -71,6 +74,7 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     prefetch_tmap(&tmap_w0);
     prefetch_tmap(&tmap_w1);
     prefetch_tmap(&tmap_t);
+    if (kTok > 16) prefetch_tmap(&tmap_h);
   }
   if (warp == 1) {
     tmem_alloc_1(smem_u32(&tmem_slot), kCols);
@@ -101,7 +105,9 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       long long issued = 0;
       bool ok = true;
       while (ok && walk.next(&s)) {
-        const int boxes = (s.rows + 15) / 16, f0 = s.block * kFeat;
+        const int f0 = s.block * kFeat;
+        const bool tall = kTok > 16 && s.rows > 32;
+        const int box = tall ? 64 : 16, boxes = (s.rows + box - 1) / box;
         for (int kb = s.kb0; kb < s.kb1; ++kb) {
           if (!wait_ready(smem_u32(&bar_empty[stage]), phase ^ 1u, wctx, kErrWaitEmpty)) {
             ok = false;
@@ -109,14 +115,14 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           }
           const uint32_t fb = smem_u32(&bar_full[stage]);
           const uint32_t sa = smem_base + stage * C::kStageBytes;
-          mbar_arrive_expect_tx(fb, C::kWeight + boxes * 16 * 128);
+          mbar_arrive_expect_tx(fb, C::kWeight + boxes * box * 128);
           const int k0 = kb * kSlabK;
           tma_load_3d_hint(sa, &tmap_w0, k0, f0, s.e, fb, once);
           if constexpr (kGated)
             tma_load_3d_hint(sa + C::kWeight / 2, &tmap_w1, k0, f0, s.e, fb, once);
           for (int i = 0; i < boxes; ++i)
-            tma_load_2d_hint(sa + C::kWeight + i * 16 * 128, &tmap_t, k0, s.row0 + i * 16, fb,
-                             keep);
+            tma_load_2d_hint(sa + C::kWeight + i * box * 128, tall ? &tmap_h : &tmap_t, k0,
+                             s.row0 + i * box, fb, keep);
           ++issued;
           if (++stage == kStages) { stage = 0; phase ^= 1u; }
         }
@@ -161,9 +167,12 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     }
     __syncwarp();
   } else {
-    const int quarter = warp & 3, tid = threadIdx.x - 64;
+    const int quarter = warp & 3, group = (warp - 2) >> 2;
+    const int tid = ((warp - 2) & 3) * 32 + lane;
+    const uint32_t staging = staging_base + (uint32_t)group * kFfnStageBytes;
     zero_unowned_rows(static_cast<T*>(o.out), o.ldo, o.feat, s_off[0], s_off[args.experts],
-                      args.rows, (long long)blockIdx.x * 128 + tid, gridDim.x * 128ll);
+                      args.rows, (long long)blockIdx.x * 256 + (threadIdx.x - 64),
+                      gridDim.x * 256ll);
     int it = 0;
     int ok = 1;
     while (walk.next(&s)) {
@@ -175,6 +184,11 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         ok = __shfl_sync(0xffffffffu, ok, 0);
       }
       tc_fence_after_sync();
+      const int c_first = group * kStageTokens;
+      if (c_first >= s.rows) {  // nothing for this group
+        if (lane == 0) mbar_arrive_local(smem_u32(&bar_acc_empty[buf]));
+        continue;
+      }
       const uint32_t tbase = tmem_base + buf * kTok + ((uint32_t)(quarter * 32) << 16);
       const bool whole = s.kb0 == 0 && s.kb1 == walk.red_blocks;
       const int f0 = s.block * kFeat;
@@ -194,7 +208,7 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         uint32_t v[16];
         tmem_ld_32x32b_x16(tbase + c, v);
         tmem_wait_ld();
-        if (c + kStageTokens >= s.rows) {
+        if (c + 2 * kStageTokens >= s.rows) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_local(smem_u32(&bar_acc_empty[buf]));
@@ -205,27 +219,27 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       if (!whole) {
         float* mine = slot(blockIdx.x);
 #pragma unroll 1
-        for (int c = 0; c < s.rows; c += kStageTokens) {
+        for (int c = c_first; c < s.rows; c += 2 * kStageTokens) {
           float acc[kStageTokens];
           load(c, acc);
 #pragma unroll
           for (int j = 0; j < 16; ++j)
             if (c + j < s.rows) __stcg(mine + (c + j) * 128, acc[j]);
         }
-        named_bar_sync(1, 128);
+        named_bar_sync(1 + group, 128);
         if (tid == 0) {
-          const bool last =
-              atomic_add_acq_rel(args.counts + c0 * 16, 1u) == (unsigned int)(c1 - c0);
-          if (last) atomicExch(args.counts + c0 * 16, 0u);
-          last_word = last;
+          unsigned int* count = args.counts + c0 * 16 + group;
+          const bool last = atomic_add_acq_rel(count, 1u) == (unsigned int)(c1 - c0);
+          if (last) atomicExch(count, 0u);
+          last_word[group] = last;
         }
-        named_bar_sync(1, 128);
-        if (last_word == 0) continue;
+        named_bar_sync(1 + group, 128);
+        if (last_word[group] == 0) continue;
       }
       with_act(o.act, [&](auto code) {
         constexpr int kAct = decltype(code)::value;
 #pragma unroll 1
-        for (int c = 0; c < s.rows; c += kStageTokens) {
+        for (int c = c_first; c < s.rows; c += 2 * kStageTokens) {
           float acc[kStageTokens];
           if (whole) {
             load(c, acc);
@@ -249,7 +263,7 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                 for (int j = 0; j < 16; ++j) acc[j] += v[i][j];
             }
           }
-          ffn_finish<kGated, kAct, T>(o, staging, 1, quarter, acc, s.row0 + c,
+          ffn_finish<kGated, kAct, T>(o, staging, 1 + group, quarter, acc, s.row0 + c,
                                       ok ? s.rows - c : 0, f0, tid, tile);
         }
       });
