@@ -23,6 +23,7 @@ struct FfnGradArgs {
   void* dz;  // null: only the bias
   long long lddz, dz_half;
   float* partial;      // (row blocks, N) sums, or null
+  void* dbias;         // the sums themselves, rounded, where one block takes all rows
   const int* offsets;  // null: all rows
   int experts, rows, feat;
   int strips;      // blocks along a row; the rest of the grid goes over the rows
@@ -124,7 +125,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
     }
   }
   if constexpr (!kGated) {
-    if (a.partial == nullptr) return;
+    if (a.partial == nullptr && a.dbias == nullptr) return;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sums[part][lane * 8 + i] = total[i];
     __syncthreads();
@@ -133,7 +134,8 @@ ffn_grad_kernel(const FfnGradArgs a) {
       float s = 0.0f;
 #pragma unroll
       for (int p = 0; p < 8; ++p) s += sums[p][threadIdx.x];
-      a.partial[(long long)block * a.feat + col] = s;
+      if (a.partial != nullptr) a.partial[(long long)block * a.feat + col] = s;
+      else static_cast<T*>(a.dbias)[col] = round_one<T>(s);
     }
   }
 }

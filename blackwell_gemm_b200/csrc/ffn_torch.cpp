@@ -312,9 +312,11 @@ struct Flat {
 
 Flat flatten(const std::vector<at::Tensor>& grads, bool written, const char* who) {
   TORCH_CHECK(!grads.empty(), who, ": needs at least one gradient");
-  for (const at::Tensor& g : grads)
-    TORCH_CHECK(g.defined() && !g._fw_grad(0).defined(), who,
-                ": forward-mode derivatives are not defined; use the backward pass");
+  const bool tangents = tangents_possible();
+  for (const at::Tensor& g : grads) {
+    TORCH_CHECK(g.defined(), who, ": gradients must be dense CUDA tensors");
+    if (tangents) check_no_tangent({g}, who);
+  }
   const c10::Device device = grads[0].device();
   const bool recording = at::GradMode::is_enabled();
   Flat f;
