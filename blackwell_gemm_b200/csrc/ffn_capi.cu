@@ -109,9 +109,9 @@ bool init_type(FfnDevice& d, int sms) {
          init_pair<kFfnDA, false, T>(sms, &d.pairs[2]) &&
          init_pair<kFfnDW, false, T>(sms, &d.pairs[3]) &&
          init_pair<kFfnDW, true, T>(sms, &d.pairs[3]) && init_stream<true, 16, T>() &&
-         init_stream<true, 64, T>() && init_stream<true, 256, T>() &&
-         init_stream<false, 16, T>() && init_stream<false, 64, T>() &&
-         init_stream<false, 256, T>();
+         init_stream<true, 64, T>() && init_stream<true, 128, T>() &&
+         init_stream<true, 256, T>() && init_stream<false, 16, T>() &&
+         init_stream<false, 64, T>();
 }
 
 int ffn_device(DeviceView* v, FfnDevice** out) {
@@ -436,8 +436,13 @@ int run_forward(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaS
   const ClusterPlan plan = cluster_plan<kMode>(c, d);
   if (use_stream<kGated>(c, plan, v, d)) {
     if (c.rows <= 16) return run_stream<kGated, 16, T>(c, v, stream);
-    if (c.rows <= 64ll * c.experts) return run_stream<kGated, 64, T>(c, v, stream);
-    return run_stream<kGated, 256, T>(c, v, stream);
+    // A tile that holds most experts' rows: an expert with more reads its weights again.
+    if constexpr (kGated) {
+      if (c.rows > 64ll * c.experts) return run_stream<kGated, 256, T>(c, v, stream);
+      if (c.rows > 24ll * c.experts && c.experts > 1)
+        return run_stream<kGated, 128, T>(c, v, stream);
+    }
+    return run_stream<kGated, 64, T>(c, v, stream);
   }
   if (plan.splits > 0) return run_plan<kMode, T>(c, plan, v, stream);
   return run_pair<kMode, T>(c, v, d, stream);
@@ -512,9 +517,9 @@ int run_grad(FfnGradArgs a, bool gated, int act, void* dbias, int dtype, cudaStr
   CHECK(half ? launch_grad<__half>(a, gated, act, blocks, stream)
              : launch_grad<__nv_bfloat16>(a, gated, act, blocks, stream));
   if (a.partial == nullptr) return B200_OK;
-  return half ? launch(ffn_bias_kernel<__half>, a.strips, 256, 0, stream, a.partial, row_blocks,
+  return half ? launch(ffn_bias_kernel<__half>, (int)ceil_div(a.feat, 32), 256, 0, stream, a.partial, row_blocks,
                        a.feat, static_cast<__half*>(dbias))
-              : launch(ffn_bias_kernel<__nv_bfloat16>, a.strips, 256, 0, stream, a.partial,
+              : launch(ffn_bias_kernel<__nv_bfloat16>, (int)ceil_div(a.feat, 32), 256, 0, stream, a.partial,
                        row_blocks, a.feat, static_cast<__nv_bfloat16*>(dbias));
 }
 

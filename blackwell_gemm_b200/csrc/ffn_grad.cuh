@@ -140,17 +140,26 @@ ffn_grad_kernel(const FfnGradArgs a) {
   }
 }
 
-// dbias[n] = the row blocks' sums, added in order.
+// dbias[n] = the row blocks' sums: 32 columns to a block, each warp every eighth of the
+// sums in order, and the eight of them in order.
 template <class T>
 __global__ void __launch_bounds__(256)
 ffn_bias_kernel(const float* __restrict__ partial, int blocks, int feat, T* __restrict__ dbias) {
+  __shared__ float sums[8][32];
   grid_wait();
   grid_launch_next();
-  const int col = blockIdx.x * 256 + threadIdx.x;
-  if (col >= feat) return;
+  const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+  const int col = blockIdx.x * 32 + lane;
   float s = 0.0f;
-#pragma unroll 8
-  for (int b = 0; b < blocks; ++b) s += partial[(long long)b * feat + col];
+  if (col < feat) {
+#pragma unroll 4
+    for (int b = part; b < blocks; b += 8) s += partial[(long long)b * feat + col];
+  }
+  sums[part][lane] = s;
+  __syncthreads();
+  if (part != 0 || col >= feat) return;
+#pragma unroll
+  for (int p = 1; p < 8; ++p) s += sums[p][lane];
   dbias[col] = round_one<T>(s);
 }
 
