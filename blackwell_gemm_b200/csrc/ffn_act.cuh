@@ -10,11 +10,13 @@
 // 16-bit outputs round by 2^-8 or 2^-11.
 //
 // Which activation is a template argument, chosen by with_act once per tile: a branch per
-// four values took 200 cycles each (8191 x 8192 x 2048 with silu: 227 us, 183 without).
+// four values took 200 cycles each (8191 rows x 8192 x 2048 with bias and gelu_tanh 227 us,
+// 183 so).
 #pragma once
 #include <stdint.h>
 
 #include "b200_ffn.h"
+#include "sm100_ptx.cuh"
 
 namespace b200 {
 
@@ -50,10 +52,6 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-__device__ __forceinline__ float logistic(float z) {
-  return fast_rcp(1.0f + fast_exp2(z * -kLog2E));
-}
-
 // s(z) and 1 - s(z) = s(-z), neither by cancellation.
 __device__ __forceinline__ void logistic_both(float z, float* s, float* rest) {
   const float e = fast_exp2(fabsf(z) * -kLog2E);
@@ -83,22 +81,68 @@ __device__ __forceinline__ float tanh_argument(float z) {
   return 2.0f * kRoot2OverPi * z * fmaf(0.044715f * z, z, 1.0f);
 }
 
-// v = act(v)
+// The same for two values at a time, where instructions are what is short (the products'
+// epilogues).
+__device__ __forceinline__ F32x2 both(float v) { return pair_of(v, v); }
+__device__ __forceinline__ F32x2 exp2_pair(F32x2 x) {
+  float a, b;
+  halves_of(x, a, b);
+  return pair_of(fast_exp2(a), fast_exp2(b));
+}
+__device__ __forceinline__ F32x2 rcp_pair(F32x2 x) {
+  float a, b;
+  halves_of(x, a, b);
+  return pair_of(fast_rcp(a), fast_rcp(b));
+}
+// s(-z / log2(e))
+__device__ __forceinline__ F32x2 logistic_pair(F32x2 exponent) {
+  return rcp_pair(add2(exp2_pair(exponent), both(1.0f)));
+}
+__device__ __forceinline__ F32x2 normal_cdf_pair(F32x2 z) {
+  float a, b, t0, t1;
+  halves_of(z, a, b);
+  const F32x2 t = rcp_pair(fma2(pair_of(fabsf(a), fabsf(b)), both(0.36f), both(1.0f)));
+  F32x2 p = fma2(both(0.0470560668f), t, both(-0.179763946f));
+  p = fma2(p, t, both(0.180953029f));
+  p = fma2(p, t, both(0.0265499685f));
+  p = fma2(p, t, both(0.139719047f));
+  p = fma2(p, t, both(0.141772489f));
+  p = fma2(p, t, both(0.143713043f));
+  const F32x2 bell = exp2_pair(mul2(mul2(z, z), both(-0.5f * kLog2E)));
+  halves_of(mul2(mul2(p, t), bell), t0, t1);
+  return pair_of(a < 0.0f ? t0 : 1.0f - t0, b < 0.0f ? t1 : 1.0f - t1);
+}
+
+// v = act(v); kN even, or 1.
 template <int kAct, int kN>
 __device__ __forceinline__ void activate(float (&v)[kN]) {
+  if constexpr (kAct == B200_ACT_NONE) return;
+  if constexpr (kN == 1) {
+    float two[2] = {v[0], v[0]};
+    activate<kAct>(two);
+    v[0] = two[0];
+  } else {
 #pragma unroll
-  for (int i = 0; i < kN; ++i) {
-    if constexpr (kAct == B200_ACT_RELU) {
-      v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
-    } else if constexpr (kAct == B200_ACT_SILU) {
-      v[i] *= logistic(v[i]);
-    } else if constexpr (kAct == B200_ACT_GELU) {
-      float bell;
-      v[i] *= normal_cdf(v[i], &bell);
-    } else if constexpr (kAct == B200_ACT_GELU_TANH) {
-      v[i] *= logistic(tanh_argument(v[i]));
-    } else if constexpr (kAct == B200_ACT_SIGMOID) {
-      v[i] = logistic(v[i]);
+    for (int i = 0; i < kN; i += 2) {
+      if constexpr (kAct == B200_ACT_RELU) {
+        v[i] = v[i] < 0.0f ? 0.0f : v[i];  // (NaN stays)
+        v[i + 1] = v[i + 1] < 0.0f ? 0.0f : v[i + 1];
+      } else {
+        const F32x2 z = pair_of(v[i], v[i + 1]);
+        F32x2 r;
+        if constexpr (kAct == B200_ACT_SILU) {
+          r = mul2(z, logistic_pair(mul2(z, both(-kLog2E))));
+        } else if constexpr (kAct == B200_ACT_GELU) {
+          r = mul2(z, normal_cdf_pair(z));
+        } else if constexpr (kAct == B200_ACT_GELU_TANH) {
+          constexpr float kScale = -2.0f * kRoot2OverPi * kLog2E;
+          const F32x2 y = mul2(z, fma2(mul2(z, both(0.044715f * kScale)), z, both(kScale)));
+          r = mul2(z, logistic_pair(y));
+        } else {
+          r = logistic_pair(mul2(z, both(-kLog2E)));
+        }
+        halves_of(r, v[i], v[i + 1]);
+      }
     }
   }
 }

@@ -34,13 +34,13 @@ std::mutex g_mu;
 FfnDevice g_ffn[kMaxDevices];
 std::atomic<int> g_kernel{0};
 
-// dW: experts whose table fits beside six stages.
+// Experts whose table fits beside six stages.
 constexpr int kFewExperts = 128;
 
 template <int kMode, bool kMany, class T>
 bool init_pair(int sms, int* pairs) {
   using C = FfnCfg<kMode, kMany>;
-  constexpr int experts = kMode == kFfnDW && !kMany ? kFewExperts : kMaxExperts;
+  constexpr int experts = kMany ? kMaxExperts : kFewExperts;
   // (512 B: more than the kernel's static shared memory)
   static_assert(C::smem_bytes(experts) <= 227 * 1024 - 512, "shared memory of one CTA");
   auto* fn = ffn_pair_kernel<kMode, kMany, T>;
@@ -105,8 +105,10 @@ bool init_type(FfnDevice& d, int sms) {
   return init_clusters<kFfnGated, T>(d, sms) && init_clusters<kFfnAct, T>(d, sms) &&
          init_clusters<kFfnDA, T>(d, sms) &&
          init_pair<kFfnGated, false, T>(sms, &d.pairs[0]) &&
+         init_pair<kFfnGated, true, T>(sms, &d.pairs[0]) &&
          init_pair<kFfnAct, false, T>(sms, &d.pairs[1]) &&
          init_pair<kFfnDA, false, T>(sms, &d.pairs[2]) &&
+         init_pair<kFfnDA, true, T>(sms, &d.pairs[2]) &&
          init_pair<kFfnDW, false, T>(sms, &d.pairs[3]) &&
          init_pair<kFfnDW, true, T>(sms, &d.pairs[3]) && init_stream<true, 16, T>() &&
          init_stream<true, 64, T>() && init_stream<true, 128, T>() &&
@@ -268,6 +270,10 @@ int run_pair(const FfnCall& c, const DeviceView& v, const FfnDevice& d, cudaStre
   a.red = red;
   a.halves = halves;
   a.o = c.o;
+  if constexpr (kMode != kFfnAct) {  // (which has one matrix)
+    if (c.experts > kFewExperts)
+      return launch_pair<kMode, true, T>(a, w[0], w[1], t, h, s, v, d, stream);
+  }
   return launch_pair<kMode, false, T>(a, w[0], w[1], t, h, s, v, d, stream);
 }
 

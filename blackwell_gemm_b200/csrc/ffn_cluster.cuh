@@ -38,7 +38,7 @@ struct FfnClusterCfg {
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
   static constexpr int kRing = 12 * kWeight;  // (at least what the exchange needs: 112 KiB)
-  static constexpr int kSmem = kRing + 2 * kFfnStageBytes + 1024;
+  static constexpr int kSmem = kRing + 2 * 2 * kFfnStageBytes + 1024;
 };
 
 // tmap_w0, tmap_w1: the weights (k, n, 1): gated gate and up, box 64 x 64; act box
@@ -255,14 +255,22 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     cluster_sync_all();  // every part has arrived
   }
   if (warp >= 2) {
-    FfnTile<kGated> s;
-    ffn_tile<kGated, T>(args.o, f0, tid, s);
-    const uint32_t staging = staging_base + (uint32_t)group * kFfnStageBytes;
+    FfnTile<kGated, T> s;
+    ffn_tile<kGated, T>(args.o, f0, row0, tid, s);
+    const uint32_t staging = staging_base + (uint32_t)group * 2 * kFfnStageBytes;
+    uint32_t turn = 0;
     auto finish = [&](auto code) {
       constexpr int kAct = decltype(code)::value;
+      FfnResidual<kGated, T> now, next;
+      auto fetch = [&](int c) {
+        next.fetch(args.o, c * kStageTokens, rows - c * kStageTokens, s);
+      };
+      fetch(part + group * splits);
 #pragma unroll 1
       for (int i = group; part + i * splits < chunks; i += 2) {
         const int c = part + i * splits;
+        now = next;
+        fetch(c + 2 * splits);
         uint32_t v[16];
         tmem_ld_32x32b_x16(tbase + c * kStageTokens, v);
         tmem_wait_ld();
@@ -289,9 +297,9 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
             from += kFfnStageBytes;
           }
         }
-        ffn_finish<kGated, kAct, T>(args.o, staging, 1 + group, quarter, acc,
-                                    row0 + c * kStageTokens, ok ? rows - c * kStageTokens : 0, f0,
-                                    tid, s);
+        ffn_finish<kGated, kAct, T, true>(args.o, staging, &turn, 1 + group, quarter, acc, row0,
+                                          c * kStageTokens, ok ? rows - c * kStageTokens : 0, f0,
+                                          tid, s, now);
       }
     };
     if constexpr (kMode == kFfnDA)

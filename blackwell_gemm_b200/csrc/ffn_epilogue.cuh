@@ -30,7 +30,7 @@ struct FfnOut {
 };
 
 constexpr int kStageTokens = 16;
-constexpr int kFfnStageBytes = kStageTokens * 128 * 4;
+constexpr int kFfnStageBytes = kStageTokens * 128 * 4;  // (a power of two)
 
 template <class T>
 __device__ __forceinline__ float widen(uint16_t bits);
@@ -50,116 +50,143 @@ __device__ __forceinline__ void store_four(T* p, const float (&v)[4]) {
 
 // One warp's part of the staging: lane's accumulator row `quarter * 32 + lane`
 // of 16 tokens.
-__device__ __forceinline__ void stage_put(uint32_t stage, int quarter, const float (&v)[16]) {
-  const uint32_t at = stage + (uint32_t)(quarter * 32 + (threadIdx.x & 31)) * 4u;
-#pragma unroll
-  for (int t = 0; t < kStageTokens; ++t) st_shared_u32(at + t * 512u, __float_as_uint(v[t]));
+template <int kFrom = 0>
+__device__ __forceinline__ void stage_put(uint32_t at, const float (&v)[16]) {
+  if constexpr (kFrom < kStageTokens) {
+    st_shared_f32_at<kFrom * 512>(at, v[kFrom]);
+    stage_put<kFrom + 1>(at, v);
+  }
 }
 
-// What a thread keeps over a tile: its features' bias, and whether all of the tile's
-// features are there, in rows that it reads and writes four at a time.
-template <bool kGated>
+// What a thread keeps over a tile: where its part of the first token begins, its features'
+// bias, and whether all of the tile's features are there, in rows that it reads and writes
+// four at a time.
+template <bool kGated, class T>
 struct FfnTile {
-  float bias[kGated ? 1 : 8];
+  T* out;
+  const T* residual;
+  float* z;
+  F32x2 bias[kGated ? 1 : 4];
   bool whole;
 };
 
-// feat0: the first feature of the 64 or 128; tid: 0..127 of the group of warps.
+// feat0: the first feature of the 64 or 128; row0: the tile's first row; tid: 0..127 of the
+// group of warps.  A thread has token tid / 16 and eight further of 16, features 4 (tid %
+// 16) on and, not gated, 64 further.
 template <bool kGated, class T>
-__device__ __forceinline__ void ffn_tile(const FfnOut& o, int feat0, int tid, FfnTile<kGated>& s) {
+__device__ __forceinline__ void ffn_tile(const FfnOut& o, int feat0, long long row0, int tid,
+                                         FfnTile<kGated, T>& s) {
+  const int f = feat0 + (tid & 15) * 4;
+  const long long row = row0 + (tid >> 4);
   s.whole = feat0 + (kGated ? 64 : 128) <= o.feat && o.vec_out &&
             (kGated || o.residual == nullptr || o.vec_res);
+  s.out = static_cast<T*>(o.out) + row * o.ldo + f;
+  s.residual = static_cast<const T*>(o.residual) + row * o.ldr + f;
+  s.z = o.z + row * o.ldz + f;
   if constexpr (!kGated) {
-    const int f = feat0 + (tid & 15) * 4;
+    if (o.bias != nullptr && s.whole) {
+      const uint16_t* b = static_cast<const uint16_t*>(o.bias) + f;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        s.bias[h * 4 + i] =
-            s.whole && o.bias != nullptr
-                ? widen<T>(static_cast<const uint16_t*>(o.bias)[f + h * 64 + i]) : 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        const uint16_t* p = b + (i >> 1) * 64 + (i & 1) * 2;
+        s.bias[i] = pair_of(widen<T>(p[0]), widen<T>(p[1]));
+      }
     }
   }
 }
 
-// A thread's part of 16 staged tokens: token tid / 16 and eight further, features
-// 4 (tid % 16) on and, not gated, 64 further.  All of it is there (FfnTile::whole, 16
-// tokens), so the loads and the arithmetic of all values run side by side.  The residual
-// is asked for before the barrier that the staged values wait at.
-template <bool kGated, int kAct, class T>
-__device__ __forceinline__ void ffn_rows_whole(const FfnOut& o, uint32_t stage, uint32_t bar,
-                                               int quarter, const float (&acc)[16],
-                                               long long row0, int feat0, int tid,
-                                               const FfnTile<kGated>& s) {
-  const int f = feat0 + (tid & 15) * 4;
-  const long long row = row0 + (tid >> 4);
-  uint2 res[2][2];
-  const bool add = !kGated && o.residual != nullptr;
-  if constexpr (!kGated) {
-    const T* r = static_cast<const T*>(o.residual) + row * o.ldr + f;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        res[j][h] = add ? *reinterpret_cast<const uint2*>(r + j * 8 * o.ldr + h * 64)
-                        : make_uint2(0, 0);
-  }
-  stage_put(stage, quarter, acc);
-  named_bar_sync(bar, 128);
-  const uint32_t at = stage + (uint32_t)(tid >> 4) * 512u + (uint32_t)(tid & 15) * 16u;
-  float v[2][2][4];
-#pragma unroll
-  for (int j = 0; j < 2; ++j)
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-      ld_shared_v4_f32(at + j * 8u * 512u + h * 256u, v[j][h][0], v[j][h][1], v[j][h][2],
-                       v[j][h][3]);
-  T* out = static_cast<T*>(o.out) + row * o.ldo + f;
-  if constexpr (!kGated) {
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[j][h][i] += s.bias[h * 4 + i];
-  }
-  if (o.z != nullptr) {
-    float* z = o.z + row * o.ldz + f;
-    const long long second = kGated ? o.z_half : 64;
-#pragma unroll
-    for (int j = 0; j < 2; ++j)
+// A thread's residual of 16 tokens, `c` from the tile's first.  The pair and cluster kernels
+// ask for it a round ahead: from HBM it takes longer than all the rest that is done with
+// them (4096 rows x 8192 x 512 with gelu 59 us; with a residual 82, and 65 so).
+template <bool kGated, class T>
+struct FfnResidual {
+  uint2 v[2][2];
+  __device__ __forceinline__ void fetch(const FfnOut& o, int c, int tokens,
+                                        const FfnTile<kGated, T>& s) {
+    if constexpr (!kGated) {
+      if (o.residual == nullptr || !s.whole || tokens < kStageTokens) return;
+      const T* r = s.residual + c * o.ldr;
+      const T* r8 = r + 8 * o.ldr;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        const float(&w)[4] = v[j][h];
-        *reinterpret_cast<float4*>(z + j * 8 * o.ldz + h * second) =
-            make_float4(w[0], w[1], w[2], w[3]);
+        v[0][h] = *reinterpret_cast<const uint2*>(r + h * 64);
+        v[1][h] = *reinterpret_cast<const uint2*>(r8 + h * 64);
       }
+    }
+  }
+};
+
+template <class T>
+__device__ __forceinline__ F32x2 widen_pair(uint32_t w) {
+  return pair_of(widen<T>((uint16_t)w), widen<T>((uint16_t)(w >> 16)));
+}
+
+// A thread's part of 16 staged tokens, `c` from the tile's first.  All of it is there
+// (FfnTile::whole, 16 tokens), so the arithmetic of all values runs side by side.
+template <bool kGated, int kAct, class T>
+__device__ __forceinline__ void ffn_rows_whole(const FfnOut& o, uint32_t stage, int c, int tid,
+                                               const FfnTile<kGated, T>& s,
+                                               const FfnResidual<kGated, T>& res) {
+  const uint32_t at = stage + (uint32_t)(tid >> 4) * 512u + (uint32_t)(tid & 15) * 16u;
+  float v[2][2][4];
+  ld_shared_v4_f32_at<0>(at, v[0][0]);
+  ld_shared_v4_f32_at<256>(at, v[0][1]);
+  ld_shared_v4_f32_at<8 * 512>(at, v[1][0]);
+  ld_shared_v4_f32_at<8 * 512 + 256>(at, v[1][1]);
+  if constexpr (!kGated) {
+    if (o.bias != nullptr) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float(&w)[4] = v[j][i >> 1];
+          const int k = (i & 1) * 2;
+          halves_of(add2(pair_of(w[k], w[k + 1]), s.bias[i]), w[k], w[k + 1]);
+        }
+    }
+  }
+  if (o.z != nullptr) {
+    float* z = s.z + c * o.ldz;
+    float* z8 = z + 8 * o.ldz;
+    const long long second = kGated ? o.z_half : 64;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const float(&a)[4] = v[0][h];
+      const float(&b)[4] = v[1][h];
+      *reinterpret_cast<float4*>(z + h * second) = make_float4(a[0], a[1], a[2], a[3]);
+      *reinterpret_cast<float4*>(z8 + h * second) = make_float4(b[0], b[1], b[2], b[3]);
+    }
   }
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
     activate<kAct>(v[j][0]);
     if constexpr (!kGated) activate<kAct>(v[j][1]);
   }
+  T* to = s.out + c * o.ldo;
 #pragma unroll
   for (int j = 0; j < 2; ++j) {
-    T* to = out + j * 8 * o.ldo;
     if constexpr (kGated) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) v[j][0][i] *= v[j][1][i];
+      for (int i = 0; i < 4; i += 2) {
+        float(&w)[4] = v[j][0];
+        halves_of(mul2(pair_of(w[i], w[i + 1]), pair_of(v[j][1][i], v[j][1][i + 1])), w[i],
+                  w[i + 1]);
+      }
       store_four(to, v[j][0]);
     } else {
+      if (o.residual != nullptr) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float(&w)[4] = v[j][h];
-        w[0] += widen<T>((uint16_t)res[j][h].x);
-        w[1] += widen<T>((uint16_t)(res[j][h].x >> 16));
-        w[2] += widen<T>((uint16_t)res[j][h].y);
-        w[3] += widen<T>((uint16_t)(res[j][h].y >> 16));
-        store_four(to + h * 64, w);
+        for (int h = 0; h < 2; ++h) {
+          float(&w)[4] = v[j][h];
+          halves_of(add2(pair_of(w[0], w[1]), widen_pair<T>(res.v[j][h].x)), w[0], w[1]);
+          halves_of(add2(pair_of(w[2], w[3]), widen_pair<T>(res.v[j][h].y)), w[2], w[3]);
+        }
       }
+      store_four(to, v[j][0]);
+      store_four(to + 64, v[j][1]);
     }
+    to += 8 * o.ldo;
   }
-  named_bar_sync(bar, 128);
 }
 
 // The same where features or tokens (of which `tokens` are there) end, or rows lie on
@@ -212,20 +239,27 @@ __device__ __forceinline__ void ffn_rows_ragged(const FfnOut& o, uint32_t stage,
   }
 }
 
-// A group of four warps: `v` staged, finished and the staging free again.
-template <bool kGated, int kAct, class T>
-__device__ __forceinline__ void ffn_finish(const FfnOut& o, uint32_t stage, uint32_t bar,
-                                           int quarter, const float (&v)[16], long long row0,
-                                           int tokens, int feat0, int tid,
-                                           const FfnTile<kGated>& s) {
-  if (s.whole && tokens >= kStageTokens) {
-    ffn_rows_whole<kGated, kAct, T>(o, stage, bar, quarter, v, row0, feat0, tid, s);
-  } else {
-    stage_put(stage, quarter, v);
-    named_bar_sync(bar, 128);
-    ffn_rows_ragged<kGated, kAct, T>(o, stage, row0, tokens, feat0, tid);
-    named_bar_sync(bar, 128);
+// A group of four warps: `v`, 16 tokens from the tile's token c on, staged and finished.
+// kTwo: there are two stagings, taken in turn (`turn`), so that one barrier is enough --
+// who writes the same one again has passed the barrier of the other, where all that read
+// this one had come by -- and the warps overlap; else the staging is free again at the end.
+template <bool kGated, int kAct, class T, bool kTwo>
+__device__ __forceinline__ void ffn_finish(const FfnOut& o, uint32_t stage, uint32_t* turn,
+                                           uint32_t bar, int quarter, const float (&v)[16],
+                                           long long row0, int c, int tokens, int feat0, int tid,
+                                           const FfnTile<kGated, T>& s,
+                                           const FfnResidual<kGated, T>& res) {
+  if constexpr (kTwo) {
+    stage += *turn;
+    *turn ^= (uint32_t)kFfnStageBytes;
   }
+  stage_put(stage + (uint32_t)(quarter * 32 + (threadIdx.x & 31)) * 4u, v);
+  named_bar_sync(bar, 128);
+  if (s.whole && tokens >= kStageTokens)
+    ffn_rows_whole<kGated, kAct, T>(o, stage, c, tid, s, res);
+  else
+    ffn_rows_ragged<kGated, kAct, T>(o, stage, row0 + c, tokens, feat0, tid);
+  if constexpr (!kTwo) named_bar_sync(bar, 128);
 }
 
 }  // namespace b200

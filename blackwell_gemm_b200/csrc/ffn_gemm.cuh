@@ -22,8 +22,11 @@
 // the others' products.  Whichever CTA arrives last adds the parts up in their order:
 // the sums do not depend on which one it was, and nobody waits for another.
 //
-// Eight epilogue warps, two groups of four: a group takes every other 16 tokens of
-// a tile, so one group's staging barriers overlap the other's arithmetic.
+// Eight epilogue warps, two groups of four: a group takes every other 16 tokens of its
+// tile.  gated and dA have sixteen, eight for each accumulator, because a round of 16
+// tokens mostly waits (4096 rows x 8192 x 256 gated 33.5 us with eight, 29.8 so); act's
+// epilogue does not fit the registers that leaves (8192 x 1024 50.1 and 54.1), so it stages
+// its rounds in turn in two places instead.
 #pragma once
 #include "ffn_epilogue.cuh"
 
@@ -48,16 +51,16 @@ struct FfnArgs {
   unsigned long long timeout_ns;
 };
 
-// dW stages 64 columns of a warp's 32 rows; for many experts (kMany) it gives up a
-// stage for the table of their rows.
+// Four stagings of 16 tokens: one to a group of epilogue warps, or two where there are two
+// groups; dW stages 64 columns of a warp's 32 rows.  For many experts (kMany) a stage is given up for the table of their rows.
 template <int kMode, bool kMany = false>
 struct FfnCfg {
   static constexpr int kStages = kMany ? 5 : 6;
   static constexpr int kOperand = 128 * kSlabK * 2;
   static constexpr int kStageBytes = 2 * kOperand;
-  static constexpr int kEpiWarps = 8;
-  static constexpr int kThreads = 32 * (2 + kEpiWarps);
-  static constexpr int kStaging = kMode == kFfnDW ? kEpiWarps * kStoreBufBytes : 2 * kFfnStageBytes;
+  static constexpr int kSets = kMode == kFfnGated || kMode == kFfnDA ? 2 : 1;  // of eight warps
+  static constexpr int kThreads = 32 * (2 + 8 * kSets);
+  static constexpr int kStaging = kMode == kFfnDW ? 8 * kStoreBufBytes : 4 * kFfnStageBytes;
   static constexpr int kFeat = kMode == kFfnGated ? 128 : 256;  // output features of a tile
   static constexpr int smem_bytes(int experts) {
     return kStages * kStageBytes + kStaging + group_table_bytes(experts) + 1024;
@@ -114,6 +117,27 @@ struct FfnUnit {
   int blocks;  // 64-long contraction blocks
   int mma_n;
 };
+
+// a / b for 0 <= a < 2^30, b > 0.  Three of them find a unit's place, on the way of
+// every tile: by the reciprocal they take a third of the compiler's division.
+__device__ __forceinline__ int quick_div(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  int q = __float2int_rz(__fdividef((float)a, (float)b));  // off by one at the most
+  const int r = a - q * b;
+  q += r >= b ? 1 : r < 0 ? -1 : 0;
+  return q;
+}
+
+// tile_coord's bands of tile-rows.
+__device__ __forceinline__ void band_coord(int t, int tiles_m, int tiles_n, int group, int* tm,
+                                           int* tn) {
+  const int band = quick_div(t, group * tiles_n);
+  const int first = band * group, width = min(tiles_m - first, group);
+  const int r = t - band * group * tiles_n;
+  const int b = quick_div(r, width);
+  *tm = first + r - b * width;
+  *tn = (band & 1) ? tiles_n - 1 - b : b;
+}
 
 // What a pair does of a unit: contraction blocks [kb0, kb1).
 struct FfnSegment : FfnUnit {
@@ -175,8 +199,8 @@ struct FfnWalk {
     int x, y;
     if constexpr (kMode == kFfnDW) {
       const int per = a.halves * tf * tc;
-      r->e = u / per;
-      tile_coord(u - r->e * per, a.halves * tf, tc, a.group, &x, &y);
+      r->e = quick_div(u, per);
+      band_coord(u - r->e * per, a.halves * tf, tc, a.group, &x, &y);
       r->half = x >= tf;
       r->row0 = off[r->e];
       r->rows = off[r->e + 1] - r->row0;
@@ -190,8 +214,8 @@ struct FfnWalk {
       r->half = 0;
       const int first = off[e], count = off[e + 1] - first;
       const int tt = tiles[e + 1] - tiles[e];
-      const int size = ((count + tt - 1) / tt + 31) & ~31;
-      tile_coord(u - tiles[e] * tf, tt, tf, a.group, &x, &y);
+      const int size = (quick_div(count + tt - 1, tt) + 31) & ~31;
+      band_coord(u - tiles[e] * tf, tt, tf, a.group, &x, &y);
       r->row0 = first + x * size;
       r->rows = min(size, count - x * size);
       r->feat0 = y * FfnCfg<kMode>::kFeat;
@@ -218,6 +242,18 @@ struct FfnWalk {
     next_unit += pairs;
     s->kb0 = 0;
     s->kb1 = s->blocks;
+    return true;
+  }
+  // next() for those whom the segment does not concern.
+  __device__ __forceinline__ bool skip() {
+    if (pos < hi) {
+      const long long end = (pos / blocks + 1) * blocks;
+      pos = end < hi ? end : hi;
+      if (pos >= hi) e = 0;
+      return true;
+    }
+    if (next_unit >= undivided) return false;
+    next_unit += pairs;
     return true;
   }
 };
@@ -248,7 +284,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   __shared__ alignas(8) uint64_t bar_drain;
   __shared__ uint32_t tmem_slot;
   __shared__ uint32_t abort_word;
-  __shared__ uint32_t last_word[2];
+  __shared__ uint32_t last_word[4];
 
   cluster_arrive_started();
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // (warp-uniform)
@@ -266,7 +302,7 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(smem_u32(&bar_acc_full[b]), 1);
-      mbar_init(smem_u32(&bar_acc_empty[b]), 2 * C::kEpiWarps);
+      mbar_init(smem_u32(&bar_acc_empty[b]), 2 * 8);  // of both CTAs
     }
     mbar_init(smem_u32(&bar_drain), 1);
     abort_word = 0;
@@ -436,30 +472,35 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
     __syncwarp();
   } else {
     // ----------------------------------------------------------- epilogue
-    const int quarter = warp & 3, group = (warp - 2) >> 2;
+    // warps 2..9 take the tiles of the first accumulator, 10..17 of the second
+    const int quarter = warp & 3, set = (warp - 2) >> 3, group = ((warp - 2) >> 2) & 1;
     const int tid = ((warp - 2) & 3) * 32 + lane;
+    const int crew = 2 * set + group;  // whose staging, barrier and word
     const uint32_t acc_empty_leader = cluster_map(smem_u32(&bar_acc_empty[0]), 0);
     T* out = static_cast<T*>(args.o.out);
     if constexpr (kMode != kFfnDW)
       zero_unowned_rows(out, args.o.ldo, args.feat, s_off[0], s_off[args.experts], args.rows,
-                        (long long)blockIdx.x * 256 + (threadIdx.x - 64), gridDim.x * 256ll);
+                        (long long)blockIdx.x * (256 * C::kSets) + (threadIdx.x - 64),
+                        gridDim.x * (256ll * C::kSets));
     const uint32_t box = store_base + (uint32_t)(warp - 2) * kStoreBufBytes;
-    const uint32_t staging = store_base + (uint32_t)group * kFfnStageBytes;
+    constexpr bool kTwo = C::kSets == 1;
+    const uint32_t staging = store_base + (uint32_t)crew * (kTwo ? 2 : 1) * kFfnStageBytes;
+    uint32_t turn = 0;
     int it = 0;
     int ok = 1;
     const int cta = blockIdx.x;
     // What the groups of all the CTAs with a part of a divided tile count in at: true
     // for the last, who takes the sum.
     auto joined = [&]() {
-      named_bar_sync(1 + group, 128);
+      named_bar_sync(1 + crew, 128);
       if (tid == 0) {
         unsigned int* count = args.counts + w.c0 * 16 + (int)rank * 2 + group;
         const bool last = atomic_add_acq_rel(count, 1u) == (unsigned int)(w.c1 - w.c0);
         if (last) atomicExch(count, 0u);
-        last_word[group] = last;
+        last_word[crew] = last;
       }
-      named_bar_sync(1 + group, 128);
-      return last_word[group] != 0;
+      named_bar_sync(1 + crew, 128);
+      return last_word[crew] != 0;
     };
     // Column `col` of this lane's accumulator row in the slot of pair c: a pair begins at
     // most one divided tile (slot 1) and ends or crosses at most one that an
@@ -468,9 +509,9 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
       return args.slots + (((long long)(2 * c + (int)rank) * 2 + (c == w.c0 ? 1 : 0)) * 256 + col) *
                               128 + quarter * 32 + lane;
     };
-    // acc = the parts' sum, `kN` columns from col on, 64 loads in flight, added in order.
+    // acc = the parts' sum, `kN` columns from col on, 32 loads in flight, added in order.
     auto add_parts = [&](int col, auto& acc) {
-      constexpr int kN = sizeof(acc) / sizeof(float), kParts = 64 / kN;
+      constexpr int kN = sizeof(acc) / sizeof(float), kParts = 32 / kN;
 #pragma unroll
       for (int j = 0; j < kN; ++j) acc[j] = 0.0f;
 #pragma unroll 1
@@ -488,7 +529,13 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
           for (int j = 0; j < kN; ++j) acc[j] += v[i][j];
       }
     };
-    while (walk.next(args, &w)) {
+    for (;;) {
+      if (C::kSets == 2 && (it & 1) != set) {
+        if (!walk.skip()) break;
+        ++it;
+        continue;
+      }
+      if (!walk.next(args, &w)) break;
       const uint32_t buf = it & 1, acc_phase = (it >> 1) & 1;
       const bool any = w.blocks != 0;
       if (any) {
@@ -588,8 +635,8 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         // (a warp whose wait ran out still comes to its group's barriers, and
         // writes nothing)
         const int f0 = w.feat0 + (int)rank * (C::kFeat / 2);
-        FfnTile<kGated> tile;
-        ffn_tile<kGated, T>(args.o, f0, tid, tile);
+        FfnTile<kGated, T> tile;
+        ffn_tile<kGated, T>(args.o, f0, w.row0, tid, tile);
         auto load = [&](int c, float (&acc)[kStageTokens]) {
           uint32_t v[16];
           tmem_ld_32x32b_x16(tbase + c, v);
@@ -615,15 +662,20 @@ ffn_pair_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         }
         auto finish = [&](auto code) {
           constexpr int kAct = decltype(code)::value;
+          FfnResidual<kGated, T> now, next;
+          next.fetch(args.o, group * kStageTokens, w.rows - group * kStageTokens, tile);
 #pragma unroll 1
           for (int c = group * kStageTokens; c < w.mma_n; c += 2 * kStageTokens) {
+            now = next;
+            next.fetch(args.o, c + 2 * kStageTokens, w.rows - c - 2 * kStageTokens, tile);
             float acc[kStageTokens];
             if (whole)
               load(c, acc);
             else
               add_parts(c, acc);
-            ffn_finish<kGated, kAct, T>(args.o, staging, 1 + group, quarter, acc, w.row0 + c,
-                                        ok ? w.rows - c : 0, f0, tid, tile);
+            ffn_finish<kGated, kAct, T, kTwo>(args.o, staging, &turn, 1 + crew, quarter, acc,
+                                              w.row0, c, ok ? w.rows - c : 0, f0, tid, tile,
+                                              now);
           }
         };
         if constexpr (kMode == kFfnDA)

@@ -202,8 +202,8 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
         return args.slots + ((long long)c * 2 + (c == c0 ? 1 : 0)) * kTok * 128 + quarter * 32 +
                lane;
       };
-      FfnTile<kGated> tile;
-      ffn_tile<kGated, T>(o, f0, tid, tile);
+      FfnTile<kGated, T> tile;
+      ffn_tile<kGated, T>(o, f0, s.row0, tid, tile);
       auto load = [&](int c, float (&acc)[kStageTokens]) {
         uint32_t v[16];
         tmem_ld_32x32b_x16(tbase + c, v);
@@ -263,8 +263,10 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
                 for (int j = 0; j < 16; ++j) acc[j] += v[i][j];
             }
           }
-          ffn_finish<kGated, kAct, T>(o, staging, 1 + group, quarter, acc, s.row0 + c,
-                                      ok ? s.rows - c : 0, f0, tid, tile);
+          FfnResidual<kGated, T> res;
+          res.fetch(o, c, s.rows - c, tile);
+          ffn_finish<kGated, kAct, T, false>(o, staging, nullptr, 1 + group, quarter, acc, s.row0,
+                                             c, ok ? s.rows - c : 0, f0, tid, tile, res);
         }
       });
     }

@@ -588,6 +588,47 @@ __device__ __forceinline__ void ld_shared_v4_u32(uint32_t addr, uint32_t (&r)[4]
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
 
+// The same with the offset in the instruction.
+template <int kOffset>
+__device__ __forceinline__ void st_shared_f32_at(uint32_t addr, float v) {
+  asm volatile("st.shared.f32 [%0+%2], %1;" :: "r"(addr), "f"(v), "n"(kOffset) : "memory");
+}
+template <int kOffset>
+__device__ __forceinline__ void ld_shared_v4_f32_at(uint32_t addr, float (&v)[4]) {
+  asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4+%5];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]) : "r"(addr), "n"(kOffset)
+               : "memory");
+}
+
+// ------------------------------------------------ two fp32 in one instruction
+// Each half rounded to nearest as by itself.
+struct F32x2 {
+  uint64_t v;
+};
+__device__ __forceinline__ F32x2 pair_of(float lo, float hi) {
+  F32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void halves_of(F32x2 p, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(p.v));
+}
+__device__ __forceinline__ F32x2 add2(F32x2 a, F32x2 b) {
+  F32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F32x2 mul2(F32x2 a, F32x2 b) {
+  F32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F32x2 fma2(F32x2 a, F32x2 b, F32x2 c) {
+  F32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+
 __device__ __forceinline__ uint16_t ld_shared_u16(uint32_t addr) {
   uint16_t v;
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr) : "memory");
