@@ -586,7 +586,7 @@ int run_norm(const b200_tensor* tensors, int n, bool clip, float max_norm, float
     return launch(norm_finish_kernel<>, 1, kNormThreads, 0, stream, partial, partials, norm);
   for (int at = 0; at < n;) {
     CHECK(norm_tables(tensors, n, &at, &table));
-    const int blocks = std::min(table.chunks, most);
+    const int blocks = table.chunks;
     if (blocks == 0) continue;
     CHECK(launch(clip_kernel<>, blocks, kNormThreads, 0, stream, table, partial, partials,
                  max_norm, norm));
