@@ -22,6 +22,9 @@
 // the others' products.  Whichever CTA arrives last adds the parts up in their order:
 // the sums do not depend on which one it was, and nobody waits for another.
 //
+// Bound by the tensor pipe (84 to 90 % active): 4095 rows, 28672 x 4096, gated 597 us, dA
+// 672, dW 617 (1.61, 1.43, 1.56 PFLOP/s, 0.87 to 0.98 of a large library product's rate).
+//
 // Eight epilogue warps, two groups of four: a group takes every other 16 tokens of its
 // tile.  gated and dA have sixteen, eight for each accumulator, because a round of 16
 // tokens mostly waits (4096 rows x 8192 x 256 gated 33.5 us with eight, 29.8 so); act's

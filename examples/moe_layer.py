@@ -2,8 +2,8 @@
 
     python examples/moe_layer.py
 
-Training: route -> dispatch -> grouped products -> combine, with gradients in
-the experts, the router and the input.  Serving: the experts' weights are
+Training: route -> dispatch -> gated and grouped products -> combine, with gradients
+in the experts, the router and the input.  Serving: the experts' weights are
 quantised to 4 bits and laid out once; single tokens go through the same
 route, dispatch and combine, and the 4-bit products.  Prints the loss of each
 step and how far the served answers are from the 16-bit layer's.
@@ -26,7 +26,7 @@ class MoELayer(torch.nn.Module):
         kw = dict(dtype=dtype, device=device)
         self.top_k, self.hidden = top_k, hidden
         self.router = torch.nn.Parameter(torch.randn(experts, width, **kw) * width ** -0.5)
-        # gate and up projections of an expert in one matrix: one grouped product
+        # gate and up projections of an expert in one matrix
         self.up = torch.nn.Parameter(torch.randn(experts, 2 * hidden, width, **kw) * width ** -0.5)
         self.down = torch.nn.Parameter(torch.randn(experts, width, hidden, **kw) * hidden ** -0.5)
         self.up4 = self.down4 = None
@@ -37,13 +37,12 @@ class MoELayer(torch.nn.Module):
         self.down4 = bg.pack_w4(*bg.quantize_w4(self.down.detach(), group))
 
     def experts(self, x, offsets):
-        serve = self.up4 is not None and not torch.is_grad_enabled()
-        h = (bg.matmul_b200_w4(x, self.up4, offsets) if serve else
-             bg.matmul_b200_grouped(x, self.up.transpose(1, 2), offsets))
-        gate, up = h.split(self.hidden, dim=1)
-        h = torch.nn.functional.silu(gate) * up
-        return (bg.matmul_b200_w4(h, self.down4, offsets) if serve else
-                bg.matmul_b200_grouped(h, self.down.transpose(1, 2), offsets))
+        if self.up4 is not None and not torch.is_grad_enabled():
+            gate, up = bg.matmul_b200_w4(x, self.up4, offsets).split(self.hidden, dim=1)
+            return bg.matmul_b200_w4(torch.nn.functional.silu(gate) * up, self.down4, offsets)
+        gate, up = self.up.transpose(1, 2).split(self.hidden, dim=2)
+        h = bg.matmul_b200_gated(x, gate, up, offsets)
+        return bg.matmul_b200_grouped(h, self.down.transpose(1, 2), offsets)
 
     def forward(self, x):
         routing = bg.route_b200(x.float() @ self.router.float().T, self.top_k)
