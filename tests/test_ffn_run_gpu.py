@@ -315,7 +315,9 @@ def finish(seconds):
         time.sleep(0.001)
 
 
-@pytest.mark.parametrize("rows,n,k,steps", [(200, 512, 512, 6000), (600, 1100, 640, 3000)])
+# clusters of single CTAs, of pairs, whole and left-over tiles
+@pytest.mark.parametrize("rows,n,k,steps", [(200, 512, 512, 6000), (256, 8192, 512, 6000),
+                                            (600, 1100, 640, 3000), (512, 2048, 2048, 3000)])
 def test_many_steps(rows, n, k, steps):
     x, g, u = randn(rows, k), randn(n, k, scale=k ** -0.5), randn(n, k, seed=1, scale=k ** -0.5)
     with torch.no_grad():
@@ -327,6 +329,48 @@ def test_many_steps(rows, n, k, steps):
                 finish(20)
         finish(20)
     assert torch.equal(first, got) and bool(torch.isfinite(back).all())
+
+
+def test_no_expert():
+    x = randn(5, 16).requires_grad_()
+    bank = randn(0, 16, 8).requires_grad_()
+    off = torch.zeros(1, dtype=torch.int32, device="cuda")
+    h = bg.matmul_b200_gated(x, bank, bank, off)
+    dx, db = torch.autograd.grad(h, (x, bank), torch.ones_like(h))
+    assert h.shape == (5, 8) and not h.any() and not dx.any() and db.shape == (0, 16, 8)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 256, 512), (300, 260, 64), (33, 75, 128)])
+def test_result_over_its_residual(m, n, k):
+    """The C ABI's C may be the residual itself."""
+    x, w, r = randn(m, k), randn(n, k, seed=1, scale=k ** -0.5), randn(m, n, seed=2)
+    for kernel in (1, 2, 3):
+        capi.ffn_set_kernel(kernel)
+        want = bg.matmul_b200_act(x, w.t(), residual=r, activation="silu")
+        c = r.clone()
+        st = capi.lib().b200_ffn_act(x.data_ptr(), w.data_ptr(), None, c.data_ptr(), c.data_ptr(),
+                                     None, m, n, k, k, k, n, n, 0, 2, capi.BF16,
+                                     torch.cuda.current_stream().cuda_stream)
+        assert st == capi.OK and torch.equal(c, want)
+
+
+def test_rows_and_columns_past_the_result_are_left():
+    """Strided results through the C ABI: what lies between rows and after them stays."""
+    m, n, k = 70, 72, 128
+    x, w = randn(m, k), randn(n, k, seed=1, scale=0.1)
+    want = bg.matmul_b200_act(x, w.t(), activation="relu")
+    for ld in (80, 75, 72):
+        for kernel in (1, 2, 3):
+            capi.ffn_set_kernel(kernel)
+            c = torch.full((m + 3, ld), 7.0, device="cuda").bfloat16()
+            z = torch.full((m + 3, 76), 5.0, device="cuda")
+            st = capi.lib().b200_ffn_act(x.data_ptr(), w.data_ptr(), None, None, c.data_ptr(),
+                                         z.data_ptr(), m, n, k, k, k, 0, ld, 76, 1, capi.BF16,
+                                         torch.cuda.current_stream().cuda_stream)
+            assert st == capi.OK
+            assert float((c[:m, :n].double() - want.double()).norm()) <= 2.0 ** -8 * float(want.double().norm())
+            assert bool((c[m:] == 7).all()) and bool((c[:, n:] == 7).all())
+            assert bool((z[m:] == 5).all()) and bool((z[:, n:] == 5).all())
 
 
 # -------------------------------------------------------------------- derivatives
