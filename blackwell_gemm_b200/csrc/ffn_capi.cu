@@ -523,9 +523,10 @@ int run_grad(FfnGradArgs a, bool gated, int act, void* dbias, int dtype, cudaStr
   CHECK(half ? launch_grad<__half>(a, gated, act, blocks, stream)
              : launch_grad<__nv_bfloat16>(a, gated, act, blocks, stream));
   if (a.partial == nullptr) return B200_OK;
-  return half ? launch(ffn_bias_kernel<__half>, (int)ceil_div(a.feat, 32), 256, 0, stream, a.partial, row_blocks,
+  const int columns = (int)ceil_div(a.feat, 32);
+  return half ? launch(ffn_bias_kernel<__half>, columns, 256, 0, stream, a.partial, row_blocks,
                        a.feat, static_cast<__half*>(dbias))
-              : launch(ffn_bias_kernel<__nv_bfloat16>, (int)ceil_div(a.feat, 32), 256, 0, stream, a.partial,
+              : launch(ffn_bias_kernel<__nv_bfloat16>, columns, 256, 0, stream, a.partial,
                        row_blocks, a.feat, static_cast<__nv_bfloat16*>(dbias));
 }
 
@@ -765,8 +766,9 @@ int run_dw(const void* dz, const void* A, const int* offsets, void* dW, int halv
   a.cols = K;
   a.halves = halves;
   a.o.out = tma ? nullptr : dW;
-  return experts > kFewExperts ? launch_pair<kFfnDW, true, T>(a, tz, ta, tz, tz, ts, v, *d, stream)
-                               : launch_pair<kFfnDW, false, T>(a, tz, ta, tz, tz, ts, v, *d, stream);
+  if (experts > kFewExperts)
+    return launch_pair<kFfnDW, true, T>(a, tz, ta, tz, tz, ts, v, *d, stream);
+  return launch_pair<kFfnDW, false, T>(a, tz, ta, tz, tz, ts, v, *d, stream);
 }
 
 }  // namespace

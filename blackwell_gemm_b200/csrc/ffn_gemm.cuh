@@ -55,7 +55,8 @@ struct FfnArgs {
 };
 
 // Four stagings of 16 tokens: one to a group of epilogue warps, or two where there are two
-// groups; dW stages 64 columns of a warp's 32 rows.  For many experts (kMany) a stage is given up for the table of their rows.
+// groups; dW stages 64 columns of a warp's 32 rows.  For many experts (kMany) a stage is
+// given up for the table of their rows.
 template <int kMode, bool kMany = false>
 struct FfnCfg {
   static constexpr int kStages = kMany ? 5 : 6;

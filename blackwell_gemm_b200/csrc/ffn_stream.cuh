@@ -59,7 +59,8 @@ ffn_stream_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   const int lane = threadIdx.x & 31;
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t staging_base = smem_base + kStages * C::kStageBytes;
-  int* s_off = reinterpret_cast<int*>(smem_raw + (staging_base + 2 * kFfnStageBytes - smem_u32(smem_raw)));
+  int* s_off = reinterpret_cast<int*>(
+      smem_raw + (staging_base + 2 * kFfnStageBytes - smem_u32(smem_raw)));
   int* s_tiles = s_off + args.experts + 1;
 
   if (threadIdx.x == 0) {

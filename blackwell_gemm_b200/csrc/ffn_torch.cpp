@@ -79,7 +79,8 @@ struct ActMatmul : torch::autograd::Function<ActMatmul> {
     // What a gradient that nobody asks for would need is not kept.
     const bool keep_a = b.requires_grad(), keep_w = a.requires_grad();
     // (detached: a view made here would answer for a weight changed meanwhile in its words)
-    ctx->save_for_backward({keep_a ? ra.t : at::Tensor(), keep_w ? rw.t.detach() : at::Tensor(), z});
+    ctx->save_for_backward(
+        {keep_a ? ra.t : at::Tensor(), keep_w ? rw.t.detach() : at::Tensor(), z});
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = bias.defined();
     ctx->saved_data["residual"] = residual.defined();

@@ -43,7 +43,8 @@ inline void check_16bit(const at::Tensor& t, const char* who, const char* name) 
               " must be bfloat16 or float16");
 }
 
-inline void check_same(const at::Tensor& t, const at::Tensor& like, const char* who, const char* name) {
+inline void check_same(const at::Tensor& t, const at::Tensor& like, const char* who,
+                       const char* name) {
   TORCH_CHECK(t.device() == like.device(), who, ": ", name, " is on another device");
   TORCH_CHECK(t.scalar_type() == like.scalar_type(), who, ": ", name, " has another dtype");
 }
