@@ -11,7 +11,7 @@
 //
 // Bound by HBM as long as the weights are most of what is read: the streaming kernel
 // spreads them over every SM evenly but joins parts through L2, which took 10 to 25 us
-// from 64 tokens on.  128 rows x 4096 x 14336: 27 us (4.5 TB/s; streaming 44, pairs 68),
+// from 64 tokens on.  128 rows x 4096 x 14336: 25.5 us (4.7 TB/s; streaming 44, pairs 68),
 // 256 rows x 2048 x 8192: 17 us (50 and 48).
 #pragma once
 #include "ffn_gemm.cuh"
@@ -34,12 +34,20 @@ struct FfnClusterArgs {
 
 template <bool kPair>
 struct FfnClusterCfg {
-  static constexpr int kMaxStages = 12;
+  static constexpr int kMaxStages = 14;
   static constexpr int kWeight = 128 * kSlabK * 2;  // per CTA and stage
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
-  static constexpr int kRing = 12 * kWeight;  // (at least what the exchange needs: 112 KiB)
-  static constexpr int kSmem = kRing + 2 * 2 * kFfnStageBytes + 1024;
+  // The ring takes all the shared memory; when its work is done (every product has
+  // completed, so every copy has landed) the parts' exchange, at most 14 x 8 KiB at 8 parts
+  // of 256 tokens, and behind it the epilogue's stagings take its place.  Against stagings
+  // of their own beside 12 stages: 4096 x 14336 at 200 rows 33.2 -> 30.3 us, at 128 rows
+  // 26.1 -> 25.5; 16384 x 4096 at 128 rows 29.1 -> 28.2; one row the same within 3%.
+  static constexpr int kRing = 14 * kWeight;
+  static constexpr int kStagingAt = 8 * kWeight;
+  static constexpr int kSmem = kRing + 1024;
+  static_assert(14 * kFfnStageBytes <= kStagingAt &&
+                kStagingAt + 2 * 2 * kFfnStageBytes <= kRing, "what takes the ring's place");
 };
 
 // tmap_w0, tmap_w1: the weights (k, n, 1): gated gate and up, box 64 x 64; act box
@@ -72,7 +80,7 @@ ffn_cluster_kernel(const __grid_constant__ CUtensorMap tmap_w0,
   const int part = (int)(crank / kCtas), splits = args.splits;
   const int tile = blockIdx.x / (splits * kCtas);
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t staging_base = smem_base + C::kRing;
+  const uint32_t staging_base = smem_base + C::kStagingAt;
   const uint32_t stages = args.stages;
 
   if (threadIdx.x == 0) {
