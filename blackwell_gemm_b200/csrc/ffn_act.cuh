@@ -182,4 +182,12 @@ __device__ __forceinline__ void activate_slope(const float (&z)[kN], float (&a)[
   }
 }
 
+// d act'(z).  relu lets through or not: what comes back to a unit that it shuts is zero
+// whatever arrives, where inf * 0 would be NaN.
+template <int kAct>
+__device__ __forceinline__ float times_slope(float d, float slope) {
+  if constexpr (kAct == B200_ACT_RELU) return slope > 0.0f ? d : 0.0f;
+  return d * slope;
+}
+
 }  // namespace b200

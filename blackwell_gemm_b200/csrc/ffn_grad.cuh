@@ -106,7 +106,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
         activate_slope<kAct>(z, g, slope);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          slope[i] = d[i] * u[i] * slope[i];
+          slope[i] = times_slope<kAct>(d[i] * u[i], slope[i]);
           g[i] = d[i] * g[i];
         }
         T* to = static_cast<T*>(a.dz) + r * a.lddz + f;
@@ -118,7 +118,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
           load_eight(a.z + r * a.ldz + f, n, z);
           activate_slope<kAct>(z, y, slope);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= slope[i];
+          for (int i = 0; i < 8; ++i) d[i] = times_slope<kAct>(d[i], slope[i]);
         }
         if (a.dz != nullptr) store_eight(static_cast<T*>(a.dz) + r * a.lddz + f, n, d);
 #pragma unroll

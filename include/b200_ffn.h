@@ -27,7 +27,7 @@ extern "C" {
 
 /* Activations.  s: the logistic function, Phi: the normal distribution's. */
 #define B200_ACT_NONE 0
-#define B200_ACT_RELU 1      /* max(z, 0); slope 0 at 0 */
+#define B200_ACT_RELU 1      /* max(z, 0); up to z = 0 nothing comes back, inf and NaN neither */
 #define B200_ACT_SILU 2      /* z s(z) */
 #define B200_ACT_GELU 3      /* z Phi(z) */
 #define B200_ACT_GELU_TANH 4 /* z (1 + tanh(c (z + 0.044715 z^3))) / 2, c = sqrt(2 / pi) */
