@@ -77,10 +77,6 @@ __device__ __forceinline__ float normal_cdf(float z, float* bell) {
   return z < 0.0f ? tail : 1.0f - tail;
 }
 
-__device__ __forceinline__ float tanh_argument(float z) {
-  return 2.0f * kRoot2OverPi * z * fmaf(0.044715f * z, z, 1.0f);
-}
-
 // The same for two values at a time, where instructions are what is short (the products'
 // epilogues).
 __device__ __forceinline__ F32x2 both(float v) { return pair_of(v, v); }
@@ -167,10 +163,12 @@ __device__ __forceinline__ void activate_slope(const float (&z)[kN], float (&a)[
       a[i] = z[i] * p;
       slope[i] = fmaf(z[i] * 0.39894228040143268f, bell, p);
     } else if constexpr (kAct == B200_ACT_GELU_TANH) {
+      // (held at 200, |z| = 67: s r is zero from there on, and stays a factor of something finite)
+      const float q = fminf(0.044715f * z[i] * z[i], 200.0f), y = 2.0f * kRoot2OverPi * z[i];
       float s, r;
-      logistic_both(tanh_argument(z[i]), &s, &r);
+      logistic_both(fmaf(y, q, y), &s, &r);
       a[i] = z[i] * s;
-      slope[i] = fmaf(a[i] * r, 2.0f * kRoot2OverPi * fmaf(0.134145f * z[i], z[i], 1.0f), s);
+      slope[i] = fmaf(a[i] * r, fmaf(6.0f * kRoot2OverPi, q, 2.0f * kRoot2OverPi), s);
     } else if constexpr (kAct == B200_ACT_SIGMOID) {
       float r;
       logistic_both(z[i], &a[i], &r);
