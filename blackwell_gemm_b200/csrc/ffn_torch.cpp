@@ -349,35 +349,96 @@ Flat flatten(const std::vector<at::Tensor>& grads, bool written, const char* who
   return f;
 }
 
-// No element may be scaled twice: seen where tensors without gaps overlap and where
-// two with gaps begin at the same element.  (These may interleave, as columns do.)
-void check_apart(const Flat& f, const char* who) {
-  struct Span {
-    const char *begin, *end;
+// Where a tensor's bytes lie: begin + the sum of stride k, 0 <= k < count, over the terms.
+struct Bytes {
+  const char *begin, *end;
+  bool dense;  // every byte from begin to end
+  const at::Tensor* t;
+};
+
+Bytes bytes_of(const at::Tensor& t) {
+  const char* p = static_cast<const char*>(t.data_ptr());
+  const bool dense = t.is_non_overlapping_and_dense();
+  int64_t last = dense ? t.numel() - 1 : 0;
+  for (int64_t i = 0; i < t.dim() && !dense; ++i) last += (t.size(i) - 1) * t.stride(i);
+  return {p, p + (last + 1) * (int64_t)t.element_size(), dense, &t};
+}
+
+// Whether two tensors have a byte in common: whether the terms of the one less those of
+// the other can make the distance of their beginnings.  A search from the largest stride
+// down, in which each term has only the few values that leave a distance the rest can
+// make; one that takes too long (strides without order among many dimensions) counts as
+// one that was found.
+struct Meeting {
+  struct Term {
+    int64_t stride, lo, hi;
+    int64_t least, most;  // what the smaller strides' terms make together
   };
-  std::vector<Span> spans;
-  spans.reserve(f.list.size());
-  auto apart = [&]() {
-    auto before = [](const Span& a, const Span& b) { return a.begin < b.begin; };
-    if (!std::is_sorted(spans.begin(), spans.end(), before))
-      std::sort(spans.begin(), spans.end(), before);
-    for (size_t i = 1; i < spans.size(); ++i)
-      TORCH_CHECK(spans[i].begin >= spans[i - 1].end && spans[i].begin != spans[i - 1].begin, who,
-                  ": gradients must not share memory");
-  };
-  // (the copies are memory of their own)
-  for (const b200_tensor& t : f.list) {
-    const char* p = static_cast<const char*>(t.data);
-    spans.push_back({p, p + t.count * (t.type == B200_FP32 ? 4 : 2)});
+  std::vector<Term> terms;
+  int budget = 100000;
+
+  void add(int64_t stride, int64_t lo, int64_t hi) {
+    for (Term& t : terms)
+      if (t.stride == stride) {
+        t.lo += lo;
+        t.hi += hi;
+        return;
+      }
+    terms.push_back({stride, lo, hi, 0, 0});
   }
-  apart();
-  if (f.back.empty()) return;
-  spans.clear();
-  for (const auto& [to, from] : f.back) {
-    const char* p = static_cast<const char*>(to.data_ptr());
-    spans.push_back({p, p});
+  void add(const Bytes& b, int sign) {
+    auto term = [&](int64_t stride, int64_t count) {
+      if (count > 1 && stride > 0)
+        add(stride, sign < 0 ? -(count - 1) : 0, sign < 0 ? 0 : count - 1);
+    };
+    const int64_t size = b.t->element_size();
+    term(1, b.dense ? b.end - b.begin : size);
+    for (int64_t i = 0; i < b.t->dim() && !b.dense; ++i)
+      term(b.t->stride(i) * size, b.t->size(i));
   }
-  apart();
+  bool reach(size_t i, int64_t distance) {
+    if (i == terms.size()) return distance == 0;
+    if (--budget < 0) return true;
+    const Term& t = terms[i];
+    auto floor_div = [](int64_t a, int64_t b) { return a / b - (a % b < 0); };
+    const int64_t lo = std::max(t.lo, -floor_div(t.most - distance, t.stride)),
+                  hi = std::min(t.hi, floor_div(distance - t.least, t.stride));
+    for (int64_t k = lo; k <= hi; ++k)
+      if (reach(i + 1, distance - k * t.stride)) return true;
+    return false;
+  }
+  static bool found(const Bytes& a, const Bytes& b) {
+    if (a.dense && b.dense) return true;  // (whose extents cross)
+    Meeting m;
+    m.add(a, 1);
+    m.add(b, -1);
+    std::sort(m.terms.begin(), m.terms.end(),
+              [](const Term& x, const Term& y) { return x.stride > y.stride; });
+    int64_t least = 0, most = 0;
+    for (size_t i = m.terms.size(); i-- > 0;) {
+      Term& t = m.terms[i];
+      t.least = least;
+      t.most = most;
+      least += t.lo * t.stride;
+      most += t.hi * t.stride;
+    }
+    return m.reach(0, b.begin - a.begin);
+  }
+};
+
+// No element may be scaled twice, nor counted twice in the norm.  (Tensors with gaps may
+// interleave, as columns do.)
+void check_apart(const std::vector<at::Tensor>& grads, const char* who) {
+  std::vector<Bytes> spans;
+  spans.reserve(grads.size());
+  for (const at::Tensor& g : grads)
+    if (g.numel() != 0) spans.push_back(bytes_of(g));
+  auto before = [](const Bytes& a, const Bytes& b) { return a.begin < b.begin; };
+  if (!std::is_sorted(spans.begin(), spans.end(), before))
+    std::sort(spans.begin(), spans.end(), before);
+  for (size_t i = 0; i < spans.size(); ++i)
+    for (size_t j = i + 1; j < spans.size() && spans[j].begin < spans[i].end; ++j)
+      TORCH_CHECK(!Meeting::found(spans[i], spans[j]), who, ": gradients must not share memory");
 }
 
 // Where the work goes; nowhere yet if the checks are going to refuse it.
@@ -401,7 +462,7 @@ at::Tensor clip_grads_b200(const std::vector<at::Tensor>& grads, double max_norm
   TORCH_CHECK(max_norm >= 0, kClip, ": max_norm must not be negative");
   const c10::cuda::OptionalCUDAGuard guard(device_of(grads));
   const Flat f = flatten(grads, true, kClip);
-  check_apart(f, kClip);
+  check_apart(grads, kClip);
   auto norm = fresh({}, at::kFloat, grads[0]);
   check_status(b200_clip_grads(f.list.data(), (int)f.list.size(), (float)max_norm,
                                norm.data_ptr<float>(), current_stream()),

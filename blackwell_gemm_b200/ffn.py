@@ -73,8 +73,9 @@ def clip_grads_b200(grads, max_norm: float):
     before that, a 0-d float32 tensor: grad_norm_b200 and the scaling in two launches
     (for each 320 tensors), without a wait for the device.  Nothing is written where
     the norm is within max_norm.  A norm that is NaN makes every gradient NaN, an
-    infinite one zero, and NaN where it was infinite.  Tensors must not share memory;
-    one with gaps between its elements goes through a copy."""
+    infinite one zero, and NaN where it was infinite.  Tensors that share memory are
+    refused (rows, columns and planes that lie between one another's do not); one with
+    gaps between its elements goes through a copy."""
     return _ext().clip_grads_b200(_list(grads), max_norm)
 
 
