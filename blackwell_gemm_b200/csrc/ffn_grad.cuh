@@ -34,13 +34,13 @@ struct FfnGradArgs {
 
 __device__ __forceinline__ void load_eight(const float* p, int n, float (&v)[8]) {
   if (n >= 8) {
-    const float4 a = __ldg(reinterpret_cast<const float4*>(p));
-    const float4 b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+    const float4 a = __ldcg(reinterpret_cast<const float4*>(p));
+    const float4 b = __ldcg(reinterpret_cast<const float4*>(p) + 1);
     v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
     v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldg(p + i) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? __ldcg(p + i) : 0.0f;
   }
 }
 
@@ -48,7 +48,7 @@ template <class T>
 __device__ __forceinline__ void load_eight(const T* p, int n, float (&v)[8]) {
   const uint16_t* h = reinterpret_cast<const uint16_t*>(p);
   if (n >= 8) {
-    const uint4 w = __ldg(reinterpret_cast<const uint4*>(h));
+    const uint4 w = __ldcg(reinterpret_cast<const uint4*>(h));
     const uint32_t x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -57,7 +57,7 @@ __device__ __forceinline__ void load_eight(const T* p, int n, float (&v)[8]) {
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = i < n ? widen<T>(__ldg(h + i)) : 0.0f;
+    for (int i = 0; i < 8; ++i) v[i] = i < n ? widen<T>(__ldcg(h + i)) : 0.0f;
   }
 }
 
@@ -146,7 +146,7 @@ ffn_grad_kernel(const FfnGradArgs a) {
 // sums in order, and the eight of them in order.
 template <class T>
 __global__ void __launch_bounds__(256)
-ffn_bias_kernel(const float* __restrict__ partial, int blocks, int feat, T* __restrict__ dbias) {
+ffn_bias_kernel(const float* partial, int blocks, int feat, T* __restrict__ dbias) {
   __shared__ float sums[8][32];
   grid_wait();
   grid_launch_next();
@@ -155,7 +155,7 @@ ffn_bias_kernel(const float* __restrict__ partial, int blocks, int feat, T* __re
   float s = 0.0f;
   if (col < feat) {
 #pragma unroll 4
-    for (int b = part; b < blocks; b += 8) s += partial[(long long)b * feat + col];
+    for (int b = part; b < blocks; b += 8) s += __ldcg(partial + (long long)b * feat + col);
   }
   sums[part][lane] = s;
   __syncthreads();

@@ -125,7 +125,7 @@ __device__ __forceinline__ double norm_chunk(const T* p, int n) {
   for (; i + (kDepth - 1) * kNormThreads < vectors; i += kDepth * kNormThreads) {
     NormVector<T> x[kDepth];
 #pragma unroll
-    for (int j = 0; j < kDepth; ++j) x[j].w = __ldg(q + i + j * kNormThreads);
+    for (int j = 0; j < kDepth; ++j) x[j].w = __ldcg(q + i + j * kNormThreads);
 #pragma unroll
     for (int j = 0; j < kDepth; ++j) {
       float v[kN];
@@ -135,7 +135,7 @@ __device__ __forceinline__ double norm_chunk(const T* p, int n) {
   }
   for (; i < vectors; i += kNormThreads) {
     NormVector<T> x;
-    x.w = __ldg(q + i);
+    x.w = __ldcg(q + i);
     float v[kN];
     x.widen_all(v);
     sum += norm_add(v);

@@ -10,8 +10,7 @@ namespace b200 {
 // 64-bit offsets as the kernels read them: what 32 bits do not hold becomes
 // something outside the rows, which build_groups clamps and reports.
 __global__ void __launch_bounds__(256)
-narrow_offsets_kernel(const long long* __restrict__ offsets, long long stride, int count,
-                      int* __restrict__ out) {
+narrow_offsets_kernel(const long long* offsets, long long stride, int count, int* out) {
   grid_wait();
   grid_launch_next();
   for (int i = threadIdx.x; i < count; i += 256)
@@ -26,9 +25,8 @@ narrow_offsets_kernel(const long long* __restrict__ offsets, long long stride, i
 // by memory: each element read and written once.  With offsets, a bank: the
 // matrices of experts without rows are left out.
 __global__ void __launch_bounds__(256)
-align_rows_kernel(const uint16_t* __restrict__ src, long long matrix_stride, long long row_stride,
-                  uint16_t* __restrict__ dst, int matrices, int rows, int cols, int ld,
-                  const int* __restrict__ offsets) {
+align_rows_kernel(const uint16_t* src, long long matrix_stride, long long row_stride, uint16_t* dst,
+                  int matrices, int rows, int cols, int ld, const int* offsets) {
   grid_wait();
   grid_launch_next();
   const int groups = ld / 8;
@@ -47,9 +45,9 @@ align_rows_kernel(const uint16_t* __restrict__ src, long long matrix_stride, lon
       const uint32_t* words = reinterpret_cast<const uint32_t*>(at & ~3ull);
       uint32_t v[5];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = __ldg(words + j);
+      for (int j = 0; j < 4; ++j) v[j] = __ldcg(words + j);
       if (at & 2) {
-        v[4] = __ldg(words + 4);
+        v[4] = __ldcg(words + 4);
 #pragma unroll
         for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(v[j], v[j + 1], 16);
       } else {

@@ -274,7 +274,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteAr
     int all = 0, before = 0;
 #pragma unroll 16
     for (int b = i / a.experts; b < (int)gridDim.x; b += shares) {
-      const int n = __ldg(a.counts + (long long)b * a.experts + e);
+      const int n = __ldcg(a.counts + (long long)b * a.experts + e);
       all += n;
       before += b < (int)blockIdx.x ? n : 0;
     }
@@ -302,7 +302,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_rank_kernel(const RouteAr
 //   over all:         p_e ([e chosen] dw_e - sum_j w_j dw_j)
 template <int kPer>
 __global__ void __launch_bounds__(256)
-route_grad_kernel(const RouteArgs a, const float* __restrict__ dweights, void* dlogits) {
+route_grad_kernel(const RouteArgs a, const float* dweights, void* dlogits) {
   grid_wait();
   grid_launch_next();
   const int lane = threadIdx.x & 31;
@@ -388,7 +388,7 @@ __device__ __forceinline__ Pack<T, kVec> load_pack(const void* base, long long i
   Pack<T, kVec> p;
   if constexpr (kVec == 8)
     *reinterpret_cast<uint4*>(&p) =
-        __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + i));
+        __ldcg(reinterpret_cast<const uint4*>(static_cast<const T*>(base) + i));
   else
     p.v[0] = static_cast<const T*>(base)[i];
   return p;
@@ -420,7 +420,7 @@ __device__ __forceinline__ void load_slots(const MoveArgs& a, long long t, int* 
 // names row r, if there is any: memory that nobody cleared, so an entry counts
 // only where that slot's row is r.
 __global__ void __launch_bounds__(256)
-mark_rows_kernel(const int* __restrict__ rows, int* __restrict__ named, int pairs) {
+mark_rows_kernel(const int* rows, int* named, int pairs) {
   grid_wait();
   grid_launch_next();
   for (long long i = blockIdx.x * 256ll + threadIdx.x; i < pairs; i += gridDim.x * 256ll) {

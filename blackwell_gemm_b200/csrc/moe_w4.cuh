@@ -1616,9 +1616,8 @@ w4_wide_kernel(const __grid_constant__ CUtensorMap tmap_t, const StreamArgs args
 // record; rows and k past the matrix get scale 0 and q = 8.  A zero point above
 // 15 is reported in the device's error word.
 __global__ void __launch_bounds__(256)
-w4_pack_kernel(const uint8_t* __restrict__ q, const uint16_t* __restrict__ scales,
-               const uint8_t* __restrict__ zeros, uint8_t* __restrict__ out, int N, int K, int group,
-               int blocks, int red_blocks, int record_bytes, int* status) {
+w4_pack_kernel(const uint8_t* q, const uint16_t* scales, const uint8_t* zeros, uint8_t* out, int N,
+               int K, int group, int blocks, int red_blocks, int record_bytes, int* status) {
   grid_wait();
   grid_launch_next();
   const long long rec = blockIdx.x;

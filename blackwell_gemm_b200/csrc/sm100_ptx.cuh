@@ -452,7 +452,9 @@ __device__ __forceinline__ void st_shared_v2(uint32_t addr, uint32_t a, uint32_t
 // --------------------------------------------------- programmatic launch order
 // A kernel launched with programmatic stream serialization may start while
 // the one before it is still running: grid_wait returns when that one has
-// finished and its writes are visible (nothing of its may be read before);
+// finished and its writes are visible (nothing of its may be read before, nor
+// through the non-coherent path, by __ldg or a const __restrict__ parameter:
+// that is for memory which nobody writes while the kernel lives);
 // grid_launch_next lets the next such kernel start.  Without the launch
 // attribute both do nothing.
 __device__ __forceinline__ void grid_wait() {
