@@ -61,8 +61,9 @@ __device__ __forceinline__ void logistic_both(float z, float* s, float* rest) {
 }
 
 // Phi(z), and exp(-z^2 / 2) on the way: Phi(-x) exp(x^2 / 2) is smooth in t =
-// 1 / (1 + 0.36 x) over [0, inf); t times a polynomial of degree 6, fitted to it with
-// equal relative errors (Lawson's weights), is off by 9e-7 of the value at most.
+// 1 / (1 + 0.36 x); t times a polynomial of degree 6, fitted to it with equal relative
+// errors (Lawson's weights), is off by 9e-7 of the value at most up to x = 14.  (From 13.2
+// on the exponential is below 2^-126 and taken for zero.)
 __device__ __forceinline__ float normal_cdf(float z, float* bell) {
   const float t = fast_rcp(fmaf(0.36f, fabsf(z), 1.0f));
   float p = 0.0470560668f;

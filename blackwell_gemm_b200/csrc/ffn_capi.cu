@@ -417,7 +417,10 @@ void by_act(int act, F&& f) {
 // in short contractions, and up to 256 where half of the pairs would have no tile (8 x
 // 14336 x 4096 gated, 512 rows: 297 us, pairs 330; 1024 rows 361 and 332; 32 x 1032 x
 // 1032, 1024 rows 30.5 and 31.9, 2048 rows 34.8 and 33.4; 4 x 744 x 6200, 400 rows 29
-// and 36).
+// and 36).  Where the steps lie, streaming's time over the pairs', banks of 8 x 8192, 16 x
+// 4096, 32 x 1032 and 64 x 1024 features, skewed counts: K = 1032 at 32 rows an expert 0.90
+// to 1.02, at 48 0.99 to 1.09; K = 2048 to 3584 at 48 0.90 to 1.01, at 64 (the pairs', by
+// this rule) 0.92 to 1.03; K = 4096 and 6144 at 64 0.92 to 1.02, at 80 1.04 to 1.20.
 template <bool kGated>
 bool use_stream(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
                 const FfnDevice& d) {
@@ -426,7 +429,8 @@ bool use_stream(const FfnCall& c, const ClusterPlan& plan, const DeviceView& v,
   if (c.offsets != nullptr) {
     if (c.rows <= (c.K >= 4096 ? 64ll : 48ll) * c.experts) return true;
     return c.rows <= 256ll * c.experts &&
-           2 * c.experts * ceil_div(c.N, kGated ? 128 : 256) <= d.pairs[kFfnAct];
+           2 * c.experts * ceil_div(c.N, kGated ? 128 : 256) <=
+               d.pairs[kGated ? kFfnGated : kFfnAct];
   }
   if (c.rows > 64) return false;
   const long long units = ceil_div(c.N, kGated ? 64 : 128), items = units * ceil_div(c.K, kSlabK);

@@ -24,7 +24,7 @@ struct FfnClusterArgs {
   int halves;      // dA: 1 or 2
   int splits;      // parts of a tile
   int tiles_t;     // token tiles, of `tokens` rows each but the last
-  int tokens;      // a multiple of 32, up to 256
+  int tokens;      // a multiple of 16 (pairs: 32), up to 256
   int stages, stage_bytes;
   int box;         // rows of a token box: a part's tokens of a stage are one box
   FfnOut o;
@@ -34,16 +34,17 @@ struct FfnClusterArgs {
 
 template <bool kPair>
 struct FfnClusterCfg {
-  static constexpr int kMaxStages = 14;
   static constexpr int kWeight = 128 * kSlabK * 2;  // per CTA and stage
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = 32 * (2 + kEpiWarps);
   // The ring takes all the shared memory; when its work is done (every product has
   // completed, so every copy has landed) the parts' exchange, at most 14 x 8 KiB at 8 parts
-  // of 256 tokens, and behind it the epilogue's stagings take its place.  Against stagings
-  // of their own beside 12 stages: 4096 x 14336 at 200 rows 33.2 -> 30.3 us, at 128 rows
-  // 26.1 -> 25.5; 16384 x 4096 at 128 rows 29.1 -> 28.2; one row the same within 3%.
-  static constexpr int kRing = 14 * kWeight;
+  // of 256 tokens, and behind it the epilogue's stagings take its place.  A stage is 18 KiB
+  // (boxes of 16 tokens) to 48 (256), so there are 12 of them to 4.  Against stagings of
+  // their own beside a ring of 192 KiB (10 to 4): 4096 x 14336 at 200 rows 33.2 -> 30.3 us,
+  // at 128 rows 26.1 -> 25.5; 16384 x 4096 at 128 rows 29.1 -> 28.2; one row the same within 3%.
+  static constexpr int kRing = 224 * 1024;
+  static constexpr int kMaxStages = kRing / (kWeight + 16 * 128);
   static constexpr int kStagingAt = 8 * kWeight;
   static constexpr int kSmem = kRing + 1024;
   static_assert(14 * kFfnStageBytes <= kStagingAt &&
