@@ -52,7 +52,7 @@ int b200_ffn_gated(const void* A, const void* Wg, const void* Wu, const int* off
                    int dtype, void* stream);
 
 /* From the gradient of b200_ffn_act's C that of its product: dz = dC * act'(z),
- * rounded (dz: rows x lddz, 16-byte aligned, lddz >= N a multiple of 8; or NULL),
+ * rounded (fp16: infinite beyond 65504; dz: rows x lddz, 16-byte aligned, lddz >= N a multiple of 8; or NULL),
  * and dbias = the unrounded sum of its rows, rounded once (N elements, or NULL).
  * z: as b200_ffn_act left it; with B200_ACT_NONE it is not read. */
 int b200_ffn_act_grad(const void* dC, const float* z, void* dz, void* dbias, int rows, int N,
@@ -92,14 +92,16 @@ typedef struct {
   int type;
 } b200_tensor;
 
-/* *norm (device memory, fp32) = the 2-norm of all elements together, summed in
- * fp64 (squares that fp32 does not hold included) and rounded once. */
+/* *norm (device memory, fp32) = the 2-norm of all elements together.  Squares are
+ * added 16 bytes of a tensor at a time in fp32 (in fp64 where fp32 does not hold them)
+ * and those sums in fp64, in one order; within 2^-21 of the norm. */
 int b200_grad_norm(const b200_tensor* tensors, int n, float* norm, void* stream);
 
 /* The same, and every element multiplied by min(1, max_norm / (norm + 1e-6)) in
  * fp32 and rounded; nothing is written where that is 1.  Tensors must not overlap.
  * A norm that is not a number makes every element one; an infinite one makes them
- * zero, and infinite elements not a number.  max_norm >= 0. */
+ * zero, and infinite elements not a number (all of them, if max_norm is infinite
+ * too).  max_norm >= 0. */
 int b200_clip_grads(const b200_tensor* tensors, int n, float max_norm, float* norm, void* stream);
 
 #ifdef __cplusplus
