@@ -365,7 +365,8 @@ Bytes bytes_of(const at::Tensor& t) {
 }
 
 // Whether two tensors have a byte in common: whether the terms of the one less those of
-// the other can make the distance of their beginnings.  A search from the largest stride
+// the other can make the distance of their beginnings.  Or two elements of one tensor:
+// whether differences of its indexes that are not all zero make none.  A search from the largest stride
 // down, in which each term has only the few values that leave a distance the rest can
 // make; one that takes too long (strides without order among many dimensions) counts as
 // one that was found.
@@ -407,22 +408,36 @@ struct Meeting {
       if (reach(i + 1, distance - k * t.stride)) return true;
     return false;
   }
-  static bool found(const Bytes& a, const Bytes& b) {
-    if (a.dense && b.dense) return true;  // (whose extents cross)
-    Meeting m;
-    m.add(a, 1);
-    m.add(b, -1);
-    std::sort(m.terms.begin(), m.terms.end(),
+  void order() {
+    std::sort(terms.begin(), terms.end(),
               [](const Term& x, const Term& y) { return x.stride > y.stride; });
     int64_t least = 0, most = 0;
-    for (size_t i = m.terms.size(); i-- > 0;) {
-      Term& t = m.terms[i];
+    for (size_t i = terms.size(); i-- > 0;) {
+      Term& t = terms[i];
       t.least = least;
       t.most = most;
       least += t.lo * t.stride;
       most += t.hi * t.stride;
     }
+  }
+  static bool between(const Bytes& a, const Bytes& b) {
+    if (a.dense && b.dense) return true;  // (whose extents cross)
+    Meeting m;
+    m.add(a, 1);
+    m.add(b, -1);
+    m.order();
     return m.reach(0, b.begin - a.begin);
+  }
+  static bool within(const at::Tensor& t) {
+    Meeting m;
+    for (int64_t i = 0; i < t.dim(); ++i)
+      if (t.size(i) > 1) m.terms.push_back({t.stride(i), 1 - t.size(i), t.size(i) - 1, 0, 0});
+    m.order();
+    // (the first difference that is not zero may be taken as positive)
+    for (size_t i = 0; i < m.terms.size(); ++i)
+      for (int64_t k = 1; k <= m.terms[i].hi && k * m.terms[i].stride <= m.terms[i].most; ++k)
+        if (m.reach(i + 1, -k * m.terms[i].stride)) return true;
+    return false;
   }
 };
 
@@ -431,14 +446,18 @@ struct Meeting {
 void check_apart(const std::vector<at::Tensor>& grads, const char* who) {
   std::vector<Bytes> spans;
   spans.reserve(grads.size());
-  for (const at::Tensor& g : grads)
-    if (g.numel() != 0) spans.push_back(bytes_of(g));
+  for (const at::Tensor& g : grads) {
+    if (g.numel() == 0) continue;
+    spans.push_back(bytes_of(g));
+    TORCH_CHECK(spans.back().dense || !Meeting::within(g), who,
+                ": gradients must not share memory");
+  }
   auto before = [](const Bytes& a, const Bytes& b) { return a.begin < b.begin; };
   if (!std::is_sorted(spans.begin(), spans.end(), before))
     std::sort(spans.begin(), spans.end(), before);
   for (size_t i = 0; i < spans.size(); ++i)
     for (size_t j = i + 1; j < spans.size() && spans[j].begin < spans[i].end; ++j)
-      TORCH_CHECK(!Meeting::found(spans[i], spans[j]), who, ": gradients must not share memory");
+      TORCH_CHECK(!Meeting::between(spans[i], spans[j]), who, ": gradients must not share memory");
 }
 
 // Where the work goes; nowhere yet if the checks are going to refuse it.

@@ -81,7 +81,7 @@ def clip_grads_b200(grads, max_norm: float):
     a norm of max_norm - 1e-6 down) nothing is written, but for tensors with gaps between
     their elements: these go through a copy and back.  A norm that is NaN makes every
     gradient NaN, an infinite one zero, and NaN where it was infinite (every one NaN if
-    max_norm is infinite too).  Tensors that share memory are refused (rows, columns and
+    max_norm is infinite too).  Elements that share memory are refused (rows, columns and
     planes that lie between one another's do not)."""
     return _ext().clip_grads_b200(_list(grads), max_norm)
 

@@ -1,4 +1,5 @@
-"""Gradients that share memory are refused wherever their elements meet, and only there."""
+"""Gradients that share memory, with one another or within themselves, are refused wherever
+their elements meet, and only there."""
 import pytest
 import torch
 
@@ -27,6 +28,10 @@ SHARED = {
     "another type": lambda x, y: [x.view(torch.float32)[:, :2], x[:, 3:8]],
     "half of an element": lambda x, y: [y[:, ::2, ::2], y.view(torch.bfloat16)[1:2, 2:3, 1:2]],
     "a diagonal": lambda x, y: [x.as_strided((8,), (17,)), x[:, 4:8]],
+    "windows of one tensor": lambda x, y: [x.as_strided((5, 8), (4, 1))],
+    "a row and the next, shifted": lambda x, y: [y, x.as_strided((3, 3), (1, 1))],
+    "two dimensions of one stride": lambda x, y: [x.as_strided((2, 2, 3), (20, 20, 3))],
+    "strides that meet": lambda x, y: [x.as_strided((4, 5), (6, 4))],
     "third among others": lambda x, y: [x[:, :4], x[:, 8:], y, x[5:6, 3:5]],
 }
 APART = {
@@ -37,6 +42,8 @@ APART = {
     "between the rows": lambda x, y: [x[:, :4], x[0, 4:16], x[1, 4:16]],
     "another type": lambda x, y: [x.view(torch.float32)[:, :2], x[:, 4:8]],
     "a diagonal": lambda x, y: [x.as_strided((4,), (17,)), x[:, 4:8]],
+    "strides that do not meet": lambda x, y: [x.as_strided((2, 4), (9, 6))],
+    "strides out of order": lambda x, y: [x.as_strided((2, 3, 4), (3, 40, 7))],
     "empty": lambda x, y: [x[:, :4], x[:, 2:2], x[3:3]],
 }
 
