@@ -38,10 +38,10 @@ def matmul_b200_act(A, B, bias=None, residual=None, *, activation: str = "none")
     element).  Its gradient is rounded to A's dtype before the products that make A's
     and B's -- in fp16 to infinity beyond 65504, where the gradients themselves might
     not be: scale the loss, or take bf16 -- and the bias' is summed before that.  What
-    comes back through relu is zero up to z = 0, whatever arrives.  The gradient of B is a (K, N) view of
-    (N, K) memory, the layout of the weight.  An operand whose rows are not on 16 bytes
-    (K no multiple of 8) costs a copy of it per call, with gradients per training
-    step."""
+    comes back through relu is zero up to z = 0, whatever arrives.  The gradient of B
+    is a (K, N) view of (N, K) memory, the layout of the weight.  An operand whose rows
+    are not on 16 bytes (K no multiple of 8) costs a copy of it per call, with gradients
+    per training step."""
     return _ext().matmul_b200_act(A, B, bias, residual, activation)
 
 
