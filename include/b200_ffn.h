@@ -53,8 +53,8 @@ int b200_ffn_gated(const void* A, const void* Wg, const void* Wu, const int* off
 
 /* From the gradient of b200_ffn_act's C that of its product: dz = dC * act'(z),
  * rounded (fp16: infinite beyond 65504; dz: rows x lddz, 16-byte aligned, lddz >= N a
- * multiple of 8; or NULL), and dbias = the unrounded sum of its rows, rounded once (N elements, or NULL).
- * z: as b200_ffn_act left it; with B200_ACT_NONE it is not read. */
+ * multiple of 8; or NULL), and dbias = the unrounded sum of its rows, rounded once
+ * (N elements, or NULL).  z: as b200_ffn_act left it; with B200_ACT_NONE it is not read. */
 int b200_ffn_act_grad(const void* dC, const float* z, void* dz, void* dbias, int rows, int N,
                       int ldc, int ldz, int lddz, int act, int dtype, void* stream);
 
