@@ -366,10 +366,10 @@ Bytes bytes_of(const at::Tensor& t) {
 
 // Whether two tensors have a byte in common: whether the terms of the one less those of
 // the other can make the distance of their beginnings.  Or two elements of one tensor:
-// whether differences of its indexes that are not all zero make none.  A search from the largest stride
-// down, in which each term has only the few values that leave a distance the rest can
-// make; one that takes too long (strides without order among many dimensions) counts as
-// one that was found.
+// whether differences of its indexes that are not all zero make none.  A search from the
+// largest stride down, in which each term has only the few values that leave a distance the
+// rest can make; one that takes too long (strides without order among many dimensions)
+// counts as one that was found.
 struct Meeting {
   struct Term {
     int64_t stride, lo, hi;

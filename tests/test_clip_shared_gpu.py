@@ -1,5 +1,8 @@
 """Gradients that share memory, with one another or within themselves, are refused wherever
 their elements meet, and only there."""
+import math
+import random
+
 import pytest
 import torch
 
@@ -72,3 +75,36 @@ def test_many_columns():
     check([x[:, i:i + 1] for i in range(300)], 0.5)
     with pytest.raises(RuntimeError, match="share memory"):
         bg.clip_grads_b200([x[:, i:i + 1] for i in range(300)] + [x[7:9, 255:257]], 0.5)
+
+
+def test_against_enumeration():
+    """Views of one buffer with any strides, of both element sizes: refused exactly where two
+    elements have a byte in common."""
+    r = random.Random(0)
+    wide = torch.randn(200, device="cuda")
+    buffers = {4: wide, 2: wide.view(torch.bfloat16)}
+    seen = [0, 0]
+    for _ in range(600):
+        views, taken, met = [], set(), False
+        for _ in range(r.randint(1, 3)):
+            size = r.choice([2, 4])
+            flat = buffers[size]
+            shape = [r.randint(1, 4) for _ in range(r.randint(1, 3))]
+            strides = [r.choice([1, 2, 3, 5, 8, 12, 16, 20]) for _ in shape]
+            start = r.randint(0, 400 // size)
+            at = [start]
+            for n, s in zip(shape, strides):
+                at = [a + i * s for a in at for i in range(n)]
+            assert max(at) < flat.numel()
+            for a in at:
+                mine = {a * size + b for b in range(size)}
+                met |= bool(mine & taken)
+                taken |= mine
+            views.append(flat.as_strided(shape, strides, start))
+        seen[met] += 1
+        if met:
+            with pytest.raises(RuntimeError, match="share memory"):
+                bg.clip_grads_b200(views, math.inf)
+        else:
+            bg.clip_grads_b200(views, math.inf)
+    assert min(seen) > 100, seen
